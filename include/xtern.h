@@ -402,6 +402,118 @@ int xt_stack_run(const xt_stack* st, void* stream);
 int xt_stack_check(xt_stack* st, int* gave_up);
 int xt_stack_destroy(xt_stack* st);
 
+/* ---- Paged key-value cache: append, attention, eviction ----
+ * What a decode step does between its projections (CausalSelfAttention::
+ * forward, src/models/llama/attention.rs:42-113, with the ring cache of
+ * src/nn/fast_attention.rs:7-75 in pages instead): rotate the new queries and
+ * keys, write keys and values into the cache, attend over it, and cut a cache
+ * that has grown too long down to the positions that were attended to most.
+ *
+ * Element types of a cache (and of logits): */
+enum { XT_F32 = 0, XT_F16 = 1, XT_BF16 = 2 };
+
+/* A pool of pages in device memory that the caller owns.  Element d of head h
+ * in slot s of page p lies at p * stride_page + s * stride_slot + h *
+ * stride_head + d of both k and v (strides in elements, of any order, pages
+ * and slots not overlapping; any alignment, 16 bytes are fastest).  score:
+ * NULL, or the attention weight that each position has received so far,
+ * [num_pages][kv_heads][page_size] f32.  head_dim 1..256, page_size
+ * 1..65536. */
+typedef struct xt_kv_cache {
+    void* k;
+    void* v;
+    float* score;
+    int dtype;
+    int kv_heads;
+    int head_dim;
+    int page_size;
+    int64_t num_pages;
+    int64_t stride_page;
+    int64_t stride_slot;
+    int64_t stride_head;
+} xt_kv_cache;
+
+/* The pages of each sequence, on the device: position i of sequence b lies in
+ * slot i % page_size of page pages[b * stride + i / page_size].  An entry
+ * outside [0, num_pages) (-1 by custom) is no page: its positions hold
+ * nothing, are never read or written, and attention skips them.  Lengths
+ * above max_pages * page_size (which is below 2^31) count as that, negative
+ * ones as 0. */
+typedef struct xt_kv_table {
+    const int32_t* pages;
+    int64_t stride;
+    int64_t seqs;
+    int64_t max_pages;
+} xt_kv_table;
+
+/* Rotary embedding tables, on the device: cos and sin [rows][dim / 2] f32, a
+ * row for each rotary position.  With h = dim / 2, element i < h of a head
+ * becomes x[i] cos[i] - x[i + h] sin[i] and element i + h becomes x[i + h]
+ * cos[i] + x[i] sin[i]; elements from dim on stay (dim even, 2..head_dim). */
+typedef struct xt_rope {
+    const float* cos;
+    const float* sin;
+    int64_t rows;
+    int dim;
+} xt_rope;
+
+/* R new tokens: k and v [R][kv_heads * head_dim] f32 (row strides ldk, ldv)
+ * go to position slots[r] of sequence seq[r] (seq NULL: sequence r), rounded
+ * to the cache's type (nearest even), k rotated first if rope is given, by
+ * row positions[r] of its tables (positions NULL: slots[r]; after an eviction
+ * a token's slot is lower than its position).  q (may be NULL)
+ * [R][q_heads * head_dim] is rotated likewise into q_out, which may be q.
+ * A cache with scores gets 0 for the new positions.  A row whose slot is
+ * negative or past the table, whose sequence or page does not exist or whose
+ * position is not in the rope tables is skipped: nothing is written for it.
+ * Two rows of one call must not name one slot (its contents are then
+ * unspecified). */
+int xt_kv_append(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
+                 const int32_t* slots, const int32_t* positions, const xt_rope* rope,
+                 const float* q, int64_t ldq, int q_heads, float* q_out, int64_t ldqo,
+                 const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t R,
+                 void* stream);
+
+/* Attention of one token per row r over the first lengths[r] positions of
+ * sequence seq[r] (seq NULL: sequence r; several rows may name one sequence,
+ * e.g. the tokens of a prompt with growing lengths): query head h of q
+ * [R][q_heads * head_dim] f32 reads key-value head h / (q_heads / kv_heads),
+ *   s_j = scale q.k_j,  out = sum_j softmax(s)_j v_j,  lse = ln sum_j exp(s_j)
+ * out [R][q_heads * head_dim] f32, lse (may be NULL) [R][q_heads].  A row
+ * without positions (or whose every s_j is -inf) gives zeros and lse = -inf.
+ * accumulate != 0 adds to the score of each position and key-value head the
+ * weight that its group's query heads gave it, sum_h softmax(s_h)_j (atomic
+ * adds: the sum over rows that share a page is in no fixed order). */
+int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
+                       const int32_t* lengths, const float* q, int64_t ldq, int q_heads,
+                       float scale, int64_t R, float* out, int64_t ldo, float* lse,
+                       int accumulate, void* stream);
+
+/* Cut every sequence b of the table that holds lengths[b] > budget positions
+ * down to budget, for each key-value head by its own scores: the first sink
+ * and the last recent positions stay, and of those between the ones of the
+ * highest score (ties to the lowest position; NaN below every number,
+ * positions without a page last).  What stays moves, in order, to positions
+ * 0..budget - 1 with its score; later positions keep their old contents.
+ * new_lengths[b] = min(lengths[b], budget) (another array than lengths);
+ * kept [seqs][kv_heads][budget] receives the old position of each that
+ * stayed, -1 past the new length.  sink + recent <= budget.  No page may
+ * belong to two positions of the table. */
+int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengths,
+                int64_t budget, int64_t sink, int64_t recent, int32_t* new_lengths,
+                int32_t* kept, void* stream);
+
+/* What a row of logits x [M][V] (row stride ld, dtype as above; -inf masks a
+ * token) says about tokens: logprobs [M][T] = x_t - ln sum exp(x) of the
+ * given tokens [M][T] (0 for a negative id, NaN for one past the
+ * vocabulary), entropy [M] = -sum p ln p in nats, and the top (0..64, at most
+ * V) most likely tokens with their log probabilities, [M][top] each, ties to
+ * the lowest id, NaN last.  A row of nothing but -inf gives -inf for every
+ * token and entropy 0; one with a NaN or +inf gives NaN. */
+int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int64_t V,
+                      const int32_t* tokens, int64_t T, float* logprobs, float* entropy, int top,
+                      int32_t* top_ids, float* top_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

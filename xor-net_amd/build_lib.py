@@ -13,7 +13,8 @@ OUT = os.path.join(HERE, "xtern", "libxtern.so")
 
 SOURCES = ["xtern_kernels.hip", "xtern_gemm.hip", "xtern_mid.hip",
            "xtern_sstack.hip", "xtern_gstream.hip", "xtern_xs.hip",
-           "xtern_api.cpp", "xtern_layout.cpp", "xtern_container.cpp"]
+           "xtern_attn.hip", "xtern_evict.hip", "xtern_probs.hip",
+           "xtern_cache_api.cpp", "xtern_api.cpp", "xtern_layout.cpp", "xtern_container.cpp"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

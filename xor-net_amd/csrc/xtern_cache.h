@@ -1,0 +1,123 @@
+// Internal declarations of the paged key-value cache (append, attention,
+// eviction) and of the token probabilities: kernel arguments and launchers
+// (xtern_attn.hip, xtern_evict.hip, xtern_probs.hip), called by
+// xtern_cache_api.cpp.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/xtern.h"
+
+namespace xt {
+
+// The cache as the kernels see it: strides in elements, score
+// [num_pages][hkv][page] or null.
+struct KvView {
+    void* k;
+    void* v;
+    float* score;
+    int64_t sp, ss, sh;  // element strides of a page, a slot, a head
+    int num_pages, page, hkv, D;
+    const int32_t* table;  // [nseq][max_pages], row stride ldt
+    int64_t ldt;
+    int nseq, max_pages;
+};
+
+struct AppendArgs {
+    KvView c;
+    const int32_t* seq;    // [R] or null (row r belongs to sequence r)
+    const int32_t* slots;  // [R] cache positions; negative: no row
+    const int32_t* pos;    // [R] rotary positions (rope only)
+    const float* cos;      // [rope_rows][rot / 2], or null (no rotation)
+    const float* sin;
+    int64_t rope_rows;
+    int rot;
+    const float* q;        // [R] rows of hq * D, stride ldq; or null
+    float* qo;
+    const float* k;
+    const float* v;
+    int64_t ldq, ldqo, ldk, ldv;
+    int hq;
+    int64_t R;
+};
+hipError_t launch_kv_append(int dtype, const AppendArgs& a, hipStream_t s);
+
+struct AttnArgs {
+    KvView c;
+    const int32_t* seq;      // [R] or null
+    const int32_t* lengths;  // [R]
+    const float* q;
+    float* out;
+    float* lse;              // [R][hq] or null
+    int64_t ldq, ldo;
+    int hq;
+    float scale;
+    int accumulate;
+    int64_t R;
+};
+hipError_t launch_paged_attention(int dtype, const AttnArgs& a, hipStream_t s);
+
+struct EvictArgs {
+    KvView c;
+    const int32_t* lengths;  // [nseq]
+    int32_t* new_lengths;    // [nseq]
+    int32_t* kept;           // [nseq][hkv][budget]
+    int budget, sink, recent;
+};
+hipError_t launch_kv_evict(int dtype, const EvictArgs& a, hipStream_t s);
+
+struct ProbsArgs {
+    const void* x;  // [M] rows of V logits, stride ld
+    int64_t ld;
+    int64_t M;
+    int V;
+    const int32_t* tokens;  // [M][T]
+    int T;
+    float* lp;       // [M][T]
+    float* entropy;  // [M]
+    int top;
+    int32_t* ids;    // [M][top]
+    float* top_lp;   // [M][top]
+};
+hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, hipStream_t s);
+
+#ifdef __HIPCC__
+
+// One element of the cache or of the logits as f32, and back (round to
+// nearest even; f16 overflows to infinity).
+template <int DT> struct Elem;
+template <> struct Elem<XT_F32> {
+    typedef float T;
+    static __device__ __forceinline__ float get(T v) { return v; }
+    static __device__ __forceinline__ T put(float v) { return v; }
+};
+template <> struct Elem<XT_F16> {
+    typedef _Float16 T;
+    static __device__ __forceinline__ float get(T v) { return (float)v; }
+    static __device__ __forceinline__ T put(float v) { return (T)v; }
+};
+template <> struct Elem<XT_BF16> {
+    typedef __bf16 T;
+    static __device__ __forceinline__ float get(T v) { return (float)v; }
+    static __device__ __forceinline__ T put(float v) { return (T)v; }
+};
+
+// The page that holds position p of sequence `seq`, or -1: a table entry
+// outside the pool holds nothing.  0 <= p < max_pages * page.
+__device__ __forceinline__ int kv_page(const KvView& c, int seq, int p) {
+    const int e = c.table[(int64_t)seq * c.ldt + p / c.page];
+    return (unsigned)e < (unsigned)c.num_pages ? e : -1;
+}
+__device__ __forceinline__ int64_t kv_offset(const KvView& c, int pg, int p, int h) {
+    return (int64_t)pg * c.sp + (int64_t)(p % c.page) * c.ss + (int64_t)h * c.sh;
+}
+// A length as the kernels use it: within the table's row.
+__device__ __forceinline__ int kv_length(const KvView& c, int n) {
+    const int64_t cap = (int64_t)c.max_pages * c.page;
+    return n < 0 ? 0 : (n > cap ? (int)cap : n);
+}
+
+#endif
+
+}  // namespace xt

@@ -14,6 +14,7 @@ Mirrored reference API (paths relative to xor-net):
   encode_sparse_tensor            src/bit1_58/sparse.rs:61-103
   TernaryLinear                   src/bit1_58/layers.rs:34-750
   DynamicLinear (Ternary arm)     src/nn/dynamic_linear.rs:610-680
+  CausalSelfAttention             src/models/llama/attention.rs:42-113
 """
 import ctypes
 import enum
@@ -280,7 +281,7 @@ def _torch():
 try:
     _raw_stream, _cur_device = _torch_mod._C._cuda_getCurrentRawStream, _torch_mod._C._cuda_getDevice
 except AttributeError:  # (a torch without them, or none)
-    _raw_stream = None
+    _raw_stream = _cur_device = None
 
 
 def _stream_ptr(stream=None):
@@ -752,8 +753,10 @@ def linear_multi_q(ws, q, inv, stream=None):
     return ys
 
 
+from .cache import (XT_F32, XT_F16, XT_BF16, KvCache, kv_append, kv_evict,  # noqa: E402,F401
+                    paged_attention, token_logprobs)
 from .layers import (TernaryLinear, DynamicLinear, TernaryRep, FastRmsNorm, Mlp,  # noqa: E402,F401
-                     Int8Linear, Int4Linear)
+                     Int8Linear, Int4Linear, CausalSelfAttention)
 
 
 class Stack:

@@ -11,8 +11,8 @@ import numpy as np
 
 from . import (XT_ERR_INVALID, XT_PACK4, XT_PACK5, XT_QUANT_AVX512, XT_XORSPARSE,
                DeviceWeights, TernaryPackType, XternError, _ternarise, encode_sparse_tensor,
-               hf_destripe, mlp_f32, mlp_q, rms_norm, XT_INT8, XT_INT4, int_quantize_host,
-               linear_f32, linear_multi_q, linear_q, pack_ternary4, pack_ternary5,
+               hf_destripe, kv_append, mlp_f32, mlp_q, paged_attention, rms_norm, XT_INT8, XT_INT4, int_quantize_host,
+               linear_f32, linear_multi_f32, linear_multi_q, linear_q, pack_ternary4, pack_ternary5,
                unpack_1_58bit_4pack, unpack_1_58bit_5pack)
 
 
@@ -327,6 +327,51 @@ class Mlp:
         return sum(l.packed_bytes() for l in (self.c_fc1, self.c_fc2, self.c_proj))
 
 
+class CausalSelfAttention:
+    """models/llama/attention.rs:42-113 over a paged cache: ternary q, k, v
+    and o projections, rotary embedding, grouped-query attention and the
+    optional attn_sub_norm."""
+
+    def __init__(self, q_proj, k_proj, v_proj, o_proj, head_dim, attn_sub_norm=None):
+        if q_proj.out_dim % head_dim or k_proj.out_dim % head_dim or v_proj.out_dim != k_proj.out_dim:
+            raise XternError(XT_ERR_INVALID, "q, k and v must be whole heads, k and v of one size")
+        if o_proj.in_dim != q_proj.out_dim:
+            raise XternError(XT_ERR_INVALID, f"Input dimension mismatch: expected {o_proj.in_dim}, "
+                                             f"got {q_proj.out_dim}")
+        self.q_proj, self.k_proj, self.v_proj, self.o_proj = q_proj, k_proj, v_proj, o_proj
+        self.head_dim = int(head_dim)
+        self.attn_sub_norm = attn_sub_norm
+
+    def forward(self, x, cache, table, slots, seq=None, positions=None, rope=None, accumulate=False,
+                mode=XT_QUANT_AVX512):
+        """x [R, hidden]: R new tokens, token r at position slots[r] (int32
+        [R], -1 for a padding row) of sequence seq[r] (default r) of table
+        (int32 [seqs, max_pages]).  Appends their keys and values to `cache`
+        (KvCache), then lets each attend over its sequence up to itself, so
+        the tokens of a prompt, in order, go in one call.  positions (int32
+        [R], default slots) are the rotary ones, rope = (cos, sin) their
+        tables.  accumulate adds the weights to cache.score.  Returns [R,
+        hidden]."""
+        if x.dim() != 2:
+            raise XternError(XT_ERR_INVALID, "x must be [rows, hidden]")
+        if x.shape[-1] != self.q_proj.in_dim:
+            raise XternError(XT_ERR_INVALID,
+                             f"Input dimension mismatch: expected {self.q_proj.in_dim}, got {x.shape[-1]}")
+        if cache.head_dim != self.head_dim or cache.kv_heads * self.head_dim != self.k_proj.out_dim:
+            raise XternError(XT_ERR_INVALID, "the cache's heads are not the projections'")
+        x = x.contiguous()
+        ws = [l.weights for l in (self.q_proj, self.k_proj, self.v_proj)]
+        if all(w.fmt == ws[0].fmt and w.in_dim == ws[0].in_dim for w in ws):
+            q, k, v = linear_multi_f32(ws, x, mode=mode)
+        else:
+            q, k, v = (linear_f32(w, x, mode=mode) for w in ws)
+        kv_append(cache, table, slots, k, v, q=q, seq=seq, positions=positions, rope=rope, q_out=q)
+        y = paged_attention(cache, table, slots + 1, q, seq=seq, accumulate=accumulate)
+        if self.attn_sub_norm is not None:
+            y = self.attn_sub_norm.forward(y)
+        return linear_f32(self.o_proj.weights, y, mode=mode)
+
+
 class DynamicLinear:
     """dynamic_linear.rs:619-643 — the Ternary arm of LinearKind."""
 
@@ -359,5 +404,5 @@ class DynamicLinear:
 
 
 __all__ = ["TernaryLinear", "DynamicLinear", "TernaryRep", "FastRmsNorm", "Mlp", "Int8Linear",
-           "Int4Linear", "TernaryPackType", "XT_PACK4",
+           "Int4Linear", "CausalSelfAttention", "TernaryPackType", "XT_PACK4",
            "XT_PACK5"]
