@@ -437,7 +437,7 @@ typedef struct xt_kv_cache {
  * slot i % page_size of page pages[b * stride + i / page_size].  An entry
  * outside [0, num_pages) (-1 by custom) is no page: its positions hold
  * nothing, are never read or written, and attention skips them.  Lengths
- * above max_pages * page_size (which is below 2^31) count as that, negative
+ * above max_pages * page_size (which is at most 2^30) count as that, negative
  * ones as 0. */
 typedef struct xt_kv_table {
     const int32_t* pages;
@@ -477,13 +477,17 @@ int xt_kv_append(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
 /* Attention of one token per row r over the first lengths[r] positions of
  * sequence seq[r] (seq NULL: sequence r; several rows may name one sequence,
  * e.g. the tokens of a prompt with growing lengths): query head h of q
- * [R][q_heads * head_dim] f32 reads key-value head h / (q_heads / kv_heads),
+ * [R][q_heads * head_dim] f32 reads key-value head h / (q_heads / kv_heads)
+ * (at most 1024 query heads each),
  *   s_j = scale q.k_j,  out = sum_j softmax(s)_j v_j,  lse = ln sum_j exp(s_j)
  * out [R][q_heads * head_dim] f32, lse (may be NULL) [R][q_heads].  A row
  * without positions (or whose every s_j is -inf) gives zeros and lse = -inf.
  * accumulate != 0 adds to the score of each position and key-value head the
  * weight that its group's query heads gave it, sum_h softmax(s_h)_j (atomic
- * adds: the sum over rows that share a page is in no fixed order). */
+ * adds: the sum over rows that share a page is in no fixed order).  Rows are
+ * split over their length; the parts, and with accumulate the R * q_heads *
+ * max_pages * page_size scores, lie in a per-stream device workspace owned by
+ * the library. */
 int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
                        const int32_t* lengths, const float* q, int64_t ldq, int q_heads,
                        float scale, int64_t R, float* out, int64_t ldo, float* lse,

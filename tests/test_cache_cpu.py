@@ -80,7 +80,7 @@ FAULTS = [
     (append, dict(r=rope(cos=None))), (append, dict(r=rope(sin=None))), (append, dict(r=rope(rows=-1))),
     (append, dict(r=rope(cos=P + 2))),
     (attend, dict(R=-1)), (attend, dict(lengths=None)), (attend, dict(q=None)), (attend, dict(out=None)),
-    (attend, dict(hq=5)), (attend, dict(hq=0)), (attend, dict(hq=-2)), (attend, dict(ldq=255)),
+    (attend, dict(hq=5)), (attend, dict(hq=2050, ldq=1 << 20, ldo=1 << 20)), (attend, dict(hq=0)), (attend, dict(hq=-2)), (attend, dict(ldq=255)),
     (attend, dict(ldo=255)), (attend, dict(scale=float("nan"))), (attend, dict(scale=float("inf"))),
     (attend, dict(c=cache(score=None), acc=1)), (attend, dict(lse=P + 2)), (attend, dict(q=P + 1)),
     (evict, dict(c=cache(score=None))), (evict, dict(budget=0)), (evict, dict(budget=1 << 31)),

@@ -63,7 +63,8 @@ int hip_fail(hipError_t e, const char* what) {
 //   kind 1: split-K partial-sum planes and arrival counters.  Zeroed when
 //           allocated; every product launch leaves the counters zero again
 //           (the last workgroup of a tile resets its counter);
-//   kind 2: the MLP's gate / up rows and requantised intermediate.
+//   kind 2: the MLP's gate / up rows and requantised intermediate;
+//   kind 3: paged attention's partial results (xtern_cache_api.cpp).
 int hipb_device(int* d) { return (int)hipGetDevice(d); }
 int hipb_alloc(void** p, size_t n) { return (int)hipMalloc(p, n); }
 int hipb_free(void* p) { return (int)hipFree(p); }
@@ -559,8 +560,12 @@ int mlp_run(const xt_weights* gate, const xt_weights* up, const xt_weights* down
 
 }  // namespace
 
-// Error reporting for the other host source files (xtern_container.cpp).
+// For the other host source files (xtern_container.cpp, xtern_cache_api.cpp).
 int xt_internal_fail(int code, const std::string& msg) { return fail(code, msg); }
+int xt_internal_workspace(hipStream_t s, size_t bytes, void** out, int kind) {
+    return workspace(s, bytes, out, kind);
+}
+int xt_internal_cus(int* cus) { return device_cus(cus); }
 
 extern "C" {
 

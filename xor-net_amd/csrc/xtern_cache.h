@@ -56,7 +56,11 @@ struct AttnArgs {
     int accumulate;
     int64_t R;
 };
-hipError_t launch_paged_attention(int dtype, const AttnArgs& a, hipStream_t s);
+// A call whose rows may be split, or that accumulates, needs a workspace
+// (attention_joins) of attention_workspace bytes; cus: compute units.
+bool attention_joins(const AttnArgs& a, int cus);
+size_t attention_workspace(const AttnArgs& a, int cus);
+hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, hipStream_t s);
 
 struct EvictArgs {
     KvView c;

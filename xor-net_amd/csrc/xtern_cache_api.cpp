@@ -13,7 +13,11 @@
 #include "../../include/xtern.h"
 #include "xtern_cache.h"
 
+// xtern_api.cpp: error message, workspace of a stream (kind 3 is this file's),
+// compute units of the current device.
 int xt_internal_fail(int code, const std::string& msg);
+int xt_internal_workspace(hipStream_t s, size_t bytes, void** out, int kind);
+int xt_internal_cus(int* cus);
 
 namespace {
 
@@ -24,6 +28,8 @@ int launched(hipError_t e, const char* what) {
 }
 
 constexpr int64_t kMaxInt = 0x7fffffff;
+constexpr int64_t kMaxLen = (int64_t)1 << 30;  // positions of a sequence
+constexpr int kMaxGroup = 1024;                // query heads of a key-value head
 
 int check_dtype(int dtype) {
     if (dtype != XT_F32 && dtype != XT_F16 && dtype != XT_BF16)
@@ -64,8 +70,8 @@ int check_cache(const xt_kv_cache* c, const xt_kv_table* t, xt::KvView* view) {
         span += x.stride * (x.extent - 1);
     }
     if (t->seqs < 0 || t->seqs > kMaxInt) return bad("seqs must be 0..2^31-1");
-    if (t->max_pages < 0 || t->max_pages * c->page_size > kMaxInt || t->max_pages > kMaxInt)
-        return bad("max_pages * page_size must be 0..2^31-1");
+    if (t->max_pages < 0 || t->max_pages > kMaxLen || t->max_pages * c->page_size > kMaxLen)
+        return bad("max_pages * page_size must be 0..2^30");
     if (t->seqs > 0 && t->max_pages > 0 && !t->pages) return bad("NULL pointer");
     if (t->stride < t->max_pages && t->seqs > 1) return bad("table rows overlap");
     if (int rc = check_align(t->pages, 4, "the page table")) return rc;
@@ -101,8 +107,8 @@ int check_count(int64_t R) {
 }
 
 int check_heads(int q_heads, int kv_heads) {
-    if (q_heads < 1 || q_heads > 65535 || q_heads % kv_heads)
-        return bad("q_heads must be a multiple of kv_heads, 1..65535");
+    if (q_heads < 1 || q_heads > 65535 || q_heads % kv_heads || q_heads / kv_heads > kMaxGroup)
+        return bad("q_heads must be a multiple of kv_heads, 1..65535, at most 1024 times kv_heads");
     return XT_OK;
 }
 
@@ -188,7 +194,14 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     a.ldo = ldo;
     a.lse = lse;
     a.accumulate = accumulate ? 1 : 0;
-    return launched(xt::launch_paged_attention(c->dtype, a, static_cast<hipStream_t>(stream)),
+    int cus = 0;
+    if (int rc = xt_internal_cus(&cus)) return rc;
+    void* ws = nullptr;
+    if (xt::attention_joins(a, cus)) {
+        if (int rc = xt_internal_workspace(static_cast<hipStream_t>(stream), xt::attention_workspace(a, cus), &ws, 3))
+            return rc;
+    }
+    return launched(xt::launch_paged_attention(c->dtype, a, cus, ws, static_cast<hipStream_t>(stream)),
                     "paged attention launch");
 }
 
