@@ -56,9 +56,8 @@ struct AttnArgs {
     int accumulate;
     int64_t R;
 };
-// A call whose rows may be split, or that accumulates, needs a workspace
-// (attention_joins) of attention_workspace bytes; cus: compute units.
-bool attention_joins(const AttnArgs& a, int cus);
+// Bytes of workspace that the call needs (0: none, ws is null); cus: compute
+// units of the device.
 size_t attention_workspace(const AttnArgs& a, int cus);
 hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, hipStream_t s);
 

@@ -197,9 +197,8 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
     void* ws = nullptr;
-    if (xt::attention_joins(a, cus)) {
-        if (int rc = xt_internal_workspace(static_cast<hipStream_t>(stream), xt::attention_workspace(a, cus), &ws, 3))
-            return rc;
+    if (const size_t bytes = xt::attention_workspace(a, cus)) {
+        if (int rc = xt_internal_workspace(static_cast<hipStream_t>(stream), bytes, &ws, 3)) return rc;
     }
     return launched(xt::launch_paged_attention(c->dtype, a, cus, ws, static_cast<hipStream_t>(stream)),
                     "paged attention launch");
