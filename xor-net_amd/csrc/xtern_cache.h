@@ -83,7 +83,8 @@ struct ProbsArgs {
     int32_t* ids;    // [M][top]
     float* top_lp;   // [M][top]
 };
-hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, hipStream_t s);
+size_t token_logprobs_workspace(const ProbsArgs& a, int cus);
+hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, hipStream_t s);
 
 #ifdef __HIPCC__
 

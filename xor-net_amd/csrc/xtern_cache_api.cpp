@@ -29,6 +29,7 @@ int launched(hipError_t e, const char* what) {
 
 constexpr int64_t kMaxInt = 0x7fffffff;
 constexpr int64_t kMaxLen = (int64_t)1 << 30;  // positions of a sequence
+constexpr int64_t kMaxRows = (int64_t)1 << 22;  // rows of a call: a workgroup each
 constexpr int kMaxGroup = 1024;                // query heads of a key-value head
 
 int check_dtype(int dtype) {
@@ -69,7 +70,7 @@ int check_cache(const xt_kv_cache* c, const xt_kv_table* t, xt::KvView* view) {
         if (x.stride > (INT64_MAX - span) / x.extent / 4) return bad("cache strides too large");
         span += x.stride * (x.extent - 1);
     }
-    if (t->seqs < 0 || t->seqs > kMaxInt) return bad("seqs must be 0..2^31-1");
+    if (t->seqs < 0 || t->seqs > kMaxRows) return bad("seqs must be 0..2^22");
     if (t->max_pages < 0 || t->max_pages > kMaxLen || t->max_pages * c->page_size > kMaxLen)
         return bad("max_pages * page_size must be 0..2^30");
     if (t->seqs > 0 && t->max_pages > 0 && !t->pages) return bad("NULL pointer");
@@ -102,7 +103,7 @@ int check_rows(const float* p, int64_t ld, int64_t R, int64_t cols, const char* 
 }
 
 int check_count(int64_t R) {
-    if (R < 0 || R > kMaxInt) return bad("row count must be 0..2^31-1");
+    if (R < 0 || R > kMaxRows) return bad("row count must be 0..2^22");
     return XT_OK;
 }
 
@@ -252,7 +253,13 @@ int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int6
     a.top = top;
     a.ids = top_ids;
     a.top_lp = top_logprobs;
-    return launched(xt::launch_token_logprobs(dtype, a, static_cast<hipStream_t>(stream)),
+    int cus = 0;
+    if (int rc = xt_internal_cus(&cus)) return rc;
+    void* ws = nullptr;
+    if (const size_t bytes = xt::token_logprobs_workspace(a, cus)) {
+        if (int rc = xt_internal_workspace(static_cast<hipStream_t>(stream), bytes, &ws, 3)) return rc;
+    }
+    return launched(xt::launch_token_logprobs(dtype, a, cus, ws, static_cast<hipStream_t>(stream)),
                     "token probabilities launch");
 }
 

@@ -6,94 +6,419 @@
 // Leaving the maximum's own 1 out of the sum keeps ln p of an almost certain
 // token exact to its last bits.  Logits of -inf have p = 0; a row of nothing
 // else gives ln p = -inf and H = 0.
+//
+// The logits are read once: HBM bounds large calls, the chain of load,
+// reduction and selection small ones.  A workgroup walks its slice of a row in
+// tiles of 8192 logits that stay in registers from the maximum over the sums to
+// the selection, the next tile in flight meanwhile; sums are per thread,
+// relative to the workgroup's running maximum, and reduced once at the end.  A
+// row is cut into slices only as far as there are too few rows for the chip
+// (then a second kernel joins them).
+//
+// Selection of the `top` largest: the minimum of G >= top disjoint groups'
+// maxima is a lower bound of the top-th largest logit, and of n logits only
+// about G ln G reach it (G = 32: 111 of 8192).  Those go to LDS, each counts
+// how many are before it, and the first `top` in that order are the list that
+// the next tile's candidates have to beat.  Where that fails (ties beyond the
+// buffer, fewer finite logits than `top`) the tile's logits are taken one
+// maximum after the other.
+#include <algorithm>
+
 #include "xtern_cache.h"
 #include "xtern_device.h"
 
 namespace xt {
 
-constexpr int kProbsThreads = 1024;
+typedef unsigned long long u64;
+
+constexpr int kProbsThreads = 512;
+constexpr int kProbsWaves = kProbsThreads / 64;
+constexpr int kProbsPer = 16;                              // logits of a thread and tile
+constexpr int kProbsTile = kProbsThreads * kProbsPer;
+constexpr int kProbsTop = 64;
+constexpr int kProbsCand = 1024;                           // candidates of a tile, with the list before it
+constexpr int kProbsSlices = 64;
+
+// Slices of a row: slice s is tiles [s * per, (s + 1) * per).
+struct ProbsPlan {
+    int slices, per, tiles;
+    float* stats;  // [M][slices][4]: m, z, xz, count of the maximum
+    u64* keys;     // [M][slices][top]
+};
 
 // Order of the alternatives: larger value first, then the lower index; NaN
-// behind everything.
-__device__ __forceinline__ unsigned long long probs_key(float x, int i) {
+// behind everything, no element (0) behind that.
+__device__ __forceinline__ u64 probs_key(float x, int i) {
     const float f = x + 0.0f;  // (-0 counts as +0)
     unsigned u = __float_as_uint(f);
     u = f != f ? 0u : u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
-    return ((unsigned long long)u << 32) | (unsigned)~i;
+    return ((u64)u << 32) | (unsigned)~i;
 }
+__device__ __forceinline__ float key_value(u64 k) {
+    const unsigned u = (unsigned)(k >> 32);
+    return __uint_as_float((u >> 31) ? u ^ 0x80000000u : ~u);
+}
+__device__ __forceinline__ int key_index(u64 k) { return (int)~(unsigned)k; }
 
-template <typename T, typename Op>
-__device__ __forceinline__ T wg_reduce(T v, T* sm, Op op) {
-    for (int o = 32; o; o >>= 1) v = op(v, (T)__shfl_xor(v, o));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sm[0];
-    for (int w = 1; w < kProbsThreads / 64; ++w) v = op(v, sm[w]);
+// Over the lanes that differ in bit `1 << s` of their number.
+template <int S>
+__device__ __forceinline__ float lane_xor(float v) {
+    if constexpr (S == 4) {
+        auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
+    } else if constexpr (S == 5) {
+        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+    } else if constexpr (S == 0) {
+        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xb1, 0xf, 0xf, true));  // quad_perm 1,0,3,2
+    } else if constexpr (S == 1) {
+        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4e, 0xf, 0xf, true));  // quad_perm 2,3,0,1
+    } else {
+        return __shfl_xor(v, 1 << S);
+    }
+}
+__device__ __forceinline__ float wave_sum_f(float v) {
+    v += lane_xor<0>(v);
+    v += lane_xor<1>(v);
+    v += lane_xor<2>(v);
+    v += lane_xor<3>(v);
+    v += lane_xor<4>(v);
+    v += lane_xor<5>(v);
     return v;
 }
 
+// Sums relative to m, of which `c` logits are m itself; to a larger maximum.
+struct ProbsSum {
+    float m, z, xz, c;
+    __device__ __forceinline__ void raise(float to) {
+        if (!(to > m)) return;
+        if (m == -INFINITY) {
+            z = z == z ? 0.0f : z;  // (a NaN stays)
+            xz = 0.0f;
+        } else {
+            const float d = m - to, f = __builtin_amdgcn_exp2f(d * 1.44269504f), s = z + c;
+            xz = f == 0.0f ? 0.0f : (xz + d * s) * f;
+            z = z == z ? (f == 0.0f ? 0.0f : s * f) : z;
+        }
+        m = to;
+        c = 0.0f;
+    }
+};
+
+struct ProbsLds {
+    float gmax[2][64];
+    float sums[3][kProbsWaves];
+    u64 cand[kProbsCand];
+    u64 list[kProbsTop];
+    u64 wbest[kProbsWaves];
+    int count;
+};
+
+// The row's results from its sums and its list of the `top` first keys.
 template <int DT>
-__global__ __launch_bounds__(kProbsThreads) void token_logprobs_kernel(ProbsArgs a) {
+__device__ void probs_finish(const ProbsArgs& a, int64_t r, ProbsSum s, const u64* list) {
     typedef Elem<DT> E;
-    const int64_t r = blockIdx.x;
-    const int t = threadIdx.x;
     const typename E::T* x = static_cast<const typename E::T*>(a.x) + r * a.ld;
-    __shared__ float smf[16];
-    __shared__ unsigned long long smk[16];
-    auto add = [](float p, float q) { return p + q; };
-    auto top = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
-    unsigned long long best = 0;
-    for (int i = t; i < a.V; i += kProbsThreads) {
-        const unsigned long long k = probs_key(E::get(x[i]), i);
-        best = top(best, k);
-    }
-    best = wg_reduce(best, smk, top);
-    const int imax = (int)~(unsigned)best;
-    const float m = E::get(x[imax]);
-    float z = 0.0f, xz = 0.0f;
-    for (int i = t; i < a.V; i += kProbsThreads) {
-        const float v = E::get(x[i]), d = v - m;
-        if (i == imax || v == -INFINITY) continue;
-        const float e = expf(d);
-        z += e;
-        xz += d * e;
-    }
-    z = wg_reduce(z, smf, add);
-    xz = wg_reduce(xz, smf, add);
-    const bool none = m == -INFINITY && z == z;  // (a NaN beside them makes the row NaN)
-    const float bad = m == INFINITY ? NAN : 0.0f;
-    const float ln = log1pf(z) + bad;
-    if (t == 0) a.entropy[r] = none ? 0.0f : ln - xz / (1.0f + z);
-    for (int i = t; i < a.T; i += kProbsThreads) {
+    s.z += s.c - 1.0f;  // one maximum left out
+    const bool none = s.m == -INFINITY && s.z == s.z;
+    const float ln = s.m == INFINITY ? NAN : log1pf(s.z);
+    if (threadIdx.x == 0) a.entropy[r] = none ? 0.0f : ln - s.xz / (1.0f + s.z);
+    auto lnp = [&](float v) { return none ? v : v - s.m - ln; };
+    for (int i = threadIdx.x; i < a.T; i += kProbsThreads) {
         const int tok = a.tokens[r * a.T + i];
-        float lp = tok < 0 ? 0.0f : NAN;
-        if (tok >= 0 && tok < a.V) lp = none ? E::get(x[tok]) : E::get(x[tok]) - m - ln;
-        a.lp[r * a.T + i] = lp;
+        a.lp[r * a.T + i] = tok < 0 ? 0.0f : (tok < a.V ? lnp(E::get(x[tok])) : NAN);
     }
-    for (int j = 0; j < a.top; ++j) {
-        if (t == 0) {
-            const int i = (int)~(unsigned)best;
-            a.ids[r * a.top + j] = i;
-            a.top_lp[r * a.top + j] = none ? E::get(x[i]) : E::get(x[i]) - m - ln;
-        }
-        unsigned long long next = 0;
-        for (int i = t; i < a.V; i += kProbsThreads) {
-            const unsigned long long k = probs_key(E::get(x[i]), i);
-            if (k < best) next = top(next, k);
-        }
-        best = wg_reduce(next, smk, top);
+    for (int i = threadIdx.x; i < a.top; i += kProbsThreads) {
+        a.ids[r * a.top + i] = key_index(list[i]);
+        a.top_lp[r * a.top + i] = lnp(key_value(list[i]));
     }
 }
 
-hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)a.M), block(kProbsThreads);
-    switch (dtype) {
-        case XT_F32: token_logprobs_kernel<XT_F32><<<grid, block, 0, s>>>(a); break;
-        case XT_F16: token_logprobs_kernel<XT_F16><<<grid, block, 0, s>>>(a); break;
-        default: token_logprobs_kernel<XT_BF16><<<grid, block, 0, s>>>(a); break;
+// The first logits of a tile and of the list before it, one maximum after
+// the other.
+__device__ void probs_one_by_one(const float* x, const int* at, int valid, int top, int* have, ProbsLds& lds) {
+    // (the list before it: a lane per entry of wave 0, taken as one more logit)
+    u64 mine = (int)threadIdx.x < *have ? lds.list[threadIdx.x] : 0, last = ~(u64)0;
+    __syncthreads();
+    const int want = min(top, *have + valid);
+    for (int j = 0; j < want; ++j) {
+        u64 best = mine < last ? mine : 0;
+        for (int i = 0; i < kProbsPer; ++i) {
+            const u64 k = at[i] >= 0 ? probs_key(x[i], at[i]) : 0;
+            if (k < last && k > best) best = k;
+        }
+        for (int o = 32; o; o >>= 1) {
+            const u64 k = __shfl_xor(best, o);
+            best = k > best ? k : best;
+        }
+        if ((threadIdx.x & 63) == 0) lds.wbest[threadIdx.x >> 6] = best;
+        __syncthreads();
+        last = lds.wbest[0];
+        for (int w = 1; w < kProbsWaves; ++w) last = max(last, lds.wbest[w]);
+        if (threadIdx.x == 0) lds.list[j] = last;
+        __syncthreads();
     }
+    *have = want;
+}
+
+// 16 logits of a thread: vectors of 16 bytes (W logits), vector v at
+// tile + (v * threads + thread) * W.
+template <int DT>
+struct ProbsTileRegs {
+    static constexpr int W = DT == XT_F32 ? 4 : 8, NV = kProbsPer / W;
+    typedef typename Elem<DT>::T T;
+    typedef T Vec __attribute__((ext_vector_type(W)));
+    typedef Vec VecU __attribute__((aligned(sizeof(T))));
+    Vec v[NV];
+    __device__ __forceinline__ void load(const T* x, int64_t base, int V) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t at = base + (int64_t)(i * kProbsThreads + (int)threadIdx.x) * W;
+            if (at + W <= V) {
+                v[i] = *reinterpret_cast<const VecU*>(x + at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < W; ++j) v[i][j] = at + j < V ? x[at + j] : (T)-INFINITY;
+            }
+        }
+    }
+};
+
+template <int DT>
+__global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsArgs a, ProbsPlan pl) {
+    typedef ProbsTileRegs<DT> R;
+    typedef typename R::T T;
+    __shared__ ProbsLds lds;
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const int64_t r = blockIdx.x / pl.slices;
+    const int slice = blockIdx.x % pl.slices;
+    const T* row = static_cast<const T*>(a.x) + r * a.ld;
+    const int t0 = slice * pl.per, t1 = min(t0 + pl.per, pl.tiles);
+    // groups of the selection: the smallest power of two that holds `top`
+    int have = 0;
+    ProbsSum s{-INFINITY, 0.0f, 0.0f, 0.0f};
+    R next;
+    next.load(row, (int64_t)t0 * kProbsTile, a.V);
+    for (int tile = t0; tile < t1; ++tile) {
+        const int base = tile * kProbsTile;  // (V <= 2^30)
+        float x[kProbsPer];
+#pragma unroll
+        for (int i = 0; i < kProbsPer; ++i) x[i] = Elem<DT>::get(next.v[i / R::W][i % R::W]);
+        if (tile + 1 < t1) next.load(row, (int64_t)(tile + 1) * kProbsTile, a.V);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kProbsPer; ++i) mx = fmaxf(mx, x[i]);
+        // maxima of 64 groups of 8 lanes
+        float gm = fmaxf(mx, lane_xor<0>(mx));
+        gm = fmaxf(gm, lane_xor<1>(gm));
+        gm = fmaxf(gm, lane_xor<2>(gm));
+        float* gmax = lds.gmax[tile & 1];
+        if ((lane & 7) == 0) gmax[t >> 3] = gm;
+        if (t == 0) lds.count = have;
+        __syncthreads();
+        gm = gmax[lane];
+        float m = gm, bound = gm;
+        m = fmaxf(m, lane_xor<0>(m));
+        m = fmaxf(m, lane_xor<1>(m));
+        m = fmaxf(m, lane_xor<2>(m));
+        m = fmaxf(m, lane_xor<3>(m));
+        m = fmaxf(m, lane_xor<4>(m));
+        m = fmaxf(m, lane_xor<5>(m));
+        const float tile_max = m;
+        m = fmaxf(m, s.m);
+        s.raise(m);
+        if (mx == m) {
+            // this thread holds a maximum (or nothing): summed apart from the rest
+            float z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kProbsPer; ++i) {
+                const float d = x[i] - m, e = __builtin_amdgcn_exp2f(d * 1.44269504f);
+                if (x[i] == m) {
+                    s.c += 1.0f;
+                } else {
+                    z += e;
+                    s.xz = fmaf(fmaxf(d, -200.0f), e, s.xz);
+                }
+            }
+            s.z += z;
+        } else {
+            float z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kProbsPer; ++i) {
+                const float d = x[i] - m, e = __builtin_amdgcn_exp2f(d * 1.44269504f);
+                z += e;
+                s.xz = fmaf(fmaxf(d, -200.0f), e, s.xz);  // (e is 0 there; -inf would give NaN)
+            }
+            s.z += z;
+        }
+        if (!a.top) continue;
+        const int valid = min(kProbsTile, a.V - base);
+        const float last = have == a.top ? key_value(lds.list[a.top - 1]) : -INFINITY;
+        const bool full = have == a.top;
+        // (uniform: nothing of the tile comes before the list's last)
+        if (full && !(tile_max > last)) {
+            if (last == last) continue;
+        }
+        // the bound: minimum over G groups' maxima
+        if (a.top <= 32) bound = fmaxf(bound, lane_xor<0>(bound));
+        else bound = fminf(bound, lane_xor<0>(bound));
+        if (a.top <= 16) bound = fmaxf(bound, lane_xor<1>(bound));
+        else bound = fminf(bound, lane_xor<1>(bound));
+        if (a.top <= 8) bound = fmaxf(bound, lane_xor<2>(bound));
+        else bound = fminf(bound, lane_xor<2>(bound));
+        if (a.top <= 4) bound = fmaxf(bound, lane_xor<3>(bound));
+        else bound = fminf(bound, lane_xor<3>(bound));
+        if (a.top <= 2) bound = fmaxf(bound, lane_xor<4>(bound));
+        else bound = fminf(bound, lane_xor<4>(bound));
+        if (a.top <= 1) bound = fmaxf(bound, lane_xor<5>(bound));
+        else bound = fminf(bound, lane_xor<5>(bound));
+        int at[kProbsPer];
+#pragma unroll
+        for (int i = 0; i < kProbsPer; ++i) {
+            at[i] = base + ((i / R::W) * kProbsThreads + t) * R::W + i % R::W;
+            if (at[i] >= a.V) at[i] = -1;
+        }
+        if (t < have) lds.cand[t] = lds.list[t];
+#pragma unroll
+        for (int i = 0; i < kProbsPer; ++i)
+            if (x[i] >= bound && x[i] > last) {
+                const int pos = atomicAdd(&lds.count, 1);
+                if (pos < kProbsCand) lds.cand[pos] = probs_key(x[i], at[i]);
+            }
+        __syncthreads();
+        const int n = lds.count;
+        if (n > kProbsCand || n < min(a.top, have + valid) || (full && last != last)) {
+            probs_one_by_one(x, at, valid, a.top, &have, lds);
+            continue;
+        }
+        for (int i = t; i < n; i += kProbsThreads) {
+            const u64 k = lds.cand[i];
+            int before = 0;
+            for (int j = 0; j < n; ++j) before += lds.cand[j] > k;
+            if (before < a.top) lds.list[before] = k;
+        }
+        have = min(a.top, n);
+        __syncthreads();
+    }
+    // the workgroup's sums
+    s.z = wave_sum_f(s.z);
+    s.xz = wave_sum_f(s.xz);
+    s.c = wave_sum_f(s.c);
+    __syncthreads();
+    if (lane == 0) {
+        lds.sums[0][wave] = s.z;
+        lds.sums[1][wave] = s.xz;
+        lds.sums[2][wave] = s.c;
+    }
+    __syncthreads();
+    s.z = s.xz = s.c = 0.0f;
+    for (int w = 0; w < kProbsWaves; ++w) {
+        s.z += lds.sums[0][w];
+        s.xz += lds.sums[1][w];
+        s.c += lds.sums[2][w];
+    }
+    if (pl.slices == 1) {
+        probs_finish<DT>(a, r, s, lds.list);
+        return;
+    }
+    if (t == 0) {
+        float* st = pl.stats + (int64_t)blockIdx.x * 4;
+        st[0] = s.m;
+        st[1] = s.z;
+        st[2] = s.xz;
+        st[3] = s.c;
+    }
+    for (int i = t; i < a.top; i += kProbsThreads)
+        pl.keys[(int64_t)blockIdx.x * a.top + i] = i < have ? lds.list[i] : 0;
+}
+
+// Joins a row's slices: the sums in slice order; of the lists, each entry
+// counts what is before it, in its own list by its place, in the others
+// (which are in order) by bisection.
+template <int DT>
+__global__ __launch_bounds__(kProbsThreads) void token_logprobs_join_kernel(ProbsArgs a, ProbsPlan pl) {
+    __shared__ u64 keys[kProbsSlices * kProbsTop];
+    __shared__ u64 list[kProbsTop];
+    const int64_t r = blockIdx.x;
+    const int n = pl.slices * a.top;
+    for (int i = threadIdx.x; i < n; i += kProbsThreads) keys[i] = pl.keys[r * n + i];
+    const float* st = pl.stats + r * pl.slices * 4;
+    const int sl = min((int)(threadIdx.x & 63), pl.slices - 1);
+    const ProbsSum mine{st[sl * 4], st[sl * 4 + 1], st[sl * 4 + 2], st[sl * 4 + 3]};
+    float m = mine.m;
+    m = fmaxf(m, lane_xor<0>(m));
+    m = fmaxf(m, lane_xor<1>(m));
+    m = fmaxf(m, lane_xor<2>(m));
+    m = fmaxf(m, lane_xor<3>(m));
+    m = fmaxf(m, lane_xor<4>(m));
+    m = fmaxf(m, lane_xor<5>(m));
+    ProbsSum s = mine;
+    s.raise(m);
+    const bool in = (int)(threadIdx.x & 63) < pl.slices;
+    s.z = wave_sum_f(in ? s.z : 0.0f);
+    s.xz = wave_sum_f(in ? s.xz : 0.0f);
+    s.c = wave_sum_f(in ? s.c : 0.0f);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kProbsThreads) {
+        const u64 k = keys[i];
+        const int own = i / a.top;
+        int before = i % a.top;
+        for (int o = 0; o < pl.slices && k && before < a.top; ++o) {
+            if (o == own) continue;
+            int lo = 0, hi = a.top;  // the first place of list o whose key is below k
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (keys[o * a.top + mid] > k) lo = mid + 1;
+                else hi = mid;
+            }
+            before += lo;
+        }
+        if (k && before < a.top) list[before] = k;
+    }
+    __syncthreads();
+    probs_finish<DT>(a, r, s, list);
+}
+
+namespace {
+
+ProbsPlan make_plan(const ProbsArgs& a, int cus) {
+    ProbsPlan pl;
+    pl.tiles = (a.V + kProbsTile - 1) / kProbsTile;
+    // slices until four workgroups per compute unit (what it holds)
+    const int64_t want = std::max<int64_t>(1, 4 * (int64_t)cus / std::max<int64_t>(a.M, 1));
+    const int slices = (int)std::min<int64_t>(std::min<int64_t>(want, kProbsSlices), pl.tiles);
+    pl.per = (pl.tiles + slices - 1) / slices;
+    pl.slices = (pl.tiles + pl.per - 1) / pl.per;
+    pl.stats = nullptr;
+    pl.keys = nullptr;
+    return pl;
+}
+
+template <int DT>
+hipError_t launch(const ProbsArgs& a, const ProbsPlan& pl, hipStream_t s) {
+    token_logprobs_kernel<DT><<<(unsigned)(a.M * pl.slices), kProbsThreads, 0, s>>>(a, pl);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || pl.slices == 1) return e;
+    token_logprobs_join_kernel<DT><<<(unsigned)a.M, kProbsThreads, 0, s>>>(a, pl);
     return hipGetLastError();
+}
+
+}  // namespace
+
+size_t token_logprobs_workspace(const ProbsArgs& a, int cus) {
+    const ProbsPlan pl = make_plan(a, cus);
+    return pl.slices == 1 ? 0 : (size_t)a.M * pl.slices * (16 + 8 * (size_t)a.top);
+}
+
+hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, hipStream_t s) {
+    ProbsPlan pl = make_plan(a, cus);
+    pl.stats = static_cast<float*>(ws);
+    pl.keys = reinterpret_cast<u64*>(pl.stats + (size_t)a.M * pl.slices * 4);
+    switch (dtype) {
+        case XT_F32: return launch<XT_F32>(a, pl, s);
+        case XT_F16: return launch<XT_F16>(a, pl, s);
+        default: return launch<XT_BF16>(a, pl, s);
+    }
 }
 
 }  // namespace xt
