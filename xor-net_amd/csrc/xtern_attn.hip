@@ -375,7 +375,7 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
 }
 
 template <int DT, int DP>
-__global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) void attention_kernel(AttnArgs a, AttnPlan pl,
+__global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 || DT != XT_F32 ? 2 : 3)) void attention_kernel(AttnArgs a, AttnPlan pl,
                                                                                    float scale2) {
     typedef AttnShape<DT, DP> S;
     typedef Elem<DT> E;
@@ -789,9 +789,9 @@ __global__ __launch_bounds__(kAttnThreads) void attention_finish_kernel(AttnArgs
 namespace {
 
 // Workgroups of attention_kernel that a compute unit holds, by registers.
-int resident(int D) { return D <= 64 ? 3 : (D <= 128 ? 2 : 1); }
+int resident(int dtype, int D) { return D > 128 ? 1 : (D > 64 || dtype != XT_F32 ? 2 : 3); }
 
-AttnPlan make_plan(const AttnArgs& a, int cus) {
+AttnPlan make_plan(int dtype, const AttnArgs& a, int cus) {
     AttnPlan pl;
     const int G = a.hq / a.c.hkv;
     pl.part_o = pl.part_ml = pl.s = nullptr;
@@ -801,7 +801,7 @@ AttnPlan make_plan(const AttnArgs& a, int cus) {
     pl.cap = (cap + 31) / 32 * 32;
     pl.per_row = a.R > kAttnPlanRows;
     const int64_t steps = a.R * std::max<int64_t>(1, (cap + kAttnStep - 1) / kAttnStep);
-    pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident(a.c.D) * cus / pl.hy));
+    pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident(dtype, a.c.D) * cus / pl.hy));
     if (pl.per_row) pl.shares = (int)a.R;
     return pl;
 }
@@ -841,13 +841,13 @@ size_t place(const AttnArgs& a, AttnPlan* pl, char* base) {
 
 }  // namespace
 
-size_t attention_workspace(const AttnArgs& a, int cus) {
-    AttnPlan pl = make_plan(a, cus);
+size_t attention_workspace(int dtype, const AttnArgs& a, int cus) {
+    AttnPlan pl = make_plan(dtype, a, cus);
     return splits(a, pl) || a.accumulate ? place(a, &pl, nullptr) : 0;
 }
 
 hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, hipStream_t s) {
-    AttnPlan pl = make_plan(a, cus);
+    AttnPlan pl = make_plan(dtype, a, cus);
     if (ws) (void)place(a, &pl, static_cast<char*>(ws));
     hipError_t e;
     switch (dtype) {

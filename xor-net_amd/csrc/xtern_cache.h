@@ -58,7 +58,7 @@ struct AttnArgs {
 };
 // Bytes of workspace that the call needs (0: none, ws is null); cus: compute
 // units of the device.
-size_t attention_workspace(const AttnArgs& a, int cus);
+size_t attention_workspace(int dtype, const AttnArgs& a, int cus);
 hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, hipStream_t s);
 
 struct EvictArgs {

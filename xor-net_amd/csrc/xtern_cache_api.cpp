@@ -198,7 +198,7 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
     void* ws = nullptr;
-    if (const size_t bytes = xt::attention_workspace(a, cus)) {
+    if (const size_t bytes = xt::attention_workspace(c->dtype, a, cus)) {
         if (int rc = xt_internal_workspace(static_cast<hipStream_t>(stream), bytes, &ws, 3)) return rc;
     }
     return launched(xt::launch_paged_attention(c->dtype, a, cus, ws, static_cast<hipStream_t>(stream)),

@@ -15,11 +15,12 @@
 // row is cut into slices only as far as there are too few rows for the chip
 // (then a second kernel joins them).
 //
-// Selection of the `top` largest: the minimum of G >= top disjoint groups'
-// maxima is a lower bound of the top-th largest logit, and of n logits only
-// about G ln G reach it (G = 32: 111 of 8192).  Those go to LDS, each counts
-// how many are before it, and the first `top` in that order are the list that
-// the next tile's candidates have to beat.  Where that fails (ties beyond the
+// Selection of the `top` largest: a wave's q-th largest lane maximum, q = top /
+// 8, is reached by at least q of its logits, so the minimum of that over the
+// eight waves is by `top` of the tile's, and by hardly more than twice as many.
+// Those go to LDS, each counts how many are before it, and the first `top` in
+// that order are the list that the next tile's candidates have to beat.  Where
+// that fails (ties beyond the
 // buffer, fewer finite logits than `top`) the tile's logits are taken one
 // maximum after the other.
 #include <algorithm>
@@ -46,6 +47,27 @@ struct ProbsPlan {
     u64* keys;     // [M][slices][top]
 };
 
+// The first `top` of keys[0 .. n) in descending order, to list[0 .. min(top,
+// n)): each counts how many are larger, four threads a key.  Zeros follow the
+// keys up to a multiple of 32.
+__device__ __forceinline__ void probs_rank(const u64* keys, int n, int top, u64* list) {
+    const int part = threadIdx.x & 3;
+    for (int i = threadIdx.x >> 2; i < n; i += kProbsThreads / 4) {
+        const u64 k = keys[i];
+        int before = 0;
+        for (int j = part; j < n; j += 32) {
+            u64 o[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) o[u] = keys[j + 4 * u];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) before += o[u] > k;
+        }
+        before += __builtin_amdgcn_mov_dpp(before, 0xb1, 0xf, 0xf, true);  // (the four lanes of a quad)
+        before += __builtin_amdgcn_mov_dpp(before, 0x4e, 0xf, 0xf, true);
+        if (part == 0 && before < top) list[before] = k;
+    }
+}
+
 // Order of the alternatives: larger value first, then the lower index; NaN
 // behind everything, no element (0) behind that.
 __device__ __forceinline__ u64 probs_key(float x, int i) {
@@ -60,31 +82,25 @@ __device__ __forceinline__ float key_value(u64 k) {
 }
 __device__ __forceinline__ int key_index(u64 k) { return (int)~(unsigned)k; }
 
-// Over the lanes that differ in bit `1 << s` of their number.
-template <int S>
-__device__ __forceinline__ float lane_xor(float v) {
-    if constexpr (S == 4) {
-        auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
-    } else if constexpr (S == 5) {
-        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-    } else if constexpr (S == 0) {
-        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xb1, 0xf, 0xf, true));  // quad_perm 1,0,3,2
-    } else if constexpr (S == 1) {
-        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4e, 0xf, 0xf, true));  // quad_perm 2,3,0,1
-    } else {
-        return __shfl_xor(v, 1 << S);
-    }
+// Reductions over the wave, the result in every lane: within 16 lanes by DPP
+// (quads, halves of a row, rows: each step meets lanes that hold the same
+// value already), then by lane swaps.
+template <typename Op>
+__device__ __forceinline__ float wave_all(float v, Op op) {
+    v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xb1, 0xf, 0xf, true)));   // quad_perm 1,0,3,2
+    v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4e, 0xf, 0xf, true)));   // quad_perm 2,3,0,1
+    v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xf, 0xf, true)));  // row_half_mirror
+    v = op(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xf, 0xf, true)));  // row_mirror
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float wave_max_f(float v) {
+    return wave_all(v, [](float p, float q) { return fmaxf(p, q); });
 }
 __device__ __forceinline__ float wave_sum_f(float v) {
-    v += lane_xor<0>(v);
-    v += lane_xor<1>(v);
-    v += lane_xor<2>(v);
-    v += lane_xor<3>(v);
-    v += lane_xor<4>(v);
-    v += lane_xor<5>(v);
-    return v;
+    return wave_all(v, [](float p, float q) { return p + q; });
 }
 
 // Sums relative to m, of which `c` logits are m itself; to a larger maximum.
@@ -106,7 +122,7 @@ struct ProbsSum {
 };
 
 struct ProbsLds {
-    float gmax[2][64];
+    float wmax[2][kProbsWaves], wbound[2][kProbsWaves];
     float sums[3][kProbsWaves];
     u64 cand[kProbsCand];
     u64 list[kProbsTop];
@@ -136,15 +152,17 @@ __device__ void probs_finish(const ProbsArgs& a, int64_t r, ProbsSum s, const u6
 
 // The first logits of a tile and of the list before it, one maximum after
 // the other.
-__device__ void probs_one_by_one(const float* x, const int* at, int valid, int top, int* have, ProbsLds& lds) {
+template <typename Index>
+__device__ void probs_one_by_one(const float* x, Index index, int V, int valid, int top, int* have, ProbsLds& lds) {
     // (the list before it: a lane per entry of wave 0, taken as one more logit)
     u64 mine = (int)threadIdx.x < *have ? lds.list[threadIdx.x] : 0, last = ~(u64)0;
     __syncthreads();
     const int want = min(top, *have + valid);
     for (int j = 0; j < want; ++j) {
         u64 best = mine < last ? mine : 0;
+#pragma unroll
         for (int i = 0; i < kProbsPer; ++i) {
-            const u64 k = at[i] >= 0 ? probs_key(x[i], at[i]) : 0;
+            const u64 k = index(i) < V ? probs_key(x[i], index(i)) : 0;
             if (k < last && k > best) best = k;
         }
         for (int o = 32; o; o >>= 1) {
@@ -195,7 +213,8 @@ __global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsA
     const T* row = static_cast<const T*>(a.x) + r * a.ld;
     const int t0 = slice * pl.per, t1 = min(t0 + pl.per, pl.tiles);
     // groups of the selection: the smallest power of two that holds `top`
-    int have = 0;
+    int have = 0, dirty = kProbsCand;
+    const int quota = (a.top + kProbsWaves - 1) / kProbsWaves;
     ProbsSum s{-INFINITY, 0.0f, 0.0f, 0.0f};
     R next;
     next.load(row, (int64_t)t0 * kProbsTile, a.V);
@@ -208,22 +227,36 @@ __global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsA
         float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kProbsPer; ++i) mx = fmaxf(mx, x[i]);
-        // maxima of 64 groups of 8 lanes
-        float gm = fmaxf(mx, lane_xor<0>(mx));
-        gm = fmaxf(gm, lane_xor<1>(gm));
-        gm = fmaxf(gm, lane_xor<2>(gm));
-        float* gmax = lds.gmax[tile & 1];
-        if ((lane & 7) == 0) gmax[t >> 3] = gm;
+        // the wave's `quota`-th largest of its lanes' maxima
+        const float wm = wave_max_f(mx);
+        float wb = wm, rest = mx;
+        // (a full list's last; a wave without anything above it has no say in
+        // the bound, and then there is none)
+        const bool full = have == a.top;
+        const float last = full && a.top ? key_value(lds.list[a.top - 1]) : -INFINITY;
+        if (full && !(wm > last)) {
+            wb = -INFINITY;
+        } else {
+            for (int i = 1; i < quota; ++i) {
+                const u64 holds = __ballot(rest == wb);
+                if (holds && lane == __builtin_ctzll(holds)) rest = -INFINITY;
+                wb = wave_max_f(rest);
+            }
+        }
+        if (lane == 0) {
+            lds.wmax[tile & 1][wave] = wm;
+            lds.wbound[tile & 1][wave] = wb;
+        }
+        for (int i = t; i < dirty; i += kProbsThreads) lds.cand[i] = 0;
+        dirty = 0;
         if (t == 0) lds.count = have;
         __syncthreads();
-        gm = gmax[lane];
-        float m = gm, bound = gm;
-        m = fmaxf(m, lane_xor<0>(m));
-        m = fmaxf(m, lane_xor<1>(m));
-        m = fmaxf(m, lane_xor<2>(m));
-        m = fmaxf(m, lane_xor<3>(m));
-        m = fmaxf(m, lane_xor<4>(m));
-        m = fmaxf(m, lane_xor<5>(m));
+        float m = lds.wmax[tile & 1][0], bound = lds.wbound[tile & 1][0];
+#pragma unroll
+        for (int w = 1; w < kProbsWaves; ++w) {
+            m = fmaxf(m, lds.wmax[tile & 1][w]);
+            bound = fminf(bound, lds.wbound[tile & 1][w]);
+        }
         const float tile_max = m;
         m = fmaxf(m, s.m);
         s.raise(m);
@@ -253,50 +286,33 @@ __global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsA
         }
         if (!a.top) continue;
         const int valid = min(kProbsTile, a.V - base);
-        const float last = have == a.top ? key_value(lds.list[a.top - 1]) : -INFINITY;
-        const bool full = have == a.top;
         // (uniform: nothing of the tile comes before the list's last)
         if (full && !(tile_max > last)) {
             if (last == last) continue;
         }
-        // the bound: minimum over G groups' maxima
-        if (a.top <= 32) bound = fmaxf(bound, lane_xor<0>(bound));
-        else bound = fminf(bound, lane_xor<0>(bound));
-        if (a.top <= 16) bound = fmaxf(bound, lane_xor<1>(bound));
-        else bound = fminf(bound, lane_xor<1>(bound));
-        if (a.top <= 8) bound = fmaxf(bound, lane_xor<2>(bound));
-        else bound = fminf(bound, lane_xor<2>(bound));
-        if (a.top <= 4) bound = fmaxf(bound, lane_xor<3>(bound));
-        else bound = fminf(bound, lane_xor<3>(bound));
-        if (a.top <= 2) bound = fmaxf(bound, lane_xor<4>(bound));
-        else bound = fminf(bound, lane_xor<4>(bound));
-        if (a.top <= 1) bound = fmaxf(bound, lane_xor<5>(bound));
-        else bound = fminf(bound, lane_xor<5>(bound));
-        int at[kProbsPer];
-#pragma unroll
-        for (int i = 0; i < kProbsPer; ++i) {
-            at[i] = base + ((i / R::W) * kProbsThreads + t) * R::W + i % R::W;
-            if (at[i] >= a.V) at[i] = -1;
-        }
         if (t < have) lds.cand[t] = lds.list[t];
+        const int at = base + t * R::W;  // of x[0]
+        auto index = [&](int i) { return at + (i / R::W) * kProbsThreads * R::W + i % R::W; };
+        if (mx >= bound && mx > last) {
+            int hits = 0;
 #pragma unroll
-        for (int i = 0; i < kProbsPer; ++i)
-            if (x[i] >= bound && x[i] > last) {
-                const int pos = atomicAdd(&lds.count, 1);
-                if (pos < kProbsCand) lds.cand[pos] = probs_key(x[i], at[i]);
-            }
+            for (int i = 0; i < kProbsPer; ++i) hits += x[i] >= bound && x[i] > last;
+            int pos = atomicAdd(&lds.count, hits);
+#pragma unroll
+            for (int i = 0; i < kProbsPer; ++i)
+                if (x[i] >= bound && x[i] > last) {
+                    if (pos < kProbsCand) lds.cand[pos] = probs_key(x[i], index(i));
+                    ++pos;
+                }
+        }
         __syncthreads();
         const int n = lds.count;
+        dirty = min(n, kProbsCand);
         if (n > kProbsCand || n < min(a.top, have + valid) || (full && last != last)) {
-            probs_one_by_one(x, at, valid, a.top, &have, lds);
+            probs_one_by_one(x, index, a.V, valid, a.top, &have, lds);
             continue;
         }
-        for (int i = t; i < n; i += kProbsThreads) {
-            const u64 k = lds.cand[i];
-            int before = 0;
-            for (int j = 0; j < n; ++j) before += lds.cand[j] > k;
-            if (before < a.top) lds.list[before] = k;
-        }
+        probs_rank(lds.cand, n, a.top, lds.list);
         have = min(a.top, n);
         __syncthreads();
     }
@@ -332,49 +348,46 @@ __global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsA
         pl.keys[(int64_t)blockIdx.x * a.top + i] = i < have ? lds.list[i] : 0;
 }
 
-// Joins a row's slices: the sums in slice order; of the lists, each entry
-// counts what is before it, in its own list by its place, in the others
-// (which are in order) by bisection.
+// Joins a row's slices: the sums, and of the lists (each in descending order)
+// the first `top`.  With q = ceil(top / slices), the slices' q-th entries have
+// a minimum that at least `top` entries reach: only those are ranked.
 template <int DT>
 __global__ __launch_bounds__(kProbsThreads) void token_logprobs_join_kernel(ProbsArgs a, ProbsPlan pl) {
     __shared__ u64 keys[kProbsSlices * kProbsTop];
     __shared__ u64 list[kProbsTop];
+    __shared__ int count;
     const int64_t r = blockIdx.x;
     const int n = pl.slices * a.top;
-    for (int i = threadIdx.x; i < n; i += kProbsThreads) keys[i] = pl.keys[r * n + i];
+    if (threadIdx.x == 0) count = 0;
+    u64 mine_k[kProbsSlices * kProbsTop / kProbsThreads];
+#pragma unroll
+    for (int i = 0; i < kProbsSlices * kProbsTop / kProbsThreads; ++i) {
+        const int at = i * kProbsThreads + threadIdx.x;
+        mine_k[i] = at < n ? pl.keys[r * n + at] : 0;
+    }
+    u64 bound = 0;
+    if (a.top) {
+        const int q = (a.top + pl.slices - 1) / pl.slices;
+        bound = pl.keys[r * n + (int64_t)min((int)(threadIdx.x & 63), pl.slices - 1) * a.top + q - 1];
+        for (int o = 32; o; o >>= 1) bound = min(bound, __shfl_xor(bound, o));
+    }
     const float* st = pl.stats + r * pl.slices * 4;
     const int sl = min((int)(threadIdx.x & 63), pl.slices - 1);
-    const ProbsSum mine{st[sl * 4], st[sl * 4 + 1], st[sl * 4 + 2], st[sl * 4 + 3]};
-    float m = mine.m;
-    m = fmaxf(m, lane_xor<0>(m));
-    m = fmaxf(m, lane_xor<1>(m));
-    m = fmaxf(m, lane_xor<2>(m));
-    m = fmaxf(m, lane_xor<3>(m));
-    m = fmaxf(m, lane_xor<4>(m));
-    m = fmaxf(m, lane_xor<5>(m));
-    ProbsSum s = mine;
+    const ProbsSum part{st[sl * 4], st[sl * 4 + 1], st[sl * 4 + 2], st[sl * 4 + 3]};
+    const float m = wave_max_f(part.m);
+    ProbsSum s = part;
     s.raise(m);
     const bool in = (int)(threadIdx.x & 63) < pl.slices;
     s.z = wave_sum_f(in ? s.z : 0.0f);
     s.xz = wave_sum_f(in ? s.xz : 0.0f);
     s.c = wave_sum_f(in ? s.c : 0.0f);
+    for (int i = threadIdx.x; i < (n + 31) / 32 * 32; i += kProbsThreads) keys[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kProbsThreads) {
-        const u64 k = keys[i];
-        const int own = i / a.top;
-        int before = i % a.top;
-        for (int o = 0; o < pl.slices && k && before < a.top; ++o) {
-            if (o == own) continue;
-            int lo = 0, hi = a.top;  // the first place of list o whose key is below k
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (keys[o * a.top + mid] > k) lo = mid + 1;
-                else hi = mid;
-            }
-            before += lo;
-        }
-        if (k && before < a.top) list[before] = k;
-    }
+#pragma unroll
+    for (int i = 0; i < kProbsSlices * kProbsTop / kProbsThreads; ++i)
+        if (mine_k[i] && mine_k[i] >= bound) keys[atomicAdd(&count, 1)] = mine_k[i];
+    __syncthreads();
+    probs_rank(keys, count, a.top, list);
     __syncthreads();
     probs_finish<DT>(a, r, s, list);
 }
