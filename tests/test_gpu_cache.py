@@ -356,7 +356,7 @@ def test_evict_rules(page, rule):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_evict_long(dtype):
-    for n, budget in ((5000, 1), (5000, 4999), (9000, 2500)):
+    for n, budget in ((5000, 1), (5000, 4999), (9000, 2500), (20011, 7000), (16384 + 4, 16380), (16385 + 4, 16000)):
         log(f"evict {dtype} {n} {budget}")
         evict_case(dtype, 1, 64, 32, [n], budget, min(4, budget), 0)
 

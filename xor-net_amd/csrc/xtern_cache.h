@@ -68,7 +68,7 @@ struct EvictArgs {
     int32_t* kept;           // [nseq][hkv][budget]
     int budget, sink, recent;
 };
-hipError_t launch_kv_evict(int dtype, const EvictArgs& a, hipStream_t s);
+hipError_t launch_kv_evict(int dtype, const EvictArgs& a, int cus, hipStream_t s);
 
 struct ProbsArgs {
     const void* x;  // [M] rows of V logits, stride ld

@@ -6,11 +6,22 @@
 // position; NaN below every number, a position without a page below that).
 // They move, in order, to positions 0 .. budget - 1.
 //
-// One workgroup per (sequence, head).  Selection: the need-th highest 32-bit
-// key by four passes of an 8-bit histogram, then one pass in position order
-// that writes the kept list.  Moving in place: the kept list is ascending, so
-// kept[j] >= j, and a chunk of targets j0 .. j1 - 1 never holds a source of a
-// later chunk; inside a chunk every load comes before the first store.
+// Two kernels.  Selection, one workgroup per (sequence, head): the scores as
+// 32-bit keys, the need-th highest by four passes of an 8-bit histogram, then
+// the kept list in position order.  Up to 16384 positions the keys stay in
+// registers, so the scores are read once; more are read again for each pass.
+// Moving: HBM bounds it (every kept row is read and written once); a
+// workgroup per (sequence, head, tensor), and per part of a row where those
+// are too few for the chip.
+//
+// Why rows can move in place: the kept list ascends, so kept[j] >= j.  A
+// workgroup moves its part of the rows in rounds of ascending j.  A source of
+// a later round is never the target of an earlier one (it is no lower than
+// its own j, which is above every earlier j), so a round needs no earlier
+// store to be done; and a target is a source only of its own or an earlier
+// round, so the barrier between a round's loads and its stores is enough.
+#include <algorithm>
+
 #include "xtern_cache.h"
 #include "xtern_device.h"
 
@@ -18,6 +29,8 @@ namespace xt {
 
 constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
+constexpr int kEvictRegs = 16;  // keys of a thread that stay in registers
+constexpr int kMoveUnits = 4;   // 16-byte pieces of a thread and round
 
 __device__ __forceinline__ unsigned evict_key(const KvView& c, int seq, int h, int p) {
     const int pg = kv_page(c, seq, p);
@@ -28,37 +41,36 @@ __device__ __forceinline__ unsigned evict_key(const KvView& c, int seq, int h, i
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// Copies rows of `units` T from position kept[j] to j for the j whose
-// position changes.
-template <typename T>
-__device__ void move_rows(const KvView& c, int seq, int h, T* base, int64_t sp, int64_t ss, int64_t sh,
-                          int units, const int32_t* kept, int j0, int budget) {
-    const int64_t total = (int64_t)(budget - j0) * units;
-    for (int64_t i0 = 0; i0 < total; i0 += kEvictThreads) {
-        const int64_t i = i0 + threadIdx.x;
-        T val{};
-        int64_t to = -1;
-        if (i < total) {
-            const int j = j0 + (int)(i / units), u = (int)(i % units), src = kept[j];
-            const int pf = kv_page(c, seq, src), pt = kv_page(c, seq, j);
-            if (src != j && pf >= 0 && pt >= 0) {
-                val = base[pf * sp + (src % c.page) * ss + h * sh + u];
-                to = pt * sp + (j % c.page) * ss + h * sh + u;
-            }
-        }
-        __syncthreads();
-        if (to >= 0) base[to] = val;
-        __syncthreads();
-    }
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int evict_scan(int v) {
+    v += dpp_id<0x111, 0xf>(v);
+    v += dpp_id<0x112, 0xf>(v);
+    v += dpp_id<0x114, 0xf>(v);
+    v += dpp_id<0x118, 0xf>(v);
+    v += dpp_id<0x142, 0xa>(v);
+    v += dpp_id<0x143, 0xc>(v);
+    return v;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kEvictThreads) void kv_evict_kernel(EvictArgs a, int per_unit) {
+// Of a 256-bin histogram, by every wave for itself: the highest bin b such
+// that bins b .. 255 hold at least `need`; *left = what b has to give.
+__device__ __forceinline__ int evict_bin(const int* hist, int need, int* left) {
+    const int lane = threadIdx.x & 63;
+    int c[4], sum = 0;  // lane l: bins 255 - 4 l downwards
+    for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - 4 * lane - i];
+    const int upto = evict_scan(sum);
+    const int l = __builtin_ctzll(__ballot(upto >= need));
+    int before = upto - sum, i = 0;
+    while (i < 3 && before + c[i] < need) before += c[i++];
+    *left = __builtin_amdgcn_readlane(need - before, l);
+    return __builtin_amdgcn_readlane(255 - 4 * lane - i, l);
+}
+
+__global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArgs a) {
     const KvView& c = a.c;
     const int seq = blockIdx.x, h = blockIdx.y, t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    __shared__ int hist[256];
-    __shared__ int wcount[2][kEvictWaves];
-    __shared__ int pick[2];
+    __shared__ int hist[4][256];
+    __shared__ int count[2][kEvictRegs * kEvictWaves];  // above and equal, by chunk of 64 positions
     const int n = kv_length(c, a.lengths[seq]);
     int32_t* kept = a.kept + ((int64_t)seq * c.hkv + h) * a.budget;
     if (h == 0 && t == 0) a.new_lengths[seq] = min(n, a.budget);
@@ -66,89 +78,206 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_kernel(EvictArgs a, in
         for (int j = t; j < a.budget; j += kEvictThreads) kept[j] = j < n ? j : -1;
         return;
     }
-    const int lo = a.sink, hi = n - a.recent;  // the positions between
+    const int lo = a.sink, hi = n - a.recent, mid = hi - lo;  // the positions between
     int need = a.budget - a.sink - a.recent;
-    unsigned prefix = 0;
-    if (need > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (t < 256) hist[t] = 0;
-            __syncthreads();
-            const unsigned mask = shift == 24 ? 0u : ~0u << (shift + 8);
-            for (int p = lo + t; p < hi; p += kEvictThreads) {
-                const unsigned k = evict_key(c, seq, h, p);
-                if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
-            }
-            __syncthreads();
-            if (t == 0) {
-                int left = need, b = 255;
-                while (hist[b] < left) left -= hist[b--];
-                pick[0] = b;
-                pick[1] = left;
-            }
-            __syncthreads();
-            prefix |= (unsigned)pick[0] << shift;
-            need = pick[1];  // of the keys equal to the prefix so far, as many stay
-        }
-    }
-    // kept: keys above `prefix`, and the first `need` equal to it
-    const bool any = a.budget > a.sink + a.recent;
-    const int per = ((hi - lo + kEvictWaves - 1) / kEvictWaves + 63) / 64 * 64;
-    const int w0 = lo + wave * per, w1 = min(w0 + per, hi);
-    int above = 0, equal = 0;
-    if (any)
-        for (int p = w0; p < w1; p += 64) {
-            const unsigned k = p + lane < w1 ? evict_key(c, seq, h, p + lane) : 0u;
-            above += __popcll(__ballot(p + lane < w1 && k > prefix));
-            equal += __popcll(__ballot(p + lane < w1 && k == prefix));
-        }
-    if (lane == 0) {
-        wcount[0][wave] = above;
-        wcount[1][wave] = equal;
-    }
     for (int j = t; j < a.sink; j += kEvictThreads) kept[j] = j;
     for (int j = t; j < a.recent; j += kEvictThreads) kept[a.budget - a.recent + j] = hi + j;
+    if (need == 0) return;
+    const bool regs = mid <= kEvictRegs * kEvictThreads;
+    unsigned key[kEvictRegs];  // position lo + 1024 i + t
+#pragma unroll
+    for (int i = 0; i < kEvictRegs; ++i) {
+        const int p = lo + i * kEvictThreads + t;
+        key[i] = regs && p < hi ? evict_key(c, seq, h, p) : 0u;
+    }
+    if (t < 256)
+        for (int i = 0; i < 4; ++i) hist[i][t] = 0;
     __syncthreads();
-    if (any) {
-        int eq = 0, at = a.sink;
-        for (int w = 0; w < wave; ++w) {
-            const int e = min(wcount[1][w], max(0, need - eq));
-            eq += wcount[1][w];
-            at += wcount[0][w] + e;
+    unsigned prefix = 0;
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        const unsigned mask = pass ? ~0u << (shift + 8) : 0u;
+        if (regs) {
+#pragma unroll
+            for (int i = 0; i < kEvictRegs; ++i)
+                if (lo + i * kEvictThreads + t < hi && (key[i] & mask) == prefix)
+                    atomicAdd(&hist[pass][(key[i] >> shift) & 255], 1);
+        } else {
+            for (int p = lo + t; p < hi; p += 4 * kEvictThreads) {
+                unsigned k[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) k[i] = evict_key(c, seq, h, min(p + i * kEvictThreads, hi - 1));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (p + i * kEvictThreads < hi && (k[i] & mask) == prefix)
+                        atomicAdd(&hist[pass][(k[i] >> shift) & 255], 1);
+            }
         }
-        const unsigned long long below = (1ull << lane) - 1;
-        for (int p = w0; p < w1; p += 64) {
-            const bool in = p + lane < w1;
-            const unsigned k = in ? evict_key(c, seq, h, p + lane) : 0u;
-            const unsigned long long me = __ballot(in && k == prefix);
-            const bool take = in && (k > prefix || (k == prefix && eq + __popcll(me & below) < need));
+        __syncthreads();
+        int left;
+        prefix |= (unsigned)evict_bin(hist[pass], need, &left) << shift;
+        need = left;  // of the keys equal to the prefix so far, as many stay
+    }
+    // kept: keys above `prefix`, and the first `need` equal to it
+    const unsigned long long below = (1ull << lane) - 1;
+    const int at0 = a.sink;
+    if (regs) {
+#pragma unroll
+        for (int i = 0; i < kEvictRegs; ++i) {
+            const bool in = lo + i * kEvictThreads + t < hi;
+            const int above = __popcll(__ballot(in && key[i] > prefix));
+            const int equal = __popcll(__ballot(in && key[i] == prefix));
+            if (lane == 0) {
+                count[0][i * kEvictWaves + wave] = above;
+                count[1][i * kEvictWaves + wave] = equal;
+            }
+        }
+        __syncthreads();
+        // sums before each chunk: wave 0 the ones above, wave 1 the equal ones
+        if (wave < 2) {
+            int* cnt = count[wave] + 4 * lane;
+            int v[4], sum = 0;
+            for (int i = 0; i < 4; ++i) sum += v[i] = cnt[i];
+            int before = evict_scan(sum) - sum;
+            for (int i = 0; i < 4; ++i) {
+                cnt[i] = before;
+                before += v[i];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEvictRegs; ++i) {
+            const int p = lo + i * kEvictThreads + t;
+            const int eq = count[1][i * kEvictWaves + wave];
+            const unsigned long long me = __ballot(p < hi && key[i] == prefix);
+            const bool take = p < hi && (key[i] > prefix || (key[i] == prefix && eq + __popcll(me & below) < need));
             const unsigned long long mt = __ballot(take);
-            if (take) kept[at + __popcll(mt & below)] = p + lane;
+            if (take) kept[at0 + count[0][i * kEvictWaves + wave] + min(eq, need) + __popcll(mt & below)] = p;
+        }
+        return;
+    }
+    // a stretch of positions per wave, counted and then written
+    const int per = ((mid + kEvictWaves - 1) / kEvictWaves + 63) / 64 * 64;
+    const int w0 = (int)min((int64_t)lo + (int64_t)wave * per, (int64_t)hi), w1 = min(w0 + per, hi);
+    int above = 0, equal = 0;
+    for (int p = w0; p < w1; p += 256) {
+        unsigned k[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = evict_key(c, seq, h, min(p + 64 * i + lane, hi - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = p + 64 * i + lane < w1;
+            above += __popcll(__ballot(in && k[i] > prefix));
+            equal += __popcll(__ballot(in && k[i] == prefix));
+        }
+    }
+    if (lane == 0) {
+        count[0][wave] = above;
+        count[1][wave] = equal;
+    }
+    __syncthreads();
+    int eq = 0, at = at0;
+    for (int w = 0; w < wave; ++w) {
+        at += count[0][w] + min(count[1][w], max(0, need - eq));
+        eq += count[1][w];
+    }
+    for (int p = w0; p < w1; p += 256) {
+        unsigned k[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = evict_key(c, seq, h, min(p + 64 * i + lane, hi - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = p + 64 * i + lane;
+            const unsigned long long me = __ballot(q < w1 && k[i] == prefix);
+            const bool take = q < w1 && (k[i] > prefix || (k[i] == prefix && eq + __popcll(me & below) < need));
+            const unsigned long long mt = __ballot(take);
+            if (take) kept[at + __popcll(mt & below)] = q;
             eq += __popcll(me);
             at += __popcll(mt);
         }
     }
-    __syncthreads();
-    const int units = c.D / per_unit;
-    move_rows<T>(c, seq, h, static_cast<T*>(c.k), c.sp / per_unit, c.ss / per_unit, c.sh / per_unit, units, kept,
-                 a.sink, a.budget);
-    move_rows<T>(c, seq, h, static_cast<T*>(c.v), c.sp / per_unit, c.ss / per_unit, c.sh / per_unit, units, kept,
-                 a.sink, a.budget);
-    move_rows<float>(c, seq, h, c.score, (int64_t)c.hkv * c.page, 1, c.page, 1, kept, a.sink, a.budget);
 }
 
-hipError_t launch_kv_evict(int dtype, const EvictArgs& a, hipStream_t s) {
+// Rows of `bytes` bytes in pieces of T (16 bytes; rows start anywhere, the last
+// piece may overlap the one before it), pieces [u0, u1) of each; or the scores.
+template <typename T>
+__device__ __forceinline__ void move_rows(const KvView& c, int seq, char* base, int64_t sp, int64_t ss, int bytes,
+                                          int u0, int u1, const int32_t* kept, int j0, int budget) {
+    const int un = u1 - u0;
+    const int64_t total = (int64_t)(budget - j0) * un;
+    typedef T U __attribute__((aligned(2)));
+    constexpr int kRound = kEvictThreads * kMoveUnits;
+    const char* from[kMoveUnits];
+    char* to[kMoveUnits];
+    auto place = [&](int64_t i0) {
+#pragma unroll
+        for (int x = 0; x < kMoveUnits; ++x) {
+            const int64_t i = i0 + x * kEvictThreads + threadIdx.x;
+            to[x] = nullptr;
+            from[x] = base;  // (read and left, where nothing moves)
+            if (i < total) {
+                const int j = j0 + (int)(i / un), src = kept[j];
+                const int off = min((u0 + (int)(i % un)) * (int)sizeof(T), bytes - (int)sizeof(T));
+                const int pf = kv_page(c, seq, src), pt = kv_page(c, seq, j);
+                if (src != j && pf >= 0 && pt >= 0) {
+                    from[x] = base + pf * sp + (src % c.page) * ss + off;
+                    to[x] = base + pt * sp + (j % c.page) * ss + off;
+                }
+            }
+        }
+    };
+    place(0);
+    for (int64_t i0 = 0; i0 < total; i0 += kRound) {
+        T val[kMoveUnits];
+        char* dst[kMoveUnits];
+#pragma unroll
+        for (int x = 0; x < kMoveUnits; ++x) {
+            dst[x] = to[x];
+            val[x] = *reinterpret_cast<const U*>(from[x]);
+        }
+        if (i0 + kRound < total) place(i0 + kRound);  // (addresses: while the rows are on their way)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every load of the round is done
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < kMoveUnits; ++x)
+            if (dst[x]) *reinterpret_cast<U*>(dst[x]) = val[x];
+    }
+}
+
+// blockIdx.y: key-value head; blockIdx.z: the parts of k's rows, of v's, the
+// scores.
+template <typename T>
+__global__ __launch_bounds__(kEvictThreads) void kv_evict_move_kernel(EvictArgs a, int es, int parts) {
+    const KvView& c = a.c;
+    const int seq = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
+    if (kv_length(c, a.lengths[seq]) <= a.budget) return;
+    const int32_t* kept = a.kept + ((int64_t)seq * c.hkv + h) * a.budget;
+    if (z == 2 * parts) {
+        move_rows<float>(c, seq, reinterpret_cast<char*>(c.score + (int64_t)h * c.page), (int64_t)c.hkv * c.page * 4, 4, 4,
+                         0, 1, kept, a.sink, a.budget);
+        return;
+    }
+    const int bytes = c.D * es, units = (bytes + (int)sizeof(T) - 1) / (int)sizeof(T), part = z % parts;
+    char* base = static_cast<char*>(z < parts ? c.k : c.v) + c.sh * h * es;
+    move_rows<T>(c, seq, base, c.sp * es, c.ss * es, bytes, units * part / parts, units * (part + 1) / parts, kept,
+                 a.sink, a.budget);
+}
+
+hipError_t launch_kv_evict(int dtype, const EvictArgs& a, int cus, hipStream_t s) {
     const KvView& c = a.c;
     const int es = dtype == XT_F32 ? 4 : 2;
-    // the widest unit that every row starts and ends on
-    const uint64_t bits = (uint64_t)reinterpret_cast<uintptr_t>(c.k) | (uint64_t)reinterpret_cast<uintptr_t>(c.v) |
-                          (uint64_t)(c.sp * es) | (uint64_t)(c.ss * es) | (uint64_t)(c.sh * es) | (uint64_t)(c.D * es);
-    const dim3 grid((unsigned)c.nseq, (unsigned)c.hkv), block(kEvictThreads);
-    if (!(bits & 15))
-        kv_evict_kernel<v4i><<<grid, block, 0, s>>>(a, 16 / es);
-    else if (!(bits & 3))
-        kv_evict_kernel<int><<<grid, block, 0, s>>>(a, 4 / es);
+    kv_evict_select_kernel<<<dim3((unsigned)c.nseq, (unsigned)c.hkv), kEvictThreads, 0, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.sink == a.budget) return e;
+    // Parts of a row until two workgroups per compute unit, of four pieces at least
+    const int bytes = c.D * es, units = (bytes + 15) / 16;
+    const int64_t rows = (int64_t)c.nseq * c.hkv * 2;
+    const int parts = bytes < 16 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(units / 4, 2 * (int64_t)cus / rows));
+    const dim3 grid((unsigned)c.nseq, (unsigned)c.hkv, (unsigned)(2 * parts + 1));
+    if (bytes >= 16)
+        kv_evict_move_kernel<v4i><<<grid, kEvictThreads, 0, s>>>(a, es, parts);
     else
-        kv_evict_kernel<short><<<grid, block, 0, s>>>(a, 1);
+        kv_evict_move_kernel<short><<<grid, kEvictThreads, 0, s>>>(a, es, parts);
     return hipGetLastError();
 }
 
