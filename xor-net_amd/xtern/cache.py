@@ -5,12 +5,9 @@ Tensors are on the current device; a call runs on torch's current stream or
 on `stream`.  With a `stream` of its own, results are allocated on that
 stream and the inputs are marked as used there.
 """
-import contextlib
 import ctypes
-import math
 
-from . import (XT_ERR_INVALID, XternError, _check, _cur_device, _i64, _lib, _raw_stream, _stream_ptr,
-               _torch, _vp)
+from . import XT_ERR_INVALID, XternError, _check, _cur_device, _i64, _lib, _stream_ptr, _torch, _torch_mod, _vp
 
 XT_F32, XT_F16, XT_BF16 = 0, 1, 2
 
@@ -46,65 +43,93 @@ def _invalid(msg):
     return XternError(XT_ERR_INVALID, msg)
 
 
-def _dtypes():
+def _torch_types():
     torch = _torch()
-    return {torch.float32: XT_F32, torch.float16: XT_F16, torch.bfloat16: XT_BF16}
+    return torch.int32, torch.float32, {torch.float32: XT_F32, torch.float16: XT_F16, torch.bfloat16: XT_BF16}
 
 
-def _ptr(t, dtype, what, shape=None):
-    """Address of a tensor of this type (and shape) on the current device."""
+_I32, _F32, _DTYPES = _torch_types() if _torch_mod is not None else (None, None, {})
+
+
+# The checks of one call's tensors cost as much as a small kernel: each makes
+# its sure case in few attribute reads and leaves the message to _refuse.
+
+def _here():
+    """The current device's index; -2 (no tensor's) without one."""
+    try:
+        return _cur_device() if _cur_device is not None else _torch().cuda.current_device()
+    except RuntimeError:
+        return -2
+
+
+def _refuse(t, dtype, what, shape, here):
     if not isinstance(t, _torch().Tensor) or not t.is_cuda:
         raise _invalid(f"{what} must be a CUDA (HIP) tensor")
     if t.dtype != dtype:
         raise _invalid(f"{what} must be {dtype}, got {t.dtype}")
-    if shape is not None and t.shape != shape:
-        raise _invalid(f"{what} must be {list(shape)}, got {list(t.shape)}")
-    here = _torch().cuda.current_device() if _raw_stream is None else _cur_device()
-    if t.device.index != here:
+    if t.get_device() != here:
         raise _invalid(f"{what} is on {t.device}, the current device is cuda:{here}")
-    return t.data_ptr()
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise _invalid(f"{what} must be {list(shape)}, got {list(t.shape)}")
+    raise _invalid(f"{what} must be contiguous")
 
 
-def _vec(t, dtype, what, shape):
-    p = _ptr(t, dtype, what, shape)
-    if not t.is_contiguous():
-        raise _invalid(f"{what} must be contiguous")
-    return p
+def _ptr(t, dtype, what, here):
+    """Address of a tensor of this type on the current device."""
+    try:
+        if t.dtype is dtype and t.get_device() == here:
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, dtype, what, None, here)
 
 
-def _head_rows(t, what, heads, D, R=None):
-    """(address, row stride) of f32 rows [R, heads * D] or [R, heads, D] whose
-    elements lie side by side; rows may be any distance apart."""
-    p = _ptr(t, _torch().float32, what)
-    s, d = t.shape, t.stride()
-    if tuple(s[1:]) not in ((heads * D,), (heads, D)):
-        raise _invalid(f"{what} must be [rows, {heads * D}] or [rows, {heads}, {D}], got {list(s)}")
+def _vec(t, dtype, what, shape, here):
+    """Address of a contiguous tensor of this type and shape."""
+    try:
+        if t.dtype is dtype and t.get_device() == here and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, dtype, what, shape, here)
+
+
+def _head_rows(t, what, D, here, R=None, heads=None):
+    """(address, row stride, heads) of float32 rows [R, heads * D] or [R,
+    heads, D] whose elements lie side by side; rows may be any distance
+    apart."""
+    p = _ptr(t, _F32, what, here)
+    s = t.shape
+    if len(s) == 3:
+        n = s[1]
+        ok = s[2] == D and n > 0 and (t.stride(2) == 1 or D == 1) and (t.stride(1) == D or n == 1)
+    else:
+        n = s[1] // D if len(s) == 2 else 0
+        ok = n > 0 and n * D == s[1] and (t.stride(1) == 1 or s[1] == 1)
+    if not ok or (heads is not None and n != heads):
+        if len(s) in (2, 3) and (s[1:] == (heads or n, D) or s[1:] == ((heads or n) * D,)) and n > 0:
+            raise _invalid(f"{what} must be contiguous within a row")
+        h = "heads" if heads is None else heads
+        raise _invalid(f"{what} must be [rows, {h} * {D}] or [rows, {h}, {D}], got {list(s)}")
     if R is not None and s[0] != R:
         raise _invalid(f"{what} must have {R} rows, got {s[0]}")
-    if (len(s) == 3 and heads > 1 and d[1] != D) or (d[-1] != 1 and s[-1] != 1):
-        raise _invalid(f"{what} must be contiguous within a row")
-    return p, d[0]
+    return p, t.stride(0), n
 
 
-def _heads_of(t, what, D):
-    """Heads of rows [R, heads * D] or [R, heads, D]."""
-    if not isinstance(t, _torch().Tensor):
-        raise _invalid(f"{what} must be a CUDA (HIP) tensor")
-    n = t.shape[-1] if t.dim() == 2 else (t.shape[1] * t.shape[2] if t.dim() == 3 else 0)
-    if t.dim() not in (2, 3) or n == 0 or n % D or (t.dim() == 3 and t.shape[2] != D):
-        raise _invalid(f"{what} must be [rows, heads * {D}] or [rows, heads, {D}], got {list(t.shape)}")
-    return n // D
-
-
-def _on(stream, *inputs):
-    """Allocations of the block belong to `stream`; inputs stay allocated
-    until its work so far is done."""
-    if stream is None:
-        return contextlib.nullcontext()
+def _mark(stream, *inputs):
+    """Keeps the inputs allocated until the stream's work so far is done."""
     for t in inputs:
         if t is not None:
             t.record_stream(stream)
-    return _torch().cuda.stream(stream)
+
+
+def _empty(stream, *shape_dtype_device):
+    """An output, on the allocator's side of the stream that writes it."""
+    shape, dtype, device = shape_dtype_device
+    if stream is None:
+        return _torch().empty(shape, dtype=dtype, device=device)
+    with _torch().cuda.stream(stream):
+        return _torch().empty(shape, dtype=dtype, device=device)
 
 
 class KvCache:
@@ -120,7 +145,7 @@ class KvCache:
                 raise _invalid(f"{what} must be a CUDA (HIP) tensor")
             if t.dim() != 4:
                 raise _invalid(f"{what} must be [num_pages, page_size, kv_heads, head_dim], got {list(t.shape)}")
-        if k.dtype not in _dtypes():
+        if k.dtype not in _DTYPES:
             raise _invalid(f"k must be float32, float16 or bfloat16, got {k.dtype}")
         if v.dtype != k.dtype or v.shape != k.shape or v.device != k.device:
             raise _invalid("k and v must have one type, shape and device")
@@ -137,7 +162,8 @@ class KvCache:
         self.k, self.v, self.score = k, v, score
         self.num_pages, self.page_size, self.kv_heads, self.head_dim = P, page, H, D
         self._c = _KvCache(k.data_ptr(), v.data_ptr(), score.data_ptr() if score is not None else None,
-                           _dtypes()[k.dtype], H, D, page, P, k.stride(0), k.stride(1), k.stride(2))
+                           _DTYPES[k.dtype], H, D, page, P, k.stride(0), k.stride(1), k.stride(2))
+        self._device, self._ref = k.get_device(), ctypes.byref(self._c)
 
     @classmethod
     def new(cls, num_pages, page_size, kv_heads, head_dim, dtype=None, score=False, device="cuda"):
@@ -149,57 +175,61 @@ class KvCache:
         return cls(k, v, torch.zeros((num_pages, kv_heads, page_size), dtype=torch.float32, device=device)
                    if score else None)
 
-    def _here(self):
-        _ptr(self.k, self.k.dtype, "the cache")
-        return ctypes.byref(self._c)
+    def _on(self, here):
+        if self._device != here:
+            raise _invalid(f"the cache is on cuda:{self._device}, the current device is cuda:{here}")
+        return self._ref
 
 
-def _table(table):
+def _table(table, here):
     """xt_kv_table of an int32 tensor [seqs, max_pages]."""
-    p = _ptr(table, _torch().int32, "table")
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+    p = _ptr(table, _I32, "table", here)
+    s = table.shape
+    if len(s) != 2 or (s[1] > 1 and table.stride(1) != 1):
         raise _invalid("table must be [seqs, max_pages], contiguous within a row")
-    return ctypes.byref(_KvTable(p, table.stride(0), table.shape[0], table.shape[1]))
+    return ctypes.byref(_KvTable(p, table.stride(0), s[0], s[1])), s[0]
 
 
 def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=None, q_out=None, stream=None):
-    """xt_kv_append: R new tokens' k and v (float32 [R, kv_heads, head_dim])
-    into position slots[r] (int32 [R]; -1 skips the row) of sequence seq[r]
-    (default r) of table (int32 [seqs, max_pages]).  rope = (cos, sin), float32
-    [rows, dim / 2] each, rotates k and q by row positions[r] (default
-    slots[r]).  Returns the rotated q (q_out if given, which may be q), or
-    None without q."""
-    torch = _torch()
-    i32, f32, D = torch.int32, torch.float32, cache.head_dim
-    c, t = cache._here(), _table(table)
-    kp, ldk = _head_rows(k, "k", cache.kv_heads, D)
+    """xt_kv_append: R new tokens' k and v (float32 [R, kv_heads, head_dim] or
+    [R, kv_heads * head_dim]) into position slots[r] (int32 [R]; -1 skips the
+    row) of sequence seq[r] (default r) of table (int32 [seqs, max_pages]).
+    rope = (cos, sin), float32 [rows, dim / 2] each, rotates k and q by row
+    positions[r] (default slots[r]).  Returns the rotated q (q_out if given,
+    which may be q), or None without q."""
+    here, D = _here(), cache.head_dim
+    c = cache._on(here)
+    t, S = _table(table, here)
+    kp, ldk, _ = _head_rows(k, "k", D, here, None, cache.kv_heads)
     R = k.shape[0]
-    vp, ldv = _head_rows(v, "v", cache.kv_heads, D, R)
-    sp = _vec(slots, i32, "slots", (R,))
-    np_ = _vec(seq, i32, "seq", (R,)) if seq is not None else None
-    if seq is None and R > table.shape[0]:
-        raise _invalid(f"{R} rows for {table.shape[0]} sequences: seq is needed")
-    pp = _vec(positions, i32, "positions", (R,)) if positions is not None else None
+    vp, ldv, _ = _head_rows(v, "v", D, here, R, cache.kv_heads)
+    sp = _vec(slots, _I32, "slots", (R,), here)
+    if seq is not None:
+        np_ = _vec(seq, _I32, "seq", (R,), here)
+    elif R > S:
+        raise _invalid(f"{R} rows for {S} sequences: seq is needed")
+    else:
+        np_ = None
+    pp = _vec(positions, _I32, "positions", (R,), here) if positions is not None else None
     rp = None
     if rope is not None:
         cos, sin = rope
-        cp = _ptr(cos, f32, "cos")
+        cp = _ptr(cos, _F32, "cos", here)
         if cos.dim() != 2 or not cos.is_contiguous():
             raise _invalid("cos must be contiguous [rows, dim / 2]")
-        rp = ctypes.byref(_Rope(cp, _vec(sin, f32, "sin", cos.shape), cos.shape[0], 2 * cos.shape[1]))
+        rp = ctypes.byref(_Rope(cp, _vec(sin, _F32, "sin", cos.shape, here), cos.shape[0], 2 * cos.shape[1]))
     qp = op = None
     ldq = ldo = hq = 0
-    with _on(stream, cache.k, cache.v, cache.score, table, slots, k, v, q, seq, positions, q_out, *(rope or ())):
-        if q is not None:
-            hq = _heads_of(q, "q", D)
-            qp, ldq = _head_rows(q, "q", hq, D, R)
-            if q_out is None:
-                q_out = torch.empty(q.shape, dtype=f32, device=q.device)
-            op, ldo = _head_rows(q_out, "q_out", hq, D, R)
-        elif q_out is not None:
-            raise _invalid("q_out without q")
-        _check(_lib.xt_kv_append(c, t, np_, sp, pp, rp, qp, ldq, hq, op, ldo, kp, ldk, vp, ldv, R,
-                                 _stream_ptr(stream)))
+    if q is not None:
+        qp, ldq, hq = _head_rows(q, "q", D, here, R)
+        if q_out is None:
+            q_out = _empty(stream, q.shape, _F32, q.device)
+        op, ldo, _ = _head_rows(q_out, "q_out", D, here, R, hq) if q_out is not q else (qp, ldq, hq)
+    elif q_out is not None:
+        raise _invalid("q_out without q")
+    if stream is not None:
+        _mark(stream, cache.k, cache.v, cache.score, table, slots, k, v, q, seq, positions, q_out, *(rope or ()))
+    _check(_lib.xt_kv_append(c, t, np_, sp, pp, rp, qp, ldq, hq, op, ldo, kp, ldk, vp, ldv, R, _stream_ptr(stream)))
     return q_out
 
 
@@ -211,25 +241,26 @@ def paged_attention(cache, table, lengths, q, seq=None, scale=None, lse=False, a
     max_pages]).  scale defaults to head_dim ** -0.5.  Returns out, shaped as
     q, or (out, lse [R, q_heads]) with lse=True; accumulate=True adds the
     weights to cache.score."""
-    torch = _torch()
-    i32, f32, D = torch.int32, torch.float32, cache.head_dim
-    c, t = cache._here(), _table(table)
-    hq = _heads_of(q, "q", D)
-    qp, ldq = _head_rows(q, "q", hq, D)
+    here, D = _here(), cache.head_dim
+    c = cache._on(here)
+    t, S = _table(table, here)
+    qp, ldq, hq = _head_rows(q, "q", D, here)
     R = q.shape[0]
-    lp = _vec(lengths, i32, "lengths", (R,))
-    sp = _vec(seq, i32, "seq", (R,)) if seq is not None else None
-    if seq is None and R > table.shape[0]:
-        raise _invalid(f"{R} rows for {table.shape[0]} sequences: seq is needed")
-    with _on(stream, cache.k, cache.v, cache.score, table, lengths, q, seq, out):
-        if out is None:
-            out = torch.empty(q.shape, dtype=f32, device=q.device)
-        op, ldo = _head_rows(out, "out", hq, D, R)
-        l = torch.empty((R, hq), dtype=f32, device=q.device) if lse else None
-        _check(_lib.xt_paged_attention(c, t, sp, lp, qp, ldq, hq,
-                                       1.0 / math.sqrt(D) if scale is None else float(scale), R, op, ldo,
-                                       l.data_ptr() if lse else None, int(bool(accumulate)),
-                                       _stream_ptr(stream)))
+    lp = _vec(lengths, _I32, "lengths", (R,), here)
+    if seq is not None:
+        sp = _vec(seq, _I32, "seq", (R,), here)
+    elif R > S:
+        raise _invalid(f"{R} rows for {S} sequences: seq is needed")
+    else:
+        sp = None
+    if out is None:
+        out = _empty(stream, q.shape, _F32, q.device)
+    op, ldo, _ = _head_rows(out, "out", D, here, R, hq)
+    l = _empty(stream, (R, hq), _F32, q.device) if lse else None
+    if stream is not None:
+        _mark(stream, cache.k, cache.v, cache.score, table, lengths, q, seq, out)
+    _check(_lib.xt_paged_attention(c, t, sp, lp, qp, ldq, hq, D ** -0.5 if scale is None else scale, R, op, ldo,
+                                   l.data_ptr() if lse else None, 1 if accumulate else 0, _stream_ptr(stream)))
     return (out, l) if lse else out
 
 
@@ -240,19 +271,17 @@ def kv_evict(cache, table, lengths, budget, sink=0, recent=0, stream=None):
     them, moved in order to the front of its pages.  Returns (new lengths
     [seqs], kept [seqs, kv_heads, budget]: each one's old position, -1 past
     the new length)."""
-    torch = _torch()
-    i32 = torch.int32
-    c, t = cache._here(), _table(table)
-    S = table.shape[0]
-    lp = _vec(lengths, i32, "lengths", (S,))
-    budget = int(budget)
-    if budget < 1:
+    here = _here()
+    c = cache._on(here)
+    t, S = _table(table, here)
+    lp = _vec(lengths, _I32, "lengths", (S,), here)
+    if not 1 <= budget < 1 << 31:
         raise _invalid("budget must be 1..2^31-1")
-    with _on(stream, cache.k, cache.v, cache.score, table, lengths):
-        new = torch.empty((S,), dtype=i32, device=table.device)
-        kept = torch.empty((S, cache.kv_heads, budget), dtype=i32, device=table.device)
-        _check(_lib.xt_kv_evict(c, t, lp, budget, int(sink), int(recent), new.data_ptr(), kept.data_ptr(),
-                                _stream_ptr(stream)))
+    new = _empty(stream, (S,), _I32, table.device)
+    kept = _empty(stream, (S, cache.kv_heads, budget), _I32, table.device)
+    if stream is not None:
+        _mark(stream, cache.k, cache.v, cache.score, table, lengths)
+    _check(_lib.xt_kv_evict(c, t, lp, budget, sink, recent, new.data_ptr(), kept.data_ptr(), _stream_ptr(stream)))
     return new, kept
 
 
@@ -262,31 +291,31 @@ def token_logprobs(logits, tokens=None, top=0, stream=None):
     int32 [M] or [M, T].  Returns (log probabilities shaped as tokens, or
     None; entropy [M]; ids int32 [M, top] of the most likely tokens and their
     log probabilities [M, top], or None, None)."""
-    torch = _torch()
-    i32, f32 = torch.int32, torch.float32
-    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
-        raise _invalid("logits must be a CUDA (HIP) tensor")
-    if logits.dtype not in _dtypes():
-        raise _invalid(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    here = _here()
+    dtype = getattr(logits, "dtype", None)
+    xp = _ptr(logits, dtype, "logits", here)
+    if dtype not in _DTYPES:
+        raise _invalid(f"logits must be float32, float16 or bfloat16, got {dtype}")
+    s = logits.shape
+    if len(s) != 2 or (s[1] > 1 and logits.stride(1) != 1):
         raise _invalid("logits must be [rows, vocabulary], contiguous within a row")
-    xp = _ptr(logits, logits.dtype, "logits")
-    (M, V), T, tp, top = logits.shape, 0, None, int(top)
-    if tokens is not None:
-        tp = _ptr(tokens, i32, "tokens")
-        if tokens.dim() not in (1, 2) or tokens.shape[0] != M or not tokens.is_contiguous():
-            raise _invalid(f"tokens must be contiguous [{M}] or [{M}, T], got {list(tokens.shape)}")
-        T = 1 if tokens.dim() == 1 else tokens.shape[1]
+    (M, V), T, tp, lp, ids, best = s, 0, None, None, None, None
     if not 0 <= top <= 64:
         raise _invalid("top must be 0..64, at most the vocabulary")
     dev = logits.device
-    with _on(stream, logits, tokens):
-        lp = torch.empty(tokens.shape, dtype=f32, device=dev) if tokens is not None else None
-        entropy = torch.empty((M,), dtype=f32, device=dev)
-        ids = torch.empty((M, top), dtype=i32, device=dev) if top else None
-        best = torch.empty((M, top), dtype=f32, device=dev) if top else None
-        _check(_lib.xt_token_logprobs(_dtypes()[logits.dtype], xp, logits.stride(0), M, V, tp, T,
-                                      lp.data_ptr() if T else None, entropy.data_ptr(), top,
-                                      ids.data_ptr() if top else None, best.data_ptr() if top else None,
-                                      _stream_ptr(stream)))
+    if tokens is not None:
+        tp = _ptr(tokens, _I32, "tokens", here)
+        n = tokens.shape
+        if len(n) not in (1, 2) or n[0] != M or not tokens.is_contiguous():
+            raise _invalid(f"tokens must be contiguous [{M}] or [{M}, T], got {list(n)}")
+        T = 1 if len(n) == 1 else n[1]
+        lp = _empty(stream, n, _F32, dev)
+    entropy = _empty(stream, (M,), _F32, dev)
+    if top:
+        ids, best = _empty(stream, (M, top), _I32, dev), _empty(stream, (M, top), _F32, dev)
+    if stream is not None:
+        _mark(stream, logits, tokens)
+    _check(_lib.xt_token_logprobs(_DTYPES[dtype], xp, logits.stride(0), M, V, tp, T, lp.data_ptr() if T else None,
+                                  entropy.data_ptr(), top, ids.data_ptr() if top else None,
+                                  best.data_ptr() if top else None, _stream_ptr(stream)))
     return lp, entropy, ids, best
