@@ -64,7 +64,10 @@ int hip_fail(hipError_t e, const char* what) {
 //           allocated; every product launch leaves the counters zero again
 //           (the last workgroup of a tile resets its counter);
 //   kind 2: the MLP's gate / up rows and requantised intermediate;
-//   kind 3: paged attention's partial results (xtern_cache_api.cpp).
+//   kind 3: partial results of paged attention and token probabilities
+//           (xtern_cache_api.cpp);
+//   kind 4: paged attention's counters.  Zeroed when allocated; a launch
+//           leaves them zero again.
 int hipb_device(int* d) { return (int)hipGetDevice(d); }
 int hipb_alloc(void** p, size_t n) { return (int)hipMalloc(p, n); }
 int hipb_free(void* p) { return (int)hipFree(p); }
@@ -127,7 +130,7 @@ int workspace(hipStream_t s, size_t bytes, void** out, int kind = 0, Scratch* sc
     }
     (void)&g_ws_thread_guard;  // (constructs this thread's guard)
     std::string err;
-    const int st = ws_table().get(s, bytes, kind, kind == 1, out, &err);
+    const int st = ws_table().get(s, bytes, kind, kind == 1 || kind == 4, out, &err);
     return ws_status(st, err);
 }
 

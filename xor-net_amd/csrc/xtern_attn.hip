@@ -1,6 +1,7 @@
 // The paged key-value cache's append (rotary embedding, rounding, scatter)
 // and the attention of one token per row over it.
 #include <algorithm>
+#include <type_traits>
 
 #include "xtern_cache.h"
 #include "xtern_device.h"
@@ -36,7 +37,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
         if (i >= nq + nk) {
             const int j = i - nq - nk, h = j / c.D, d = j % c.D;
             vc[kv_offset(c, pg, slot, h) + d] = E::put(a.v[r * a.ldv + j]);
-            if (c.score && d == 0) c.score[((int64_t)pg * c.hkv + h) * c.page + slot % c.page] = 0.0f;
+            if (c.score && d == 0) c.score[((int64_t)pg * c.hkv + h) * c.page + kv_slot(c, slot)] = 0.0f;
             continue;
         }
         const bool isq = i < nq;
@@ -108,6 +109,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 // (rows may start at any element: the hardware loads unaligned vectors)
 typedef v4i v4iu __attribute__((aligned(2)));
 typedef v2i v2iu __attribute__((aligned(2)));
+typedef v4f v4fu __attribute__((aligned(4)));
 
 constexpr int kAttnThreads = 256;
 constexpr int kAttnWaves = kAttnThreads / 64;
@@ -121,9 +123,17 @@ constexpr int kAttnPlanRows = 1024;  // rows whose work is split by its total
 // sums go to slot (workgroup + row), which both grow along the line, so no two
 // segments share one and a row's slots are consecutive.
 // More than kAttnPlanRows rows: one workgroup per row.
+// The workgroup that ends a row's last segment joins them.  Segments and their
+// count are written and read at device scope, as the chip's eight L2s need it
+// (a fence would write back and drop whole caches): 131072 positions of one
+// row take 98 + 4 us in one kernel against 98 + 6.7 in two, without the second
+// launch.
 struct AttnPlan {
-    float* part_o;   // [slots][hy][16][D], unnormalised, relative to the segment's maximum
-    float* part_ml;  // [slots][hy][2][16]: maximum (base 2), sum
+    float* part_o;   // [slots][hy][16][dp], unnormalised, relative to the segment's maximum
+    float* part_ml;  // [slots][hy][16][2]: maximum (base 2), sum
+    unsigned* count; // [R][hy]: segments of the row done, zero between calls
+    float* ml;       // accumulate: maximum and sum of the whole row, [R][hq][2]
+    int dp;          // D, made even
     float* s;        // accumulate: S in base 2, [R][hq][cap]
     int64_t cap;     // positions of a row of s, a multiple of 32
     int hy;          // workgroups per share: kv heads x tiles of 16 query heads
@@ -164,11 +174,15 @@ struct AttnLine {
     int len, upto;       // the lane's row (R <= 64)
     int64_t* ends;       // LDS, [R] (R > 64)
     int64_t total;       // steps
+    int64_t per;         // steps of a share
+    double inv;          // 1 / per
     int x;               // shares that the line is cut into
 
     __device__ AttnLine(const AttnArgs& a_, const AttnPlan& pl_, int64_t* lds) : a(a_), pl(pl_), ends(lds) {
         if (pl.per_row) {
             total = x = (int)a.R;
+            per = 1;
+            inv = 1.0;
             return;
         }
         if (a.R <= 64) {
@@ -193,11 +207,19 @@ struct AttnLine {
             }
             __syncthreads();
         }
-        x = (int)min((int64_t)pl.shares, total);
+        // (whole numbers below 2^53: a quotient in doubles is off by one at most)
+        per = max((int64_t)1, (int64_t)((double)total / (double)pl.shares));
+        while (per * pl.shares < total) ++per;
+        inv = 1.0 / (double)per;
+        x = share_of(total - 1) + 1;
     }
     // First step of share b; the share that holds a step.
-    __device__ int64_t begin(int b) const { return (int64_t)b * total / x; }
-    __device__ int share_of(int64_t step) const { return (int)(((step + 1) * x - 1) / total); }
+    __device__ int64_t begin(int b) const { return min(b * per, total); }
+    __device__ int share_of(int64_t step) const {
+        int b = (int)((double)step * inv);
+        b -= b * per > step;
+        return b + ((b + 1) * per <= step);
+    }
     // First row that ends after `step`.
     __device__ int row_at(int64_t step) const {
         if (pl.per_row) return (int)step;
@@ -311,7 +333,6 @@ struct AttnShape {
     static constexpr int NJ = TK / 4;              // positions of a lane's V piece
     static constexpr int UE = DP / 16 < KU ? DP / 16 : KU;  // elements of a value load
     static constexpr int NU = DP / 16 / UE;        // value loads per position
-    static constexpr int QV = F32 ? KS : KS * Split<F32 ? (int)XT_BF16 : DT>::N;  // query registers (16 bytes)
 };
 
 // One chunk [p0, p1) of a row for the heads h0 .. h0 + nh - 1, in plain f32
@@ -374,23 +395,171 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
     __syncthreads();
 }
 
+// Two floats at device scope.
+__device__ __forceinline__ void st2_device(float* p, float x, float y) {
+    const unsigned long long v = ((unsigned long long)__float_as_uint(y) << 32) | __float_as_uint(x);
+    __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 ld2_device(const float* p) {
+    const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
+}
+
+__device__ __forceinline__ float row_lse(float m, float l) {
+    return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+}
+
+constexpr int kJoinBlock = 64;  // segments whose factors are in LDS at a time
+struct JoinLds {
+    float m[16], l[16], f[16 * kJoinBlock], fl[16 * kJoinBlock];
+};
+
+// Joins the segments of a row for the heads h0 .. h0 + nh - 1.  A wave adds up
+// one head's columns, a pair a lane, over the segments; with one or two heads
+// the waves share the segments.  Bound by the latency of device-scope loads,
+// so up to 32 of them are in flight.
+template <int DP>
+__device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int h0, int nh, JoinLds& lds,
+                               float* scratch) {
+    const int D = a.c.D, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+    const int64_t first = it.slot * pl.hy + blockIdx.y, step = (int64_t)pl.hy * 16 * pl.dp;
+    // Maxima and sums of a block of segments to LDS
+    auto stats = [&](int c0, int cnt) {
+#pragma unroll 1
+        for (int i = t; i < nh * kJoinBlock; i += kAttnThreads) {
+            const int h = i / kJoinBlock, c = i % kJoinBlock;
+            if (c >= cnt) continue;
+            const float2 x = ld2_device(pl.part_ml + ((first + (int64_t)(c0 + c) * pl.hy) * 16 + h) * 2);
+            lds.f[i] = x.x;
+            lds.fl[i] = x.y;
+        }
+    };
+    if (t < 16) {
+        lds.m[t] = -INFINITY;
+        lds.l[t] = 0.0f;
+    }
+#pragma unroll 1
+    for (int c0 = 0; c0 < it.nc; c0 += kJoinBlock) {
+        const int cnt = min(kJoinBlock, it.nc - c0);
+        stats(c0, cnt);
+        __syncthreads();
+#pragma unroll 1
+        for (int h = wave; h < nh; h += kAttnWaves) {
+            const float m = lane < cnt ? lds.f[h * kJoinBlock + lane] : -INFINITY;
+            const float l = lane < cnt ? lds.fl[h * kJoinBlock + lane] : 0.0f;
+            const float old = lds.m[h], mn = fmaxf(old, wave_max(m)), base = mn == -INFINITY ? 0.0f : mn;
+            const float sum = wave_sum(l * pow2(m - base)) + lds.l[h] * pow2(old - base);
+            if (lane == 0) {
+                lds.m[h] = mn;
+                lds.l[h] = sum;
+            }
+        }
+        __syncthreads();
+    }
+    constexpr int NK = DP > 128 ? 2 : 1, N = 32 / NK;  // pairs of a lane, segments in flight
+    const int share = nh == 1 ? 4 : (nh == 2 ? 2 : 1), part = wave & (share - 1);
+#pragma unroll 1
+    for (int hb = 0; hb < nh; hb += kAttnWaves / share) {
+        const int h = hb + wave / share;
+        float2 v[NK];
+#pragma unroll
+        for (int k = 0; k < NK; ++k) v[k] = float2{0.0f, 0.0f};
+#pragma unroll 1
+        for (int c0 = 0; c0 < it.nc; c0 += kJoinBlock) {
+            const int cnt = min(kJoinBlock, it.nc - c0);
+            if (it.nc > kJoinBlock) {
+                __syncthreads();
+                stats(c0, cnt);
+                __syncthreads();
+            }
+            if (h >= nh) continue;
+            const float base = lds.m[h] == -INFINITY ? 0.0f : lds.m[h];
+            const float fc = lane < cnt ? pow2(lds.f[h * kJoinBlock + lane] - base) : 0.0f;  // the lane's segment's
+            const float* o = pl.part_o + ((first + (int64_t)c0 * pl.hy) * 16 + h) * pl.dp;
+            auto add = [&](int c, auto batch) {
+                constexpr int B = decltype(batch)::value;
+                float2 x[B][NK];
+#pragma unroll
+                for (int i = 0; i < B; ++i)
+#pragma unroll
+                    for (int k = 0; k < NK; ++k)
+                        if (2 * lane + 128 * k < D)
+                            x[i][k] = ld2_device(o + min(c + i * share, cnt - 1) * step + 2 * lane + 128 * k);
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    const int ci = c + i * share;
+                    const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fc), min(ci, 63)));
+#pragma unroll
+                    for (int k = 0; k < NK; ++k)
+                        if (ci < cnt && 2 * lane + 128 * k < D) {
+                            v[k].x += f * x[i][k].x;
+                            v[k].y += f * x[i][k].y;
+                        }
+                }
+            };
+            int c = part;
+#pragma unroll 1
+            for (; c + N / 2 * share < cnt; c += N * share) add(c, std::integral_constant<int, N>());
+#pragma unroll 1
+            for (; c < cnt; c += 8 * share) add(c, std::integral_constant<int, 8>());
+        }
+        if (share > 1) {  // scratch [4][256]
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                scratch[wave * 256 + 2 * lane + 128 * k] = v[k].x;
+                scratch[wave * 256 + 2 * lane + 128 * k + 1] = v[k].y;
+            }
+            __syncthreads();
+            if (part == 0)
+                for (int w = 1; w < share; ++w)
+#pragma unroll
+                    for (int k = 0; k < NK; ++k) {
+                        v[k].x += scratch[(wave + w) * 256 + 2 * lane + 128 * k];
+                        v[k].y += scratch[(wave + w) * 256 + 2 * lane + 128 * k + 1];
+                    }
+        }
+        if (h < nh && part == 0) {
+            const float l = lds.l[h];
+            float* to = a.out + it.row * a.ldo + (int64_t)(h0 + h) * D;
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                const int d = 2 * lane + 128 * k;
+                if (d < D) to[d] = l == 0.0f ? 0.0f : v[k].x / l;
+                if (d + 1 < D) to[d + 1] = l == 0.0f ? 0.0f : v[k].y / l;
+            }
+        }
+    }
+    if (t < nh) {
+        const int64_t at = (int64_t)it.row * a.hq + h0 + t;
+        if (a.lse) a.lse[at] = row_lse(lds.m[t], lds.l[t]);
+        if (pl.ml) {
+            pl.ml[2 * at] = lds.m[t];
+            pl.ml[2 * at + 1] = lds.l[t];
+        }
+    }
+}
+
 template <int DT, int DP>
-__global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 || DT != XT_F32 ? 2 : 3)) void attention_kernel(AttnArgs a, AttnPlan pl,
+__global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) void attention_kernel(AttnArgs a, AttnPlan pl,
                                                                                    float scale2) {
     typedef AttnShape<DT, DP> S;
     typedef Elem<DT> E;
     typedef typename E::T T;
     const KvView& c = a.c;
     constexpr int kLdsRow = DP + 4;  // floats; the pad keeps heads apart in the banks
-    __shared__ float lds_o[kAttnWaves * 16 * kLdsRow];
+    __shared__ v4i lds_mem[kAttnWaves * 16 * kLdsRow / 4];
+    v4i* lds_q = lds_mem;                                // the queries, then
+    float* lds_o = reinterpret_cast<float*>(lds_mem);    // the waves' sums
     __shared__ float lds_ml[kAttnWaves][2][16];
     __shared__ int64_t lds_off[kAttnWaves][2][32];
+    __shared__ JoinLds lds_join;
+    __shared__ int lds_last;
     __shared__ int64_t lds_ends[kAttnPlanRows];
     const int hk = blockIdx.y / pl.tiles, G = a.hq / c.hkv;
     const int h0 = hk * G + (blockIdx.y % pl.tiles) * 16, nh = min(16, hk * G + G - h0);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int D = c.D;
-    const bool fast = D >= S::KU;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const AttnLine line(a, pl, lds_ends);
     if ((int)blockIdx.x >= line.x) return;
     int64_t at = line.begin(blockIdx.x);
@@ -399,6 +568,12 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 || DT != X
         int64_t row_end;
         const AttnSeg it = line.segment(r, at, to_step, &row_end);
         at = row_end;
+        // (opaque to the compiler: it would keep every index that follows from
+        // them in registers from segment to segment, and spill)
+        int D = c.D, lane = threadIdx.x & 63;
+        asm volatile("" : "+s"(D), "+v"(lane));
+        const int n = lane & 15, g = lane >> 4;
+        const bool fast = D >= S::KU;
         const int sq = a.seq ? a.seq[r] : r;
         const int ntiles = it.p1 > it.p0 ? (it.p1 - it.p0 + S::TK - 1) / S::TK : 0;
 
@@ -407,7 +582,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 || DT != X
     #pragma unroll
         for (int i = 0; i < S::NU * S::UE; ++i) o[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-        if (fast && wave < ntiles) {
+        if (fast && ntiles > 0) {
             const T* kc = static_cast<const T*>(c.k);
             const T* vc = static_cast<const T*>(c.v);
             // byte offsets of the lane's pieces in a key's and a value's row
@@ -423,7 +598,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 || DT != X
             // LDS; -1: no position there (masked, read from offset 0)
             auto entry = [&](int i) {  // the lane's table entry of tile i
                 const int p = it.p0 + i * S::TK + (lane & (S::TK - 1));
-                return p < it.p1 ? c.table[(int64_t)sq * c.ldt + p / c.page] : -1;
+                return p < it.p1 ? c.table[(int64_t)sq * c.ldt + kv_page_of(c, p)] : -1;
             };
             auto offsets = [&](int i, int e) {
                 const int p = it.p0 + i * S::TK + (lane & (S::TK - 1));
@@ -459,63 +634,91 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 || DT != X
 
             int next_e = entry(wave);
             const int after_e = entry(wave + kAttnWaves);
-            // the lane's pieces of the query rows: head h0 + n, elements from
-            // min(KU (4 s + g), D - KU); where pieces overlap (D no multiple of
-            // KU, or past D) the earlier one counts, the later one holds zeros
+            // The query rows as the lanes' operands, to LDS (in registers they
+            // would take 48 of 256 at D = 128), a wave every fourth piece: head
+            // h0 + n, elements from min(KU (4 s + g), D - KU); where pieces
+            // overlap (D no multiple of KU, or past D) the earlier one counts,
+            // the later one holds zeros.
             const float* q = a.q + it.row * a.ldq + (int64_t)(h0 + (n < nh ? n : 0)) * D;
-            float qf[S::KS * S::KU];
-    #pragma unroll
-            for (int i = 0; i < S::KS * S::KU; ++i) qf[i] = q[kd[i / S::KU] + i % S::KU];
-            bool full = offsets(wave, next_e);
-            next_e = after_e;
-            load_k(wave);
-            load_v(wave);
-            // (the queries' arithmetic while the first tile is on its way)
-    #pragma unroll
-            for (int i = 0; i < S::KS * S::KU; ++i)
-                if (n >= nh || kd[i / S::KU] + i % S::KU < S::KU * (4 * (i / S::KU) + g)) qf[i] = 0.0f;
-            typename Split<S::F32 ? (int)XT_BF16 : DT>::V qp[S::F32 ? 1 : S::KS][3];
-            if constexpr (!S::F32) {
-                if constexpr (DT == XT_F16) {
-                    // the row's largest element at 2^14 .. 2^15: f16's two pieces
-                    // then hold 22 bits of every element, or 2^-39 of the largest
-                    float mx = 0.0f;
-    #pragma unroll
-                    for (int i = 0; i < S::KS * S::KU; ++i) mx = fmaxf(mx, fabsf(qf[i]));
-                    mx = rows_max(mx);
-                    int e = 0;
-                    if (mx > 0.0f && mx < INFINITY) {
-                        (void)frexpf(mx, &e);
-                        e = max(-100, min(100, 15 - e));
-                    }
-                    const float up = ldexpf(1.0f, e);
-                    qs = scale2 * ldexpf(1.0f, -e);
-    #pragma unroll
-                    for (int i = 0; i < S::KS * S::KU; ++i) qf[i] *= up;
+            auto q_load = [&](int s, float* x) {
+                const int nom = S::KU * (4 * s + g), d = min(nom, D - S::KU);
+#pragma unroll
+                for (int i = 0; i < S::KU; i += 4) {
+                    const v4f f = *reinterpret_cast<const v4fu*>(q + d + i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[i + e] = n < nh && d + i + e >= nom ? f[e] : 0.0f;
                 }
-    #pragma unroll
-                for (int s = 0; s < S::KS; ++s) split8<DT>(&qf[s * S::KU], qp[s]);
+            };
+            float up = 1.0f;
+            if constexpr (DT == XT_F16) {
+                // the row's largest element at 2^14 .. 2^15: f16's two pieces
+                // then hold 22 bits of every element, or 2^-39 of the largest
+                float mx = 0.0f;
+#pragma unroll
+                for (int s = 0; s < S::KS; ++s) {
+                    float x[8];
+                    q_load(s, x);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[i]));
+                }
+                mx = rows_max(mx);
+                int e = 0;
+                if (mx > 0.0f && mx < INFINITY) {
+                    (void)frexpf(mx, &e);
+                    e = max(-100, min(100, 15 - e));
+                }
+                up = ldexpf(1.0f, e);
+                qs = scale2 * ldexpf(1.0f, -e);
             }
+#pragma unroll 1
+            for (int s = wave; s < S::KS; s += kAttnWaves) {
+                float x[S::KU];
+                q_load(s, x);
+                if constexpr (S::F32) {
+                    lds_q[s * 64 + lane] = __builtin_bit_cast(v4i, v4f{x[0], x[1], x[2], x[3]});
+                } else {
+                    typename Split<DT>::V pieces[3];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] *= up;
+                    split8<DT>(x, pieces);
+#pragma unroll
+                    for (int k = 0; k < Split<DT>::N; ++k)
+                        lds_q[(s * Split<DT>::N + k) * 64 + lane] = __builtin_bit_cast(v4i, pieces[k]);
+                }
+            }
+            bool full = false;
+            if (wave < ntiles) {
+                full = offsets(wave, next_e);
+                next_e = after_e;
+                load_k(wave);
+                load_v(wave);
+            }
+            __syncthreads();
             for (int i = wave; i < ntiles; i += kAttnWaves) {
+                asm volatile("" ::: "memory");  // (the queries stay in LDS)
                 // S of the tile
                 v4f sc[S::NT];
-    #pragma unroll
-                for (int t = 0; t < S::NT; ++t) {
-                    sc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int t = 0; t < S::NT; ++t) sc[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < S::KS; ++s) {
                     if constexpr (S::F32) {
-    #pragma unroll
-                        for (int s = 0; s < S::KS; ++s)
-    #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(kr[t][s][x]), qf[s * 4 + x],
-                                                                             sc[t], 0, 0, 0);
+                        const v4f qv = __builtin_bit_cast(v4f, lds_q[s * 64 + lane]);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+#pragma unroll
+                            for (int t = 0; t < S::NT; ++t)
+                                sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(kr[t][s][x]), qv[x], sc[t],
+                                                                             0, 0, 0);
                     } else {
-    #pragma unroll
-                        for (int s = 0; s < S::KS; ++s)
-    #pragma unroll
-                            for (int x = Split<DT>::N - 1; x >= 0; --x)
-                                sc[t] = Split<DT>::mfma(__builtin_bit_cast(typename Split<DT>::V, kr[t][s]), qp[s][x],
-                                                        sc[t]);
+                        typedef typename Split<DT>::V V;
+#pragma unroll
+                        for (int x = Split<DT>::N - 1; x >= 0; --x) {
+                            const V qv = __builtin_bit_cast(V, lds_q[(s * Split<DT>::N + x) * 64 + lane]);
+#pragma unroll
+                            for (int t = 0; t < S::NT; ++t)
+                                sc[t] = Split<DT>::mfma(__builtin_bit_cast(V, kr[t][s]), qv, sc[t]);
+                        }
                     }
                 }
                 // the next tile's keys, in flight under this tile's softmax and values
@@ -643,92 +846,39 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 || DT != X
         // has a maximum of -inf and comes here too.)
         if (__syncthreads_or(bad)) attn_plain<DT>(a, pl, it, hk, h0, nh, scale2, lds_o, &lds_ml[0][0][0], kLdsRow);
 
-        const bool whole = it.nc == 1;
-        const int64_t item = ((int64_t)blockIdx.x + it.row) * pl.hy + blockIdx.y;
-        float* to = whole ? a.out + it.row * a.ldo + (int64_t)h0 * D : pl.part_o + item * 16 * D;
-        for (int x = threadIdx.x; x < nh * D; x += kAttnThreads) {
-            const int h = x / D, d = x % D;
-            const float v = lds_o[h * kLdsRow + d], lt = lds_ml[0][1][h];
-            to[x] = !whole ? v : (lt == 0.0f ? 0.0f : v / lt);
-        }
-        if (threadIdx.x < nh) {
-            const float mm = lds_ml[0][0][n], lt = lds_ml[0][1][n];
-            if (whole && a.lse)
-                a.lse[(int64_t)it.row * a.hq + h0 + n] = lt == 0.0f ? -INFINITY : (mm + log2f(lt)) * 0.69314718056f;
-            if (pl.part_ml) {
-                pl.part_ml[item * 32 + n] = mm;
-                pl.part_ml[item * 32 + 16 + n] = lt;
+        if (it.nc == 1) {
+            float* to = a.out + it.row * a.ldo + (int64_t)h0 * D;
+            for (int h = wave; h < nh; h += kAttnWaves) {
+                const float lt = lds_ml[0][1][h];
+                for (int d = lane; d < D; d += 64) to[h * D + d] = lt == 0.0f ? 0.0f : lds_o[h * kLdsRow + d] / lt;
             }
-        }
-        __syncthreads();
-    }
-}
-
-// Joins the segments of a row: one workgroup per (row, query head).  The
-// factors of 256 segments at a time go to LDS, then every thread adds up four
-// columns of every eighth (or fourth) segment, eight loads in flight.
-__device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const AttnLine& line, int row) {
-    int64_t row_end;
-    const AttnSeg it = line.segment(row, 0, INT64_MAX, &row_end);
-    if (it.nc == 1) return;
-    const int G = a.hq / a.c.hkv, h = blockIdx.y, hk = h / G, tile = (h % G) / 16, n = (h % G) % 16;
-    const int D = a.c.D, t = threadIdx.x, wave = t >> 6;
-    __shared__ float sf[kAttnThreads];
-    __shared__ float so[kAttnThreads * 4];
-    __shared__ float sm[2][kAttnWaves];
-    const int64_t first = (int64_t)it.slot * pl.hy + hk * pl.tiles + tile;
-    const int64_t stride = (int64_t)pl.hy * 16 * D;  // of part_o, chunk to chunk
-    const float* po = pl.part_o + (first * 16 + n) * D;
-    const int cols = D <= 128 ? 32 : 64, groups = kAttnThreads / cols;
-    const int c4 = (t % cols) * 4, grp = t / cols;
-    float m = -INFINITY, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = 0; c0 < it.nc; c0 += kAttnThreads) {
-        const int cnt = min(kAttnThreads, it.nc - c0);
-        const float* ml = pl.part_ml + (first + (int64_t)(c0 + min(t, cnt - 1)) * pl.hy) * 32 + n;
-        const float mc = t < cnt ? ml[0] : -INFINITY, lc = t < cnt ? ml[16] : 0.0f;
-        const float mw = wave_max(mc);
-        __syncthreads();  // (the last round's factors are used up)
-        if ((t & 63) == 0) sm[0][wave] = mw;
-        __syncthreads();
-        const float mn = fmaxf(m, fmaxf(fmaxf(sm[0][0], sm[0][1]), fmaxf(sm[0][2], sm[0][3])));
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float f = pow2(m - base), fc = pow2(mc - base);
-        sf[t] = fc;
-        const float lw = wave_sum(lc * fc);
-        if ((t & 63) == 0) sm[1][wave] = lw;
-        m = mn;
-        __syncthreads();
-        l = l * f + ((sm[1][0] + sm[1][1]) + (sm[1][2] + sm[1][3]));
-#pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] *= f;
-        for (int c = grp; c < cnt; c += 8 * groups) {
-            float ld[8][4], w[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int cu = c + u * groups;
-                w[u] = cu < cnt ? sf[cu] : 0.0f;
-                const float* o = po + (int64_t)(c0 + min(cu, cnt - 1)) * stride;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) ld[u][x] = o[min(c4 + x, D - 1)];
+            if (threadIdx.x < nh) {
+                const int64_t row_h = (int64_t)it.row * a.hq + h0 + n;
+                const float mm = lds_ml[0][0][n], lt = lds_ml[0][1][n];
+                if (a.lse) a.lse[row_h] = row_lse(mm, lt);
+                if (pl.ml) {
+                    pl.ml[2 * row_h] = mm;
+                    pl.ml[2 * row_h + 1] = lt;
+                }
             }
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) v[x] += c + u * groups < cnt ? w[u] * ld[u][x] : 0.0f;
+        } else {
+            const int64_t item = ((int64_t)blockIdx.x + it.row) * pl.hy + blockIdx.y;
+            for (int h = wave; h < nh; h += kAttnWaves)
+                for (int d = 2 * lane; d < D; d += 128)
+                    st2_device(pl.part_o + (item * 16 + h) * pl.dp + d, lds_o[h * kLdsRow + d],
+                               d + 1 < D ? lds_o[h * kLdsRow + d + 1] : 0.0f);
+            if (threadIdx.x < nh) st2_device(pl.part_ml + (item * 16 + n) * 2, lds_ml[0][0][n], lds_ml[0][1][n]);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every store has arrived
+            __syncthreads();
+            // (the count wraps to zero by itself, for the next call)
+            if (threadIdx.x == 0)
+                lds_last = atomicInc(pl.count + (int64_t)it.row * pl.hy + blockIdx.y, (unsigned)it.nc - 1) ==
+                           (unsigned)it.nc - 1;
+            __syncthreads();
+            if (lds_last) attention_join<DP>(a, pl, it, h0, nh, lds_join, lds_o);
         }
+        __syncthreads();
     }
-    // [group][4 cols]
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < 4; ++x) so[grp * 4 * cols + c4 + x] = v[x];
-    __syncthreads();
-    if (t < D) {
-        float s = 0.0f;
-        for (int gI = 0; gI < groups; ++gI) s += so[gI * 4 * cols + t];
-        a.out[it.row * a.ldo + (int64_t)h * D + t] = l == 0.0f ? 0.0f : s / l;
-    }
-    if (t == 0 && a.lse)
-        a.lse[(int64_t)it.row * a.hq + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
 }
 
 // Adds the attention weights of a segment to the scores: one workgroup per
@@ -737,22 +887,10 @@ __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const At
     const KvView& c = a.c;
     const int G = a.hq / c.hkv, sq = a.seq ? a.seq[it.row] : it.row;
     extern __shared__ float hm[];  // [G] maximum, [G] 1 / sum
-    // a wave per head, a lane per chunk
-    for (int h = threadIdx.x >> 6; h < G; h += kAttnWaves) {
-        const int64_t first = (int64_t)it.slot * pl.hy + hk * pl.tiles + h / 16;
-        float m = -INFINITY, l = 0.0f;
-        for (int x = threadIdx.x & 63; x < it.nc; x += 64) {
-            const float* ml = pl.part_ml + (first + (int64_t)x * pl.hy) * 32 + h % 16;
-            const float mn = fmaxf(m, ml[0]), base = mn == -INFINITY ? 0.0f : mn;
-            l = l * pow2(m - base) + ml[16] * pow2(ml[0] - base);
-            m = mn;
-        }
-        const float mw = wave_max(m), base = mw == -INFINITY ? 0.0f : mw;
-        l = wave_sum(l * pow2(m - base));
-        if ((threadIdx.x & 63) == 0) {
-            hm[h] = base;
-            hm[G + h] = l == 0.0f ? 0.0f : 1.0f / l;
-        }
+    for (int h = threadIdx.x; h < G; h += kAttnThreads) {
+        const float* ml = pl.ml + 2 * ((int64_t)it.row * a.hq + hk * G + h);
+        hm[h] = ml[0] == -INFINITY ? 0.0f : ml[0];
+        hm[G + h] = ml[1] == 0.0f ? 0.0f : 1.0f / ml[1];
     }
     __syncthreads();
     for (int p = it.p0 + threadIdx.x; p < it.p1; p += kAttnThreads) {
@@ -761,19 +899,13 @@ __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const At
         float w = 0.0f;
         for (int h = 0; h < G; ++h)
             w += pow2(pl.s[((int64_t)it.row * a.hq + hk * G + h) * pl.cap + p] - hm[h]) * hm[G + h];
-        atomicAdd(&c.score[((int64_t)pg * c.hkv + hk) * c.page + p % c.page], w);
+        atomicAdd(&c.score[((int64_t)pg * c.hkv + hk) * c.page + kv_slot(c, p)], w);
     }
 }
 
-// What follows the attention kernel: workgroups (x, y < hq) join row x of
-// query head y, workgroups (x, hq + kv head) add share x's weights.
-__global__ __launch_bounds__(kAttnThreads) void attention_finish_kernel(AttnArgs a, AttnPlan pl) {
+__global__ __launch_bounds__(kAttnThreads) void attention_score_kernel(AttnArgs a, AttnPlan pl) {
     __shared__ int64_t lds_ends[kAttnPlanRows];
     const AttnLine line(a, pl, lds_ends);
-    if ((int)blockIdx.y < a.hq) {
-        if (blockIdx.x < a.R) attention_join(a, pl, line, blockIdx.x);
-        return;
-    }
     if ((int64_t)blockIdx.x >= line.x) return;
     int64_t at = line.begin(blockIdx.x);
     const int64_t to = line.begin(blockIdx.x + 1);
@@ -781,7 +913,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_finish_kernel(AttnArgs
         int64_t row_end;
         const AttnSeg it = line.segment(r, at, to, &row_end);
         at = row_end;
-        attention_scores(a, pl, it, (int)blockIdx.y - a.hq);
+        attention_scores(a, pl, it, blockIdx.y);
         __syncthreads();
     }
 }
@@ -789,19 +921,21 @@ __global__ __launch_bounds__(kAttnThreads) void attention_finish_kernel(AttnArgs
 namespace {
 
 // Workgroups of attention_kernel that a compute unit holds, by registers.
-int resident(int dtype, int D) { return D > 128 ? 1 : (D > 64 || dtype != XT_F32 ? 2 : 3); }
+int resident(int D) { return D > 128 ? 1 : (D > 64 ? 2 : 3); }
 
-AttnPlan make_plan(int dtype, const AttnArgs& a, int cus) {
+AttnPlan make_plan(const AttnArgs& a, int cus) {
     AttnPlan pl;
     const int G = a.hq / a.c.hkv;
-    pl.part_o = pl.part_ml = pl.s = nullptr;
+    pl.part_o = pl.part_ml = pl.s = pl.ml = nullptr;
+    pl.count = nullptr;
+    pl.dp = (a.c.D + 1) / 2 * 2;
     pl.tiles = (G + 15) / 16;
     pl.hy = a.c.hkv * pl.tiles;
     const int64_t cap = (int64_t)a.c.max_pages * a.c.page;
     pl.cap = (cap + 31) / 32 * 32;
     pl.per_row = a.R > kAttnPlanRows;
     const int64_t steps = a.R * std::max<int64_t>(1, (cap + kAttnStep - 1) / kAttnStep);
-    pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident(dtype, a.c.D) * cus / pl.hy));
+    pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident(a.c.D) * cus / pl.hy));
     if (pl.per_row) pl.shares = (int)a.R;
     return pl;
 }
@@ -833,34 +967,38 @@ size_t place(const AttnArgs& a, AttnPlan* pl, char* base) {
         return p;
     };
     const size_t slots = (size_t)pl->shares + (size_t)a.R;
-    pl->part_ml = take(slots * pl->hy * 32);
-    if (splits(a, *pl)) pl->part_o = take(slots * pl->hy * 16 * a.c.D);
-    if (a.accumulate) pl->s = take((size_t)a.R * a.hq * pl->cap);
+    if (splits(a, *pl)) {
+        pl->part_ml = take(slots * pl->hy * 32);
+        pl->part_o = take(slots * pl->hy * 16 * pl->dp);
+    }
+    if (a.accumulate) {
+        pl->ml = take((size_t)a.R * a.hq * 2);
+        pl->s = take((size_t)a.R * a.hq * pl->cap);
+    }
     return at;
 }
 
 }  // namespace
 
-size_t attention_workspace(int dtype, const AttnArgs& a, int cus) {
-    AttnPlan pl = make_plan(dtype, a, cus);
-    return splits(a, pl) || a.accumulate ? place(a, &pl, nullptr) : 0;
+size_t attention_workspace(const AttnArgs& a, int cus, size_t* counters) {
+    AttnPlan pl = make_plan(a, cus);
+    *counters = splits(a, pl) ? (size_t)a.R * pl.hy * sizeof(unsigned) : 0;
+    return place(a, &pl, nullptr);
 }
 
-hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, hipStream_t s) {
-    AttnPlan pl = make_plan(dtype, a, cus);
-    if (ws) (void)place(a, &pl, static_cast<char*>(ws));
+hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, void* counters, hipStream_t s) {
+    AttnPlan pl = make_plan(a, cus);
+    (void)place(a, &pl, static_cast<char*>(ws));
+    pl.count = static_cast<unsigned*>(counters);
     hipError_t e;
     switch (dtype) {
         case XT_F32: e = launch_attention<XT_F32>(a, pl, s); break;
         case XT_F16: e = launch_attention<XT_F16>(a, pl, s); break;
         default: e = launch_attention<XT_BF16>(a, pl, s); break;
     }
-    if (e != hipSuccess || !ws) return e;
-    // (rows are not joined where none is split)
-    const dim3 grid((unsigned)std::max<int64_t>(a.R, a.accumulate ? pl.shares : 0),
-                    (unsigned)(a.hq + (a.accumulate ? a.c.hkv : 0)));
-    const size_t lds = a.accumulate ? 2 * sizeof(float) * (size_t)(a.hq / a.c.hkv) : 0;
-    attention_finish_kernel<<<grid, kAttnThreads, lds, s>>>(a, pl);
+    if (e != hipSuccess || !a.accumulate) return e;
+    const size_t lds = 2 * sizeof(float) * (size_t)(a.hq / a.c.hkv);
+    attention_score_kernel<<<dim3((unsigned)pl.shares, (unsigned)a.c.hkv), kAttnThreads, lds, s>>>(a, pl);
     return hipGetLastError();
 }
 

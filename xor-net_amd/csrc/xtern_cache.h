@@ -19,6 +19,8 @@ struct KvView {
     float* score;
     int64_t sp, ss, sh;  // element strides of a page, a slot, a head
     int num_pages, page, hkv, D;
+    unsigned page_mul;  // p / page = p * page_mul >> page_shift for p < 2^31:
+    int page_shift;     // ceil(2^(31 + s) / page) and 31 + s, 2^s >= page
     const int32_t* table;  // [nseq][max_pages], row stride ldt
     int64_t ldt;
     int nseq, max_pages;
@@ -56,10 +58,10 @@ struct AttnArgs {
     int accumulate;
     int64_t R;
 };
-// Bytes of workspace that the call needs (0: none, ws is null); cus: compute
-// units of the device.
-size_t attention_workspace(int dtype, const AttnArgs& a, int cus);
-hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, hipStream_t s);
+// Bytes of workspace that the call needs, and of counters that are zero before
+// and after it (0: none, null); cus: compute units of the device.
+size_t attention_workspace(const AttnArgs& a, int cus, size_t* counters);
+hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, void* counters, hipStream_t s);
 
 struct EvictArgs {
     KvView c;
@@ -86,6 +88,16 @@ struct ProbsArgs {
 size_t token_logprobs_workspace(const ProbsArgs& a, int cus);
 hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, hipStream_t s);
 
+// page_mul and page_shift of a page size (1 .. 65536): the error of page_mul,
+// below page <= 2^s, grows to less than 2^(31 + s) in a product with p < 2^31.
+inline void set_page(KvView* c, int page) {
+    int s = 0;
+    while ((1 << s) < page) ++s;
+    c->page = page;
+    c->page_shift = 31 + s;
+    c->page_mul = (unsigned)((((uint64_t)1 << (31 + s)) + (uint64_t)page - 1) / (uint64_t)page);
+}
+
 #ifdef __HIPCC__
 
 // One element of the cache or of the logits as f32, and back (round to
@@ -107,14 +119,19 @@ template <> struct Elem<XT_BF16> {
     static __device__ __forceinline__ T put(float v) { return (T)v; }
 };
 
+__device__ __forceinline__ int kv_page_of(const KvView& c, int p) {
+    return (int)(((uint64_t)(unsigned)p * c.page_mul) >> c.page_shift);
+}
 // The page that holds position p of sequence `seq`, or -1: a table entry
 // outside the pool holds nothing.  0 <= p < max_pages * page.
 __device__ __forceinline__ int kv_page(const KvView& c, int seq, int p) {
-    const int e = c.table[(int64_t)seq * c.ldt + p / c.page];
+    const int e = c.table[(int64_t)seq * c.ldt + kv_page_of(c, p)];
     return (unsigned)e < (unsigned)c.num_pages ? e : -1;
 }
+// Its slot there.
+__device__ __forceinline__ int kv_slot(const KvView& c, int p) { return p - kv_page_of(c, p) * c.page; }
 __device__ __forceinline__ int64_t kv_offset(const KvView& c, int pg, int p, int h) {
-    return (int64_t)pg * c.sp + (int64_t)(p % c.page) * c.ss + (int64_t)h * c.sh;
+    return (int64_t)pg * c.sp + (int64_t)kv_slot(c, p) * c.ss + (int64_t)h * c.sh;
 }
 // A length as the kernels use it: within the table's row.
 __device__ __forceinline__ int kv_length(const KvView& c, int n) {

@@ -13,7 +13,7 @@
 #include "../../include/xtern.h"
 #include "xtern_cache.h"
 
-// xtern_api.cpp: error message, workspace of a stream (kind 3 is this file's),
+// xtern_api.cpp: error message, workspace of a stream (kinds 3 and 4 are this file's),
 // compute units of the current device.
 int xt_internal_fail(int code, const std::string& msg);
 int xt_internal_workspace(hipStream_t s, size_t bytes, void** out, int kind);
@@ -84,7 +84,7 @@ int check_cache(const xt_kv_cache* c, const xt_kv_table* t, xt::KvView* view) {
     view->ss = c->page_size == 1 ? 0 : c->stride_slot;
     view->sh = c->kv_heads == 1 ? 0 : c->stride_head;
     view->num_pages = (int)c->num_pages;
-    view->page = c->page_size;
+    xt::set_page(view, c->page_size);
     view->hkv = c->kv_heads;
     view->D = c->head_dim;
     view->table = t->pages;
@@ -197,11 +197,16 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     a.accumulate = accumulate ? 1 : 0;
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
-    void* ws = nullptr;
-    if (const size_t bytes = xt::attention_workspace(c->dtype, a, cus)) {
-        if (int rc = xt_internal_workspace(static_cast<hipStream_t>(stream), bytes, &ws, 3)) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    void *ws = nullptr, *counters = nullptr;
+    size_t nc = 0;
+    if (const size_t bytes = xt::attention_workspace(a, cus, &nc)) {
+        if (int rc = xt_internal_workspace(st, bytes, &ws, 3)) return rc;
     }
-    return launched(xt::launch_paged_attention(c->dtype, a, cus, ws, static_cast<hipStream_t>(stream)),
+    if (nc) {
+        if (int rc = xt_internal_workspace(st, nc, &counters, 4)) return rc;
+    }
+    return launched(xt::launch_paged_attention(c->dtype, a, cus, ws, counters, st),
                     "paged attention launch");
 }
 

@@ -35,7 +35,7 @@ constexpr int kMoveUnits = 4;   // 16-byte pieces of a thread and round
 __device__ __forceinline__ unsigned evict_key(const KvView& c, int seq, int h, int p) {
     const int pg = kv_page(c, seq, p);
     if (pg < 0) return 0u;
-    const float f = c.score[((int64_t)pg * c.hkv + h) * c.page + p % c.page] + 0.0f;  // (-0 counts as +0)
+    const float f = c.score[((int64_t)pg * c.hkv + h) * c.page + kv_slot(c, p)] + 0.0f;  // (-0 counts as +0)
     if (f != f) return 1u;
     const unsigned u = __float_as_uint(f);
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
@@ -220,8 +220,8 @@ __device__ __forceinline__ void move_rows(const KvView& c, int seq, char* base, 
                 const int off = min((u0 + (int)(i % un)) * (int)sizeof(T), bytes - (int)sizeof(T));
                 const int pf = kv_page(c, seq, src), pt = kv_page(c, seq, j);
                 if (src != j && pf >= 0 && pt >= 0) {
-                    from[x] = base + pf * sp + (src % c.page) * ss + off;
-                    to[x] = base + pt * sp + (j % c.page) * ss + off;
+                    from[x] = base + pf * sp + (kv_slot(c, src)) * ss + off;
+                    to[x] = base + pt * sp + (kv_slot(c, j)) * ss + off;
                 }
             }
         }
