@@ -1,7 +1,6 @@
 // The paged key-value cache's append (rotary embedding, rounding, scatter)
 // and the attention of one token per row over it.
 #include <algorithm>
-#include <type_traits>
 
 #include "xtern_cache.h"
 #include "xtern_device.h"
@@ -410,84 +409,51 @@ __device__ __forceinline__ float row_lse(float m, float l) {
     return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
 }
 
-constexpr int kJoinBlock = 64;  // segments whose factors are in LDS at a time
-struct JoinLds {
-    float m[16], l[16], f[16 * kJoinBlock], fl[16 * kJoinBlock];
-};
-
 // Joins the segments of a row for the heads h0 .. h0 + nh - 1.  A wave adds up
-// one head's columns, a pair a lane, over the segments; with one or two heads
-// the waves share the segments.  Bound by the latency of device-scope loads,
-// so up to 32 of them are in flight.
+// one head's columns, a pair a lane, over 64 segments at a time, whose maxima
+// and sums are a lane's each; with one or two heads the waves share the
+// segments.  Bound by the latency of device-scope loads: the first segments'
+// columns are requested together with the statistics that weigh them.
 template <int DP>
-__device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int h0, int nh, JoinLds& lds,
+__device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int h0, int nh,
                                float* scratch) {
-    const int D = a.c.D, t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+    constexpr int NK = DP > 128 ? 2 : 1, N = 16;  // pairs of a lane, segments in flight
+    const int D = a.c.D, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t first = it.slot * pl.hy + blockIdx.y, step = (int64_t)pl.hy * 16 * pl.dp;
-    // Maxima and sums of a block of segments to LDS
-    auto stats = [&](int c0, int cnt) {
-#pragma unroll 1
-        for (int i = t; i < nh * kJoinBlock; i += kAttnThreads) {
-            const int h = i / kJoinBlock, c = i % kJoinBlock;
-            if (c >= cnt) continue;
-            const float2 x = ld2_device(pl.part_ml + ((first + (int64_t)(c0 + c) * pl.hy) * 16 + h) * 2);
-            lds.f[i] = x.x;
-            lds.fl[i] = x.y;
-        }
-    };
-    if (t < 16) {
-        lds.m[t] = -INFINITY;
-        lds.l[t] = 0.0f;
-    }
-#pragma unroll 1
-    for (int c0 = 0; c0 < it.nc; c0 += kJoinBlock) {
-        const int cnt = min(kJoinBlock, it.nc - c0);
-        stats(c0, cnt);
-        __syncthreads();
-#pragma unroll 1
-        for (int h = wave; h < nh; h += kAttnWaves) {
-            const float m = lane < cnt ? lds.f[h * kJoinBlock + lane] : -INFINITY;
-            const float l = lane < cnt ? lds.fl[h * kJoinBlock + lane] : 0.0f;
-            const float old = lds.m[h], mn = fmaxf(old, wave_max(m)), base = mn == -INFINITY ? 0.0f : mn;
-            const float sum = wave_sum(l * pow2(m - base)) + lds.l[h] * pow2(old - base);
-            if (lane == 0) {
-                lds.m[h] = mn;
-                lds.l[h] = sum;
-            }
-        }
-        __syncthreads();
-    }
-    constexpr int NK = DP > 128 ? 2 : 1, N = 32 / NK;  // pairs of a lane, segments in flight
     const int share = nh == 1 ? 4 : (nh == 2 ? 2 : 1), part = wave & (share - 1);
 #pragma unroll 1
     for (int hb = 0; hb < nh; hb += kAttnWaves / share) {
         const int h = hb + wave / share;
+        float m = -INFINITY, l = 0.0f;
         float2 v[NK];
 #pragma unroll
         for (int k = 0; k < NK; ++k) v[k] = float2{0.0f, 0.0f};
 #pragma unroll 1
-        for (int c0 = 0; c0 < it.nc; c0 += kJoinBlock) {
-            const int cnt = min(kJoinBlock, it.nc - c0);
-            if (it.nc > kJoinBlock) {
-                __syncthreads();
-                stats(c0, cnt);
-                __syncthreads();
-            }
-            if (h >= nh) continue;
-            const float base = lds.m[h] == -INFINITY ? 0.0f : lds.m[h];
-            const float fc = lane < cnt ? pow2(lds.f[h * kJoinBlock + lane] - base) : 0.0f;  // the lane's segment's
+        for (int c0 = 0; c0 < it.nc && h < nh; c0 += 64) {
+            const int cnt = min(64, it.nc - c0);
             const float* o = pl.part_o + ((first + (int64_t)c0 * pl.hy) * 16 + h) * pl.dp;
-            auto add = [&](int c, auto batch) {
-                constexpr int B = decltype(batch)::value;
-                float2 x[B][NK];
+            const float2 ml = ld2_device(pl.part_ml + ((first + (int64_t)(c0 + min(lane, cnt - 1)) * pl.hy) * 16 + h) * 2);
+            float fc = 0.0f;  // the factor of the lane's segment
+#pragma unroll 1
+            for (int c = part; c < cnt || c == part; c += N * share) {
+                float2 x[N][NK];
 #pragma unroll
-                for (int i = 0; i < B; ++i)
+                for (int i = 0; i < N; ++i)
 #pragma unroll
                     for (int k = 0; k < NK; ++k)
                         if (2 * lane + 128 * k < D)
                             x[i][k] = ld2_device(o + min(c + i * share, cnt - 1) * step + 2 * lane + 128 * k);
+                if (c == part) {
+                    const float mc = lane < cnt ? ml.x : -INFINITY, mn = fmaxf(m, wave_max(mc));
+                    const float base = mn == -INFINITY ? 0.0f : mn, f = pow2(m - base);
+                    fc = pow2(mc - base);
+                    l = l * f + wave_sum(lane < cnt ? ml.y * fc : 0.0f);
 #pragma unroll
-                for (int i = 0; i < B; ++i) {
+                    for (int k = 0; k < NK; ++k) v[k].x *= f, v[k].y *= f;
+                    m = mn;
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
                     const int ci = c + i * share;
                     const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fc), min(ci, 63)));
 #pragma unroll
@@ -497,12 +463,7 @@ __device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const Attn
                             v[k].y += f * x[i][k].y;
                         }
                 }
-            };
-            int c = part;
-#pragma unroll 1
-            for (; c + N / 2 * share < cnt; c += N * share) add(c, std::integral_constant<int, N>());
-#pragma unroll 1
-            for (; c < cnt; c += 8 * share) add(c, std::integral_constant<int, 8>());
+            }
         }
         if (share > 1) {  // scratch [4][256]
             __syncthreads();
@@ -520,23 +481,21 @@ __device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const Attn
                         v[k].y += scratch[(wave + w) * 256 + 2 * lane + 128 * k + 1];
                     }
         }
-        if (h < nh && part == 0) {
-            const float l = lds.l[h];
-            float* to = a.out + it.row * a.ldo + (int64_t)(h0 + h) * D;
+        if (h >= nh || part) continue;
+        float* to = a.out + it.row * a.ldo + (int64_t)(h0 + h) * D;
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                const int d = 2 * lane + 128 * k;
-                if (d < D) to[d] = l == 0.0f ? 0.0f : v[k].x / l;
-                if (d + 1 < D) to[d + 1] = l == 0.0f ? 0.0f : v[k].y / l;
-            }
+        for (int k = 0; k < NK; ++k) {
+            const int d = 2 * lane + 128 * k;
+            if (d < D) to[d] = l == 0.0f ? 0.0f : v[k].x / l;
+            if (d + 1 < D) to[d + 1] = l == 0.0f ? 0.0f : v[k].y / l;
         }
-    }
-    if (t < nh) {
-        const int64_t at = (int64_t)it.row * a.hq + h0 + t;
-        if (a.lse) a.lse[at] = row_lse(lds.m[t], lds.l[t]);
-        if (pl.ml) {
-            pl.ml[2 * at] = lds.m[t];
-            pl.ml[2 * at + 1] = lds.l[t];
+        if (lane == 0) {
+            const int64_t at = (int64_t)it.row * a.hq + h0 + h;
+            if (a.lse) a.lse[at] = row_lse(m, l);
+            if (pl.ml) {
+                pl.ml[2 * at] = m;
+                pl.ml[2 * at + 1] = l;
+            }
         }
     }
 }
@@ -554,7 +513,6 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
     float* lds_o = reinterpret_cast<float*>(lds_mem);    // the waves' sums
     __shared__ float lds_ml[kAttnWaves][2][16];
     __shared__ int64_t lds_off[kAttnWaves][2][32];
-    __shared__ JoinLds lds_join;
     __shared__ int lds_last;
     __shared__ int64_t lds_ends[kAttnPlanRows];
     const int hk = blockIdx.y / pl.tiles, G = a.hq / c.hkv;
@@ -875,7 +833,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 lds_last = atomicInc(pl.count + (int64_t)it.row * pl.hy + blockIdx.y, (unsigned)it.nc - 1) ==
                            (unsigned)it.nc - 1;
             __syncthreads();
-            if (lds_last) attention_join<DP>(a, pl, it, h0, nh, lds_join, lds_o);
+            if (lds_last) attention_join<DP>(a, pl, it, h0, nh, lds_o);
         }
         __syncthreads();
     }
