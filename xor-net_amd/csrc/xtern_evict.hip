@@ -233,14 +233,14 @@ __device__ __forceinline__ void move_rows(const KvView& c, int seq, char* base, 
 #pragma unroll
         for (int x = 0; x < kMoveUnits; ++x) {
             dst[x] = to[x];
-            val[x] = *reinterpret_cast<const U*>(from[x]);
+            val[x] = __builtin_nontemporal_load(reinterpret_cast<const U*>(from[x]));
         }
         if (i0 + kRound < total) place(i0 + kRound);  // (addresses: while the rows are on their way)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every load of the round is done
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < kMoveUnits; ++x)
-            if (dst[x]) *reinterpret_cast<U*>(dst[x]) = val[x];
+            if (dst[x]) __builtin_nontemporal_store(val[x], reinterpret_cast<U*>(dst[x]));
     }
 }
 

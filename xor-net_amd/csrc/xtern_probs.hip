@@ -193,7 +193,7 @@ struct ProbsTileRegs {
         for (int i = 0; i < NV; ++i) {
             const int64_t at = base + (int64_t)(i * kProbsThreads + (int)threadIdx.x) * W;
             if (at + W <= V) {
-                v[i] = *reinterpret_cast<const VecU*>(x + at);
+                v[i] = __builtin_nontemporal_load(reinterpret_cast<const VecU*>(x + at));
             } else {
 #pragma unroll
                 for (int j = 0; j < W; ++j) v[i][j] = at + j < V ? x[at + j] : (T)-INFINITY;
