@@ -66,8 +66,8 @@ int hip_fail(hipError_t e, const char* what) {
 //   kind 2: the MLP's gate / up rows and requantised intermediate;
 //   kind 3: partial results of paged attention and token probabilities
 //           (xtern_cache_api.cpp);
-//   kind 4: paged attention's counters.  Zeroed when allocated; a launch
-//           leaves them zero again.
+//   kind 4: their counters.  Zeroed when allocated; a launch leaves the ones
+//           it uses zero again.
 int hipb_device(int* d) { return (int)hipGetDevice(d); }
 int hipb_alloc(void** p, size_t n) { return (int)hipMalloc(p, n); }
 int hipb_free(void* p) { return (int)hipFree(p); }

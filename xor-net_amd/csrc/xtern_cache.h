@@ -85,8 +85,8 @@ struct ProbsArgs {
     int32_t* ids;    // [M][top]
     float* top_lp;   // [M][top]
 };
-size_t token_logprobs_workspace(const ProbsArgs& a, int cus);
-hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, hipStream_t s);
+size_t token_logprobs_workspace(const ProbsArgs& a, int cus, size_t* counters);
+hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, void* counters, hipStream_t s);
 
 // page_mul and page_shift of a page size (1 .. 65536): the error of page_mul,
 // below page <= 2^s, grows to less than 2^(31 + s) in a product with p < 2^31.

@@ -113,6 +113,15 @@ int check_heads(int q_heads, int kv_heads) {
     return XT_OK;
 }
 
+// The workspace and the counters of a call (either may be none).
+int get_workspace(hipStream_t s, size_t bytes, size_t counters, void** ws, void** cnt) {
+    *ws = *cnt = nullptr;
+    if (bytes) {
+        if (int rc = xt_internal_workspace(s, bytes, ws, 3)) return rc;
+    }
+    return counters ? xt_internal_workspace(s, counters, cnt, 4) : XT_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -198,14 +207,10 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    void *ws = nullptr, *counters = nullptr;
-    size_t nc = 0;
-    if (const size_t bytes = xt::attention_workspace(a, cus, &nc)) {
-        if (int rc = xt_internal_workspace(st, bytes, &ws, 3)) return rc;
-    }
-    if (nc) {
-        if (int rc = xt_internal_workspace(st, nc, &counters, 4)) return rc;
-    }
+    void *ws, *counters;
+    size_t nc;
+    const size_t bytes = xt::attention_workspace(a, cus, &nc);
+    if (int rc = get_workspace(st, bytes, nc, &ws, &counters)) return rc;
     return launched(xt::launch_paged_attention(c->dtype, a, cus, ws, counters, st),
                     "paged attention launch");
 }
@@ -262,11 +267,12 @@ int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int6
     a.top_lp = top_logprobs;
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
-    void* ws = nullptr;
-    if (const size_t bytes = xt::token_logprobs_workspace(a, cus)) {
-        if (int rc = xt_internal_workspace(static_cast<hipStream_t>(stream), bytes, &ws, 3)) return rc;
-    }
-    return launched(xt::launch_token_logprobs(dtype, a, cus, ws, static_cast<hipStream_t>(stream)),
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    void *ws, *counters;
+    size_t nc;
+    const size_t bytes = xt::token_logprobs_workspace(a, cus, &nc);
+    if (int rc = get_workspace(st, bytes, nc, &ws, &counters)) return rc;
+    return launched(xt::launch_token_logprobs(dtype, a, cus, ws, counters, st),
                     "token probabilities launch");
 }
 

@@ -12,8 +12,9 @@
 // tiles of 8192 logits that stay in registers from the maximum over the sums to
 // the selection, the next tile in flight meanwhile; sums are per thread,
 // relative to the workgroup's running maximum, and reduced once at the end.  A
-// row is cut into slices only as far as there are too few rows for the chip
-// (then a second kernel joins them).
+// row is cut into slices only as far as there are too few rows for the chip;
+// the workgroup that ends a row's last slice joins them (results and count at
+// device scope, as the chip's eight L2s need it).
 //
 // Selection of the `top` largest: a wave's q-th largest lane maximum, q = top /
 // 8, is reached by at least q of its logits, so the minimum of that over the
@@ -43,8 +44,9 @@ constexpr int kProbsSlices = 64;
 // Slices of a row: slice s is tiles [s * per, (s + 1) * per).
 struct ProbsPlan {
     int slices, per, tiles;
-    float* stats;  // [M][slices][4]: m, z, xz, count of the maximum
-    u64* keys;     // [M][slices][top]
+    u64* stats;       // [M][slices][2]: m and z, xz and the count of the maximum
+    u64* keys;        // [M][slices][top]
+    unsigned* count;  // [M]: slices done, zero between calls
 };
 
 // The first `top` of keys[0 .. n) in descending order, to list[0 .. min(top,
@@ -121,13 +123,25 @@ struct ProbsSum {
     }
 };
 
+__device__ __forceinline__ void st_device(u64* p, u64 v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ u64 ld_device(const u64* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ u64 pack2(float lo, float hi) {
+    return ((u64)__float_as_uint(hi) << 32) | __float_as_uint(lo);
+}
+__device__ __forceinline__ float low(u64 v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float high(u64 v) { return __uint_as_float((unsigned)(v >> 32)); }
+
 struct ProbsLds {
     float wmax[2][kProbsWaves], wbound[2][kProbsWaves];
     float sums[3][kProbsWaves];
     u64 cand[kProbsCand];
     u64 list[kProbsTop];
     u64 wbest[kProbsWaves];
-    int count;
+    int count, last;
 };
 
 // The row's results from its sums and its list of the `top` first keys.
@@ -202,11 +216,49 @@ struct ProbsTileRegs {
     }
 };
 
+// Joins a row's slices: the sums, and of the lists (each in descending order)
+// the first `top`.  With q = ceil(top / slices), the slices' q-th entries have
+// a minimum that at least `top` entries reach: only those are ranked.
+template <int DT>
+__device__ void probs_join(const ProbsArgs& a, const ProbsPlan& pl, int64_t r, u64* keys, ProbsLds& lds) {
+    const int n = pl.slices * a.top, sl = min((int)(threadIdx.x & 63), pl.slices - 1);
+    constexpr int kMine = kProbsSlices * kProbsTop / kProbsThreads;
+    u64 mine[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+        const int at = i * kProbsThreads + threadIdx.x;
+        mine[i] = at < n ? ld_device(pl.keys + r * n + at) : 0;
+    }
+    const u64 s0 = ld_device(pl.stats + (r * pl.slices + sl) * 2), s1 = ld_device(pl.stats + (r * pl.slices + sl) * 2 + 1);
+    u64 bound = 0;
+    if (a.top) {
+        bound = ld_device(pl.keys + r * n + (int64_t)sl * a.top + (a.top + pl.slices - 1) / pl.slices - 1);
+        for (int o = 32; o; o >>= 1) bound = min(bound, __shfl_xor(bound, o));
+    }
+    ProbsSum s{low(s0), high(s0), low(s1), high(s1)};
+    s.raise(wave_max_f(s.m));
+    const bool in = (int)(threadIdx.x & 63) < pl.slices;
+    s.z = wave_sum_f(in ? s.z : 0.0f);
+    s.xz = wave_sum_f(in ? s.xz : 0.0f);
+    s.c = wave_sum_f(in ? s.c : 0.0f);
+    for (int i = threadIdx.x; i < (n + 31) / 32 * 32; i += kProbsThreads) keys[i] = 0;
+    if (threadIdx.x == 0) lds.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        if (mine[i] && mine[i] >= bound) keys[atomicAdd(&lds.count, 1)] = mine[i];
+    __syncthreads();
+    probs_rank(keys, lds.count, a.top, lds.list);
+    __syncthreads();
+    probs_finish<DT>(a, r, s, lds.list);
+}
+
 template <int DT>
 __global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsArgs a, ProbsPlan pl) {
     typedef ProbsTileRegs<DT> R;
     typedef typename R::T T;
     __shared__ ProbsLds lds;
+    __shared__ u64 join_keys[kProbsSlices * kProbsTop];
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t r = blockIdx.x / pl.slices;
     const int slice = blockIdx.x % pl.slices;
@@ -338,58 +390,17 @@ __global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsA
         return;
     }
     if (t == 0) {
-        float* st = pl.stats + (int64_t)blockIdx.x * 4;
-        st[0] = s.m;
-        st[1] = s.z;
-        st[2] = s.xz;
-        st[3] = s.c;
+        st_device(pl.stats + (int64_t)blockIdx.x * 2, pack2(s.m, s.z));
+        st_device(pl.stats + (int64_t)blockIdx.x * 2 + 1, pack2(s.xz, s.c));
     }
     for (int i = t; i < a.top; i += kProbsThreads)
-        pl.keys[(int64_t)blockIdx.x * a.top + i] = i < have ? lds.list[i] : 0;
-}
-
-// Joins a row's slices: the sums, and of the lists (each in descending order)
-// the first `top`.  With q = ceil(top / slices), the slices' q-th entries have
-// a minimum that at least `top` entries reach: only those are ranked.
-template <int DT>
-__global__ __launch_bounds__(kProbsThreads) void token_logprobs_join_kernel(ProbsArgs a, ProbsPlan pl) {
-    __shared__ u64 keys[kProbsSlices * kProbsTop];
-    __shared__ u64 list[kProbsTop];
-    __shared__ int count;
-    const int64_t r = blockIdx.x;
-    const int n = pl.slices * a.top;
-    if (threadIdx.x == 0) count = 0;
-    u64 mine_k[kProbsSlices * kProbsTop / kProbsThreads];
-#pragma unroll
-    for (int i = 0; i < kProbsSlices * kProbsTop / kProbsThreads; ++i) {
-        const int at = i * kProbsThreads + threadIdx.x;
-        mine_k[i] = at < n ? pl.keys[r * n + at] : 0;
-    }
-    u64 bound = 0;
-    if (a.top) {
-        const int q = (a.top + pl.slices - 1) / pl.slices;
-        bound = pl.keys[r * n + (int64_t)min((int)(threadIdx.x & 63), pl.slices - 1) * a.top + q - 1];
-        for (int o = 32; o; o >>= 1) bound = min(bound, __shfl_xor(bound, o));
-    }
-    const float* st = pl.stats + r * pl.slices * 4;
-    const int sl = min((int)(threadIdx.x & 63), pl.slices - 1);
-    const ProbsSum part{st[sl * 4], st[sl * 4 + 1], st[sl * 4 + 2], st[sl * 4 + 3]};
-    const float m = wave_max_f(part.m);
-    ProbsSum s = part;
-    s.raise(m);
-    const bool in = (int)(threadIdx.x & 63) < pl.slices;
-    s.z = wave_sum_f(in ? s.z : 0.0f);
-    s.xz = wave_sum_f(in ? s.xz : 0.0f);
-    s.c = wave_sum_f(in ? s.c : 0.0f);
-    for (int i = threadIdx.x; i < (n + 31) / 32 * 32; i += kProbsThreads) keys[i] = 0;
+        st_device(pl.keys + (int64_t)blockIdx.x * a.top + i, i < have ? lds.list[i] : 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every store has arrived
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kProbsSlices * kProbsTop / kProbsThreads; ++i)
-        if (mine_k[i] && mine_k[i] >= bound) keys[atomicAdd(&count, 1)] = mine_k[i];
+    // (the count wraps to zero by itself, for the next call)
+    if (t == 0) lds.last = atomicInc(pl.count + r, (unsigned)pl.slices - 1) == (unsigned)pl.slices - 1;
     __syncthreads();
-    probs_rank(keys, count, a.top, list);
-    __syncthreads();
-    probs_finish<DT>(a, r, s, list);
+    if (lds.last) probs_join<DT>(a, pl, r, join_keys, lds);
 }
 
 namespace {
@@ -402,31 +413,30 @@ ProbsPlan make_plan(const ProbsArgs& a, int cus) {
     const int slices = (int)std::min<int64_t>(std::min<int64_t>(want, kProbsSlices), pl.tiles);
     pl.per = (pl.tiles + slices - 1) / slices;
     pl.slices = (pl.tiles + pl.per - 1) / pl.per;
-    pl.stats = nullptr;
-    pl.keys = nullptr;
+    pl.stats = pl.keys = nullptr;
+    pl.count = nullptr;
     return pl;
 }
 
 template <int DT>
 hipError_t launch(const ProbsArgs& a, const ProbsPlan& pl, hipStream_t s) {
     token_logprobs_kernel<DT><<<(unsigned)(a.M * pl.slices), kProbsThreads, 0, s>>>(a, pl);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || pl.slices == 1) return e;
-    token_logprobs_join_kernel<DT><<<(unsigned)a.M, kProbsThreads, 0, s>>>(a, pl);
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t token_logprobs_workspace(const ProbsArgs& a, int cus) {
+size_t token_logprobs_workspace(const ProbsArgs& a, int cus, size_t* counters) {
     const ProbsPlan pl = make_plan(a, cus);
-    return pl.slices == 1 ? 0 : (size_t)a.M * pl.slices * (16 + 8 * (size_t)a.top);
+    *counters = pl.slices == 1 ? 0 : (size_t)a.M * sizeof(unsigned);
+    return pl.slices == 1 ? 0 : (size_t)a.M * pl.slices * (2 + (size_t)a.top) * sizeof(u64);
 }
 
-hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, hipStream_t s) {
+hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, void* counters, hipStream_t s) {
     ProbsPlan pl = make_plan(a, cus);
-    pl.stats = static_cast<float*>(ws);
-    pl.keys = reinterpret_cast<u64*>(pl.stats + (size_t)a.M * pl.slices * 4);
+    pl.stats = static_cast<u64*>(ws);
+    pl.keys = pl.stats + (size_t)a.M * pl.slices * 2;
+    pl.count = static_cast<unsigned*>(counters);
     switch (dtype) {
         case XT_F32: return launch<XT_F32>(a, pl, s);
         case XT_F16: return launch<XT_F16>(a, pl, s);
