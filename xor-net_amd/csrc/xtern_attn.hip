@@ -3,7 +3,6 @@
 #include <algorithm>
 
 #include "xtern_cache.h"
-#include "xtern_device.h"
 
 namespace xt {
 
@@ -122,15 +121,16 @@ constexpr int kAttnPlanRows = 1024;  // rows whose work is split by its total
 // sums go to slot (workgroup + row), which both grow along the line, so no two
 // segments share one and a row's slots are consecutive.
 // More than kAttnPlanRows rows: one workgroup per row.
-// The workgroup that ends a row's last segment joins them.  Segments and their
-// count are written and read at device scope, as the chip's eight L2s need it
-// (a fence would write back and drop whole caches): 131072 positions of one
-// row take 98 + 4 us in one kernel against 98 + 6.7 in two, without the second
-// launch.
+// The workgroup that ends the last of a row's segments joins them, from 32
+// segments on in two levels (groups of 32, then the groups): what one
+// workgroup can read at device scope, about 20 GB/s, bounds a join.  Segments
+// and counts are written and read at device scope, as the chip's eight L2s
+// need it (a fence would write back and drop whole caches).
 struct AttnPlan {
     float* part_o;   // [slots][hy][16][dp], unnormalised, relative to the segment's maximum
     float* part_ml;  // [slots][hy][16][2]: maximum (base 2), sum
-    unsigned* count; // [R][hy]: segments of the row done, zero between calls
+    unsigned* count; // [slots][hy]: segments of the group done that begins there; zero between calls
+    unsigned* tops;  // [R][hy]: groups of the row done; zero between calls
     float* ml;       // accumulate: maximum and sum of the whole row, [R][hq][2]
     int dp;          // D, made even
     float* s;        // accumulate: S in base 2, [R][hq][cap]
@@ -153,17 +153,6 @@ __device__ __forceinline__ int attn_len(const AttnArgs& a, int64_t r) {
     return (unsigned)sq < (unsigned)a.c.nseq ? kv_length(a.c, a.lengths[r]) : 0;
 }
 __device__ __forceinline__ int attn_steps(int len) { return max(1, (len + kAttnStep - 1) / kAttnStep); }
-
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += dpp_id<0x111, 0xf>(v);
-    v += dpp_id<0x112, 0xf>(v);
-    v += dpp_id<0x114, 0xf>(v);
-    v += dpp_id<0x118, 0xf>(v);
-    v += dpp_id<0x142, 0xa>(v);
-    v += dpp_id<0x143, 0xc>(v);
-    return v;
-}
 
 // The line as every wave of the workgroup sees it: 64 rows, a lane each, in
 // registers (no barrier), or the rows' ends in LDS.
@@ -409,60 +398,56 @@ __device__ __forceinline__ float row_lse(float m, float l) {
     return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
 }
 
-// Joins the segments of a row for the heads h0 .. h0 + nh - 1.  A wave adds up
-// one head's columns, a pair a lane, over 64 segments at a time, whose maxima
-// and sums are a lane's each; with one or two heads the waves share the
-// segments.  Bound by the latency of device-scope loads: the first segments'
-// columns are requested together with the statistics that weigh them.
+constexpr int kJoinGroup = 32;
+
+// Joins `cnt` (at most 64) segments, in every `every`-th slot from slot0, for
+// the heads h0 .. h0 + nh - 1: into the row's results (last), or into slot0.
+// A wave adds up one head's columns, a pair a lane; the segments' maxima and
+// sums are a lane's each; with one or two heads the waves share the segments.
+// Bound by the latency of device-scope loads: the first segments' columns are
+// requested together with the statistics that weigh them.
 template <int DP>
-__device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int h0, int nh,
-                               float* scratch) {
+__device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, int row, int64_t slot0, int every, int cnt,
+                               bool last, int h0, int nh, float* scratch) {
     constexpr int NK = DP > 128 ? 2 : 1, N = 16;  // pairs of a lane, segments in flight
     const int D = a.c.D, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t first = it.slot * pl.hy + blockIdx.y, step = (int64_t)pl.hy * 16 * pl.dp;
+    const int64_t first = slot0 * pl.hy + blockIdx.y, step = (int64_t)every * pl.hy * 16 * pl.dp;
     const int share = nh == 1 ? 4 : (nh == 2 ? 2 : 1), part = wave & (share - 1);
 #pragma unroll 1
     for (int hb = 0; hb < nh; hb += kAttnWaves / share) {
-        const int h = hb + wave / share;
-        float m = -INFINITY, l = 0.0f;
+        const int h = min(hb + wave / share, nh - 1);  // (a head too many: a repeat, not written)
+        float* o = pl.part_o + (first * 16 + h) * pl.dp;
+        float* ml = pl.part_ml + (first * 16 + h) * 2;
+        const float2 st = ld2_device(ml + (int64_t)min(lane, cnt - 1) * every * pl.hy * 32);
+        float m = 0.0f, l = 0.0f, fc = 0.0f;  // fc: the factor of the lane's segment
         float2 v[NK];
 #pragma unroll
         for (int k = 0; k < NK; ++k) v[k] = float2{0.0f, 0.0f};
 #pragma unroll 1
-        for (int c0 = 0; c0 < it.nc && h < nh; c0 += 64) {
-            const int cnt = min(64, it.nc - c0);
-            const float* o = pl.part_o + ((first + (int64_t)c0 * pl.hy) * 16 + h) * pl.dp;
-            const float2 ml = ld2_device(pl.part_ml + ((first + (int64_t)(c0 + min(lane, cnt - 1)) * pl.hy) * 16 + h) * 2);
-            float fc = 0.0f;  // the factor of the lane's segment
-#pragma unroll 1
-            for (int c = part; c < cnt || c == part; c += N * share) {
-                float2 x[N][NK];
+        for (int c = part; c < cnt || c == part; c += N * share) {
+            float2 x[N][NK];
 #pragma unroll
-                for (int i = 0; i < N; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-                    for (int k = 0; k < NK; ++k)
-                        if (2 * lane + 128 * k < D)
-                            x[i][k] = ld2_device(o + min(c + i * share, cnt - 1) * step + 2 * lane + 128 * k);
-                if (c == part) {
-                    const float mc = lane < cnt ? ml.x : -INFINITY, mn = fmaxf(m, wave_max(mc));
-                    const float base = mn == -INFINITY ? 0.0f : mn, f = pow2(m - base);
-                    fc = pow2(mc - base);
-                    l = l * f + wave_sum(lane < cnt ? ml.y * fc : 0.0f);
+                for (int k = 0; k < NK; ++k)
+                    if (2 * lane + 128 * k < D)
+                        x[i][k] = ld2_device(o + min(c + i * share, cnt - 1) * step + 2 * lane + 128 * k);
+            if (c == part) {
+                const float mc = lane < cnt ? st.x : -INFINITY;
+                m = wave_max(mc);
+                fc = pow2(mc - (m == -INFINITY ? 0.0f : m));
+                l = wave_sum(lane < cnt ? st.y * fc : 0.0f);
+            }
 #pragma unroll
-                    for (int k = 0; k < NK; ++k) v[k].x *= f, v[k].y *= f;
-                    m = mn;
-                }
+            for (int i = 0; i < N; ++i) {
+                const int ci = c + i * share;
+                const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fc), min(ci, 63)));
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const int ci = c + i * share;
-                    const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fc), min(ci, 63)));
-#pragma unroll
-                    for (int k = 0; k < NK; ++k)
-                        if (ci < cnt && 2 * lane + 128 * k < D) {
-                            v[k].x += f * x[i][k].x;
-                            v[k].y += f * x[i][k].y;
-                        }
-                }
+                for (int k = 0; k < NK; ++k)
+                    if (ci < cnt && 2 * lane + 128 * k < D) {
+                        v[k].x += f * x[i][k].x;
+                        v[k].y += f * x[i][k].y;
+                    }
             }
         }
         if (share > 1) {  // scratch [4][256]
@@ -481,8 +466,16 @@ __device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const Attn
                         v[k].y += scratch[(wave + w) * 256 + 2 * lane + 128 * k + 1];
                     }
         }
-        if (h >= nh || part) continue;
-        float* to = a.out + it.row * a.ldo + (int64_t)(h0 + h) * D;
+        if (hb + wave / share >= nh || part) continue;
+        if (!last) {
+            // (the wave itself has read what lay there)
+#pragma unroll
+            for (int k = 0; k < NK; ++k)
+                if (2 * lane + 128 * k < D) st2_device(o + 2 * lane + 128 * k, v[k].x, v[k].y);
+            if (lane == 0) st2_device(ml, m, l);
+            continue;
+        }
+        float* to = a.out + row * a.ldo + (int64_t)(h0 + h) * D;
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
             const int d = 2 * lane + 128 * k;
@@ -490,7 +483,7 @@ __device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const Attn
             if (d + 1 < D) to[d + 1] = l == 0.0f ? 0.0f : v[k].y / l;
         }
         if (lane == 0) {
-            const int64_t at = (int64_t)it.row * a.hq + h0 + h;
+            const int64_t at = (int64_t)row * a.hq + h0 + h;
             if (a.lse) a.lse[at] = row_lse(m, l);
             if (pl.ml) {
                 pl.ml[2 * at] = m;
@@ -498,6 +491,16 @@ __device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, const Attn
             }
         }
     }
+}
+
+// Counts one of `of` results, stored by this workgroup, and says whether it
+// was the last.  (The count wraps to zero by itself, for the next call.)
+__device__ __forceinline__ bool attention_count(unsigned* count, int of, int* lds_last) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every store has arrived
+    __syncthreads();
+    if (threadIdx.x == 0) *lds_last = atomicInc(count, (unsigned)of - 1) == (unsigned)of - 1;
+    __syncthreads();
+    return *lds_last;
 }
 
 template <int DT, int DP>
@@ -830,14 +833,16 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                     st2_device(pl.part_o + (item * 16 + h) * pl.dp + d, lds_o[h * kLdsRow + d],
                                d + 1 < D ? lds_o[h * kLdsRow + d + 1] : 0.0f);
             if (threadIdx.x < nh) st2_device(pl.part_ml + (item * 16 + n) * 2, lds_ml[0][0][n], lds_ml[0][1][n]);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every store has arrived
-            __syncthreads();
-            // (the count wraps to zero by itself, for the next call)
-            if (threadIdx.x == 0)
-                lds_last = atomicInc(pl.count + (int64_t)it.row * pl.hy + blockIdx.y, (unsigned)it.nc - 1) ==
-                           (unsigned)it.nc - 1;
-            __syncthreads();
-            if (lds_last) attention_join<DP>(a, pl, it, h0, nh, lds_o);
+            const int64_t slot = (int64_t)blockIdx.x + it.row, group = (slot - it.slot) / kJoinGroup;
+            const int groups = (it.nc + kJoinGroup - 1) / kJoinGroup;
+            const int64_t g0 = it.slot + group * kJoinGroup;
+            const int in_group = (int)min((int64_t)kJoinGroup, it.slot + it.nc - g0);
+            if (attention_count(pl.count + g0 * pl.hy + blockIdx.y, in_group, &lds_last)) {
+                attention_join<DP>(a, pl, it.row, g0, 1, in_group, groups == 1, h0, nh, lds_o);
+                if (groups > 1 &&
+                    attention_count(pl.tops + (int64_t)it.row * pl.hy + blockIdx.y, groups, &lds_last))
+                    attention_join<DP>(a, pl, it.row, it.slot, kJoinGroup, groups, true, h0, nh, lds_o);
+            }
         }
         __syncthreads();
     }
@@ -889,7 +894,7 @@ AttnPlan make_plan(const AttnArgs& a, int cus) {
     AttnPlan pl;
     const int G = a.hq / a.c.hkv;
     pl.part_o = pl.part_ml = pl.s = pl.ml = nullptr;
-    pl.count = nullptr;
+    pl.count = pl.tops = nullptr;
     pl.dp = (a.c.D + 1) / 2 * 2;
     pl.tiles = (G + 15) / 16;
     pl.hy = a.c.hkv * pl.tiles;
@@ -898,6 +903,7 @@ AttnPlan make_plan(const AttnArgs& a, int cus) {
     pl.per_row = a.R > kAttnPlanRows;
     const int64_t steps = a.R * std::max<int64_t>(1, (cap + kAttnStep - 1) / kAttnStep);
     pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident(a.c.D) * cus / pl.hy));
+    pl.shares = std::min(pl.shares, 64 * kJoinGroup);  // (as many as two levels join)
     if (pl.per_row) pl.shares = (int)a.R;
     return pl;
 }
@@ -944,7 +950,7 @@ size_t place(const AttnArgs& a, AttnPlan* pl, char* base) {
 
 size_t attention_workspace(const AttnArgs& a, int cus, size_t* counters) {
     AttnPlan pl = make_plan(a, cus);
-    *counters = splits(a, pl) ? (size_t)a.R * pl.hy * sizeof(unsigned) : 0;
+    *counters = splits(a, pl) ? ((size_t)pl.shares + 2 * (size_t)a.R) * pl.hy * sizeof(unsigned) : 0;
     return place(a, &pl, nullptr);
 }
 
@@ -952,6 +958,7 @@ hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* w
     AttnPlan pl = make_plan(a, cus);
     (void)place(a, &pl, static_cast<char*>(ws));
     pl.count = static_cast<unsigned*>(counters);
+    pl.tops = pl.count + ((size_t)pl.shares + (size_t)a.R) * pl.hy;
     hipError_t e;
     switch (dtype) {
         case XT_F32: e = launch_attention<XT_F32>(a, pl, s); break;

@@ -69,8 +69,11 @@ struct EvictArgs {
     int32_t* new_lengths;    // [nseq]
     int32_t* kept;           // [nseq][hkv][budget]
     int budget, sink, recent;
+    unsigned* keys;  // workspace (set by the launcher): [nseq][hkv][ldk]
+    int64_t ldk;
 };
-hipError_t launch_kv_evict(int dtype, const EvictArgs& a, int cus, hipStream_t s);
+size_t evict_workspace(const EvictArgs& a);
+hipError_t launch_kv_evict(int dtype, EvictArgs a, int cus, void* ws, hipStream_t s);
 
 struct ProbsArgs {
     const void* x;  // [M] rows of V logits, stride ld
@@ -99,6 +102,49 @@ inline void set_page(KvView* c, int page) {
 }
 
 #ifdef __HIPCC__
+}  // namespace xt
+#include "xtern_device.h"
+namespace xt {
+
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += dpp_id<0x111, 0xf>(v);
+    v += dpp_id<0x112, 0xf>(v);
+    v += dpp_id<0x114, 0xf>(v);
+    v += dpp_id<0x118, 0xf>(v);
+    v += dpp_id<0x142, 0xa>(v);
+    v += dpp_id<0x143, 0xc>(v);
+    return v;
+}
+
+// Counts bin `bin` of a histogram in LDS for every lane that is `in`: one add
+// for a wave whose lanes agree (a tile of equal values would otherwise add to
+// one address lane by lane).
+__device__ __forceinline__ void hist_add(int* hist, int bin, bool in) {
+    const unsigned long long who = __ballot(in);
+    if (!who) return;
+    const int first = __builtin_ctzll(who), b = __builtin_amdgcn_readlane(bin, first);
+    if (__ballot(in && bin == b) == who) {
+        if ((int)(threadIdx.x & 63) == first) atomicAdd(&hist[b], (int)__popcll(who));
+    } else if (in) {
+        atomicAdd(&hist[bin], 1);
+    }
+}
+
+// Of a 256-bin histogram in LDS, by every wave for itself: the highest bin b
+// such that bins b .. 255 hold at least `need`; *left = what b has to give.
+// One step of finding the need-th largest of many 32-bit keys, 8 bits a pass.
+__device__ __forceinline__ int radix_bin(const int* hist, int need, int* left) {
+    const int lane = threadIdx.x & 63;
+    int c[4], sum = 0;  // lane l: bins 255 - 4 l downwards
+    for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - 4 * lane - i];
+    const int upto = wave_scan(sum);
+    const int l = __builtin_ctzll(__ballot(upto >= need));
+    int before = upto - sum, i = 0;
+    while (i < 3 && before + c[i] < need) before += c[i++];
+    *left = __builtin_amdgcn_readlane(need - before, l);
+    return __builtin_amdgcn_readlane(255 - 4 * lane - i, l);
+}
 
 // One element of the cache or of the logits as f32, and back (round to
 // nearest even; f16 overflows to infinity).

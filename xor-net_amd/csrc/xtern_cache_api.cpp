@@ -235,7 +235,10 @@ int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengt
     a.recent = (int)recent;
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
-    return launched(xt::launch_kv_evict(c->dtype, a, cus, static_cast<hipStream_t>(stream)), "cache eviction launch");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    void *ws, *counters;
+    if (int rc = get_workspace(st, xt::evict_workspace(a), 0, &ws, &counters)) return rc;
+    return launched(xt::launch_kv_evict(c->dtype, a, cus, ws, st), "cache eviction launch");
 }
 
 int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int64_t V, const int32_t* tokens,

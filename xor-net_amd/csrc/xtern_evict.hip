@@ -9,7 +9,9 @@
 // Two kernels.  Selection, one workgroup per (sequence, head): the scores as
 // 32-bit keys, the need-th highest by four passes of an 8-bit histogram, then
 // the kept list in position order.  Up to 16384 positions the keys stay in
-// registers, so the scores are read once; more are read again for each pass.
+// registers; more are written to a workspace by the first pass and read back
+// by the others, which costs a few instructions a key where finding the score
+// again takes forty (90000 positions of 8 heads: 140 against 222 us).
 // Moving: HBM bounds it (every kept row is read and written once); a
 // workgroup per (sequence, head, tensor), and per part of a row where those
 // are too few for the chip.
@@ -23,7 +25,6 @@
 #include <algorithm>
 
 #include "xtern_cache.h"
-#include "xtern_device.h"
 
 namespace xt {
 
@@ -31,6 +32,7 @@ constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kEvictRegs = 16;  // keys of a thread that stay in registers
 constexpr int kMoveUnits = 4;   // 16-byte pieces of a thread and round
+constexpr int kEvictAhead = 8;  // keys of a thread in flight where they are read again
 
 __device__ __forceinline__ unsigned evict_key(const KvView& c, int seq, int h, int p) {
     const int pg = kv_page(c, seq, p);
@@ -39,31 +41,6 @@ __device__ __forceinline__ unsigned evict_key(const KvView& c, int seq, int h, i
     if (f != f) return 1u;
     const unsigned u = __float_as_uint(f);
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
-}
-
-// Inclusive sum over the wave's lanes.
-__device__ __forceinline__ int evict_scan(int v) {
-    v += dpp_id<0x111, 0xf>(v);
-    v += dpp_id<0x112, 0xf>(v);
-    v += dpp_id<0x114, 0xf>(v);
-    v += dpp_id<0x118, 0xf>(v);
-    v += dpp_id<0x142, 0xa>(v);
-    v += dpp_id<0x143, 0xc>(v);
-    return v;
-}
-
-// Of a 256-bin histogram, by every wave for itself: the highest bin b such
-// that bins b .. 255 hold at least `need`; *left = what b has to give.
-__device__ __forceinline__ int evict_bin(const int* hist, int need, int* left) {
-    const int lane = threadIdx.x & 63;
-    int c[4], sum = 0;  // lane l: bins 255 - 4 l downwards
-    for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - 4 * lane - i];
-    const int upto = evict_scan(sum);
-    const int l = __builtin_ctzll(__ballot(upto >= need));
-    int before = upto - sum, i = 0;
-    while (i < 3 && before + c[i] < need) before += c[i++];
-    *left = __builtin_amdgcn_readlane(need - before, l);
-    return __builtin_amdgcn_readlane(255 - 4 * lane - i, l);
 }
 
 __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArgs a) {
@@ -84,6 +61,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
     for (int j = t; j < a.recent; j += kEvictThreads) kept[a.budget - a.recent + j] = hi + j;
     if (need == 0) return;
     const bool regs = mid <= kEvictRegs * kEvictThreads;
+    unsigned* keys = a.keys + ((int64_t)seq * c.hkv + h) * a.ldk;  // (where they do not fit)
     unsigned key[kEvictRegs];  // position lo + 1024 i + t
 #pragma unroll
     for (int i = 0; i < kEvictRegs; ++i) {
@@ -100,22 +78,27 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
         if (regs) {
 #pragma unroll
             for (int i = 0; i < kEvictRegs; ++i)
-                if (lo + i * kEvictThreads + t < hi && (key[i] & mask) == prefix)
-                    atomicAdd(&hist[pass][(key[i] >> shift) & 255], 1);
+                hist_add(hist[pass], (key[i] >> shift) & 255,
+                         lo + i * kEvictThreads + t < hi && (key[i] & mask) == prefix);
         } else {
-            for (int p = lo + t; p < hi; p += 4 * kEvictThreads) {
-                unsigned k[4];
+            for (int p = t; p < mid; p += kEvictAhead * kEvictThreads) {
+                unsigned k[kEvictAhead];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) k[i] = evict_key(c, seq, h, min(p + i * kEvictThreads, hi - 1));
+                for (int i = 0; i < kEvictAhead; ++i) {
+                    const int q = min(p + i * kEvictThreads, mid - 1);
+                    k[i] = pass ? keys[q] : evict_key(c, seq, h, lo + q);
+                }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (p + i * kEvictThreads < hi && (k[i] & mask) == prefix)
-                        atomicAdd(&hist[pass][(k[i] >> shift) & 255], 1);
+                for (int i = 0; i < kEvictAhead; ++i) {
+                    const bool in = p + i * kEvictThreads < mid;
+                    if (in && !pass) keys[p + i * kEvictThreads] = k[i];
+                    hist_add(hist[pass], (k[i] >> shift) & 255, in && (k[i] & mask) == prefix);
+                }
             }
         }
         __syncthreads();
         int left;
-        prefix |= (unsigned)evict_bin(hist[pass], need, &left) << shift;
+        prefix |= (unsigned)radix_bin(hist[pass], need, &left) << shift;
         need = left;  // of the keys equal to the prefix so far, as many stay
     }
     // kept: keys above `prefix`, and the first `need` equal to it
@@ -138,7 +121,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
             int* cnt = count[wave] + 4 * lane;
             int v[4], sum = 0;
             for (int i = 0; i < 4; ++i) sum += v[i] = cnt[i];
-            int before = evict_scan(sum) - sum;
+            int before = wave_scan(sum) - sum;
             for (int i = 0; i < 4; ++i) {
                 cnt[i] = before;
                 before += v[i];
@@ -160,12 +143,12 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
     const int per = ((mid + kEvictWaves - 1) / kEvictWaves + 63) / 64 * 64;
     const int w0 = (int)min((int64_t)lo + (int64_t)wave * per, (int64_t)hi), w1 = min(w0 + per, hi);
     int above = 0, equal = 0;
-    for (int p = w0; p < w1; p += 256) {
-        unsigned k[4];
+    for (int p = w0; p < w1; p += 64 * kEvictAhead) {
+        unsigned k[kEvictAhead];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = evict_key(c, seq, h, min(p + 64 * i + lane, hi - 1));
+        for (int i = 0; i < kEvictAhead; ++i) k[i] = keys[min(p + 64 * i + lane, hi - 1) - lo];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kEvictAhead; ++i) {
             const bool in = p + 64 * i + lane < w1;
             above += __popcll(__ballot(in && k[i] > prefix));
             equal += __popcll(__ballot(in && k[i] == prefix));
@@ -181,12 +164,12 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
         at += count[0][w] + min(count[1][w], max(0, need - eq));
         eq += count[1][w];
     }
-    for (int p = w0; p < w1; p += 256) {
-        unsigned k[4];
+    for (int p = w0; p < w1; p += 64 * kEvictAhead) {
+        unsigned k[kEvictAhead];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = evict_key(c, seq, h, min(p + 64 * i + lane, hi - 1));
+        for (int i = 0; i < kEvictAhead; ++i) k[i] = keys[min(p + 64 * i + lane, hi - 1) - lo];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kEvictAhead; ++i) {
             const int q = p + 64 * i + lane;
             const unsigned long long me = __ballot(q < w1 && k[i] == prefix);
             const bool take = q < w1 && (k[i] > prefix || (k[i] == prefix && eq + __popcll(me & below) < need));
@@ -198,36 +181,36 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
     }
 }
 
-// Rows of `bytes` bytes in pieces of T (16 bytes; rows start anywhere, the last
+// Rows of `bytes` bytes in pieces of T, kMoveUnits a thread and round (16 bytes; rows start anywhere, the last
 // piece may overlap the one before it), pieces [u0, u1) of each; or the scores.
 template <typename T>
 __device__ __forceinline__ void move_rows(const KvView& c, int seq, char* base, int64_t sp, int64_t ss, int bytes,
                                           int u0, int u1, const int32_t* kept, int j0, int budget) {
-    const int un = u1 - u0;
-    const int64_t total = (int64_t)(budget - j0) * un;
+    // Lanes: the row's pieces, rounded up to a power of two, then rows
     typedef T U __attribute__((aligned(2)));
-    constexpr int kRound = kEvictThreads * kMoveUnits;
+    const int un = u1 - u0, lg = un > 1 ? 32 - __builtin_clz(un - 1) : 0;
+    const int u = threadIdx.x & ((1 << lg) - 1), rows = kEvictThreads >> lg, r0 = threadIdx.x >> lg;
+    const int off = min((u0 + u) * (int)sizeof(T), bytes - (int)sizeof(T));
     const char* from[kMoveUnits];
     char* to[kMoveUnits];
-    auto place = [&](int64_t i0) {
+    auto place = [&](int jr) {  // (budget < length <= 2^30)
 #pragma unroll
         for (int x = 0; x < kMoveUnits; ++x) {
-            const int64_t i = i0 + x * kEvictThreads + threadIdx.x;
+            const int j = jr + x * rows + r0;
             to[x] = nullptr;
             from[x] = base;  // (read and left, where nothing moves)
-            if (i < total) {
-                const int j = j0 + (int)(i / un), src = kept[j];
-                const int off = min((u0 + (int)(i % un)) * (int)sizeof(T), bytes - (int)sizeof(T));
+            if (j < budget && u < un) {
+                const int src = kept[j];
                 const int pf = kv_page(c, seq, src), pt = kv_page(c, seq, j);
                 if (src != j && pf >= 0 && pt >= 0) {
-                    from[x] = base + pf * sp + (kv_slot(c, src)) * ss + off;
-                    to[x] = base + pt * sp + (kv_slot(c, j)) * ss + off;
+                    from[x] = base + pf * sp + kv_slot(c, src) * ss + off;
+                    to[x] = base + pt * sp + kv_slot(c, j) * ss + off;
                 }
             }
         }
     };
-    place(0);
-    for (int64_t i0 = 0; i0 < total; i0 += kRound) {
+    place(j0);
+    for (int jr = j0; jr < budget; jr += kMoveUnits * rows) {
         T val[kMoveUnits];
         char* dst[kMoveUnits];
 #pragma unroll
@@ -235,7 +218,7 @@ __device__ __forceinline__ void move_rows(const KvView& c, int seq, char* base, 
             dst[x] = to[x];
             val[x] = __builtin_nontemporal_load(reinterpret_cast<const U*>(from[x]));
         }
-        if (i0 + kRound < total) place(i0 + kRound);  // (addresses: while the rows are on their way)
+        place(jr + kMoveUnits * rows);  // (addresses: while the rows are on their way)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every load of the round is done
         __syncthreads();
 #pragma unroll
@@ -247,7 +230,7 @@ __device__ __forceinline__ void move_rows(const KvView& c, int seq, char* base, 
 // blockIdx.y: key-value head; blockIdx.z: the parts of k's rows, of v's, the
 // scores.
 template <typename T>
-__global__ __launch_bounds__(kEvictThreads) void kv_evict_move_kernel(EvictArgs a, int es, int parts) {
+__global__ __launch_bounds__(kEvictThreads, 8) void kv_evict_move_kernel(EvictArgs a, int es, int parts) {
     const KvView& c = a.c;
     const int seq = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
     if (kv_length(c, a.lengths[seq]) <= a.budget) return;
@@ -263,7 +246,14 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_move_kernel(EvictArgs 
                  a.sink, a.budget);
 }
 
-hipError_t launch_kv_evict(int dtype, const EvictArgs& a, int cus, hipStream_t s) {
+size_t evict_workspace(const EvictArgs& a) {
+    const int64_t cap = (int64_t)a.c.max_pages * a.c.page - a.sink - a.recent;
+    return cap > kEvictRegs * kEvictThreads ? (size_t)a.c.nseq * a.c.hkv * cap * sizeof(unsigned) : 0;
+}
+
+hipError_t launch_kv_evict(int dtype, EvictArgs a, int cus, void* ws, hipStream_t s) {
+    a.keys = static_cast<unsigned*>(ws);
+    a.ldk = (int64_t)a.c.max_pages * a.c.page - a.sink - a.recent;
     const KvView& c = a.c;
     const int es = dtype == XT_F32 ? 4 : 2;
     kv_evict_select_kernel<<<dim3((unsigned)c.nseq, (unsigned)c.hkv), kEvictThreads, 0, s>>>(a);

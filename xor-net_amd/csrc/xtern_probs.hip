@@ -22,12 +22,11 @@
 // Those go to LDS, each counts how many are before it, and the first `top` in
 // that order are the list that the next tile's candidates have to beat.  Where
 // that fails (ties beyond the
-// buffer, fewer finite logits than `top`) the tile's logits are taken one
-// maximum after the other.
+// buffer, fewer finite logits than `top`) the tile is selected from by the
+// digits of its logits.
 #include <algorithm>
 
 #include "xtern_cache.h"
-#include "xtern_device.h"
 
 namespace xt {
 
@@ -140,7 +139,7 @@ struct ProbsLds {
     float sums[3][kProbsWaves];
     u64 cand[kProbsCand];
     u64 list[kProbsTop];
-    u64 wbest[kProbsWaves];
+    u64 wbest[kProbsWaves + 1];
     int count, last;
 };
 
@@ -164,32 +163,78 @@ __device__ void probs_finish(const ProbsArgs& a, int64_t r, ProbsSum s, const u6
     }
 }
 
-// The first logits of a tile and of the list before it, one maximum after
-// the other.
-template <typename Index>
-__device__ void probs_one_by_one(const float* x, Index index, int V, int valid, int top, int* have, ProbsLds& lds) {
-    // (the list before it: a lane per entry of wave 0, taken as one more logit)
-    u64 mine = (int)threadIdx.x < *have ? lds.list[threadIdx.x] : 0, last = ~(u64)0;
+// The first `top` of a tile's logits and of the list before it, whatever they
+// are: the last one's value by four passes of a histogram, then everything
+// above it, and of its equals the list's and then the lowest indices.
+template <int W, typename Index>
+__device__ void probs_select(const float* x, Index index, int V, int valid, int top, int* have, ProbsLds& lds) {
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+    const u64 mine = t < *have ? lds.list[t] : 0;  // (wave 0: an entry a lane)
+    const unsigned mine_v = (unsigned)(mine >> 32);
+    int* hist = reinterpret_cast<int*>(lds.cand);  // [4][256]
+    __syncthreads();
+    for (int i = t; i < 4 * 256; i += kProbsThreads) hist[i] = 0;
     __syncthreads();
     const int want = min(top, *have + valid);
-    for (int j = 0; j < want; ++j) {
-        u64 best = mine < last ? mine : 0;
+    int need = want;
+    unsigned value = 0;
+    auto word = [&](int i) { return (unsigned)(probs_key(x[i], 0) >> 32); };
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        const unsigned mask = pass ? ~0u << (shift + 8) : 0u;
 #pragma unroll
-        for (int i = 0; i < kProbsPer; ++i) {
-            const u64 k = index(i) < V ? probs_key(x[i], index(i)) : 0;
-            if (k < last && k > best) best = k;
-        }
-        for (int o = 32; o; o >>= 1) {
-            const u64 k = __shfl_xor(best, o);
-            best = k > best ? k : best;
-        }
-        if ((threadIdx.x & 63) == 0) lds.wbest[threadIdx.x >> 6] = best;
+        for (int i = 0; i < kProbsPer; ++i)
+            hist_add(hist + 256 * pass, (word(i) >> shift) & 255, index(i) < V && (word(i) & mask) == value);
+        if (mine && (mine_v & mask) == value) atomicAdd(&hist[256 * pass + ((mine_v >> shift) & 255)], 1);
         __syncthreads();
-        last = lds.wbest[0];
-        for (int w = 1; w < kProbsWaves; ++w) last = max(last, lds.wbest[w]);
-        if (threadIdx.x == 0) lds.list[j] = last;
-        __syncthreads();
+        int left;
+        value |= (unsigned)radix_bin(hist + 256 * pass, need, &left) << shift;
+        need = left;
     }
+    __syncthreads();
+    // `need` of the equals: the list's entries come first
+    const u64 of_list = __ballot(mine && mine_v == value);
+    if (t == 0) lds.wbest[kProbsWaves] = of_list;
+    // The tile's equals before this thread's, for each run of W indices: 16
+    // bits each, 8192 in all at most
+    u64 eq = 0;
+#pragma unroll
+    for (int i = 0; i < kProbsPer; ++i)
+        if (index(i) < V && word(i) == value) eq += (u64)1 << (16 * (i / W));
+    u64 before = eq;
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 y = __shfl_up(before, o);
+        if (lane >= o) before += y;
+    }
+    if (lane == 63) lds.wbest[wave] = before;
+    before -= eq;
+    for (int i = t; i < 96; i += kProbsThreads) lds.cand[i] = 0;
+    if (t == 0) lds.count = 0;
+    __syncthreads();
+    const u64 listed = lds.wbest[kProbsWaves];
+    u64 total = 0;
+    for (int w = 0; w < kProbsWaves; ++w) {
+        if (w < wave) before += lds.wbest[w];
+        total += lds.wbest[w];
+    }
+    const int rest = need - min(need, (int)__popcll(listed));
+    if (mine && (mine_v > value || (mine_v == value && (int)__popcll(listed & (((u64)1 << lane) - 1)) < need)))
+        lds.cand[atomicAdd(&lds.count, 1)] = mine;
+    int run = 0;  // the tile's equals before run i / W
+#pragma unroll
+    for (int i = 0; i < kProbsPer; ++i) {
+        if (i && i % W == 0) run += (int)((total >> (16 * (i / W - 1))) & 0xffff);
+        if (index(i) >= V) continue;
+        bool take = word(i) > value;
+        if (word(i) == value) {
+            take = run + (int)((before >> (16 * (i / W))) & 0xffff) < rest;
+            before += (u64)1 << (16 * (i / W));
+        }
+        if (take) lds.cand[atomicAdd(&lds.count, 1)] = probs_key(x[i], index(i));
+    }
+    __syncthreads();
+    probs_rank(lds.cand, want, top, lds.list);
+    __syncthreads();
     *have = want;
 }
 
@@ -361,7 +406,8 @@ __global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsA
         const int n = lds.count;
         dirty = min(n, kProbsCand);
         if (n > kProbsCand || n < min(a.top, have + valid) || (full && last != last)) {
-            probs_one_by_one(x, index, a.V, valid, a.top, &have, lds);
+            probs_select<R::W>(x, index, a.V, valid, a.top, &have, lds);
+            dirty = kProbsCand;
             continue;
         }
         probs_rank(lds.cand, n, a.top, lds.list);
