@@ -11,6 +11,19 @@
 
 namespace xt {
 
+// n / d for n < 2^31 as n * mul >> shift: mul = ceil(2^(31 + s) / d), shift =
+// 31 + s, 2^s >= d (d <= 65536); the error of mul, below d <= 2^s, grows to
+// less than 2^(31 + s) in the product.
+struct FastDiv {
+    unsigned mul;
+    int shift;
+};
+inline FastDiv fast_div(int d) {
+    int s = 0;
+    while ((1 << s) < d) ++s;
+    return FastDiv{(unsigned)((((uint64_t)1 << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d), 31 + s};
+}
+
 // The cache as the kernels see it: strides in elements, score
 // [num_pages][hkv][page] or null.
 struct KvView {
@@ -19,8 +32,7 @@ struct KvView {
     float* score;
     int64_t sp, ss, sh;  // element strides of a page, a slot, a head
     int num_pages, page, hkv, D;
-    unsigned page_mul;  // p / page = p * page_mul >> page_shift for p < 2^31:
-    int page_shift;     // ceil(2^(31 + s) / page) and 31 + s, 2^s >= page
+    FastDiv by_page;
     const int32_t* table;  // [nseq][max_pages], row stride ldt
     int64_t ldt;
     int nseq, max_pages;
@@ -42,8 +54,9 @@ struct AppendArgs {
     int64_t ldq, ldqo, ldk, ldv;
     int hq;
     int64_t R;
+    FastDiv by_per, by_vals;  // set by the launcher
 };
-hipError_t launch_kv_append(int dtype, const AppendArgs& a, hipStream_t s);
+hipError_t launch_kv_append(int dtype, AppendArgs a, hipStream_t s);
 
 struct AttnArgs {
     KvView c;
@@ -90,16 +103,6 @@ struct ProbsArgs {
 };
 size_t token_logprobs_workspace(const ProbsArgs& a, int cus, size_t* counters);
 hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, void* counters, hipStream_t s);
-
-// page_mul and page_shift of a page size (1 .. 65536): the error of page_mul,
-// below page <= 2^s, grows to less than 2^(31 + s) in a product with p < 2^31.
-inline void set_page(KvView* c, int page) {
-    int s = 0;
-    while ((1 << s) < page) ++s;
-    c->page = page;
-    c->page_shift = 31 + s;
-    c->page_mul = (unsigned)((((uint64_t)1 << (31 + s)) + (uint64_t)page - 1) / (uint64_t)page);
-}
 
 #ifdef __HIPCC__
 }  // namespace xt
@@ -165,9 +168,10 @@ template <> struct Elem<XT_BF16> {
     static __device__ __forceinline__ T put(float v) { return (T)v; }
 };
 
-__device__ __forceinline__ int kv_page_of(const KvView& c, int p) {
-    return (int)(((uint64_t)(unsigned)p * c.page_mul) >> c.page_shift);
+__device__ __forceinline__ int fast_quot(int n, FastDiv d) {
+    return (int)(((uint64_t)(unsigned)n * d.mul) >> d.shift);
 }
+__device__ __forceinline__ int kv_page_of(const KvView& c, int p) { return fast_quot(p, c.by_page); }
 // The page that holds position p of sequence `seq`, or -1: a table entry
 // outside the pool holds nothing.  0 <= p < max_pages * page.
 __device__ __forceinline__ int kv_page(const KvView& c, int seq, int p) {

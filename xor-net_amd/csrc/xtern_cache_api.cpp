@@ -84,7 +84,8 @@ int check_cache(const xt_kv_cache* c, const xt_kv_table* t, xt::KvView* view) {
     view->ss = c->page_size == 1 ? 0 : c->stride_slot;
     view->sh = c->kv_heads == 1 ? 0 : c->stride_head;
     view->num_pages = (int)c->num_pages;
-    xt::set_page(view, c->page_size);
+    view->page = c->page_size;
+    view->by_page = xt::fast_div(c->page_size);
     view->hkv = c->kv_heads;
     view->D = c->head_dim;
     view->table = t->pages;
