@@ -409,7 +409,7 @@ int xt_stack_destroy(xt_stack* st);
  * keys, write keys and values into the cache, attend over it, and cut a cache
  * that has grown too long down to the positions that were attended to most.
  *
- * Every call takes at most 2^22 rows or sequences.  Element types of a cache
+ * Every call takes at most 2^21 rows or sequences.  Element types of a cache
  * (and of logits): */
 enum { XT_F32 = 0, XT_F16 = 1, XT_BF16 = 2 };
 

@@ -58,7 +58,7 @@ CACHE_FAULTS = [dict(dtype=3), dict(dtype=-1), dict(kv_heads=0), dict(kv_heads=1
                 dict(num_pages=1 << 31), dict(k=None), dict(v=None), dict(k=P + 1), dict(v=P + 1), dict(score=P + 2),
                 dict(dtype=0, k=P + 2), dict(stride_slot=63), dict(stride_head=1023), dict(stride_page=2047),
                 dict(stride_page=0), dict(stride_head=0), dict(stride_page=-2048), dict(stride_page=1 << 61)]
-TABLE_FAULTS = [dict(seqs=-1), dict(seqs=1 << 31), dict(max_pages=-1), dict(max_pages=1 << 27, stride=1 << 27),
+TABLE_FAULTS = [dict(seqs=-1), dict(seqs=1 << 31), dict(seqs=(1 << 21) + 1), dict(max_pages=-1), dict(max_pages=1 << 27, stride=1 << 27),
                 dict(max_pages=1 << 62, stride=1 << 62), dict(pages=None), dict(stride=2), dict(pages=P + 1)]
 
 
@@ -72,7 +72,7 @@ def test_bad_caches_and_tables(call):
 
 
 FAULTS = [
-    (append, dict(R=-1)), (append, dict(R=1 << 31)), (append, dict(slots=None)), (append, dict(k=None)),
+    (append, dict(R=-1)), (append, dict(R=1 << 31)), (attend, dict(R=(1 << 21) + 1)), (probs, dict(M=(1 << 21) + 1)), (append, dict(slots=None)), (append, dict(k=None)),
     (append, dict(v=None)), (append, dict(qo=None)), (append, dict(ldk=127)), (append, dict(ldv=127)),
     (append, dict(ldq=255)), (append, dict(ldqo=255)), (append, dict(hq=3)), (append, dict(hq=0)),
     (append, dict(hq=1 << 16)), (append, dict(ldqo=257)), (append, dict(k=P + 2)), (append, dict(ldk=1 << 60)),
@@ -100,6 +100,13 @@ def test_bad_arguments(i):
     call, f = FAULTS[i]
     assert call(**f) == xtern.XT_ERR_INVALID, (call.__name__, f)
     assert L.xt_last_error()
+
+
+def test_workspaces_beyond_any_device():
+    """Sizes that a size_t would wrap."""
+    t = table(seqs=1 << 21, max_pages=1 << 26, stride=1 << 26)
+    assert attend(t=t, R=1 << 21, hq=2048, ldq=1 << 17, ldo=1 << 17, acc=1) == xtern.XT_ERR_NOMEM
+    assert evict(t=t) == xtern.XT_ERR_NOMEM
 
 
 def test_null_structs():

@@ -145,6 +145,17 @@ def test_attention_holes(dtype):
     attention_case(dtype, 8, 2, 64, 16, lens=[100, 40, 300, 200, 33, 64, 50], edit=edit, accumulate=True)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_attention_freed_front(dtype):
+    """The front pages of long sequences given back (a sliding window): whole
+    segments of the split hold nothing."""
+    def edit(table, lengths, pool):
+        table[0, :240] = -1
+        table[1, 10:100] = -1
+
+    attention_case(dtype, 8, 2, 64, 16, lens=[4000, 2000, 30], edit=edit, accumulate=True)
+
+
 def test_attention_rows_of_one_sequence():
     """A prompt: each token attends up to itself; rows that name no sequence."""
     for dtype in DTYPES:
@@ -178,6 +189,33 @@ def test_attention_infinities(dtype):
     out, lse = xtern.paged_attention(cache, torch.from_numpy(table).cuda(), torch.from_numpy(lengths).cuda(),
                                      q.cuda(), lse=True)
     assert bool((out == 0).all()) and bool((lse == -float("inf")).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_attention_infinities_of_a_split_row(dtype):
+    """An infinite key or value far into a long row: NaN or infinity where the
+    formula has them, the other heads and rows untouched by it."""
+    page, H, D, n = 16, 2, 64, 3000
+    rng = np.random.default_rng(8)
+    pool = Pool(rng, 2 * 188 + 2, page, H, D, dtype, score=True)
+    table = ref.tables(rng, [n, n], page, pool.P)
+    pool.fill(rng, table, [n, n])
+    q = torch.from_numpy(rng.standard_normal((2, 4, D)).astype(np.float32))
+    clean = ref.attention(pool.k, pool.v, table, page, q, [n, n], None, D ** -0.5)
+    pg, sl = int(table[0, 2500 // page]), 2500 % page
+    pool.v[pg, sl, 0, 3] = float("inf")
+    pool.k[int(table[0, 700 // page]), 700 % page, 1, :] = float("nan")
+    cache = pool.upload()
+    out, lse = xtern.paged_attention(cache, torch.from_numpy(table).cuda(), torch.tensor([n, n], dtype=torch.int32).cuda(),
+                                     q.cuda(), lse=True)
+    out, lse = out.cpu(), lse.cpu()
+    ref.close(out[1], clean[0][1], clean[3][1], "the other row")
+    ref.close(lse[1], clean[1][1], clean[4][1], "its lse")
+    rest = [d for d in range(D) if d != 3]
+    ref.close(out[0, :2][:, rest], clean[0][0, :2][:, rest], clean[3][0, :2][:, rest], "the other columns")
+    assert bool((out[0, :2, 3] == float("inf")).all())
+    ref.close(lse[0, :2], clean[1][0, :2], clean[4][0, :2], "lse")
+    assert bool(torch.isnan(out[0, 2:]).all()) and bool(torch.isnan(lse[0, 2:]).all())
 
 
 def test_attention_strided_rows():

@@ -132,9 +132,13 @@ hipError_t launch_kv_append(int dtype, AppendArgs a, hipStream_t s) {
 //   the softmax factors of a head are then the lane's own, also for O^T.
 // 16-bit caches: q and p in f32 are split into bf16 (three pieces) or f16 (two,
 // scaled by a power of two against its short range), whose products with k, v
-// the 16-bit MFMA adds up exactly in f32: the matrix cores have that to spare
-// (24 instructions of 16 cycles per 32 positions and piece-of-three against
-// 6700 cycles of HBM time).  f32 caches take the f32 MFMA.
+// the 16-bit MFMA adds up in f32: the matrix cores have that to spare (at D =
+// 128, 48 instructions of 16 cycles per 32 positions against the 6700 cycles
+// that their 16 KB take a SIMD at 6 TB/s).  f32 caches take the f32 MFMA.
+// Measured (kernel time): 64 rows of up to 8192 positions, 32 query and 8 kv
+// heads of 128, f16, 180 us (6.0 TB/s of cache); 131072 positions of one row,
+// bf16, 95 us (5.6 TB/s); 700 positions of 20 and 5 heads 11.5 us, where the
+// chain of dependent loads (lengths, table, keys, then the join's) counts.
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
@@ -362,8 +366,8 @@ struct AttnShape {
 // One chunk [p0, p1) of a row for the heads h0 .. h0 + nh - 1, in plain f32
 // operations: what the matrix cores' split operands cannot give (infinities
 // and NaN among the inputs, sums past f32's range in a piece) and head sizes
-// below one load.  256 positions at a time, one head after the other.  Writes
-// the sums as attention_item does.
+// below one load.  256 positions at a time, one head after the other; the sums
+// go where the matrix cores' would be.
 template <int DT>
 __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int hk, int h0, int nh,
                            float scale2, float* lds_o, float* lds_ml, int ldo) {
@@ -832,7 +836,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                     lt += lds_ml[w][1][n] * pow2(lds_ml[w][0][n] - (mm == -INFINITY ? 0.0f : mm));
                 lds_ml[0][0][n] = mm;
                 lds_ml[0][1][n] = lt;
-                bad = n < nh && !(fabsf(mm) < INFINITY && lt < INFINITY) && it.p1 > it.p0;
+                bad = n < nh && !(mm < INFINITY && lt < INFINITY);
             }
             for (int x = threadIdx.x; x < nh * D; x += kAttnThreads) {
                 const int h = x / D, d = x % D;
@@ -843,8 +847,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 bad |= !(fabsf(v) < INFINITY);
             }
         }
-        // Not all finite (or a tiny head): in plain operations.  (A row of holes
-        // has a maximum of -inf and comes here too.)
+        // Not all finite (or a tiny head): in plain operations.  (A segment of
+        // nothing but holes has a maximum of -inf, sums of 0, and is done.)
         if (__syncthreads_or(bad)) attn_plain<DT>(a, pl, it, hk, h0, nh, scale2, lds_o, &lds_ml[0][0][0], kLdsRow);
 
         if (it.nc == 1) {

@@ -29,7 +29,7 @@ int launched(hipError_t e, const char* what) {
 
 constexpr int64_t kMaxInt = 0x7fffffff;
 constexpr int64_t kMaxLen = (int64_t)1 << 30;  // positions of a sequence
-constexpr int64_t kMaxRows = (int64_t)1 << 22;  // rows of a call: a workgroup each
+constexpr int64_t kMaxRows = (int64_t)1 << 21;  // rows of a call: a workgroup each
 constexpr int kMaxGroup = 1024;                // query heads of a key-value head
 
 int check_dtype(int dtype) {
@@ -70,7 +70,7 @@ int check_cache(const xt_kv_cache* c, const xt_kv_table* t, xt::KvView* view) {
         if (x.stride > (INT64_MAX - span) / x.extent / 4) return bad("cache strides too large");
         span += x.stride * (x.extent - 1);
     }
-    if (t->seqs < 0 || t->seqs > kMaxRows) return bad("seqs must be 0..2^22");
+    if (t->seqs < 0 || t->seqs > kMaxRows) return bad("seqs must be 0..2^21");
     if (t->max_pages < 0 || t->max_pages > kMaxLen || t->max_pages * c->page_size > kMaxLen)
         return bad("max_pages * page_size must be 0..2^30");
     if (t->seqs > 0 && t->max_pages > 0 && !t->pages) return bad("NULL pointer");
@@ -104,13 +104,20 @@ int check_rows(const float* p, int64_t ld, int64_t R, int64_t cols, const char* 
 }
 
 int check_count(int64_t R) {
-    if (R < 0 || R > kMaxRows) return bad("row count must be 0..2^22");
+    if (R < 0 || R > kMaxRows) return bad("row count must be 0..2^21");
     return XT_OK;
 }
 
 int check_heads(int q_heads, int kv_heads) {
     if (q_heads < 1 || q_heads > 65535 || q_heads % kv_heads || q_heads / kv_heads > kMaxGroup)
         return bad("q_heads must be a multiple of kv_heads, 1..65535, at most 1024 times kv_heads");
+    return XT_OK;
+}
+
+// Workspaces that no device holds (and whose size a size_t may not).
+int check_workspace(double bytes) {
+    if (bytes > 1e13)
+        return xt_internal_fail(XT_ERR_NOMEM, "the call would need a workspace of " + std::to_string(bytes) + " bytes");
     return XT_OK;
 }
 
@@ -205,6 +212,10 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     a.ldo = ldo;
     a.lse = lse;
     a.accumulate = accumulate ? 1 : 0;
+    if (a.accumulate) {
+        const double cap = (double)t->max_pages * c->page_size + 32;
+        if (int rc = check_workspace(4.0 * (double)R * q_heads * cap)) return rc;
+    }
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -234,6 +245,7 @@ int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengt
     a.budget = (int)budget;
     a.sink = (int)sink;
     a.recent = (int)recent;
+    if (int rc = check_workspace(4.0 * (double)t->seqs * c->kv_heads * (double)t->max_pages * c->page_size)) return rc;
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
