@@ -399,6 +399,16 @@ def test_evict_long(dtype):
         evict_case(dtype, 1, 64, 32, [n], budget, min(4, budget), 0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("D,layout", [(64, "page_head_slot"), (100, "odd"), (37, "joint"), (256, "head_first")])
+def test_evict_many_rows_of_few_heads(dtype, D, layout):
+    """Thousands of kept rows: moved through a workspace where heads are few,
+    in place where they are many."""
+    log(f"evict {dtype} {D} {layout}")
+    evict_case(dtype, 1, D, 16, [6000, 4500, 4300], 4400, 7, 100, layout=layout)
+    evict_case(dtype, 2, D, 48, [5000], 4096 + 3, 3, 0, layout=layout)
+
+
 def test_evict_scores():
     """Equal scores, NaN, infinities, negative ones, holes in the table,
     lengths that the table does not hold."""

@@ -82,10 +82,13 @@ struct EvictArgs {
     int32_t* new_lengths;    // [nseq]
     int32_t* kept;           // [nseq][hkv][budget]
     int budget, sink, recent;
-    unsigned* keys;  // workspace (set by the launcher): [nseq][hkv][ldk]
+    // workspace (set by the launcher): keys [nseq][hkv][ldk], staged rows
+    unsigned* keys;
     int64_t ldk;
+    int __attribute__((ext_vector_type(4)))* stage;
+    float* stage_score;
 };
-size_t evict_workspace(const EvictArgs& a);
+size_t evict_workspace(int dtype, const EvictArgs& a, int cus);
 hipError_t launch_kv_evict(int dtype, EvictArgs a, int cus, void* ws, hipStream_t s);
 
 struct ProbsArgs {

@@ -250,7 +250,7 @@ int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengt
     if (int rc = xt_internal_cus(&cus)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     void *ws, *counters;
-    if (int rc = get_workspace(st, xt::evict_workspace(a), 0, &ws, &counters)) return rc;
+    if (int rc = get_workspace(st, xt::evict_workspace(c->dtype, a, cus), 0, &ws, &counters)) return rc;
     return launched(xt::launch_kv_evict(c->dtype, a, cus, ws, st), "cache eviction launch");
 }
 

@@ -6,15 +6,17 @@
 // position; NaN below every number, a position without a page below that).
 // They move, in order, to positions 0 .. budget - 1.
 //
-// Two kernels.  Selection, one workgroup per (sequence, head): the scores as
+// First the selection, one workgroup per (sequence, head): the scores as
 // 32-bit keys, the need-th highest by four passes of an 8-bit histogram, then
 // the kept list in position order.  Up to 16384 positions the keys stay in
 // registers; more are written to a workspace by the first pass and read back
 // by the others, which costs a few instructions a key where finding the score
 // again takes forty (90000 positions of 8 heads: 140 against 222 us).
-// Moving: HBM bounds it (every kept row is read and written once); a
+// Then the moving: HBM bounds it (every kept row is read and written once); a
 // workgroup per (sequence, head, tensor), and per part of a row where those
-// are too few for the chip.
+// are too few for the chip.  32 sequences of up to 8192 positions and 8 heads
+// of 128 in f16, cut to 2048: 17 + 95 us (4.3 TB/s moved; a large copy reaches
+// 4.8); one of 1027 positions and 5 heads cut to 512: 11 + 6 us.
 //
 // Why rows can move in place: the kept list ascends, so kept[j] >= j.  A
 // workgroup moves its part of the rows in rounds of ascending j.  A source of
@@ -246,28 +248,124 @@ __global__ __launch_bounds__(kEvictThreads, 8) void kv_evict_move_kernel(EvictAr
                  a.sink, a.budget);
 }
 
-size_t evict_workspace(const EvictArgs& a) {
-    const int64_t cap = (int64_t)a.c.max_pages * a.c.page - a.sink - a.recent;
-    return cap > kEvictRegs * kEvictThreads ? (size_t)a.c.nseq * a.c.hkv * cap * sizeof(unsigned) : 0;
+// The same through a workspace, for calls of few heads and many rows: there the
+// in-place rounds leave most of the chip idle, while here every row is copied
+// on its own, all of them out (PUT false), then all of them in.  Staged:
+// [seq][head][row][2 units pieces], and the scores.  Measured with 8 heads of
+// 128 in bf16, both kernels against in place: 1200 rows 13 against 10 us, 2500
+// 17 / 18, 5000 23 / 30, 30000 93 / 174.
+template <bool PUT>
+__global__ __launch_bounds__(256) void kv_evict_stage_kernel(EvictArgs a, int es) {
+    typedef v4i U __attribute__((aligned(2)));
+    const KvView& c = a.c;
+    const int seq = blockIdx.z, h = blockIdx.y;
+    if (kv_length(c, a.lengths[seq]) <= a.budget) return;
+    const int64_t head = (int64_t)seq * c.hkv + h;
+    const int32_t* kept = a.kept + head * a.budget;
+    const int bytes = c.D * es, units = (bytes + 15) / 16, lg = 32 - __builtin_clz(2 * units - 1);
+    const int u = threadIdx.x & ((1 << lg) - 1), rows = 256 >> lg;
+    if (u >= 2 * units) return;
+    const bool val = u >= units;
+    const int off = min((val ? u - units : u) * 16, bytes - 16);
+    char* base = static_cast<char*>(val ? c.v : c.k) + c.sh * h * es + off;
+    v4i* stage = a.stage + head * (a.budget - a.sink) * 2 * units + u;
+    float* scores = a.stage_score + head * (a.budget - a.sink);
+    const int j0 = a.sink + blockIdx.x * kMoveUnits * rows + (threadIdx.x >> lg);
+    v4i x[kMoveUnits];
+    float sc[kMoveUnits];
+    int64_t to[kMoveUnits];  // slot of the row that is written (PUT), -1: none
+#pragma unroll
+    for (int i = 0; i < kMoveUnits; ++i) {
+        const int j = j0 + i * rows;
+        to[i] = -1;
+        if (j >= a.budget) continue;
+        const int src = kept[j], pf = kv_page(c, seq, src), pt = kv_page(c, seq, j);
+        if (src == j || pf < 0 || pt < 0) continue;
+        to[i] = PUT ? pt : 0;
+        if (PUT) {
+            x[i] = stage[(int64_t)(j - a.sink) * 2 * units];
+            if (u == 0) sc[i] = scores[j - a.sink];
+        } else {
+            const int slot = kv_slot(c, src);
+            x[i] = __builtin_nontemporal_load(reinterpret_cast<const U*>(base + (pf * c.sp + slot * c.ss) * es));
+            if (u == 0) sc[i] = c.score[((int64_t)pf * c.hkv + h) * c.page + slot];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMoveUnits; ++i) {
+        const int j = j0 + i * rows;
+        if (to[i] < 0) continue;
+        if (PUT) {
+            const int slot = kv_slot(c, j);
+            *reinterpret_cast<U*>(base + (to[i] * c.sp + slot * c.ss) * es) = x[i];
+            if (u == 0) c.score[(to[i] * c.hkv + h) * c.page + slot] = sc[i];
+        } else {
+            stage[(int64_t)(j - a.sink) * 2 * units] = x[i];
+            if (u == 0) scores[j - a.sink] = sc[i];
+        }
+    }
+}
+
+namespace {
+
+struct EvictPlan {
+    size_t keys, stage, scores;  // bytes of the workspace's parts
+    int parts;                   // of a row, moved in place
+    bool moves, staged;
+};
+
+EvictPlan make_plan(int dtype, const EvictArgs& a, int cus) {
+    EvictPlan pl;
+    const int64_t cap = (int64_t)a.c.max_pages * a.c.page, mid = cap - a.sink - a.recent;
+    const int64_t heads = (int64_t)a.c.nseq * a.c.hkv, kept = a.budget - a.sink;
+    pl.keys = mid > kEvictRegs * kEvictThreads ? (size_t)(heads * mid) * sizeof(unsigned) : 0;
+    pl.keys = (pl.keys + 255) / 256 * 256;
+    pl.moves = kept > 0 && cap > a.budget;
+    // Parts of a row until two workgroups per compute unit, of four pieces at least
+    const int bytes = a.c.D * (dtype == XT_F32 ? 4 : 2), units = (bytes + 15) / 16;
+    pl.parts = bytes < 16 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(units / 4, (int64_t)cus / heads));
+    // Through the workspace where that leaves compute units without a
+    // workgroup and there are rows enough to pay for the second kernel
+    const double stage = (double)heads * kept * (32.0 * units + 4);
+    pl.staged = pl.moves && bytes >= 16 && 2 * heads * pl.parts <= cus && kept >= 4096 && stage < 4e9;
+    pl.stage = pl.staged ? (size_t)(heads * kept) * 32 * units : 0;
+    pl.scores = pl.staged ? (size_t)(heads * kept) * sizeof(float) : 0;
+    return pl;
+}
+
+}  // namespace
+
+size_t evict_workspace(int dtype, const EvictArgs& a, int cus) {
+    const EvictPlan pl = make_plan(dtype, a, cus);
+    return pl.keys + pl.stage + pl.scores;
 }
 
 hipError_t launch_kv_evict(int dtype, EvictArgs a, int cus, void* ws, hipStream_t s) {
-    a.keys = static_cast<unsigned*>(ws);
-    a.ldk = (int64_t)a.c.max_pages * a.c.page - a.sink - a.recent;
+    const EvictPlan pl = make_plan(dtype, a, cus);
     const KvView& c = a.c;
-    const int es = dtype == XT_F32 ? 4 : 2;
+    a.keys = static_cast<unsigned*>(ws);
+    a.ldk = (int64_t)c.max_pages * c.page - a.sink - a.recent;
+    a.stage = reinterpret_cast<v4i*>(static_cast<char*>(ws) + pl.keys);
+    a.stage_score = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.keys + pl.stage);
+    const int es = dtype == XT_F32 ? 4 : 2, units = (c.D * es + 15) / 16;
     kv_evict_select_kernel<<<dim3((unsigned)c.nseq, (unsigned)c.hkv), kEvictThreads, 0, s>>>(a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.sink == a.budget) return e;
-    // Parts of a row until two workgroups per compute unit, of four pieces at least
-    const int bytes = c.D * es, units = (bytes + 15) / 16;
-    const int64_t rows = (int64_t)c.nseq * c.hkv * 2;
-    const int parts = bytes < 16 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(units / 4, 2 * (int64_t)cus / rows));
-    const dim3 grid((unsigned)c.nseq, (unsigned)c.hkv, (unsigned)(2 * parts + 1));
-    if (bytes >= 16)
-        kv_evict_move_kernel<v4i><<<grid, kEvictThreads, 0, s>>>(a, es, parts);
+    if (e != hipSuccess || !pl.moves) return e;
+    if (pl.staged) {
+        int lg = 0;
+        while ((1 << lg) < 2 * units) ++lg;
+        const int rows = kMoveUnits * (256 >> lg);  // of a workgroup
+        const dim3 grid((unsigned)((a.budget - a.sink + rows - 1) / rows), (unsigned)c.hkv, (unsigned)c.nseq);
+        kv_evict_stage_kernel<false><<<grid, 256, 0, s>>>(a, es);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        kv_evict_stage_kernel<true><<<grid, 256, 0, s>>>(a, es);
+        return hipGetLastError();
+    }
+    const dim3 grid((unsigned)c.nseq, (unsigned)c.hkv, (unsigned)(2 * pl.parts + 1));
+    if (c.D * es >= 16)
+        kv_evict_move_kernel<v4i><<<grid, kEvictThreads, 0, s>>>(a, es, pl.parts);
     else
-        kv_evict_move_kernel<short><<<grid, kEvictThreads, 0, s>>>(a, es, parts);
+        kv_evict_move_kernel<short><<<grid, kEvictThreads, 0, s>>>(a, es, pl.parts);
     return hipGetLastError();
 }
 

@@ -24,6 +24,10 @@
 // that fails (ties beyond the
 // buffer, fewer finite logits than `top`) the tile is selected from by the
 // digits of its logits.
+//
+// Measured (kernel time): 1024 rows of 128256 f32 logits 83 us without
+// alternatives (6.3 TB/s), 91 / 117 us with 1 / 20; one row with 20 10.7 us,
+// where the chain of load, reduction, selection and join counts.
 #include <algorithm>
 
 #include "xtern_cache.h"
