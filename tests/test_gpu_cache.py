@@ -122,6 +122,30 @@ def test_attention_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("heads", [(1, 1, 64), (2, 1, 130), (4, 2, 255), (6, 2, 200), (17, 1, 64), (10, 5, 36)], ids=str)
+def test_attention_long_heads(dtype, heads):
+    """Rows in many segments for one, two and more query heads of a group."""
+    log(f"attention {dtype} {heads} long")
+    attention_case(dtype, *heads, page=16, lens=[9000, 140], accumulate=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_attention_row_counts(dtype):
+    """More rows than a wave has lanes, some of them split; more rows than are
+    split at all, several to a sequence."""
+    rng = np.random.default_rng(4)
+    lens = [int(x) for x in rng.integers(0, 60, 150)]
+    lens[3], lens[70], lens[149] = 3000, 1500, 2500
+    log(f"attention {dtype} 150 rows")
+    attention_case(dtype, 4, 2, 64, 16, lens=lens, accumulate=True)
+    log(f"attention {dtype} 1100 rows")
+    seq = [i % 5 for i in range(1100)]
+    attention_case(dtype, 4, 2, 64, 16, lens=[300, 20, 1, 150, 64], seq=seq,
+                   lengths=[(37 * i) % (l + 1) for i, l in enumerate([[300, 20, 1, 150, 64][b] for b in seq])],
+                   accumulate=dtype == torch.float32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 def test_attention_spread(dtype):
     """Scores hundreds apart, equal scores, a scale below zero."""
     for scale, std in ((2.0, 3.0), (0.0, 1.0), (-0.3, 1.0), (1e-3, 100.0 if dtype != torch.float16 else 50.0)):
@@ -329,6 +353,27 @@ def test_append_forms(page):
         append_case(dtype, 4, 2, 64, 64, page if page > 1 else 8, "joint", with_q=False, seed=page)
 
 
+def test_append_parts_of_wider_rows():
+    """q, k and v as columns of one fused tensor, q rotated where it lies."""
+    rng = np.random.default_rng(9)
+    hq, H, D, page = 4, 2, 64, 16
+    for dtype in DTYPES:
+        fused = torch.from_numpy(rng.standard_normal((5, (hq + 2 * H) * D + 3)).astype(np.float32)).cuda()
+        q, k, v = (fused[:, a * D + 1:b * D + 1] for a, b in ((0, hq), (hq, hq + H), (hq + H, hq + 2 * H)))
+        table = torch.arange(10, dtype=torch.int32, device="cuda").reshape(5, 2)
+        slots = torch.tensor([0, 31, 16, 15, -1], dtype=torch.int32, device="cuda")
+        ang = torch.rand((40, D // 2), device="cuda")
+        rope = (ang.cos().contiguous(), ang.sin().contiguous())
+        a, b = (xtern.KvCache.new(10, page, H, D, dtype=dtype) for _ in range(2))
+        want = xtern.kv_append(a, table, slots, k.contiguous(), v.contiguous(), q=q.contiguous(), rope=rope,
+                               q_out=q.contiguous().clone())
+        before = fused.clone()
+        xtern.kv_append(b, table, slots, k, v, q=q, rope=rope, q_out=q)
+        assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v) and torch.equal(q, want)
+        before[:, 1:hq * D + 1] = q
+        assert torch.equal(before, fused)
+
+
 def test_append_special_values():
     """Overflow to infinity, subnormals, ties to even, NaN."""
     vals = torch.tensor([65519.0, 65520.0, 1e38, -1e38, 3.4e38, 1e-8, -6e-8, 5.9e-8, 1 + 2 ** -8, 1 + 3 * 2 ** -8,
@@ -407,6 +452,14 @@ def test_evict_many_rows_of_few_heads(dtype, D, layout):
     log(f"evict {dtype} {D} {layout}")
     evict_case(dtype, 1, D, 16, [6000, 4500, 4300], 4400, 7, 100, layout=layout)
     evict_case(dtype, 2, D, 48, [5000], 4096 + 3, 3, 0, layout=layout)
+
+
+def test_evict_budgets_and_lengths():
+    """Budgets above the table's capacity; several long sequences whose keys
+    go through the workspace."""
+    evict_case(torch.bfloat16, 2, 32, 16, [100, 50], 5000, 3, 4)
+    evict_case(torch.float16, 2, 8, 16, [17000, 20000, 300], 400, 2, 5)
+    evict_case(torch.float16, 1, 4, 16, [17000, 20000], 16700, 0, 5)  # (rows below one piece)
 
 
 def test_evict_scores():

@@ -65,6 +65,15 @@ def test_row_counts(dtype, M):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_slices_of_several_tiles(dtype):
+    """Enough rows that a row has few slices, each of several tiles."""
+    rng = np.random.default_rng(5)
+    for M, V, top in ((400, 40000, 20), (130, 70001, 64), (1030, 17000, 1)):
+        log(f"logprobs {dtype} M={M} V={V} top={top}")
+        case(rows(rng, M, V, dtype), toks(rng, M, 2, V), top)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("std", [0.0, 1e-3, 30.0, 3000.0])
 def test_spread(dtype, std):
     """All logits equal (every alternative a tie), almost equal, far apart."""
@@ -159,6 +168,13 @@ def test_nan_and_infinity():
         assert ids[3].tolist() == [0, 1]
         y = torch.full((1, 3), float("nan"), dtype=dtype, device="cuda")
         assert xtern.token_logprobs(y, top=3)[2].tolist() == [[0, 1, 2]]
+
+
+def test_no_tokens():
+    x = torch.zeros((2, 64), device="cuda")
+    lp, H, ids, tlp = xtern.token_logprobs(x, torch.zeros((2, 0), dtype=torch.int32, device="cuda"), top=64)
+    assert lp.shape == (2, 0) and ids.tolist() == [list(range(64))] * 2
+    ref.close(tlp, torch.full((2, 64), -np.log(64.0), dtype=torch.float64), torch.full((2, 64), 8 * ref.EPS * np.log(64.0)), "uniform")
 
 
 def test_no_rows():

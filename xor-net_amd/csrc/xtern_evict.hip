@@ -64,11 +64,13 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
     if (need == 0) return;
     const bool regs = mid <= kEvictRegs * kEvictThreads;
     unsigned* keys = a.keys + ((int64_t)seq * c.hkv + h) * a.ldk;  // (where they do not fit)
+    const int used = regs ? (mid + kEvictThreads - 1) / kEvictThreads : 0;  // registers in use
     unsigned key[kEvictRegs];  // position lo + 1024 i + t
 #pragma unroll
     for (int i = 0; i < kEvictRegs; ++i) {
         const int p = lo + i * kEvictThreads + t;
-        key[i] = regs && p < hi ? evict_key(c, seq, h, p) : 0u;
+        key[i] = 0u;
+        if (i < used && p < hi) key[i] = evict_key(c, seq, h, p);
     }
     if (t < 256)
         for (int i = 0; i < 4; ++i) hist[i][t] = 0;
@@ -80,8 +82,9 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
         if (regs) {
 #pragma unroll
             for (int i = 0; i < kEvictRegs; ++i)
-                hist_add(hist[pass], (key[i] >> shift) & 255,
-                         lo + i * kEvictThreads + t < hi && (key[i] & mask) == prefix);
+                if (i < used)
+                    hist_add(hist[pass], (key[i] >> shift) & 255,
+                             lo + i * kEvictThreads + t < hi && (key[i] & mask) == prefix);
         } else {
             for (int p = t; p < mid; p += kEvictAhead * kEvictThreads) {
                 unsigned k[kEvictAhead];
@@ -109,6 +112,10 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
     if (regs) {
 #pragma unroll
         for (int i = 0; i < kEvictRegs; ++i) {
+            if (i >= used) {
+                if (lane == 0) count[0][i * kEvictWaves + wave] = count[1][i * kEvictWaves + wave] = 0;
+                continue;
+            }
             const bool in = lo + i * kEvictThreads + t < hi;
             const int above = __popcll(__ballot(in && key[i] > prefix));
             const int equal = __popcll(__ballot(in && key[i] == prefix));
@@ -132,6 +139,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kEvictRegs; ++i) {
+            if (i >= used) continue;
             const int p = lo + i * kEvictThreads + t;
             const int eq = count[1][i * kEvictWaves + wave];
             const unsigned long long me = __ballot(p < hi && key[i] == prefix);

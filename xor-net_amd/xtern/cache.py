@@ -98,6 +98,14 @@ def _head_rows(t, what, D, here, R=None, heads=None):
     """(address, row stride, heads) of float32 rows [R, heads * D] or [R,
     heads, D] whose elements lie side by side; rows may be any distance
     apart."""
+    try:
+        if t.dtype is _F32 and t.get_device() == here and t.is_contiguous():
+            s = t.shape
+            n = s[1] if len(s) == 3 and s[2] == D else (s[1] // D if len(s) == 2 and not s[1] % D else 0)
+            if n and (R is None or s[0] == R) and (heads is None or n == heads):
+                return t.data_ptr(), n * D, n
+    except AttributeError:
+        pass
     p = _ptr(t, _F32, what, here)
     s = t.shape
     if len(s) == 3:
