@@ -9,14 +9,14 @@
 // First the selection, one workgroup per (sequence, head): the scores as
 // 32-bit keys, the need-th highest by four passes of an 8-bit histogram, then
 // the kept list in position order.  Up to 16384 positions the keys stay in
-// registers; more are written to a workspace by the first pass and read back
-// by the others, which costs a few instructions a key where finding the score
-// again takes forty (90000 positions of 8 heads: 140 against 222 us).
+// registers; for more, a kernel of its own writes them to a workspace first
+// (finding a score takes forty instructions, reading a key a few: 40000
+// positions of 8 heads 8 + 48 us, 80 with the selecting workgroup finding its own).
 // Then the moving: HBM bounds it (every kept row is read and written once); a
 // workgroup per (sequence, head, tensor), and per part of a row where those
 // are too few for the chip.  32 sequences of up to 8192 positions and 8 heads
 // of 128 in f16, cut to 2048: 17 + 95 us (4.3 TB/s moved; a large copy reaches
-// 4.8); one of 1027 positions and 5 heads cut to 512: 11 + 6 us.
+// 4.8); one of 1027 positions and 5 heads cut to 512: 9 + 6 us.
 //
 // Why rows can move in place: the kept list ascends, so kept[j] >= j.  A
 // workgroup moves its part of the rows in rounds of ascending j.  A source of
@@ -34,7 +34,8 @@ constexpr int kEvictThreads = 1024;
 constexpr int kEvictWaves = kEvictThreads / 64;
 constexpr int kEvictRegs = 16;  // keys of a thread that stay in registers
 constexpr int kMoveUnits = 4;   // 16-byte pieces of a thread and round
-constexpr int kEvictAhead = 8;  // keys of a thread in flight where they are read again
+constexpr int kEvictAhead = 8;  // keys of a thread in flight where they go through memory
+constexpr int kEvictTile = 256 * kEvictAhead;
 
 __device__ __forceinline__ unsigned evict_key(const KvView& c, int seq, int h, int p) {
     const int pg = kv_page(c, seq, p);
@@ -43,6 +44,25 @@ __device__ __forceinline__ unsigned evict_key(const KvView& c, int seq, int h, i
     if (f != f) return 1u;
     const unsigned u = __float_as_uint(f);
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+
+// Keys of the positions between, to the workspace, by the whole chip: for
+// calls whose heads may have more than a workgroup's registers hold.
+__global__ __launch_bounds__(256) void kv_evict_keys_kernel(EvictArgs a) {
+    const KvView& c = a.c;
+    const int seq = blockIdx.x, h = blockIdx.y, n = kv_length(c, a.lengths[seq]);
+    const int mid = n - a.recent - a.sink;
+    if (n <= a.budget || mid <= kEvictRegs * kEvictThreads) return;
+    unsigned* keys = a.keys + ((int64_t)seq * c.hkv + h) * a.ldk;
+    for (int64_t p0 = (int64_t)blockIdx.z * kEvictTile + threadIdx.x; p0 < mid; p0 += (int64_t)gridDim.z * kEvictTile) {
+        unsigned k[kEvictAhead];
+#pragma unroll
+        for (int i = 0; i < kEvictAhead; ++i)
+            k[i] = evict_key(c, seq, h, a.sink + (int)min(p0 + 256 * i, (int64_t)mid - 1));
+#pragma unroll
+        for (int i = 0; i < kEvictAhead; ++i)
+            if (p0 + 256 * i < mid) keys[p0 + 256 * i] = k[i];
+    }
 }
 
 __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArgs a) {
@@ -89,14 +109,10 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
             for (int p = t; p < mid; p += kEvictAhead * kEvictThreads) {
                 unsigned k[kEvictAhead];
 #pragma unroll
-                for (int i = 0; i < kEvictAhead; ++i) {
-                    const int q = min(p + i * kEvictThreads, mid - 1);
-                    k[i] = pass ? keys[q] : evict_key(c, seq, h, lo + q);
-                }
+                for (int i = 0; i < kEvictAhead; ++i) k[i] = keys[min(p + i * kEvictThreads, mid - 1)];
 #pragma unroll
                 for (int i = 0; i < kEvictAhead; ++i) {
                     const bool in = p + i * kEvictThreads < mid;
-                    if (in && !pass) keys[p + i * kEvictThreads] = k[i];
                     hist_add(hist[pass], (k[i] >> shift) & 255, in && (k[i] & mask) == prefix);
                 }
             }
@@ -356,9 +372,14 @@ hipError_t launch_kv_evict(int dtype, EvictArgs a, int cus, void* ws, hipStream_
     a.stage = reinterpret_cast<v4i*>(static_cast<char*>(ws) + pl.keys);
     a.stage_score = reinterpret_cast<float*>(static_cast<char*>(ws) + pl.keys + pl.stage);
     const int es = dtype == XT_F32 ? 4 : 2, units = (c.D * es + 15) / 16;
+    hipError_t e;
+    if (pl.keys) {
+        const int64_t tiles = std::min<int64_t>((a.ldk + kEvictTile - 1) / kEvictTile, 65535);
+        kv_evict_keys_kernel<<<dim3((unsigned)c.nseq, (unsigned)c.hkv, (unsigned)tiles), 256, 0, s>>>(a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     kv_evict_select_kernel<<<dim3((unsigned)c.nseq, (unsigned)c.hkv), kEvictThreads, 0, s>>>(a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !pl.moves) return e;
+    if ((e = hipGetLastError()) != hipSuccess || !pl.moves) return e;
     if (pl.staged) {
         int lg = 0;
         while ((1 << lg) < 2 * units) ++lg;
