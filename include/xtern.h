@@ -481,8 +481,8 @@ int xt_kv_append(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
  * [R][q_heads * head_dim] f32 reads key-value head h / (q_heads / kv_heads)
  * (at most 1024 query heads each),
  *   s_j = scale q.k_j,  out = sum_j softmax(s)_j v_j,  lse = ln sum_j exp(s_j)
- * out [R][q_heads * head_dim] f32, lse (may be NULL) [R][q_heads].  A row
- * without positions (or whose every s_j is -inf) gives zeros and lse = -inf.
+ * out [R][q_heads * head_dim] f32, which may be q, lse (may be NULL)
+ * [R][q_heads].  A row without positions (or whose every s_j is -inf) gives zeros and lse = -inf.
  * accumulate != 0 adds to the score of each position and key-value head the
  * weight that its group's query heads gave it, sum_h softmax(s_h)_j (atomic
  * adds: the sum over rows that share a page is in no fixed order).  Rows are

@@ -91,7 +91,7 @@ FAULTS = [
     (probs, dict(T=-1)), (probs, dict(T=1 << 21)), (probs, dict(top=-1)), (probs, dict(top=65)),
     (probs, dict(V=2, top=3)), (probs, dict(x=None)), (probs, dict(H=None)), (probs, dict(tokens=None)),
     (probs, dict(lp=None)), (probs, dict(ids=None)), (probs, dict(tlp=None)), (probs, dict(ld=99)),
-    (probs, dict(ld=1 << 62)), (probs, dict(x=P + 2)), (probs, dict(dtype=1, x=P + 1)),
+    (probs, dict(ld=1 << 62)), (probs, dict(x=P + 2)), (probs, dict(dtype=1, x=P + 1)), (attend, dict(ldo=257)),
 ]
 
 

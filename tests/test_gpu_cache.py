@@ -261,6 +261,31 @@ def test_attention_strided_rows():
     assert bool((res[:, :2] == 7).all()) and bool((res[:, -1] == 7).all())
 
 
+def test_attention_in_place():
+    """out = q: whole rows, rows in parts, rows in plain operations (a tiny
+    head; infinite values), many rows, columns of a wider tensor."""
+    g = torch.Generator().manual_seed(11)
+    for dtype in DTYPES:
+        for hq, H, D, R, length in ((8, 2, 128, 3, 90), (20, 1, 64, 2, 9000), (4, 2, 3, 5, 300), (4, 4, 256, 300, 40)):
+            pages = -(-length // 16)
+            c = xtern.KvCache.new(pages, 16, H, D, dtype=dtype, score=True)
+            c.k.copy_(torch.randn(c.k.shape, generator=g))
+            c.v.copy_(torch.randn(c.v.shape, generator=g))
+            c.v[0, 3, 0, 0] = float("inf")
+            table = torch.arange(pages, dtype=torch.int32, device="cuda").reshape(1, pages)
+            seq = torch.zeros(R, dtype=torch.int32, device="cuda")
+            lengths = torch.randint(0, length + 1, (R,), generator=g, dtype=torch.int32).cuda()
+            lengths[0] = length
+            wide = torch.randn((R, hq * D + 5), generator=g).cuda()
+            q = wide[:, 2:hq * D + 2]
+            want, lse = xtern.paged_attention(c, table, lengths, q.clone(), seq=seq, lse=True)
+            edge = wide.clone()
+            got, lse2 = xtern.paged_attention(c, table, lengths, q, seq=seq, lse=True, out=q, accumulate=True)
+            assert got is q and same_bits(got, want) and same_bits(lse, lse2), (dtype, D)
+            edge[:, 2:hq * D + 2] = want
+            assert same_bits(wide, edge)
+
+
 def test_attention_empty_calls():
     cache = xtern.KvCache.new(4, 16, 2, 64)
     i32 = dict(dtype=torch.int32, device="cuda")

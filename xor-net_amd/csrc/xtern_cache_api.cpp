@@ -201,6 +201,9 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     if (int rc = check_rows(q, ldq, R, cols, "q")) return rc;
     if (int rc = check_rows(out, ldo, R, cols, "out")) return rc;
     if (int rc = check_align(lse, 4, "lse")) return rc;
+    // (in place is fine: the workgroups that read a row's head have read it
+    // before the one that writes it does)
+    if (q == out && ldq != ldo && R > 1) return bad("out overlaps q at another stride");
     a.seq = seq;
     a.lengths = lengths;
     a.q = q;

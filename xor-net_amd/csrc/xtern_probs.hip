@@ -21,9 +21,8 @@
 // eight waves is by `top` of the tile's, and by hardly more than twice as many.
 // Those go to LDS, each counts how many are before it, and the first `top` in
 // that order are the list that the next tile's candidates have to beat.  Where
-// that fails (ties beyond the
-// buffer, fewer finite logits than `top`) the tile is selected from by the
-// digits of its logits.
+// that fails (ties beyond the buffer, fewer finite logits than `top`) the tile
+// is selected from by the digits of its logits.
 //
 // Measured (kernel time): 1024 rows of 128256 f32 logits 83 us without
 // alternatives (6.3 TB/s), 91 / 117 us with 1 / 20; one row with 20 10.7 us,
@@ -313,8 +312,7 @@ __global__ __launch_bounds__(kProbsThreads, 4) void token_logprobs_kernel(ProbsA
     const int slice = blockIdx.x % pl.slices;
     const T* row = static_cast<const T*>(a.x) + r * a.ld;
     const int t0 = slice * pl.per, t1 = min(t0 + pl.per, pl.tiles);
-    // groups of the selection: the smallest power of two that holds `top`
-    int have = 0, dirty = kProbsCand;
+    int have = 0, dirty = kProbsCand;  // entries of the list; of the buffer, to be cleared
     const int quota = (a.top + kProbsWaves - 1) / kProbsWaves;
     ProbsSum s{-INFINITY, 0.0f, 0.0f, 0.0f};
     R next;

@@ -248,8 +248,8 @@ def paged_attention(cache, table, lengths, q, seq=None, scale=None, lse=False, a
     """xt_paged_attention: row r of q (float32 [R, q_heads, head_dim] or [R,
     q_heads * head_dim]) attends over the first lengths[r] (int32 [R])
     positions of sequence seq[r] (default r) of table (int32 [seqs,
-    max_pages]).  scale defaults to head_dim ** -0.5.  Returns out, shaped as
-    q, or (out, lse [R, q_heads]) with lse=True; accumulate=True adds the
+    max_pages]).  scale defaults to head_dim ** -0.5.  Returns out (which may
+    be q), shaped as q, or (out, lse [R, q_heads]) with lse=True; accumulate=True adds the
     weights to cache.score."""
     here, D = _here(), cache.head_dim
     c = cache._on(here)
