@@ -487,6 +487,40 @@ def test_evict_budgets_and_lengths():
     evict_case(torch.float16, 1, 4, 16, [17000, 20000], 16700, 0, 5)  # (rows below one piece)
 
 
+def test_evict_largest_budget():
+    """A list of 2^31 - 1 entries, none of it past its end."""
+    c = xtern.KvCache.new(4, 16, 1, 8, score=True)
+    c.k.copy_(torch.randn(c.k.shape))
+    before = c.k.clone()
+    table = torch.arange(4, dtype=torch.int32, device="cuda").reshape(1, 4)
+    lengths = torch.tensor([50], dtype=torch.int32, device="cuda")
+    new, kept = xtern.kv_evict(c, table, lengths, 2 ** 31 - 1, sink=2 ** 30, recent=2 ** 30 - 1)
+    assert new.tolist() == [50] and kept[0, 0, :50].tolist() == list(range(50))
+    assert int(kept[0, 0, 50:].max()) == -1 and int(kept[0, 0, 50:].min()) == -1
+    assert torch.equal(c.k, before)
+    del kept
+    torch.cuda.empty_cache()
+
+
+def test_evict_more_sequences_than_a_grid_side():
+    """70000 sequences, the last one long: as in a call of its own."""
+    S, page = 70000, 16500
+    k, v = (torch.randn((2, page, 1, 8)).half().cuda() for _ in range(2))
+    score = torch.rand((2, 1, page)).cuda()
+    one, many = (xtern.KvCache(k.clone(), v.clone(), score.clone()) for _ in range(2))
+    table = torch.full((S, 1), -1, dtype=torch.int32, device="cuda")
+    table[-1] = 1
+    lengths = torch.arange(S, dtype=torch.int32, device="cuda") % 9
+    lengths[-1] = page
+    new, kept = xtern.kv_evict(many, table, lengths, 40, sink=2, recent=3)
+    new1, kept1 = xtern.kv_evict(one, table[-1:], lengths[-1:], 40, sink=2, recent=3)
+    assert torch.equal(new[:-1], lengths[:-1]) and int(new[-1]) == int(new1[0]) == 40
+    assert torch.equal(kept[-1:], kept1) and int(kept1.min()) == 0
+    assert torch.equal(one.k, many.k) and torch.equal(one.v, many.v) and torch.equal(one.score, many.score)
+    want = torch.where(torch.arange(40, device="cuda") < lengths[:-1, None], torch.arange(40, device="cuda"), -1)
+    assert torch.equal(kept[:-1, 0], want.int())
+
+
 def test_evict_scores():
     """Equal scores, NaN, infinities, negative ones, holes in the table,
     lengths that the table does not hold."""

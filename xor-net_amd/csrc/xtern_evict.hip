@@ -74,7 +74,8 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictArg
     int32_t* kept = a.kept + ((int64_t)seq * c.hkv + h) * a.budget;
     if (h == 0 && t == 0) a.new_lengths[seq] = min(n, a.budget);
     if (n <= a.budget) {
-        for (int j = t; j < a.budget; j += kEvictThreads) kept[j] = j < n ? j : -1;
+        for (unsigned j = t; j < (unsigned)a.budget; j += kEvictThreads)  // (up to 2^31 - 1)
+            kept[j] = (int)j < n ? (int)j : -1;
         return;
     }
     const int lo = a.sink, hi = n - a.recent, mid = hi - lo;  // the positions between
