@@ -29,17 +29,11 @@ ROPE_BASE = 10000.0
 
 
 def _xtern():
-    """The package, imported by the first call that needs it (as a program
-    does once, not on every call)."""
-    global _package
-    if _package is None:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xor-net_amd"))
-        import xtern
-        _package = xtern
-    return _package
-
-
-_package = None
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xor-net_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import xtern
+    return xtern
 
 
 # --- the cases -------------------------------------------------------------
