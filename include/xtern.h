@@ -497,13 +497,17 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
 /* Cut every sequence b of the table that holds lengths[b] > budget positions
  * down to budget, for each key-value head by its own scores: the first sink
  * and the last recent positions stay, and of those between the ones of the
- * highest score (ties to the lowest position; NaN below every number,
- * positions without a page last).  What stays moves, in order, to positions
- * 0..budget - 1 with its score; later positions keep their old contents.
- * new_lengths[b] = min(lengths[b], budget) (another array than lengths);
- * kept [seqs][kv_heads][budget] receives the old position of each that
- * stayed, -1 past the new length.  sink + recent <= budget.  No page may
- * belong to two positions of the table. */
+ * highest score (ties to the lowest position; NaN below every number).  What
+ * stays moves, in order, to positions 0..budget - 1 with its score; later
+ * positions keep their old contents.  new_lengths[b] = min(lengths[b], budget)
+ * (another array than lengths); kept [seqs][kv_heads][budget] receives the old
+ * position of each that stayed, -1 behind the last.
+ * Positions without a page hold nothing and do not count: in a sequence that
+ * is cut, sink, recent and budget count the positions that have one, what
+ * stays moves to the first of those, and new_lengths[b] ends behind the last
+ * that it took (more than budget where a page before it is missing; a sequence
+ * with at most budget positions left keeps them all where they are).
+ * sink + recent <= budget.  No page may belong to two positions of the table. */
 int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengths,
                 int64_t budget, int64_t sink, int64_t recent, int32_t* new_lengths,
                 int32_t* kept, void* stream);

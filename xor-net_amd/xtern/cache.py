@@ -278,9 +278,10 @@ def kv_evict(cache, table, lengths, budget, sink=0, recent=0, stream=None):
     """xt_kv_evict: every sequence of table with lengths[b] (int32 [seqs]) >
     budget is cut down to budget positions per key-value head, the first
     `sink`, the last `recent` and those of the highest cache.score between
-    them, moved in order to the front of its pages.  Returns (new lengths
-    [seqs], kept [seqs, kv_heads, budget]: each one's old position, -1 past
-    the new length)."""
+    them, moved in order to the front of its pages.  Positions without a page
+    do not count and are not moved to.  Returns (new lengths [seqs], up to the
+    last position in use; kept [seqs, kv_heads, budget]: the old position of
+    each that stayed, then -1)."""
     here = _here()
     c = cache._on(here)
     t, S = _table(table, here)
