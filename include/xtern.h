@@ -475,6 +475,16 @@ int xt_kv_append(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
                  const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t R,
                  void* stream);
 
+/* xt_kv_append that also says how many positions each new token sees:
+ * lengths [R] (an array of its own) receives slots[r] + 1, or 0 for a row that
+ * was skipped.  These are the lengths for xt_paged_attention: a skipped row's
+ * slot holds some other token, or nothing, and its query is not rotated. */
+int xt_kv_append_lengths(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
+                         const int32_t* slots, const int32_t* positions, const xt_rope* rope,
+                         const float* q, int64_t ldq, int q_heads, float* q_out, int64_t ldqo,
+                         const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t R,
+                         int32_t* lengths, void* stream);
+
 /* Attention of one token per row r over the first lengths[r] positions of
  * sequence seq[r] (seq NULL: sequence r; several rows may name one sequence,
  * e.g. the tokens of a prompt with growing lengths): query head h of q

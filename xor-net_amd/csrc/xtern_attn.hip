@@ -36,9 +36,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     const int slot = a.slots[r];
     const int sq = a.seq ? a.seq[r] : (int)r;
     const int pos = a.cos ? a.pos[r] : 0;
-    if (slot < 0 || slot >= (int64_t)c.max_pages * c.page || (unsigned)sq >= (unsigned)c.nseq) return;
-    if (a.cos && (pos < 0 || pos >= a.rope_rows)) return;
-    const int pg = kv_page(c, sq, slot);
+    int pg = -1;
+    if (slot >= 0 && slot < (int64_t)c.max_pages * c.page && (unsigned)sq < (unsigned)c.nseq &&
+        (!a.cos || (pos >= 0 && pos < a.rope_rows)))
+        pg = kv_page(c, sq, slot);
+    if (a.lengths && threadIdx.x == 0) a.lengths[r] = pg < 0 ? 0 : slot + 1;
     if (pg < 0) return;
     const int half = a.cos ? a.rot / 2 : 0, per = (c.D - half) / W;  // work items of one rotated head
     const int nq = (a.q ? a.hq : 0) * per, nk = c.hkv * per, vals = c.D / W, nv = c.hkv * vals;

@@ -51,6 +51,7 @@ struct AppendArgs {
     float* qo;
     const float* k;
     const float* v;
+    int32_t* lengths;      // [R] or null: positions that the row's token sees, 0 for a skipped row
     int64_t ldq, ldqo, ldk, ldv;
     int hq;
     int64_t R;

@@ -138,6 +138,14 @@ int xt_kv_append(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
                  const int32_t* positions, const xt_rope* rope, const float* q, int64_t ldq, int q_heads,
                  float* q_out, int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv,
                  int64_t R, void* stream) {
+    return xt_kv_append_lengths(c, t, seq, slots, positions, rope, q, ldq, q_heads, q_out, ldqo, k, ldk, v, ldv, R,
+                                nullptr, stream);
+}
+
+int xt_kv_append_lengths(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq, const int32_t* slots,
+                         const int32_t* positions, const xt_rope* rope, const float* q, int64_t ldq, int q_heads,
+                         float* q_out, int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv,
+                         int64_t R, int32_t* lengths, void* stream) {
     xt::AppendArgs a;
     memset(&a, 0, sizeof a);
     if (int rc = check_cache(c, t, &a.c)) return rc;
@@ -163,6 +171,10 @@ int xt_kv_append(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
         if (int rc = check_rows(q_out, ldqo, R, q_heads * D, "q_out")) return rc;
         if (q == q_out && ldq != ldqo && R > 1) return bad("q_out overlaps q at another stride");
     }
+    if (int rc = check_align(lengths, 4, "lengths")) return rc;
+    if (lengths && (lengths == slots || lengths == seq || lengths == positions))
+        return bad("lengths must not be slots, seq or positions");
+    a.lengths = lengths;
     a.seq = seq;
     a.slots = slots;
     a.pos = positions ? positions : slots;

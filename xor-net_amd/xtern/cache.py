@@ -32,6 +32,7 @@ class _Rope(ctypes.Structure):
 _cache_p, _table_p, _rope_p = (ctypes.POINTER(t) for t in (_KvCache, _KvTable, _Rope))
 _lib.xt_kv_append.argtypes = [_cache_p, _table_p, _vp, _vp, _vp, _rope_p, _vp, _i64, ctypes.c_int, _vp, _i64,
                               _vp, _i64, _vp, _i64, _i64, _vp]
+_lib.xt_kv_append_lengths.argtypes = _lib.xt_kv_append.argtypes[:-1] + [_vp, _vp]
 _lib.xt_paged_attention.argtypes = [_cache_p, _table_p, _vp, _vp, _vp, _i64, ctypes.c_int, ctypes.c_float, _i64,
                                     _vp, _i64, _vp, ctypes.c_int, _vp]
 _lib.xt_kv_evict.argtypes = [_cache_p, _table_p, _vp, _i64, _i64, _i64, _vp, _vp, _vp]
@@ -200,13 +201,15 @@ def _table(table, here):
     return ctypes.byref(_KvTable(p, table.stride(0), s[0], s[1])), s[0]
 
 
-def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=None, q_out=None, stream=None):
+def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=None, q_out=None, stream=None,
+              lengths=None):
     """xt_kv_append: R new tokens' k and v (float32 [R, kv_heads, head_dim] or
     [R, kv_heads * head_dim]) into position slots[r] (int32 [R]; -1 skips the
     row) of sequence seq[r] (default r) of table (int32 [seqs, max_pages]).
     rope = (cos, sin), float32 [rows, dim / 2] each, rotates k and q by row
-    positions[r] (default slots[r]).  Returns the rotated q (q_out if given,
-    which may be q), or None without q."""
+    positions[r] (default slots[r]).  lengths (int32 [R], if given) receives
+    what each token sees, slots[r] + 1, or 0 for a row that was skipped.
+    Returns the rotated q (q_out if given, which may be q), or None without q."""
     here, D = _here(), cache.head_dim
     c = cache._on(here)
     t, S = _table(table, here)
@@ -221,6 +224,7 @@ def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=
     else:
         np_ = None
     pp = _vec(positions, _I32, "positions", (R,), here) if positions is not None else None
+    lp = _vec(lengths, _I32, "lengths", (R,), here) if lengths is not None else None
     rp = None
     if rope is not None:
         cos, sin = rope
@@ -238,8 +242,9 @@ def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=
     elif q_out is not None:
         raise _invalid("q_out without q")
     if stream is not None:
-        _mark(stream, cache.k, cache.v, cache.score, table, slots, k, v, q, seq, positions, q_out, *(rope or ()))
-    _check(_lib.xt_kv_append(c, t, np_, sp, pp, rp, qp, ldq, hq, op, ldo, kp, ldk, vp, ldv, R, _stream_ptr(stream)))
+        _mark(stream, cache.k, cache.v, cache.score, table, slots, k, v, q, seq, positions, q_out, lengths, *(rope or ()))
+    _check(_lib.xt_kv_append_lengths(c, t, np_, sp, pp, rp, qp, ldq, hq, op, ldo, kp, ldk, vp, ldv, R, lp,
+                                     _stream_ptr(stream)))
     return q_out
 
 

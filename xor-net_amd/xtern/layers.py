@@ -14,6 +14,7 @@ from . import (XT_ERR_INVALID, XT_PACK4, XT_PACK5, XT_QUANT_AVX512, XT_XORSPARSE
                hf_destripe, kv_append, mlp_f32, mlp_q, paged_attention, rms_norm, XT_INT8, XT_INT4, int_quantize_host,
                linear_f32, linear_multi_f32, linear_multi_q, linear_q, pack_ternary4, pack_ternary5,
                unpack_1_58bit_4pack, unpack_1_58bit_5pack)
+from .cache import _I32, _empty
 
 
 class TernaryRep(enum.Enum):
@@ -350,8 +351,10 @@ class CausalSelfAttention:
         (KvCache), then lets each attend over its sequence up to itself, so
         the tokens of a prompt, in order, go in one call.  positions (int32
         [R], default slots) are the rotary ones, rope = (cos, sin) their
-        tables.  accumulate adds the weights to cache.score.  Returns [R,
-        hidden]."""
+        tables.  A row that cannot be appended (a slot, a page or a sequence
+        that is not there, a position without a row in the tables) sees
+        nothing: its attention is zero.  accumulate adds the weights to
+        cache.score.  Returns [R, hidden]."""
         if x.dim() != 2:
             raise XternError(XT_ERR_INVALID, "x must be [rows, hidden]")
         if x.shape[-1] != self.q_proj.in_dim:
@@ -365,8 +368,9 @@ class CausalSelfAttention:
             q, k, v = linear_multi_f32(ws, x, mode=mode)
         else:
             q, k, v = (linear_f32(w, x, mode=mode) for w in ws)
-        kv_append(cache, table, slots, k, v, q=q, seq=seq, positions=positions, rope=rope, q_out=q)
-        y = paged_attention(cache, table, slots + 1, q, seq=seq, accumulate=accumulate)
+        lengths = _empty(None, _I32, x.device, x.shape[0])
+        kv_append(cache, table, slots, k, v, q=q, seq=seq, positions=positions, rope=rope, q_out=q, lengths=lengths)
+        y = paged_attention(cache, table, lengths, q, seq=seq, accumulate=accumulate)
         if self.attn_sub_norm is not None:
             y = self.attn_sub_norm.forward(y)
         return linear_f32(self.o_proj.weights, y, mode=mode)
