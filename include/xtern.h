@@ -496,9 +496,10 @@ int xt_kv_append_lengths(const xt_kv_cache* c, const xt_kv_table* t, const int32
  * accumulate != 0 adds to the score of each position and key-value head the
  * weight that its group's query heads gave it, sum_h softmax(s_h)_j (atomic
  * adds: the sum over rows that share a page is in no fixed order).  Rows are
- * split over their length; the parts, and with accumulate the R * q_heads *
- * max_pages * page_size scores, lie in a per-stream device workspace owned by
- * the library. */
+ * split over their length; the parts, and with accumulate the q_heads *
+ * max_pages * page_size scores of each row, lie in a per-stream device workspace
+ * owned by the library.  Scores beyond 1 GiB (and beyond one row's) are not
+ * held at once: the rows then go in several launches. */
 int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq,
                        const int32_t* lengths, const float* q, int64_t ldq, int q_heads,
                        float scale, int64_t R, float* out, int64_t ldo, float* lse,

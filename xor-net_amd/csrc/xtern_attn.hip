@@ -942,7 +942,7 @@ AttnPlan make_plan(const AttnArgs& a, int cus) {
     pl.hy = a.c.hkv * pl.tiles;
     const int64_t cap = (int64_t)a.c.max_pages * a.c.page;
     pl.cap = (cap + 31) / 32 * 32;
-    pl.per_row = a.R > kAttnPlanRows;
+    pl.per_row = a.call_rows > kAttnPlanRows;
     const int64_t steps = a.R * std::max<int64_t>(1, (cap + kAttnStep - 1) / kAttnStep);
     pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident(a.c.D) * cus / pl.hy));
     pl.shares = std::min(pl.shares, 64 * kJoinGroup);  // (as many as two levels join)

@@ -71,6 +71,7 @@ struct AttnArgs {
     float scale;
     int accumulate;
     int64_t R;
+    int64_t call_rows;       // of the call whose rows, or a part of them, these are
 };
 // Bytes of workspace that the call needs, and of counters that are zero before
 // and after it (0: none, null); cus: compute units of the device.

@@ -116,9 +116,40 @@ int check_heads(int q_heads, int kv_heads) {
 
 // Workspaces that no device holds (and whose size a size_t may not).
 int check_workspace(double bytes) {
-    if (bytes > 1e13)
+    if (bytes > 1e12)
         return xt_internal_fail(XT_ERR_NOMEM, "the call would need a workspace of " + std::to_string(bytes) + " bytes");
     return XT_OK;
+}
+
+// What a workspace holds for each position that the table could have (a row's
+// scores) stays within this: the lengths are on the device, so a wide table
+// would else take memory for positions that nobody wrote.  Calls that need more
+// run in parts, one after the other in the same workspace.  4096 rows of a
+// prompt with scores, 32 heads, a table for 32768 positions: 3.8 ms whole (16
+// GiB), 4.2 in parts of 1 GiB, 4.1 of 2 GiB, 5.1 of 256 MiB.
+constexpr int64_t kMaxScratch = (int64_t)1 << 30;
+int64_t part_of(int64_t n, int64_t bytes_each) {
+    const int64_t most = std::max<int64_t>(1, kMaxScratch / std::max<int64_t>(bytes_each, 1));
+    const int64_t parts = (n + most - 1) / most;
+    return (n + parts - 1) / parts;  // (parts of one size)
+}
+
+// The table from sequence `at` on.
+void skip_sequences(xt::KvView* c, int64_t at) {
+    c->table += at * c->ldt;
+    c->nseq = (int)std::max<int64_t>(0, c->nseq - at);
+}
+
+// Rows [r0, r0 + n) of a call.
+xt::AttnArgs rows_of(xt::AttnArgs a, int64_t r0, int64_t n) {
+    a.R = n;
+    a.q += r0 * a.ldq;
+    a.out += r0 * a.ldo;
+    if (a.lse) a.lse += r0 * a.hq;
+    a.lengths += r0;
+    if (a.seq) a.seq += r0;
+    else skip_sequences(&a.c, r0);
+    return a;
 }
 
 // The workspace and the counters of a call (either may be none).
@@ -222,24 +253,32 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     a.ldq = ldq;
     a.hq = q_heads;
     a.scale = scale;
-    a.R = R;
+    a.R = a.call_rows = R;
     a.out = out;
     a.ldo = ldo;
     a.lse = lse;
     a.accumulate = accumulate ? 1 : 0;
+    int64_t part = R;  // rows at a time
     if (a.accumulate) {
-        const double cap = (double)t->max_pages * c->page_size + 32;
-        if (int rc = check_workspace(4.0 * (double)R * q_heads * cap)) return rc;
+        const int64_t row = 4 * (int64_t)q_heads * t->max_pages * c->page_size;
+        part = part_of(R, row);
+        if (int rc = check_workspace((double)part * (double)row)) return rc;
     }
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     void *ws, *counters;
-    size_t nc;
-    const size_t bytes = xt::attention_workspace(a, cus, &nc);
-    if (int rc = get_workspace(st, bytes, nc, &ws, &counters)) return rc;
-    return launched(xt::launch_paged_attention(c->dtype, a, cus, ws, counters, st),
-                    "paged attention launch");
+    size_t nc, nc_last;
+    const xt::AttnArgs last = rows_of(a, (R - 1) / part * part, R - (R - 1) / part * part);
+    const size_t bytes_last = xt::attention_workspace(last, cus, &nc_last);
+    const size_t bytes = std::max(bytes_last, xt::attention_workspace(rows_of(a, 0, part), cus, &nc));
+    if (int rc = get_workspace(st, bytes, std::max(nc, nc_last), &ws, &counters)) return rc;
+    for (int64_t r0 = 0; r0 < R; r0 += part) {
+        const xt::AttnArgs b = rows_of(a, r0, std::min(part, R - r0));
+        if (int rc = launched(xt::launch_paged_attention(c->dtype, b, cus, ws, counters, st), "paged attention launch"))
+            return rc;
+    }
+    return XT_OK;
 }
 
 int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengths, int64_t budget, int64_t sink,
