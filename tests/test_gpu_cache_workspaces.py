@@ -98,3 +98,23 @@ def test_more_rows_than_sequences_are_none():
     torch.cuda.synchronize()
     assert bool(out[0].any()) and not bool(out[1:].any())
     assert float((c.score - first).sum()) == pytest.approx(hq, rel=1e-4)
+
+def test_eviction_of_a_wide_table():
+    """48 sequences of 16 heads over a table for 2^20 positions: 3.2 GB of keys
+    if all were held at once."""
+    rng = np.random.default_rng(8)
+    S, H, D = 48, 16, 8
+    lens = [20000, 300, 17000, 0] + [int(x) for x in rng.integers(0, 200, S - 5)] + [18011]
+    P, narrow, wide = tables(rng, lens, S)
+    first = cache_of(rng, P, H, D, torch.bfloat16)
+    lengths = torch.tensor(lens, **I32)
+
+    def call(small):
+        c = xtern.KvCache(*(x.clone() for x in (first.k, first.v, first.score)))
+        out = xtern.kv_evict(c, narrow if small else wide, lengths, 150, sink=4, recent=30)
+        return (*out, c.k, c.v, c.score)
+
+    out, took = used(call)
+    assert all(torch.equal(a, b) for a, b in zip(out, call(small=True)))
+    log(f"took {took / 2 ** 20:.0f} MiB")
+    assert took < BOUND

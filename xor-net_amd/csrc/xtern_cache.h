@@ -90,6 +90,8 @@ struct EvictArgs {
     int __attribute__((ext_vector_type(4)))* stage;
     float* stage_score;
 };
+// Bytes of keys in it for each sequence; the whole of it.
+size_t evict_key_bytes(const EvictArgs& a);
 size_t evict_workspace(int dtype, const EvictArgs& a, int cus);
 hipError_t launch_kv_evict(int dtype, EvictArgs a, int cus, void* ws, hipStream_t s);
 

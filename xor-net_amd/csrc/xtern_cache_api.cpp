@@ -114,15 +114,15 @@ int check_heads(int q_heads, int kv_heads) {
     return XT_OK;
 }
 
-// Workspaces that no device holds (and whose size a size_t may not).
-int check_workspace(double bytes) {
+// Memory that no device holds (and whose size a size_t may not).
+int check_fits(double bytes, const char* what) {
     if (bytes > 1e12)
-        return xt_internal_fail(XT_ERR_NOMEM, "the call would need a workspace of " + std::to_string(bytes) + " bytes");
+        return xt_internal_fail(XT_ERR_NOMEM, std::string(what) + " would take " + std::to_string(bytes) + " bytes");
     return XT_OK;
 }
 
 // What a workspace holds for each position that the table could have (a row's
-// scores) stays within this: the lengths are on the device, so a wide table
+// scores, a sequence's keys) stays within this: the lengths are on the device, so a wide table
 // would else take memory for positions that nobody wrote.  Calls that need more
 // run in parts, one after the other in the same workspace.  4096 rows of a
 // prompt with scores, 32 heads, a table for 32768 positions: 3.8 ms whole (16
@@ -149,6 +149,16 @@ xt::AttnArgs rows_of(xt::AttnArgs a, int64_t r0, int64_t n) {
     a.lengths += r0;
     if (a.seq) a.seq += r0;
     else skip_sequences(&a.c, r0);
+    return a;
+}
+
+// At most n sequences of a call, from b0 on.
+xt::EvictArgs sequences_of(xt::EvictArgs a, int64_t b0, int64_t n) {
+    skip_sequences(&a.c, b0);
+    a.c.nseq = (int)std::min<int64_t>(a.c.nseq, n);
+    a.lengths += b0;
+    a.new_lengths += b0;
+    a.kept += b0 * a.c.hkv * a.budget;
     return a;
 }
 
@@ -262,7 +272,7 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     if (a.accumulate) {
         const int64_t row = 4 * (int64_t)q_heads * t->max_pages * c->page_size;
         part = part_of(R, row);
-        if (int rc = check_workspace((double)part * (double)row)) return rc;
+        if (int rc = check_fits((double)part * (double)row, "the workspace")) return rc;
     }
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
@@ -299,13 +309,21 @@ int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengt
     a.budget = (int)budget;
     a.sink = (int)sink;
     a.recent = (int)recent;
-    if (int rc = check_workspace(4.0 * (double)t->seqs * c->kv_heads * (double)t->max_pages * c->page_size)) return rc;
+    const int64_t keys = (int64_t)xt::evict_key_bytes(a), part = part_of(t->seqs, keys);  // sequences at a time
+    if (int rc = check_fits(4.0 * (double)t->seqs * (double)t->max_pages, "the page table")) return rc;
+    if (int rc = check_fits((double)keys, "the workspace")) return rc;
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
     hipStream_t st = static_cast<hipStream_t>(stream);
     void *ws, *counters;
-    if (int rc = get_workspace(st, xt::evict_workspace(c->dtype, a, cus), 0, &ws, &counters)) return rc;
-    return launched(xt::launch_kv_evict(c->dtype, a, cus, ws, st), "cache eviction launch");
+    const size_t bytes_last = xt::evict_workspace(c->dtype, sequences_of(a, (t->seqs - 1) / part * part, part), cus);
+    const size_t bytes = std::max(bytes_last, xt::evict_workspace(c->dtype, sequences_of(a, 0, part), cus));
+    if (int rc = get_workspace(st, bytes, 0, &ws, &counters)) return rc;
+    for (int64_t b0 = 0; b0 < t->seqs; b0 += part)
+        if (int rc = launched(xt::launch_kv_evict(c->dtype, sequences_of(a, b0, part), cus, ws, st),
+                              "cache eviction launch"))
+            return rc;
+    return XT_OK;
 }
 
 int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int64_t V, const int32_t* tokens,

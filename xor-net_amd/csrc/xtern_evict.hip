@@ -468,6 +468,11 @@ __global__ __launch_bounds__(256) void kv_evict_stage_kernel(EvictArgs a, int es
     }
 }
 
+size_t evict_key_bytes(const EvictArgs& a) {
+    const int64_t mid = (int64_t)a.c.max_pages * a.c.page - a.sink - a.recent;
+    return mid > kEvictRegs * kEvictThreads ? (size_t)(a.c.hkv * mid) * sizeof(unsigned) : 0;
+}
+
 namespace {
 
 struct EvictPlan {
@@ -478,10 +483,9 @@ struct EvictPlan {
 
 EvictPlan make_plan(int dtype, const EvictArgs& a, int cus) {
     EvictPlan pl;
-    const int64_t cap = (int64_t)a.c.max_pages * a.c.page, mid = cap - a.sink - a.recent;
+    const int64_t cap = (int64_t)a.c.max_pages * a.c.page;
     const int64_t heads = (int64_t)a.c.nseq * a.c.hkv, kept = a.budget - a.sink;
-    pl.keys = mid > kEvictRegs * kEvictThreads ? (size_t)(heads * mid) * sizeof(unsigned) : 0;
-    pl.keys = (pl.keys + 255) / 256 * 256;
+    pl.keys = ((size_t)a.c.nseq * evict_key_bytes(a) + 255) / 256 * 256;
     pl.moves = kept > 0 && cap > a.budget;
     // Parts of a row until two workgroups per compute unit, of four pieces at least
     const int bytes = a.c.D * (dtype == XT_F32 ? 4 : 2), units = (bytes + 15) / 16;
