@@ -132,13 +132,13 @@ hipError_t launch_kv_append(int dtype, AppendArgs a, hipStream_t s) {
 //     column of eight positions, which the lane loads as eight row pieces and
 //     transposes in registers (v_perm);
 //   the softmax factors of a head are then the lane's own, also for O^T.
-// 16-bit caches: q and p in f32 are split into bf16 (three pieces) or f16 (two,
-// scaled by a power of two against its short range), whose products with k, v
-// the 16-bit MFMA adds up in f32: the matrix cores have that to spare (at D =
-// 128, 48 instructions of 16 cycles per 32 positions against the 6700 cycles
-// that their 16 KB take a SIMD at 6 TB/s).  f32 caches take the f32 MFMA.
+// 16-bit caches: q and p in f32 are split into three bf16 or f16 pieces (f16's
+// raised against its short range), whose products with k, v the 16-bit MFMA
+// adds up in f32: the matrix cores have that to spare (at D = 128, 48
+// instructions of 16 cycles per 32 positions against the 6700 cycles that their
+// 16 KB take a SIMD at 6 TB/s).  f32 caches take the f32 MFMA.
 // Measured (kernel time): 64 rows of up to 8192 positions, 32 query and 8 kv
-// heads of 128, f16, 180 us (6.0 TB/s of cache); 131072 positions of one row,
+// heads of 128, f16, 186 us (5.8 TB/s of cache); 131072 positions of one row,
 // bf16, 95 us (5.6 TB/s); 700 positions of 20 and 5 heads 11.5 us, where the
 // chain of dependent loads (lengths, table, keys, then the join's) counts.
 
@@ -317,10 +317,13 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 __device__ __forceinline__ float pow2(float v) { return __builtin_amdgcn_exp2f(v); }
 
-template <int DT> struct Split;  // pieces of an f32 operand
+// Pieces of an f32 operand x: the first is x rounded, each further one STEP
+// times what the one before left of it.
+template <int DT> struct Split;
 template <> struct Split<XT_BF16> {
     typedef v8bf V;
     static constexpr int N = 3;
+    static constexpr float STEP = 1.0f;
     static constexpr float P = 1.0f;  // scale of the probabilities
     static __device__ __forceinline__ v4f mfma(V a, V b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -328,9 +331,14 @@ template <> struct Split<XT_BF16> {
 };
 template <> struct Split<XT_F16> {
     typedef v8h V;
-    static constexpr int N = 2;
-    // p <= 1: 2^14 p fits f16, and what its two pieces leave is below 2^-25 of
-    // the largest
+    static constexpr int N = 3;
+    // f16 has 11 bits, and none below 2^-24: raised by 2^11, the next piece holds
+    // the next 11 bits, and what three pieces leave is below 2^-47.  With p <= 1
+    // as 2^14 p, weights down to 2^-37 of the row's largest keep all 24 bits, and
+    // smaller ones are off by 2^-61 of it at most.  (Two pieces without the raise,
+    // steps of 2^-39: weights of 2^-26 had lost their last 11 bits; heads of 64 /
+    // 128 / 256 took 53 / 182 / 172 us and take 55 / 186 / 184.)
+    static constexpr float STEP = 2048.0f;
     static constexpr float P = 16384.0f;
     static __device__ __forceinline__ v4f mfma(V a, V b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -347,7 +355,7 @@ __device__ __forceinline__ void split8(const float* x, typename Split<DT>::V* ou
         for (int i = 0; i < 8; ++i) {
             const T p = (T)r[i];
             out[n][i] = p;
-            r[i] -= (float)p;
+            r[i] = (r[i] - (float)p) * Split<DT>::STEP;
         }
 }
 
@@ -658,8 +666,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             };
             float up = 1.0f;
             if constexpr (DT == XT_F16) {
-                // the row's largest element at 2^14 .. 2^15: f16's two pieces
-                // then hold 22 bits of every element, or 2^-39 of the largest
+                // the row's largest element at 2^14 .. 2^15: the pieces then hold
+                // every element down to 2^-37 of it, and 2^-61 of it of the others
                 float mx = 0.0f;
 #pragma unroll
                 for (int s = 0; s < S::KS; ++s) {
@@ -717,7 +725,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                             for (int t = 0; t < S::NT; ++t)
                                 sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__int_as_float(kr[t][s][x]), qv[x], sc[t],
                                                                              0, 0, 0);
-                    } else {
+                    } else if constexpr (Split<DT>::STEP == 1.0f) {
                         typedef typename Split<DT>::V V;
 #pragma unroll
                         for (int x = Split<DT>::N - 1; x >= 0; --x) {
@@ -726,6 +734,22 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                             for (int t = 0; t < S::NT; ++t)
                                 sc[t] = Split<DT>::mfma(__builtin_bit_cast(V, kr[t][s]), qv, sc[t]);
                         }
+                    }
+                }
+                if constexpr (DT == XT_F16) {  // a piece at a time, the last first
+                    typedef typename Split<DT>::V V;
+#pragma unroll
+                    for (int x = Split<DT>::N - 1; x >= 0; --x) {
+#pragma unroll
+                        for (int s = 0; s < S::KS; ++s) {
+                            const V qv = __builtin_bit_cast(V, lds_q[(s * Split<DT>::N + x) * 64 + lane]);
+#pragma unroll
+                            for (int t = 0; t < S::NT; ++t)
+                                sc[t] = Split<DT>::mfma(__builtin_bit_cast(V, kr[t][s]), qv, sc[t]);
+                        }
+                        if (x)
+#pragma unroll
+                            for (int t = 0; t < S::NT; ++t) sc[t] *= 1.0f / Split<DT>::STEP;
                     }
                 }
                 // the next tile's keys, in flight under this tile's softmax and values
@@ -795,10 +819,18 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                             for (int x = 0; x < 4; ++x)
                                 col[x] = (int)__builtin_amdgcn_perm((unsigned)vr[2 * x + 1][u][e / 2],
                                                                     (unsigned)vr[2 * x][u][e / 2], sel);
+                            const auto cv = __builtin_bit_cast(typename Split<DT>::V, col);
+                            v4f& sum = o[u * S::UE + e];
+                            if constexpr (Split<DT>::STEP == 1.0f) {
     #pragma unroll
-                            for (int x = Split<DT>::N - 1; x >= 0; --x)
-                                o[u * S::UE + e] = Split<DT>::mfma(__builtin_bit_cast(typename Split<DT>::V, col), pp[x],
-                                                                   o[u * S::UE + e]);
+                                for (int x = Split<DT>::N - 1; x >= 0; --x) sum = Split<DT>::mfma(cv, pp[x], sum);
+                            } else {
+                                v4f low = {0.0f, 0.0f, 0.0f, 0.0f};
+    #pragma unroll
+                                for (int x = Split<DT>::N - 1; x > 0; --x)
+                                    low = Split<DT>::mfma(cv, pp[x], low) * (1.0f / Split<DT>::STEP);
+                                sum = Split<DT>::mfma(cv, pp[0], sum + low);
+                            }
                         }
                 }
                 if (i + kAttnWaves < ntiles) load_v(i + kAttnWaves);
