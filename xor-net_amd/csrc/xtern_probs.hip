@@ -24,9 +24,11 @@
 // that fails (ties beyond the buffer, fewer finite logits than `top`) the tile
 // is selected from by the digits of its logits.
 //
-// Measured (kernel time): 1024 rows of 128256 f32 logits 83 us without
-// alternatives (6.3 TB/s), 91 / 117 us with 1 / 20; one row with 20 10.7 us,
-// where the chain of load, reduction, selection and join counts.
+// Measured: 1024 rows of 128256 f32 logits 83 us without alternatives (6.3
+// TB/s), 91 / 114 with 1 / 20; of f16 or bf16 65 us (4.0 TB/s) and 107 / 157 with
+// 20 / 64, where the instructions count: the exponentials, and for alternatives
+// the barriers of each tile.  One row of f32 with 20 10.7 us, where the chain of
+// load, reduction, selection and join counts.
 #include <algorithm>
 
 #include "xtern_cache.h"
@@ -456,8 +458,12 @@ namespace {
 ProbsPlan make_plan(const ProbsArgs& a, int cus) {
     ProbsPlan pl;
     pl.tiles = (a.V + kProbsTile - 1) / kProbsTile;
-    // slices until four workgroups per compute unit (what it holds)
-    const int64_t want = std::max<int64_t>(1, 4 * (int64_t)cus / std::max<int64_t>(a.M, 1));
+    // slices until two workgroups per compute unit (what it holds, by registers).
+    // One of 128256 f32 logits each, 20 alternatives, against slices for four and
+    // for eight a unit: 37 rows 18 us (21, 20), 128 rows 27 (37, 47), 512 rows 63
+    // (74, 90); 300 rows 59 (55, 68).  From 513 rows on, 85 us, a row is one slice,
+    // and the ones that do not fit at once wait for the others.
+    const int64_t want = std::max<int64_t>(1, 2 * (int64_t)cus / std::max<int64_t>(a.M, 1));
     const int slices = (int)std::min<int64_t>(std::min<int64_t>(want, kProbsSlices), pl.tiles);
     pl.per = (pl.tiles + slices - 1) / slices;
     pl.slices = (pl.tiles + pl.per - 1) / pl.per;
