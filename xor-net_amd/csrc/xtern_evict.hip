@@ -490,10 +490,16 @@ EvictPlan make_plan(int dtype, const EvictArgs& a, int cus) {
     // Parts of a row until two workgroups per compute unit, of four pieces at least
     const int bytes = a.c.D * (dtype == XT_F32 ? 4 : 2), units = (bytes + 15) / 16;
     pl.parts = bytes < 16 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(units / 4, (int64_t)cus / heads));
-    // Through the workspace where that leaves compute units without a
-    // workgroup and there are rows enough to pay for the second kernel
+    // Through the workspace where that leaves half the compute units without a
+    // workgroup and there are rows enough to pay for the second kernel.  Whole
+    // calls, staged against in place, 6000 / 12000 rows: 12 heads of 128 in bf16 (96
+    // workgroups) 96 / 165 us against 104 / 190, 16 heads (128) 104 / 181 against
+    // 101 / 185, 24 heads (192) 124 / 217 against 110 / 200, 32 heads (256) 138 / 270
+    // against 117 / 220; 8 heads in f32 (128) 103 / 178 against 102 / 189, 16 heads
+    // (256) 136 / 266 against 121 / 225.  4096 rows of 8 heads: 68 either way; of one
+    // head of 64 in f16 52 against 67, and 33 against 37 at 2000 (not taken).
     const double stage = (double)heads * kept * (32.0 * units + 4);
-    pl.staged = pl.moves && bytes >= 16 && 2 * heads * pl.parts <= cus && kept >= 4096 && stage < 4e9;
+    pl.staged = pl.moves && bytes >= 16 && 4 * heads * pl.parts <= cus && kept >= 4096 && stage < 4e9;
     pl.stage = pl.staged ? (size_t)(heads * kept) * 32 * units : 0;
     pl.scores = pl.staged ? (size_t)(heads * kept) * sizeof(float) : 0;
     return pl;
