@@ -162,7 +162,13 @@ constexpr int kAttnPlanRows = 1024;  // rows whose work is split by its total
 // of one row, whole rows and the start of another: its segments.  A segment's
 // sums go to slot (workgroup + row), which both grow along the line, so no two
 // segments share one and a row's slots are consecutive.
-// More than kAttnPlanRows rows: one workgroup per row.
+// More than kAttnPlanRows rows: one workgroup per row and group of heads.  With
+// that many rows of like lengths they fill the chip by themselves, and the
+// line costs its scan: 1000 / 2000 rows of up to 2000 positions, 32 and 8 heads
+// of 128 in bf16, 699 / 1415 us on the line, 658 / 1331 a workgroup each; of 2000 to
+// 4000, 1000 rows, 1927 against 2040.  What the limit costs is a long row among
+// many short ones: 1000 rows, one of 60000 positions and the others of 100, 193
+// us on the line and 1018 without; 1100 rows 972 as it is, 210 on the line.
 // The workgroup that ends the last of a row's segments joins them, from 32
 // segments on in two levels (groups of 32, then the groups): what one
 // workgroup can read at device scope, about 20 GB/s, bounds a join.  Segments
@@ -961,7 +967,11 @@ __global__ __launch_bounds__(kAttnThreads) void attention_score_kernel(AttnArgs 
 
 namespace {
 
-// Workgroups of attention_kernel that a compute unit holds, by registers.
+// Workgroups of attention_kernel per compute unit that the work is split for:
+// as many as it holds by registers with a 16-bit cache.  The f32 kernels take
+// fewer and one more of each would fit up to 128: measured slower (9 rows, 32
+// heads of 100: 86 us with two, 95 with three; 64 rows, 8 kv heads of 128, 182 and
+// 190; of 64, 100 with three and 102 with four).
 int resident(int D) { return D > 128 ? 1 : (D > 64 ? 2 : 3); }
 
 AttnPlan make_plan(const AttnArgs& a, int cus) {
