@@ -1,9 +1,10 @@
 """What xt_kv_append_lengths refuses, on the CPU: as xt_kv_append, and lengths
-that are another argument or not aligned."""
+that are another argument or not aligned.  And scales whose multiple in base 2
+is infinite."""
 import pytest
 
 import xtern
-from test_cache_cpu import CACHE_FAULTS, L, P, TABLE_FAULTS, cache, ref_, rope, table
+from test_cache_cpu import CACHE_FAULTS, L, P, TABLE_FAULTS, attend, cache, ref_, rope, table
 
 
 def append(c=None, t=None, slots=P, seq=P, pos=P, lengths=P + 64, R=2, k=P):
@@ -27,3 +28,9 @@ def test_bad_arguments(f):
 
 def test_no_rows():
     assert append(R=0) == xtern.XT_OK
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, 2.36e38, float("inf"), float("nan")])
+def test_scales(scale):
+    assert attend(scale=scale) == xtern.XT_ERR_INVALID
+    assert attend(scale=scale / 10, R=0) == (xtern.XT_OK if abs(scale) < float("inf") else xtern.XT_ERR_INVALID)

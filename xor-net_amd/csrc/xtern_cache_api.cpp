@@ -246,7 +246,8 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     if (int rc = check_cache(c, t, &a.c)) return rc;
     if (int rc = check_count(R)) return rc;
     if (int rc = check_heads(q_heads, c->kv_heads)) return rc;
-    if (!isfinite(scale)) return bad("scale must be finite");
+    // (the kernels work with scale in base 2)
+    if (!isfinite((float)((double)scale * 1.4426950408889634))) return bad("scale must be finite, at most 2.3e38");
     if (accumulate && !c->score) return bad("accumulate needs a cache with scores");
     if (R == 0) return XT_OK;
     if (!lengths) return bad("NULL pointer");
