@@ -24,7 +24,8 @@
  * synchronises or clears memory while its stream is being captured: a call
  * whose workspace would have to grow fails with XT_ERR_UNSUPPORTED instead.
  * Make one eager call of the largest shape on the capturing stream and
- * thread first.  A graph uses the workspace of the thread and stream it was
+ * thread first; of the cache and probability calls, one of each shape that is
+ * captured (fewer rows are split further, and may need more).  A graph uses the workspace of the thread and stream it was
  * captured on; replay it on that stream, or order it against eager calls of
  * that thread on that stream.
  *

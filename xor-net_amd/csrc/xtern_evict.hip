@@ -19,7 +19,7 @@
 // workgroup per (sequence, head, tensor), and per part of a row where those
 // are too few for the chip.  32 sequences of up to 8192 positions and 8 heads
 // of 128 in f16, cut to 2048: 17 + 95 us (4.3 TB/s moved; a large copy reaches
-// 4.8); one of 1027 positions and 5 heads cut to 512: 9 + 6 us.
+// 4.8); one of 1027 positions and 5 heads cut to 512: 10 + 6 us.
 //
 // Why rows can move in place: the kept list ascends and is part of L, so
 // kept[j] >= L[j].  A workgroup moves its part of the rows in rounds of

@@ -24,8 +24,8 @@
 // that fails (ties beyond the buffer, fewer finite logits than `top`) the tile
 // is selected from by the digits of its logits.
 //
-// Measured: 1024 rows of 128256 f32 logits 83 us without alternatives (6.3
-// TB/s), 91 / 114 with 1 / 20; of f16 or bf16 65 us (4.0 TB/s) and 107 / 157 with
+// Measured: 1024 rows of 128256 f32 logits 84 us without alternatives (6.3
+// TB/s), 91 / 124 / 176 with 1 / 20 / 64; of f16 or bf16 65 us (4.0 TB/s) and 107 / 157 with
 // 20 / 64, where the instructions count: the exponentials, and for alternatives
 // the barriers of each tile.  One row of f32 with 20 10.7 us, where the chain of
 // load, reduction, selection and join counts.

@@ -78,7 +78,7 @@ public:
         if (cap_active) {
             *err = "workspace of " + std::to_string(bytes) +
                    " bytes would have to be allocated during graph capture; make one eager call "
-                   "of the largest shape on this stream and thread before capturing";
+                   "of this shape on this stream and thread before capturing";
             return kCapture;
         }
         if (!w.ptr) {  // a first buffer for this key: adopt a pooled one
