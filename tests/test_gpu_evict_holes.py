@@ -96,7 +96,7 @@ def test_long(dtype):
     than a workgroup has threads."""
     for n, page, budget, lost in ((5000, 1, 700, range(100, 2300)), (20011, 32, 3000, range(0, 40)),
                                   (20011, 32, 3000, range(3, 500, 7)), (17000, 16, 900, range(0, 1000)),
-                                  (16384 + 64, 16, 16383, [5])):
+                                  (16384 + 64, 16, 16383, [5]), (14000, 5000, 800, [0]), (40000, 20000, 900, [1])):
         log(f"evict holes {dtype} {n} {page} {budget}")
         case(dtype, 8, 4 if dtype == torch.float32 else 8, page, [n, 40], budget, min(4, budget), 33, {0: lost, 1: [0]})
 
