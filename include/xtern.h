@@ -403,7 +403,7 @@ int xt_stack_run(const xt_stack* st, void* stream);
 int xt_stack_check(xt_stack* st, int* gave_up);
 int xt_stack_destroy(xt_stack* st);
 
-/* ---- Paged key-value cache: append, attention, eviction ----
+/* ---- Paged key-value cache: append, read-back, attention, eviction ----
  * What a decode step does between its projections (CausalSelfAttention::
  * forward, src/models/llama/attention.rs:42-113, with the ring cache of
  * src/nn/fast_attention.rs:7-75 in pages instead): rotate the new queries and
@@ -413,6 +413,10 @@ int xt_stack_destroy(xt_stack* st);
  * Every call takes at most 2^21 rows or sequences.  Element types of a cache
  * (and of logits): */
 enum { XT_F32 = 0, XT_F16 = 1, XT_BF16 = 2 };
+/* and of a cache alone: 8-bit codes, with a scale for each position and head
+ * (xt_kv_scales); taken by xt_kv_store, xt_kv_read and
+ * xt_paged_attention_window. */
+enum { XT_I8 = 3 };
 
 /* A pool of pages in device memory that the caller owns.  Element d of head h
  * in slot s of page p lies at p * stride_page + s * stride_slot + h *
@@ -434,6 +438,14 @@ typedef struct xt_kv_cache {
     int64_t stride_slot;
     int64_t stride_head;
 } xt_kv_cache;
+
+/* The scales of an XT_I8 cache, [num_pages][kv_heads][page_size] f32 each: code c
+ * of a key (a value) stands for c times its position's and head's scale.  Such a
+ * cache keeps no score. */
+typedef struct xt_kv_scales {
+    float* k;
+    float* v;
+} xt_kv_scales;
 
 /* The pages of each sequence, on the device: position i of sequence b lies in
  * slot i % page_size of page pages[b * stride + i / page_size].  An entry
@@ -486,6 +498,36 @@ int xt_kv_append_lengths(const xt_kv_cache* c, const xt_kv_table* t, const int32
                          const float* k, int64_t ldk, const float* v, int64_t ldv, int64_t R,
                          int32_t* lengths, void* stream);
 
+/* Norms of the query and key heads: x becomes w x / sqrt(mean x^2 + eps), w
+ * [head_dim] f32 on the device; eps finite, >= 0. */
+typedef struct xt_head_norm {
+    const float* q;
+    const float* k;
+    double eps;
+} xt_head_norm;
+
+/* xt_kv_append_lengths with norms of q's and k's heads before the rotation
+ * (norm NULL: none) and into a cache of any type; scales: an XT_I8 cache's, else
+ * NULL.  The heads are normed, rotated and quantised in 64 bits and rounded once.
+ * An XT_I8 cache gets, of a head y of k or v with a = max |y|, the scale s = a /
+ * 127 (rounded to f32) and the codes round(y / s) (nearest, ties to even); s and
+ * codes 0 where a < 2^-119; NaN and codes 0 where the head has an infinity or
+ * NaN.  lengths may be NULL. */
+int xt_kv_store(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t,
+                const int32_t* seq, const int32_t* slots, const int32_t* positions,
+                const xt_rope* rope, const xt_head_norm* norm, const float* q, int64_t ldq,
+                int q_heads, float* q_out, int64_t ldqo, const float* k, int64_t ldk,
+                const float* v, int64_t ldv, int64_t R, int32_t* lengths, void* stream);
+
+/* Keys and values of R positions as the cache holds them: row r of k and v
+ * [R][kv_heads * head_dim] (row strides ldk, ldv; type out: XT_F32, XT_F16 or
+ * XT_BF16, rounded to nearest even) gets position slots[r] of sequence seq[r]
+ * (seq NULL: sequence r), zeros where the slot is negative or past the table or
+ * the sequence or page does not exist. */
+int xt_kv_read(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t,
+               const int32_t* seq, const int32_t* slots, int64_t R, int out, void* k, int64_t ldk,
+               void* v, int64_t ldv, void* stream);
+
 /* Attention of one token per row r over the first lengths[r] positions of
  * sequence seq[r] (seq NULL: sequence r; several rows may name one sequence,
  * e.g. the tokens of a prompt with growing lengths): query head h of q
@@ -505,6 +547,25 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
                        const int32_t* lengths, const float* q, int64_t ldq, int q_heads,
                        float scale, int64_t R, float* out, int64_t ldo, float* lse,
                        int accumulate, void* stream);
+
+/* xt_paged_attention over a cache of any type (scales: an XT_I8 cache's, else
+ * NULL), with a window and with several tokens of a sequence:
+ * window > 0: a row of length n sees position p only if p < sink or p >= n -
+ *   window (the newest `window`, the last one its own); 0: every p < n, and sink
+ *   has to be 0.  Both at most 2^30.
+ * tokens (1..65536, a divisor of R): the rows go in groups of `tokens` that
+ *   belong to one sequence, the one that seq names for the group's first row
+ *   (seq NULL: group g to sequence g); their lengths may be any, 0 for padding.
+ *   Over an XT_I8 cache as many rows of a group as have 16 query heads between
+ *   them share one pass over its positions; over the others every row makes its
+ *   own.
+ * Positions that no row sees are not read.  Queries and an XT_I8 cache's codes
+ * meet in whole numbers of 24 and 8 bits: results keep the precision of f32. */
+int xt_paged_attention_window(const xt_kv_cache* c, const xt_kv_scales* scales,
+                              const xt_kv_table* t, const int32_t* seq, const int32_t* lengths,
+                              int64_t tokens, int64_t window, int64_t sink, const float* q,
+                              int64_t ldq, int q_heads, float scale, int64_t R, float* out,
+                              int64_t ldo, float* lse, int accumulate, void* stream);
 
 /* Cut every sequence b of the table that holds lengths[b] > budget positions
  * down to budget, for each key-value head by its own scores: the first sink
@@ -534,6 +595,30 @@ int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengt
 int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int64_t V,
                       const int32_t* tokens, int64_t T, float* logprobs, float* entropy, int top,
                       int32_t* top_ids, float* top_logprobs, void* stream);
+
+/* Verification of T (0..64) drafted tokens for each of S sequences, S (2 T + 1)
+ * at most 2^21.  target: logits [S][T + 1][V] (V at most 2^30; strides ld_seq,
+ * ld_row in elements; -inf masks a token), at place t those of the token after
+ * drafted[b][t - 1]; draft: the logits [S][T][V] that the drafts were drawn from
+ * (strides ldd_seq, ldd_row), or NULL: each was certain.  counts [S] (NULL: T
+ * each): drafts of a sequence, at most T; negative: no sequence.  With p and q
+ * the probabilities softmax(x / temperature) and given uniforms [S][T + 1] in
+ * [0, 1): drafts are accepted while uniforms[b][t] q(x_t) < p(x_t); the token
+ * after them is drawn with uniforms[b][T] from max(p - q, 0) of the first that
+ * was not (an id outside the vocabulary ends the drafts before it, as counts
+ * does), or from p after the last: the lowest id up to which the sum is above
+ * that share of the whole.
+ * temperature >= 0 for every sequence, or temperatures [S]; at 0 all of p lies
+ * on the largest logit (the lowest id of equals).  accepted [S]: drafts that
+ * were; tokens [S][T + 1]: these, the drawn one, then -1; logprobs [S][T + 1]: ln
+ * p of each, then 0.  A row that has to be looked at and has NaN, +inf or
+ * nothing but -inf, or a temperature that is none, ends the sequence with -1 in
+ * the drawn token's place. */
+int xt_verify_drafts(int dtype, const void* target, int64_t ld_seq, int64_t ld_row,
+                     const void* draft, int64_t ldd_seq, int64_t ldd_row, int64_t S, int64_t T,
+                     int64_t V, const int32_t* drafted, const int32_t* counts,
+                     const float* uniforms, float temperature, const float* temperatures,
+                     int32_t* accepted, int32_t* tokens, float* logprobs, void* stream);
 
 #ifdef __cplusplus
 }

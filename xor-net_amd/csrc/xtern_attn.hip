@@ -1,8 +1,6 @@
 // The paged key-value cache's append (rotary embedding, rounding, scatter)
 // and the attention of one token per row over it.
-#include <algorithm>
-
-#include "xtern_cache.h"
+#include "xtern_attn.h"
 
 namespace xt {
 
@@ -142,186 +140,11 @@ hipError_t launch_kv_append(int dtype, AppendArgs a, hipStream_t s) {
 // bf16, 95 us (5.6 TB/s); 700 positions of 20 and 5 heads 11.5 us, where the
 // chain of dependent loads (lengths, table, keys, then the join's) counts.
 
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef int v2i __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 // (rows may start at any element: the hardware loads unaligned vectors)
 typedef v4i v4iu __attribute__((aligned(2)));
 typedef v2i v2iu __attribute__((aligned(2)));
-typedef v4f v4fu __attribute__((aligned(4)));
-
-constexpr int kAttnThreads = 256;
-constexpr int kAttnWaves = kAttnThreads / 64;
-constexpr int kAttnStep = 128;       // positions: the unit of the split
-constexpr int kAttnPlanRows = 1024;  // rows whose work is split by its total
-
-// The split.  The steps of all rows (an empty row has one, for its zeros) form
-// one line, cut into equal shares for as many workgroups as run at once: rows
-// of any lengths keep all of them busy to the end.  A share may cover the end
-// of one row, whole rows and the start of another: its segments.  A segment's
-// sums go to slot (workgroup + row), which both grow along the line, so no two
-// segments share one and a row's slots are consecutive.
-// More than kAttnPlanRows rows: one workgroup per row and group of heads.  With
-// that many rows of like lengths they fill the chip by themselves, and the
-// line costs its scan: 1000 / 2000 rows of up to 2000 positions, 32 and 8 heads
-// of 128 in bf16, 699 / 1415 us on the line, 658 / 1331 a workgroup each; of 2000 to
-// 4000, 1000 rows, 1927 against 2040.  What the limit costs is a long row among
-// many short ones: 1000 rows, one of 60000 positions and the others of 100, 193
-// us on the line and 1018 without; 1100 rows 972 as it is, 210 on the line.
-// The workgroup that ends the last of a row's segments joins them, from 32
-// segments on in two levels (groups of 32, then the groups): what one
-// workgroup can read at device scope, about 20 GB/s, bounds a join.  Segments
-// and counts are written and read at device scope, as the chip's eight L2s
-// need it (a fence would write back and drop whole caches).
-struct AttnPlan {
-    float* part_o;   // [slots][hy][16][dp], unnormalised, relative to the segment's maximum
-    float* part_ml;  // [slots][hy][16][2]: maximum (base 2), sum
-    unsigned* count; // [slots][hy]: segments of the group done that begins there; zero between calls
-    unsigned* tops;  // [R][hy]: groups of the row done; zero between calls
-    float* ml;       // accumulate: maximum and sum of the whole row, [R][hq][2]
-    int dp;          // D, made even
-    float* s;        // accumulate: S in base 2, [R][hq][cap]
-    int64_t cap;     // positions of a row of s, a multiple of 32
-    int hy;          // workgroups per share: kv heads x tiles of 16 query heads
-    int tiles;       // of 16 query heads per kv head
-    int shares;      // at most
-    bool per_row;
-};
-
-// A row's part of the line, and of it what one share covers.
-struct AttnSeg {
-    int row, n, p0, p1;  // positions [p0, p1) of n
-    int nc;              // segments of the row
-    int64_t slot;        // of its first one
-};
-
-__device__ __forceinline__ int attn_len(const AttnArgs& a, int64_t r) {
-    const int sq = a.seq ? a.seq[r] : (int)r;
-    return (unsigned)sq < (unsigned)a.c.nseq ? kv_length(a.c, a.lengths[r]) : 0;
-}
-__device__ __forceinline__ int attn_steps(int len) { return max(1, (len + kAttnStep - 1) / kAttnStep); }
-
-// The line as every wave of the workgroup sees it: 64 rows, a lane each, in
-// registers (no barrier), or the rows' ends in LDS.
-struct AttnLine {
-    const AttnArgs& a;
-    const AttnPlan& pl;
-    int len, upto;       // the lane's row (R <= 64)
-    int64_t* ends;       // LDS, [R] (R > 64)
-    int64_t total;       // steps
-    int64_t per;         // steps of a share
-    double inv;          // 1 / per
-    int x;               // shares that the line is cut into
-
-    __device__ AttnLine(const AttnArgs& a_, const AttnPlan& pl_, int64_t* lds) : a(a_), pl(pl_), ends(lds) {
-        if (pl.per_row) {
-            total = x = (int)a.R;
-            per = 1;
-            inv = 1.0;
-            return;
-        }
-        if (a.R <= 64) {
-            const int lane = threadIdx.x & 63;
-            len = lane < a.R ? attn_len(a, lane) : -1;
-            upto = wave_scan(len < 0 ? 0 : attn_steps(len));  // (64 rows of 2^30 positions: 2^29)
-            total = __builtin_amdgcn_readlane(upto, 63);
-        } else {
-            // wave w: rows 64 w .. 64 w + 63 and every 256 behind them
-            __shared__ int block[kAttnPlanRows / 64];
-            const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-            for (int r = wave * 64; r < a.R; r += kAttnThreads) {
-                const int up = wave_scan(r + lane < a.R ? attn_steps(attn_len(a, r + lane)) : 0);
-                if (r + lane < a.R) ends[r + lane] = up;
-                if (lane == 63) block[r / 64] = up;
-            }
-            __syncthreads();
-            total = 0;
-            for (int r = 0; r < a.R; r += 64) {
-                if ((r / 64) % kAttnWaves == wave && r + lane < a.R) ends[r + lane] += total;
-                total += block[r / 64];
-            }
-            __syncthreads();
-        }
-        // (whole numbers below 2^53: a quotient in doubles is off by one at most)
-        per = max((int64_t)1, (int64_t)((double)total / (double)pl.shares));
-        while (per * pl.shares < total) ++per;
-        inv = 1.0 / (double)per;
-        x = share_of(total - 1) + 1;
-    }
-    // First step of share b; the share that holds a step.
-    __device__ int64_t begin(int b) const { return min(b * per, total); }
-    __device__ int share_of(int64_t step) const {
-        int b = (int)((double)step * inv);
-        b -= b * per > step;
-        return b + ((b + 1) * per <= step);
-    }
-    // First row that ends after `step`.
-    __device__ int row_at(int64_t step) const {
-        if (pl.per_row) return (int)step;
-        if (a.R <= 64) return __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(step < upto)));
-        int lo = 0, hi = (int)a.R - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (step < ends[mid]) hi = mid;
-            else lo = mid + 1;
-        }
-        return __builtin_amdgcn_readfirstlane(lo);
-    }
-    // Row r, from step `from` (of the line) up to step `to`.
-    __device__ AttnSeg segment(int r, int64_t from, int64_t to, int64_t* end) const {
-        AttnSeg g;
-        g.row = r;
-        if (pl.per_row) {
-            g.n = attn_len(a, r);
-            g.p0 = 0;
-            g.p1 = g.n;
-            g.nc = 1;
-            g.slot = 2 * (int64_t)r;  // (share r + row r)
-            *end = r + 1;
-            return g;
-        }
-        int64_t first;
-        if (a.R <= 64) {
-            g.n = __builtin_amdgcn_readlane(len, r);
-            *end = __builtin_amdgcn_readlane(upto, r);
-            first = *end - attn_steps(g.n);
-        } else {
-            g.n = attn_len(a, r);
-            *end = ends[r];
-            first = r ? ends[r - 1] : 0;
-        }
-        g.p0 = (int)(max(from, first) - first) * kAttnStep;
-        g.p1 = min((int)(min(to, *end) - first) * kAttnStep, g.n);
-        g.nc = share_of(*end - 1) - share_of(first) + 1;
-        g.slot = share_of(first) + r;
-        return g;
-    }
-};
-
-__device__ __forceinline__ float rows_max(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float rows_sum(float v) {
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-// Over the wave, in every lane.
-__device__ __forceinline__ float wave_max(float v) {
-    for (int o = 1; o < 16; o <<= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return rows_max(v);
-}
-__device__ __forceinline__ float wave_sum(float v) {
-    for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o);
-    return rows_sum(v);
-}
-__device__ __forceinline__ float pow2(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // Pieces of an f32 operand x: the first is x rounded, each further one STEP
 // times what the one before left of it.
@@ -389,7 +212,7 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
                            float scale2, float* lds_o, float* lds_ml, int ldo) {
     typedef Elem<DT> E;
     const KvView& c = a.c;
-    const int t = threadIdx.x, sq = a.seq ? a.seq[it.row] : it.row;
+    const int t = threadIdx.x, sq = attn_unit(a, it.row).seq;
     __shared__ float sp[kAttnThreads];
     __shared__ int64_t so[kAttnThreads];
     __shared__ float sm[kAttnWaves];
@@ -399,7 +222,7 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
         const float* q = a.q + it.row * a.ldq + (int64_t)(h0 + h) * c.D;
         float m = -INFINITY, l = 0.0f, o = 0.0f;
         for (int p0 = it.p0; p0 < it.p1; p0 += kAttnThreads) {
-            const int p = p0 + t, pg = p < it.p1 ? kv_page(c, sq, p) : -1;
+            const int i = p0 + t, p = attn_pos(a, it.gap, i), pg = i < it.p1 ? kv_page(c, sq, p) : -1;
             const int64_t off = pg < 0 ? -1 : kv_offset(c, pg, p, hk);
             float s = -INFINITY;
             if (off >= 0) {
@@ -407,7 +230,7 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
                 for (int d = 0; d < c.D; ++d) acc += q[d] * E::get(kc[off + d]);
                 s = acc * scale2;
             }
-            if (pl.s && p < it.p1) pl.s[((int64_t)it.row * a.hq + h0 + h) * pl.cap + p] = s;
+            if (pl.s && i < it.p1) pl.s[((int64_t)it.row * a.hq + h0 + h) * pl.cap + i] = s;
             float v = s;
             for (int x = 32; x; x >>= 1) v = fmaxf(v, __shfl_xor(v, x));
             __syncthreads();
@@ -437,126 +260,6 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
         }
     }
     __syncthreads();
-}
-
-// Two floats at device scope.
-__device__ __forceinline__ void st2_device(float* p, float x, float y) {
-    const unsigned long long v = ((unsigned long long)__float_as_uint(y) << 32) | __float_as_uint(x);
-    __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 ld2_device(const float* p) {
-    const unsigned long long v = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED,
-                                                   __HIP_MEMORY_SCOPE_AGENT);
-    return float2{__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32))};
-}
-
-__device__ __forceinline__ float row_lse(float m, float l) {
-    return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
-}
-
-constexpr int kJoinGroup = 32;
-
-// Joins `cnt` (at most 64) segments, in every `every`-th slot from slot0, for
-// the heads h0 .. h0 + nh - 1: into the row's results (last), or into slot0.
-// A wave adds up one head's columns, a pair a lane; the segments' maxima and
-// sums are a lane's each; with one or two heads the waves share the segments.
-// Bound by the latency of device-scope loads: the first segments' columns are
-// requested together with the statistics that weigh them.
-template <int DP>
-__device__ void attention_join(const AttnArgs& a, const AttnPlan& pl, int row, int64_t slot0, int every, int cnt,
-                               bool last, int h0, int nh, float* scratch) {
-    constexpr int NK = DP > 128 ? 2 : 1, N = 16;  // pairs of a lane, segments in flight
-    const int D = a.c.D, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t first = slot0 * pl.hy + blockIdx.y, step = (int64_t)every * pl.hy * 16 * pl.dp;
-    const int share = nh == 1 ? 4 : (nh == 2 ? 2 : 1), part = wave & (share - 1);
-#pragma unroll 1
-    for (int hb = 0; hb < nh; hb += kAttnWaves / share) {
-        const int h = min(hb + wave / share, nh - 1);  // (a head too many: a repeat, not written)
-        float* o = pl.part_o + (first * 16 + h) * pl.dp;
-        float* ml = pl.part_ml + (first * 16 + h) * 2;
-        const float2 st = ld2_device(ml + (int64_t)min(lane, cnt - 1) * every * pl.hy * 32);
-        float m = 0.0f, l = 0.0f, fc = 0.0f;  // fc: the factor of the lane's segment
-        float2 v[NK];
-#pragma unroll
-        for (int k = 0; k < NK; ++k) v[k] = float2{0.0f, 0.0f};
-#pragma unroll 1
-        for (int c = part; c < cnt || c == part; c += N * share) {
-            float2 x[N][NK];
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-#pragma unroll
-                for (int k = 0; k < NK; ++k)
-                    if (2 * lane + 128 * k < D)
-                        x[i][k] = ld2_device(o + min(c + i * share, cnt - 1) * step + 2 * lane + 128 * k);
-            if (c == part) {
-                const float mc = lane < cnt ? st.x : -INFINITY;
-                m = wave_max(mc);
-                fc = pow2(mc - (m == -INFINITY ? 0.0f : m));
-                l = wave_sum(lane < cnt ? st.y * fc : 0.0f);
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int ci = c + i * share;
-                const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(fc), min(ci, 63)));
-#pragma unroll
-                for (int k = 0; k < NK; ++k)
-                    if (ci < cnt && 2 * lane + 128 * k < D) {
-                        v[k].x += f * x[i][k].x;
-                        v[k].y += f * x[i][k].y;
-                    }
-            }
-        }
-        if (share > 1) {  // scratch [4][256]
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                scratch[wave * 256 + 2 * lane + 128 * k] = v[k].x;
-                scratch[wave * 256 + 2 * lane + 128 * k + 1] = v[k].y;
-            }
-            __syncthreads();
-            if (part == 0)
-                for (int w = 1; w < share; ++w)
-#pragma unroll
-                    for (int k = 0; k < NK; ++k) {
-                        v[k].x += scratch[(wave + w) * 256 + 2 * lane + 128 * k];
-                        v[k].y += scratch[(wave + w) * 256 + 2 * lane + 128 * k + 1];
-                    }
-        }
-        if (hb + wave / share >= nh || part) continue;
-        if (!last) {
-            // (the wave itself has read what lay there)
-#pragma unroll
-            for (int k = 0; k < NK; ++k)
-                if (2 * lane + 128 * k < D) st2_device(o + 2 * lane + 128 * k, v[k].x, v[k].y);
-            if (lane == 0) st2_device(ml, m, l);
-            continue;
-        }
-        float* to = a.out + row * a.ldo + (int64_t)(h0 + h) * D;
-#pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            const int d = 2 * lane + 128 * k;
-            if (d < D) to[d] = l == 0.0f ? 0.0f : v[k].x / l;
-            if (d + 1 < D) to[d + 1] = l == 0.0f ? 0.0f : v[k].y / l;
-        }
-        if (lane == 0) {
-            const int64_t at = (int64_t)row * a.hq + h0 + h;
-            if (a.lse) a.lse[at] = row_lse(m, l);
-            if (pl.ml) {
-                pl.ml[2 * at] = m;
-                pl.ml[2 * at + 1] = l;
-            }
-        }
-    }
-}
-
-// Counts one of `of` results, stored by this workgroup, and says whether it
-// was the last.  (The count wraps to zero by itself, for the next call.)
-__device__ __forceinline__ bool attention_count(unsigned* count, int of, int* lds_last) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every store has arrived
-    __syncthreads();
-    if (threadIdx.x == 0) *lds_last = atomicInc(count, (unsigned)of - 1) == (unsigned)of - 1;
-    __syncthreads();
-    return *lds_last;
 }
 
 template <int DT, int DP>
@@ -591,7 +294,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
         asm volatile("" : "+s"(D), "+v"(lane));
         const int n = lane & 15, g = lane >> 4;
         const bool fast = D >= S::KU;
-        const int sq = a.seq ? a.seq[r] : r;
+        const int sq = attn_unit(a, r).seq;
         const int ntiles = it.p1 > it.p0 ? (it.p1 - it.p0 + S::TK - 1) / S::TK : 0;
 
         float m = -INFINITY, l = 0.0f, qs = scale2;
@@ -615,10 +318,10 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             // LDS; -1: no position there (masked, read from offset 0)
             auto entry = [&](int i) {  // the lane's table entry of tile i
                 const int p = it.p0 + i * S::TK + (lane & (S::TK - 1));
-                return p < it.p1 ? c.table[(int64_t)sq * c.ldt + kv_page_of(c, p)] : -1;
+                return p < it.p1 ? c.table[(int64_t)sq * c.ldt + kv_page_of(c, attn_pos(a, it.gap, p))] : -1;
             };
             auto offsets = [&](int i, int e) {
-                const int p = it.p0 + i * S::TK + (lane & (S::TK - 1));
+                const int p = attn_pos(a, it.gap, it.p0 + i * S::TK + (lane & (S::TK - 1)));
                 const int64_t off = (unsigned)e < (unsigned)c.num_pages ? kv_offset(c, e, p, hk) : -1;
                 if (lane < S::TK) lds_off[wave][(i / kAttnWaves) & 1][lane] = off;
                 return __ballot(off < 0) == 0;
@@ -916,12 +619,13 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             const int64_t slot = (int64_t)blockIdx.x + it.row, group = (slot - it.slot) / kJoinGroup;
             const int groups = (it.nc + kJoinGroup - 1) / kJoinGroup;
             const int64_t g0 = it.slot + group * kJoinGroup;
+            auto where = [&](int h) { return AttnPlace{it.row, h0 + h}; };
             const int in_group = (int)min((int64_t)kJoinGroup, it.slot + it.nc - g0);
             if (attention_count(pl.count + g0 * pl.hy + blockIdx.y, in_group, &lds_last)) {
-                attention_join<DP>(a, pl, it.row, g0, 1, in_group, groups == 1, h0, nh, lds_o);
+                attention_join<DP>(a, pl, where, g0, 1, in_group, groups == 1, nh, lds_o);
                 if (groups > 1 &&
                     attention_count(pl.tops + (int64_t)it.row * pl.hy + blockIdx.y, groups, &lds_last))
-                    attention_join<DP>(a, pl, it.row, it.slot, kJoinGroup, groups, true, h0, nh, lds_o);
+                    attention_join<DP>(a, pl, where, it.slot, kJoinGroup, groups, true, nh, lds_o);
             }
         }
         __syncthreads();
@@ -932,7 +636,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
 // (share, kv head), every query head of the group.
 __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int hk) {
     const KvView& c = a.c;
-    const int G = a.hq / c.hkv, sq = a.seq ? a.seq[it.row] : it.row;
+    const int G = a.hq / c.hkv, sq = attn_unit(a, it.row).seq;
     extern __shared__ float hm[];  // [G] maximum, [G] 1 / sum
     for (int h = threadIdx.x; h < G; h += kAttnThreads) {
         const float* ml = pl.ml + 2 * ((int64_t)it.row * a.hq + hk * G + h);
@@ -940,12 +644,12 @@ __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const At
         hm[G + h] = ml[1] == 0.0f ? 0.0f : 1.0f / ml[1];
     }
     __syncthreads();
-    for (int p = it.p0 + threadIdx.x; p < it.p1; p += kAttnThreads) {
-        const int pg = kv_page(c, sq, p);
+    for (int i = it.p0 + threadIdx.x; i < it.p1; i += kAttnThreads) {
+        const int p = attn_pos(a, it.gap, i), pg = kv_page(c, sq, p);
         if (pg < 0) continue;
         float w = 0.0f;
         for (int h = 0; h < G; ++h)
-            w += pow2(pl.s[((int64_t)it.row * a.hq + hk * G + h) * pl.cap + p] - hm[h]) * hm[G + h];
+            w += pow2(pl.s[((int64_t)it.row * a.hq + hk * G + h) * pl.cap + i] - hm[h]) * hm[G + h];
         atomicAdd(&c.score[((int64_t)pg * c.hkv + hk) * c.page + kv_slot(c, p)], w);
     }
 }
@@ -974,29 +678,6 @@ namespace {
 // 190; of 64, 100 with three and 102 with four).
 int resident(int D) { return D > 128 ? 1 : (D > 64 ? 2 : 3); }
 
-AttnPlan make_plan(const AttnArgs& a, int cus) {
-    AttnPlan pl;
-    const int G = a.hq / a.c.hkv;
-    pl.part_o = pl.part_ml = pl.s = pl.ml = nullptr;
-    pl.count = pl.tops = nullptr;
-    pl.dp = (a.c.D + 1) / 2 * 2;
-    pl.tiles = (G + 15) / 16;
-    pl.hy = a.c.hkv * pl.tiles;
-    const int64_t cap = (int64_t)a.c.max_pages * a.c.page;
-    pl.cap = (cap + 31) / 32 * 32;
-    pl.per_row = a.call_rows > kAttnPlanRows;
-    const int64_t steps = a.R * std::max<int64_t>(1, (cap + kAttnStep - 1) / kAttnStep);
-    pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident(a.c.D) * cus / pl.hy));
-    pl.shares = std::min(pl.shares, 64 * kJoinGroup);  // (as many as two levels join)
-    if (pl.per_row) pl.shares = (int)a.R;
-    return pl;
-}
-
-// Whether a row may be in more than one segment.
-bool splits(const AttnArgs& a, const AttnPlan& pl) {
-    return !pl.per_row && (int64_t)a.c.max_pages * a.c.page > kAttnStep;
-}
-
 template <int DT>
 hipError_t launch_attention(const AttnArgs& a, const AttnPlan& pl, hipStream_t s) {
     const dim3 grid((unsigned)pl.shares, (unsigned)pl.hy), block(kAttnThreads);
@@ -1010,39 +691,21 @@ hipError_t launch_attention(const AttnArgs& a, const AttnPlan& pl, hipStream_t s
     return hipGetLastError();
 }
 
-// Bytes of the plan's arrays in one workspace.
-size_t place(const AttnArgs& a, AttnPlan* pl, char* base) {
-    size_t at = 0;
-    auto take = [&](size_t floats) {
-        float* p = reinterpret_cast<float*>(base + at);
-        at += (floats * 4 + 255) / 256 * 256;
-        return p;
-    };
-    const size_t slots = (size_t)pl->shares + (size_t)a.R;
-    if (splits(a, *pl)) {
-        pl->part_ml = take(slots * pl->hy * 32);
-        pl->part_o = take(slots * pl->hy * 16 * pl->dp);
-    }
-    if (a.accumulate) {
-        pl->ml = take((size_t)a.R * a.hq * 2);
-        pl->s = take((size_t)a.R * a.hq * pl->cap);
-    }
-    return at;
-}
-
 }  // namespace
 
+// (a row to a unit: tokens of one sequence share nothing here)
 size_t attention_workspace(const AttnArgs& a, int cus, size_t* counters) {
-    AttnPlan pl = make_plan(a, cus);
-    *counters = splits(a, pl) ? ((size_t)pl.shares + 2 * (size_t)a.R) * pl.hy * sizeof(unsigned) : 0;
-    return place(a, &pl, nullptr);
+    AttnPlan pl = plan_attention(a, cus, 1, resident(a.c.D));
+    *counters = attention_counters(a, pl);
+    return place_attention(a, &pl, attention_splits(a, pl), nullptr);
 }
 
-hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, void* counters, hipStream_t s) {
-    AttnPlan pl = make_plan(a, cus);
-    (void)place(a, &pl, static_cast<char*>(ws));
-    pl.count = static_cast<unsigned*>(counters);
-    pl.tops = pl.count + ((size_t)pl.shares + (size_t)a.R) * pl.hy;
+hipError_t launch_paged_attention(int dtype, AttnArgs a, int cus, void* ws, void* counters, hipStream_t s) {
+    AttnPlan pl = plan_attention(a, cus, 1, resident(a.c.D));
+    attention_memory(a, &pl, ws, counters);
+    a.unit_rows = 1;
+    a.units = a.tokens;
+    a.by_units = fast_div(a.units);
     hipError_t e;
     switch (dtype) {
         case XT_F32: e = launch_attention<XT_F32>(a, pl, s); break;

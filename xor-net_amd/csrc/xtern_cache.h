@@ -1,7 +1,8 @@
-// Internal declarations of the paged key-value cache (append, attention,
-// eviction) and of the token probabilities: kernel arguments and launchers
-// (xtern_attn.hip, xtern_evict.hip, xtern_probs.hip), called by
-// xtern_cache_api.cpp.
+// Internal declarations of the paged key-value cache (append, read-back,
+// attention, eviction), of the token probabilities and of the verification of
+// drafted tokens: kernel arguments and launchers (xtern_attn.hip,
+// xtern_attn8.hip, xtern_store.hip, xtern_evict.hip, xtern_probs.hip,
+// xtern_verify.hip), called by xtern_cache_api.cpp.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stddef.h>
@@ -30,6 +31,8 @@ struct KvView {
     void* k;
     void* v;
     float* score;
+    float* ks;  // 8-bit codes: the scales [num_pages][hkv][page] of keys and of values
+    float* vs;
     int64_t sp, ss, sh;  // element strides of a page, a slot, a head
     int num_pages, page, hkv, D;
     FastDiv by_page;
@@ -56,8 +59,25 @@ struct AppendArgs {
     int hq;
     int64_t R;
     FastDiv by_per, by_vals;  // set by the launcher
+    const float* q_norm;      // [D] weights of a head's norm, or null (no norms)
+    const float* k_norm;
+    double eps;
 };
 hipError_t launch_kv_append(int dtype, AppendArgs a, hipStream_t s);
+// With norms, or into 8-bit codes; cus: compute units of the device.
+hipError_t launch_kv_store(int dtype, AppendArgs a, int cus, hipStream_t s);
+
+struct ReadArgs {
+    KvView c;
+    const int32_t* seq;    // [R] or null
+    const int32_t* slots;  // [R]
+    void* k;               // [R] rows of hkv * D, strides ldk, ldv
+    void* v;
+    int64_t ldk, ldv;
+    int64_t R;
+    FastDiv by_per;        // set by the launcher
+};
+hipError_t launch_kv_read(int dtype, int out, ReadArgs a, int cus, hipStream_t s);
 
 struct AttnArgs {
     KvView c;
@@ -72,11 +92,19 @@ struct AttnArgs {
     int accumulate;
     int64_t R;
     int64_t call_rows;       // of the call whose rows, or a part of them, these are
+    int window, sink;        // a row of length n sees p < sink and p >= n - window (2^30: every p)
+    int tokens;              // rows r of one sequence: r / tokens
+    // set by the launcher: a sequence's rows, in units of unit_rows
+    int unit_rows, units;
+    FastDiv by_units;
 };
 // Bytes of workspace that the call needs, and of counters that are zero before
 // and after it (0: none, null); cus: compute units of the device.
 size_t attention_workspace(const AttnArgs& a, int cus, size_t* counters);
-hipError_t launch_paged_attention(int dtype, const AttnArgs& a, int cus, void* ws, void* counters, hipStream_t s);
+hipError_t launch_paged_attention(int dtype, AttnArgs a, int cus, void* ws, void* counters, hipStream_t s);
+// The same over a cache of 8-bit codes.
+size_t attention8_workspace(const AttnArgs& a, int cus, size_t* counters);
+hipError_t launch_paged_attention8(AttnArgs a, int cus, void* ws, void* counters, hipStream_t s);
 
 struct EvictArgs {
     KvView c;
@@ -110,6 +138,25 @@ struct ProbsArgs {
 };
 size_t token_logprobs_workspace(const ProbsArgs& a, int cus, size_t* counters);
 hipError_t launch_token_logprobs(int dtype, const ProbsArgs& a, int cus, void* ws, void* counters, hipStream_t s);
+
+constexpr int kVerifyDrafts = 64;  // of a sequence: a lane each
+
+struct VerifyArgs {
+    const void* target;  // [S][T + 1][V], strides in elements
+    const void* draft;   // [S][T][V] or null
+    int64_t ld_seq, ld_row, ldd_seq, ldd_row;
+    int S, T, V;
+    const int32_t* drafted;  // [S][T]
+    const int32_t* counts;   // [S] or null
+    const float* uniforms;   // [S][T + 1]
+    const float* temps;      // [S] or null
+    float temp;
+    int32_t* accepted;       // [S]
+    int32_t* tokens;         // [S][T + 1]
+    float* logprobs;         // [S][T + 1]
+};
+size_t verify_workspace(const VerifyArgs& a, int cus, size_t* counters);
+hipError_t launch_verify(int dtype, const VerifyArgs& a, int cus, void* ws, void* counters, hipStream_t s);
 
 #ifdef __HIPCC__
 }  // namespace xt

@@ -1,5 +1,5 @@
-// C ABI of the paged key-value cache and of the token probabilities
-// (include/xtern.h): argument checks and kernel dispatch.  Every pointer,
+// C ABI of the paged key-value cache, of the token probabilities and of the
+// verification of drafted tokens (include/xtern.h): argument checks and kernel dispatch.  Every pointer,
 // shape and stride is checked here; what only the device knows (lengths,
 // table entries, token ids) the kernels check themselves.
 #include <hip/hip_runtime.h>
@@ -44,16 +44,27 @@ int check_align(const void* p, int size, const char* what) {
     return XT_OK;
 }
 
-// The cache and the table as the kernels see them.  `view` gets every field.
-int check_cache(const xt_kv_cache* c, const xt_kv_table* t, xt::KvView* view) {
+// The cache, its scales (XT_I8) and the table as the kernels see them.  `view`
+// gets every field.
+int check_cache(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t, xt::KvView* view) {
     if (!c || !t) return bad("cache or table is NULL");
-    if (int rc = check_dtype(c->dtype)) return rc;
+    const bool codes = c->dtype == XT_I8;
+    if (codes) {
+        if (!scales) return bad("a cache of 8-bit codes needs its scales");
+        if (!scales->k || !scales->v) return bad("NULL pointer");
+        if (c->score) return bad("a cache of 8-bit codes keeps no score");
+        if (int rc = check_align(scales->k, 4, "the key scales")) return rc;
+        if (int rc = check_align(scales->v, 4, "the value scales")) return rc;
+    } else {
+        if (int rc = check_dtype(c->dtype)) return rc;
+        if (scales) return bad("scales belong to a cache of 8-bit codes");
+    }
     if (c->head_dim < 1 || c->head_dim > 256) return bad("head_dim must be 1..256");
     if (c->kv_heads < 1 || c->kv_heads > 65535) return bad("kv_heads must be 1..65535");
     if (c->page_size < 1 || c->page_size > 65536) return bad("page_size must be 1..65536");
     if (c->num_pages < 1 || c->num_pages > kMaxInt) return bad("num_pages must be 1..2^31-1");
     if (!c->k || !c->v) return bad("NULL pointer");
-    const int es = c->dtype == XT_F32 ? 4 : 2;
+    const int es = codes ? 1 : (c->dtype == XT_F32 ? 4 : 2);
     if (int rc = check_align(c->k, es, "the key cache")) return rc;
     if (int rc = check_align(c->v, es, "the value cache")) return rc;
     if (int rc = check_align(c->score, 4, "the score cache")) return rc;
@@ -80,6 +91,8 @@ int check_cache(const xt_kv_cache* c, const xt_kv_table* t, xt::KvView* view) {
     view->k = c->k;
     view->v = c->v;
     view->score = c->score;
+    view->ks = codes ? scales->k : nullptr;
+    view->vs = codes ? scales->v : nullptr;
     view->sp = c->num_pages == 1 ? 0 : c->stride_page;
     view->ss = c->page_size == 1 ? 0 : c->stride_slot;
     view->sh = c->kv_heads == 1 ? 0 : c->stride_head;
@@ -95,12 +108,22 @@ int check_cache(const xt_kv_cache* c, const xt_kv_table* t, xt::KvView* view) {
     return XT_OK;
 }
 
-// R rows of `cols` f32 elements at stride ld; out: rows that are written.
-int check_rows(const float* p, int64_t ld, int64_t R, int64_t cols, const char* what) {
+// R rows of `cols` elements (f32, or of `size` bytes) at stride ld.
+int check_rows(const void* p, int64_t ld, int64_t R, int64_t cols, const char* what, int size = 4) {
     if (!p) return bad("NULL pointer");
     if (R > 1 && ld < cols) return bad(std::string(what) + " rows overlap");
     if (ld > INT64_MAX / 8 / std::max<int64_t>(R, 1)) return bad(std::string(what) + " stride too large");
-    return check_align(p, 4, what);
+    return check_align(p, size, what);
+}
+
+// [S][rows] rows of V logits of `size` bytes; they may overlap (one row shown to
+// several sequences).
+int check_logits(const void* p, int64_t ld_seq, int64_t ld_row, int64_t S, int64_t rows, int64_t V, const char* what,
+                 int size) {
+    const int64_t most = INT64_MAX / 16;
+    if ((S > 1 && (ld_seq < 0 || ld_seq > most / S)) || (rows > 1 && (ld_row < 0 || ld_row > most / rows)))
+        return bad(std::string(what) + " strides must not be negative or too large");
+    return check_align(p, size, what);
 }
 
 int check_count(int64_t R) {
@@ -140,7 +163,7 @@ void skip_sequences(xt::KvView* c, int64_t at) {
     c->nseq = (int)std::max<int64_t>(0, c->nseq - at);
 }
 
-// Rows [r0, r0 + n) of a call.
+// Rows [r0, r0 + n) of a call, whole groups.
 xt::AttnArgs rows_of(xt::AttnArgs a, int64_t r0, int64_t n) {
     a.R = n;
     a.q += r0 * a.ldq;
@@ -148,7 +171,7 @@ xt::AttnArgs rows_of(xt::AttnArgs a, int64_t r0, int64_t n) {
     if (a.lse) a.lse += r0 * a.hq;
     a.lengths += r0;
     if (a.seq) a.seq += r0;
-    else skip_sequences(&a.c, r0);
+    else skip_sequences(&a.c, r0 / a.tokens);
     return a;
 }
 
@@ -171,25 +194,14 @@ int get_workspace(hipStream_t s, size_t bytes, size_t counters, void** ws, void*
     return counters ? xt_internal_workspace(s, counters, cnt, 4) : XT_OK;
 }
 
-}  // namespace
-
-extern "C" {
-
-int xt_kv_append(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq, const int32_t* slots,
-                 const int32_t* positions, const xt_rope* rope, const float* q, int64_t ldq, int q_heads,
-                 float* q_out, int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv,
-                 int64_t R, void* stream) {
-    return xt_kv_append_lengths(c, t, seq, slots, positions, rope, q, ldq, q_heads, q_out, ldqo, k, ldk, v, ldv, R,
-                                nullptr, stream);
-}
-
-int xt_kv_append_lengths(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq, const int32_t* slots,
-                         const int32_t* positions, const xt_rope* rope, const float* q, int64_t ldq, int q_heads,
-                         float* q_out, int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv,
-                         int64_t R, int32_t* lengths, void* stream) {
-    xt::AppendArgs a;
+// The arguments of an append, of R > 0 rows where it returns XT_OK.
+int append_args(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t, const int32_t* seq,
+                const int32_t* slots, const int32_t* positions, const xt_rope* rope, const xt_head_norm* norm,
+                const float* q, int64_t ldq, int q_heads, float* q_out, int64_t ldqo, const float* k, int64_t ldk,
+                const float* v, int64_t ldv, int64_t R, int32_t* lengths, xt::AppendArgs* args) {
+    xt::AppendArgs& a = *args;
     memset(&a, 0, sizeof a);
-    if (int rc = check_cache(c, t, &a.c)) return rc;
+    if (int rc = check_cache(c, scales, t, &a.c)) return rc;
     if (int rc = check_count(R)) return rc;
     if (q) {
         if (int rc = check_heads(q_heads, c->kv_heads)) return rc;
@@ -201,6 +213,12 @@ int xt_kv_append_lengths(const xt_kv_cache* c, const xt_kv_table* t, const int32
         if (!rope->cos || !rope->sin) return bad("NULL pointer");
         if (int rc = check_align(rope->cos, 4, "cos")) return rc;
         if (int rc = check_align(rope->sin, 4, "sin")) return rc;
+    }
+    if (norm) {
+        if (!norm->k || (q && !norm->q)) return bad("NULL pointer");
+        if (!(norm->eps >= 0.0) || !isfinite(norm->eps)) return bad("norm eps must be finite, >= 0");
+        if (int rc = check_align(norm->q, 4, "the query norm")) return rc;
+        if (int rc = check_align(norm->k, 4, "the key norm")) return rc;
     }
     if (R == 0) return XT_OK;
     if (!slots) return bad("NULL pointer");
@@ -235,16 +253,95 @@ int xt_kv_append_lengths(const xt_kv_cache* c, const xt_kv_table* t, const int32
     a.ldk = ldk;
     a.ldv = ldv;
     a.R = R;
+    if (norm) {
+        a.q_norm = norm->q;
+        a.k_norm = norm->k;
+        a.eps = norm->eps;
+    }
+    return XT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int xt_kv_append(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq, const int32_t* slots,
+                 const int32_t* positions, const xt_rope* rope, const float* q, int64_t ldq, int q_heads,
+                 float* q_out, int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv,
+                 int64_t R, void* stream) {
+    return xt_kv_append_lengths(c, t, seq, slots, positions, rope, q, ldq, q_heads, q_out, ldqo, k, ldk, v, ldv, R,
+                                nullptr, stream);
+}
+
+int xt_kv_append_lengths(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq, const int32_t* slots,
+                         const int32_t* positions, const xt_rope* rope, const float* q, int64_t ldq, int q_heads,
+                         float* q_out, int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv,
+                         int64_t R, int32_t* lengths, void* stream) {
+    xt::AppendArgs a;
+    if (int rc = append_args(c, nullptr, t, seq, slots, positions, rope, nullptr, q, ldq, q_heads, q_out, ldqo, k, ldk,
+                             v, ldv, R, lengths, &a))
+        return rc;
+    if (R == 0) return XT_OK;
     return launched(xt::launch_kv_append(c->dtype, a, static_cast<hipStream_t>(stream)), "cache append launch");
+}
+
+int xt_kv_store(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t, const int32_t* seq,
+                const int32_t* slots, const int32_t* positions, const xt_rope* rope, const xt_head_norm* norm,
+                const float* q, int64_t ldq, int q_heads, float* q_out, int64_t ldqo, const float* k, int64_t ldk,
+                const float* v, int64_t ldv, int64_t R, int32_t* lengths, void* stream) {
+    xt::AppendArgs a;
+    if (int rc = append_args(c, scales, t, seq, slots, positions, rope, norm, q, ldq, q_heads, q_out, ldqo, k, ldk, v,
+                             ldv, R, lengths, &a))
+        return rc;
+    if (R == 0) return XT_OK;
+    int cus = 0;
+    if (int rc = xt_internal_cus(&cus)) return rc;
+    return launched(xt::launch_kv_store(c->dtype, a, cus, static_cast<hipStream_t>(stream)), "cache store launch");
+}
+
+int xt_kv_read(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t, const int32_t* seq,
+               const int32_t* slots, int64_t R, int out, void* k, int64_t ldk, void* v, int64_t ldv, void* stream) {
+    xt::ReadArgs a;
+    memset(&a, 0, sizeof a);
+    if (int rc = check_cache(c, scales, t, &a.c)) return rc;
+    if (int rc = check_dtype(out)) return rc;
+    if (int rc = check_count(R)) return rc;
+    if (R == 0) return XT_OK;
+    if (!slots) return bad("NULL pointer");
+    const int64_t cols = (int64_t)c->kv_heads * c->head_dim;
+    const int es = out == XT_F32 ? 4 : 2;
+    if (int rc = check_rows(k, ldk, R, cols, "k", es)) return rc;
+    if (int rc = check_rows(v, ldv, R, cols, "v", es)) return rc;
+    a.seq = seq;
+    a.slots = slots;
+    a.k = k;
+    a.v = v;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.R = R;
+    int cus = 0;
+    if (int rc = xt_internal_cus(&cus)) return rc;
+    return launched(xt::launch_kv_read(c->dtype, out, a, cus, static_cast<hipStream_t>(stream)), "cache read launch");
 }
 
 int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* seq, const int32_t* lengths,
                        const float* q, int64_t ldq, int q_heads, float scale, int64_t R, float* out, int64_t ldo,
                        float* lse, int accumulate, void* stream) {
+    return xt_paged_attention_window(c, nullptr, t, seq, lengths, 1, 0, 0, q, ldq, q_heads, scale, R, out, ldo, lse,
+                                     accumulate, stream);
+}
+
+int xt_paged_attention_window(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t,
+                              const int32_t* seq, const int32_t* lengths, int64_t tokens, int64_t window,
+                              int64_t sink, const float* q, int64_t ldq, int q_heads, float scale, int64_t R,
+                              float* out, int64_t ldo, float* lse, int accumulate, void* stream) {
     xt::AttnArgs a;
     memset(&a, 0, sizeof a);
-    if (int rc = check_cache(c, t, &a.c)) return rc;
+    if (int rc = check_cache(c, scales, t, &a.c)) return rc;
     if (int rc = check_count(R)) return rc;
+    if (tokens < 1 || tokens > 65536 || R % tokens) return bad("tokens must be 1..65536, a divisor of the rows");
+    if (window < 0 || window > kMaxLen || sink < 0 || sink > kMaxLen) return bad("window and sink must be 0..2^30");
+    if (sink && !window) return bad("sink without a window");
     if (int rc = check_heads(q_heads, c->kv_heads)) return rc;
     // (the kernels work with scale in base 2)
     if (!isfinite((float)((double)scale * 1.4426950408889634))) return bad("scale must be finite, at most 2.3e38");
@@ -269,10 +366,13 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     a.ldo = ldo;
     a.lse = lse;
     a.accumulate = accumulate ? 1 : 0;
+    a.window = (int)(window ? window : kMaxLen);
+    a.sink = (int)sink;
+    a.tokens = (int)tokens;
     int64_t part = R;  // rows at a time
     if (a.accumulate) {
         const int64_t row = 4 * (int64_t)q_heads * t->max_pages * c->page_size;
-        part = part_of(R, row);
+        part = part_of(R / tokens, row * tokens) * tokens;
         if (int rc = check_fits((double)part * (double)row, "the workspace")) return rc;
     }
     int cus = 0;
@@ -281,13 +381,16 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
     void *ws, *counters;
     size_t nc, nc_last;
     const xt::AttnArgs last = rows_of(a, (R - 1) / part * part, R - (R - 1) / part * part);
-    const size_t bytes_last = xt::attention_workspace(last, cus, &nc_last);
-    const size_t bytes = std::max(bytes_last, xt::attention_workspace(rows_of(a, 0, part), cus, &nc));
+    const bool codes = c->dtype == XT_I8;
+    const auto workspace = codes ? xt::attention8_workspace : xt::attention_workspace;
+    const size_t bytes_last = workspace(last, cus, &nc_last);
+    const size_t bytes = std::max(bytes_last, workspace(rows_of(a, 0, part), cus, &nc));
     if (int rc = get_workspace(st, bytes, std::max(nc, nc_last), &ws, &counters)) return rc;
     for (int64_t r0 = 0; r0 < R; r0 += part) {
         const xt::AttnArgs b = rows_of(a, r0, std::min(part, R - r0));
-        if (int rc = launched(xt::launch_paged_attention(c->dtype, b, cus, ws, counters, st), "paged attention launch"))
-            return rc;
+        const hipError_t e = codes ? xt::launch_paged_attention8(b, cus, ws, counters, st)
+                                   : xt::launch_paged_attention(c->dtype, b, cus, ws, counters, st);
+        if (int rc = launched(e, "paged attention launch")) return rc;
     }
     return XT_OK;
 }
@@ -296,7 +399,7 @@ int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengt
                 int64_t recent, int32_t* new_lengths, int32_t* kept, void* stream) {
     xt::EvictArgs a;
     memset(&a, 0, sizeof a);
-    if (int rc = check_cache(c, t, &a.c)) return rc;
+    if (int rc = check_cache(c, nullptr, t, &a.c)) return rc;
     if (!c->score) return bad("eviction needs a cache with scores");
     if (budget < 1 || budget > kMaxInt) return bad("budget must be 1..2^31-1");
     if (sink < 0 || recent < 0 || sink > budget || recent > budget - sink)
@@ -363,6 +466,58 @@ int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int6
     if (int rc = get_workspace(st, bytes, nc, &ws, &counters)) return rc;
     return launched(xt::launch_token_logprobs(dtype, a, cus, ws, counters, st),
                     "token probabilities launch");
+}
+
+int xt_verify_drafts(int dtype, const void* target, int64_t ld_seq, int64_t ld_row, const void* draft, int64_t ldd_seq,
+                     int64_t ldd_row, int64_t S, int64_t T, int64_t V, const int32_t* drafted, const int32_t* counts,
+                     const float* uniforms, float temperature, const float* temperatures, int32_t* accepted,
+                     int32_t* tokens, float* logprobs, void* stream) {
+    if (int rc = check_dtype(dtype)) return rc;
+    if (T < 0 || T > xt::kVerifyDrafts) return bad("drafts of a sequence must be 0..64");
+    if (S < 0 || S * (2 * T + 1) > kMaxRows || S > kMaxRows) return bad("sequences times 2 drafts + 1 must be 0..2^21");
+    if (V < 1 || V > (1 << 30)) return bad("vocabulary must be 1..2^30");
+    if (!temperatures && !(temperature >= 0.0f && isfinite(temperature))) return bad("temperature must be finite, >= 0");
+    if (S == 0) return XT_OK;
+    if (!target || !uniforms || !accepted || !tokens || !logprobs || (T > 0 && !drafted)) return bad("NULL pointer");
+    const int es = dtype == XT_F32 ? 4 : 2;
+    if (int rc = check_logits(target, ld_seq, ld_row, S, T + 1, V, "target", es)) return rc;
+    if (draft && T > 0) {
+        if (int rc = check_logits(draft, ldd_seq, ldd_row, S, T, V, "draft", es)) return rc;
+    }
+    const struct {
+        const void* p;
+        const char* what;
+    } words[] = {{drafted, "drafted"},   {counts, "counts"}, {uniforms, "uniforms"}, {temperatures, "temperatures"},
+                 {accepted, "accepted"}, {tokens, "tokens"}, {logprobs, "logprobs"}};
+    for (const auto& w : words)
+        if (int rc = check_align(w.p, 4, w.what)) return rc;
+    xt::VerifyArgs a;
+    memset(&a, 0, sizeof a);
+    a.target = target;
+    a.draft = T > 0 ? draft : nullptr;
+    a.ld_seq = S > 1 ? ld_seq : 0;
+    a.ld_row = T > 0 ? ld_row : 0;
+    a.ldd_seq = S > 1 ? ldd_seq : 0;
+    a.ldd_row = T > 1 ? ldd_row : 0;
+    a.S = (int)S;
+    a.T = (int)T;
+    a.V = (int)V;
+    a.drafted = drafted;
+    a.counts = counts;
+    a.uniforms = uniforms;
+    a.temps = temperatures;
+    a.temp = temperature;
+    a.accepted = accepted;
+    a.tokens = tokens;
+    a.logprobs = logprobs;
+    int cus = 0;
+    if (int rc = xt_internal_cus(&cus)) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    void *ws, *counters;
+    size_t nc;
+    const size_t bytes = xt::verify_workspace(a, cus, &nc);
+    if (int rc = get_workspace(st, bytes, nc, &ws, &counters)) return rc;
+    return launched(xt::launch_verify(dtype, a, cus, ws, counters, st), "draft verification launch");
 }
 
 }  // extern "C"

@@ -1,0 +1,297 @@
+// New tokens into a paged cache with norms of their heads and, for a cache of
+// 8-bit codes, a scale for each token and head; and cached positions read back.
+#include <algorithm>
+
+#include "xtern_cache.h"
+
+namespace xt {
+
+// A head x of D elements, of q and k with weights w and eps:
+//   y_i = w_i x_i / sqrt(sum x^2 / D + eps)        (no norm: y = x)
+// then the rotation of the pairs i, i + h as in kv_append_kernel; of v: y = x.
+// q_out = y.  A cache of 8-bit codes holds y as c = round(y / s), s = a / 127
+// rounded to f32, a = max |y| of the head as f32: |c| <= 127 and |c s - y| <=
+// s / 2.  Below a = 2^-119 (1 / s would leave f32's normal numbers) s and c are
+// 0; a head with an infinity or NaN has s = NaN, c = 0, so that what reads it
+// sees NaN.
+//
+// All of it in 64 bits, rounded once (to f32, then to the cache's type): a value
+// next to the border of two codes falls where the exact one does, in whatever
+// order sums are taken.  The f64 units take 4 cycles an instruction like the
+// f32 ones, and a call is bound by its bytes or by its launch.
+//
+// A head is 16, 32 or 64 lanes of one wave, W = 4 elements each (D and h
+// multiples of four; no alignment is needed), or 64 lanes of every 64th
+// element; each lane also loads the elements that its own are rotated with.  The
+// heads of a row go to several workgroups where rows are few.
+template <int DT> struct Held;
+template <> struct Held<XT_I8> { typedef int8_t T; };
+template <> struct Held<XT_F32> { typedef float T; };
+template <> struct Held<XT_F16> { typedef _Float16 T; };
+template <> struct Held<XT_BF16> { typedef __bf16 T; };
+
+constexpr int kStoreThreads = 256;
+constexpr float kLeastHead = 0x1p-119f;
+
+template <typename T>
+__device__ __forceinline__ T lanes_sum(T v, int lanes) {
+    for (int o = lanes / 2; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ unsigned lanes_max(unsigned v, int lanes) {
+    for (int o = lanes / 2; o; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
+    return v;
+}
+
+template <int DT, int W>
+__global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a, int lanes) {
+    typedef typename Held<DT>::T T;
+    typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+    const KvView& c = a.c;
+    const int64_t r = blockIdx.x;
+    const int slot = a.slots[r];
+    const int sq = a.seq ? a.seq[r] : (int)r;
+    const int pos = a.cos ? a.pos[r] : 0;
+    int pg = -1;
+    if (slot >= 0 && slot < (int64_t)c.max_pages * c.page && (unsigned)sq < (unsigned)c.nseq &&
+        (!a.cos || (pos >= 0 && pos < a.rope_rows)))
+        pg = kv_page(c, sq, slot);
+    if (a.lengths && blockIdx.y == 0 && threadIdx.x == 0) a.lengths[r] = pg < 0 ? 0 : slot + 1;
+    if (pg < 0) return;
+    if (c.score && blockIdx.y == 0)
+        for (int h = threadIdx.x; h < c.hkv; h += kStoreThreads)
+            c.score[((int64_t)pg * c.hkv + h) * c.page + kv_slot(c, slot)] = 0.0f;
+    const int D = c.D, half = a.cos ? a.rot / 2 : 0, hq = a.q ? a.hq : 0;
+    const int l = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = kStoreThreads / lanes;
+    const int64_t at = kv_offset(c, pg, slot, 0);
+    // element e of the lane; what it is rotated with, and by which pair
+    int d[4], other[4], pair[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        d[e] = W == 4 ? 4 * l + e : l + 64 * e;
+        other[e] = d[e] < half ? d[e] + half : d[e] - half;
+        pair[e] = d[e] < half ? d[e] : d[e] - half;
+    }
+    // The four elements at i[0], side by side, or those of them that are of the head
+    auto get = [&](const float* p, const int* i, float* x) {
+        if constexpr (W == 4) {
+            const F4 v = *reinterpret_cast<const F4*>(p + i[0]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = d[e] < D ? p[i[e]] : 0.0f;
+        }
+    };
+    const bool any = W == 4 ? d[0] < D : true;  // (W 4: all four or none)
+    // (d and half are multiples of four then: one test for the lane)
+    auto turns = [&](int e) { return d[W == 4 ? 0 : e] < 2 * half; };
+    for (int h = blockIdx.y * groups + group; h < hq + 2 * c.hkv; h += gridDim.y * groups) {
+        const bool isq = h < hq, isv = h >= hq + c.hkv;
+        const int head = isq ? h : (isv ? h - hq - c.hkv : h - hq);
+        const float* src = (isq ? a.q + r * a.ldq : (isv ? a.v + r * a.ldv : a.k + r * a.ldk)) + (int64_t)head * D;
+        const float* w = isq ? a.q_norm : (isv ? nullptr : a.k_norm);
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (any) get(src, d, x);
+        double y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = x[e];
+        double inv = 1.0;
+        if (w) {
+            const double sum = lanes_sum(fma(y[0], y[0], fma(y[1], y[1], fma(y[2], y[2], y[3] * y[3]))), lanes);
+            inv = 1.0 / sqrt(sum / D + a.eps);
+            if (any) {
+                float g[4];
+                get(w, d, g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = y[e] * inv * g[e];
+            }
+        }
+        if (half && !isv && any) {
+            float z[4], g[4] = {1.0f, 1.0f, 1.0f, 1.0f}, cs[4], sn[4];
+            int o[4], p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[e] = turns(e) ? other[e] : d[e];
+                p[e] = turns(e) ? pair[e] : 0;
+            }
+            get(src, o, z);
+            if (w) get(w, o, g);
+            get(a.cos + (int64_t)pos * half, p, cs);
+            get(a.sin + (int64_t)pos * half, p, sn);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const double u = (double)z[e] * inv * g[e];
+                const double t = d[e] < half ? -(u * sn[e]) : u * sn[e];
+                if (turns(e)) y[e] = fma(y[e], (double)cs[e], t);
+            }
+        }
+        float f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = (float)y[e];
+        if (isq) {
+            float* to = a.qo + r * a.ldqo + (int64_t)head * D;
+            if constexpr (W == 4) {
+                if (any) *reinterpret_cast<F4*>(to + d[0]) = F4{f[0], f[1], f[2], f[3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d[e] < D) to[d[e]] = f[e];
+            }
+            continue;
+        }
+        T* to = static_cast<T*>(isv ? c.v : c.k) + at + head * c.sh;
+        T held[4];
+        if constexpr (DT == XT_I8) {
+            unsigned top = 0;  // (as whole numbers: NaN above infinity above the rest)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d[e] < D) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+            const float m = __uint_as_float(lanes_max(top, lanes));
+            const bool zero = !(m >= kLeastHead && m < INFINITY);  // (or NaN)
+            const float scale = m < kLeastHead ? 0.0f : (m < INFINITY ? (float)((double)m / 127.0) : NAN);
+            const double up = zero ? 0.0 : 1.0 / (double)scale;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) held[e] = zero ? 0 : (int8_t)(int)rint(y[e] * up);
+            if (l == 0) (isv ? c.vs : c.ks)[((int64_t)pg * c.hkv + head) * c.page + kv_slot(c, slot)] = scale;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) held[e] = Elem<DT>::put(f[e]);
+        }
+        if constexpr (W == 4) {
+            typedef T V __attribute__((ext_vector_type(4)));
+            typedef V U __attribute__((aligned(sizeof(T))));
+            if (any) *reinterpret_cast<U*>(to + d[0]) = V{held[0], held[1], held[2], held[3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d[e] < D) to[d[e]] = held[e];
+        }
+    }
+}
+
+// Rows r of k and v: position slots[r] of its sequence, codes times their scale
+// (or elements) rounded to the output's type; zeros for a row that names no
+// position.  Bound by HBM: a workgroup takes N rows, whose places N threads look
+// up side by side, then copies them, W elements (16 bytes of output) a thread.
+template <int DT, int OT, int W>
+__global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a, int rows) {
+    typedef typename Held<DT>::T T;
+    typedef typename Elem<OT>::T O;
+    const KvView& c = a.c;
+    constexpr int kMost = 32;
+    __shared__ int64_t off[kMost], sc[kMost];
+    const int64_t r0 = (int64_t)blockIdx.x * rows;
+    const int n = (int)min((int64_t)rows, a.R - r0);
+    if ((int)threadIdx.x < n) {
+        const int64_t r = r0 + threadIdx.x;
+        const int slot = a.slots[r], sq = a.seq ? a.seq[r] : (int)r;
+        int pg = -1;
+        if (slot >= 0 && slot < (int64_t)c.max_pages * c.page && (unsigned)sq < (unsigned)c.nseq) pg = kv_page(c, sq, slot);
+        off[threadIdx.x] = pg < 0 ? -1 : kv_offset(c, pg, slot, 0);
+        sc[threadIdx.x] = pg < 0 ? 0 : (int64_t)pg * c.hkv * c.page + kv_slot(c, slot);
+    }
+    __syncthreads();
+    const int per = c.D / W, row = c.hkv * per, both = 2 * row;
+    // threads of a row: as many as it has pieces, rounded up to a power of two
+    const int lg = min(8, 32 - __builtin_clz(both - 1)), step = 256 >> lg;
+    typedef T V __attribute__((ext_vector_type(W)));
+    typedef V VU __attribute__((aligned(sizeof(T))));
+    typedef O X __attribute__((ext_vector_type(W)));
+    typedef X XU __attribute__((aligned(sizeof(O))));
+    for (int x = threadIdx.x >> lg; x < n; x += step) {
+        for (int j = threadIdx.x & ((1 << lg) - 1); j < both; j += 1 << lg) {
+            const bool isv = j >= row;
+            const int k = isv ? j - row : j, h = fast_quot(k, a.by_per), e = (k - h * per) * W;
+            O* out = static_cast<O*>(isv ? a.v : a.k) + (r0 + x) * (isv ? a.ldv : a.ldk) + (int64_t)h * c.D + e;
+            X y;
+            if (off[x] < 0) {
+#pragma unroll
+                for (int u = 0; u < W; ++u) y[u] = Elem<OT>::put(0.0f);
+            } else {
+                const V v = *reinterpret_cast<const VU*>(static_cast<const T*>(isv ? c.v : c.k) + off[x] + h * c.sh + e);
+                [[maybe_unused]] float s = 1.0f;
+                if constexpr (DT == XT_I8) s = (isv ? c.vs : c.ks)[sc[x] + (int64_t)h * c.page];
+#pragma unroll
+                for (int u = 0; u < W; ++u) {
+                    if constexpr (DT == XT_I8) {
+                        float f = s * (float)v[u];
+                        // (an f32 of its own: with one element a thread the
+                        // compiler would round the product to f16 at once)
+                        asm("" : "+v"(f));
+                        y[u] = Elem<OT>::put(f);
+                    } else {
+                        y[u] = Elem<OT>::put(Elem<DT>::get(v[u]));
+                    }
+                }
+            }
+            *reinterpret_cast<XU*>(out) = y;
+        }
+    }
+}
+
+namespace {
+
+template <int DT>
+hipError_t launch_store(AppendArgs& a, int cus, hipStream_t s) {
+    const int half = a.cos ? a.rot / 2 : 0, D = a.c.D;
+    const bool wide = D % 4 == 0 && half % 4 == 0;
+    const int lanes = !wide || D > 128 ? 64 : (D > 64 ? 32 : 16), groups = kStoreThreads / lanes;
+    const int64_t heads = (a.q ? a.hq : 0) + 2 * (int64_t)a.c.hkv;
+    // workgroups of a row: until two per compute unit
+    const int64_t want = std::max<int64_t>(1, 2 * (int64_t)cus / a.R);
+    const dim3 grid((unsigned)a.R, (unsigned)std::min((heads + groups - 1) / groups, want));
+    if (wide)
+        kv_store_kernel<DT, 4><<<grid, kStoreThreads, 0, s>>>(a, lanes);
+    else
+        kv_store_kernel<DT, 1><<<grid, kStoreThreads, 0, s>>>(a, lanes);
+    return hipGetLastError();
+}
+
+template <int DT, int OT>
+hipError_t launch_read(ReadArgs& a, int cus, hipStream_t s) {
+    constexpr int kWide = OT == XT_F32 ? 4 : 8;
+    const int w = a.c.D % kWide == 0 ? kWide : 1;
+    a.by_per = fast_div(a.c.D / w);
+    const int64_t both = 2 * (int64_t)a.c.hkv * (a.c.D / w);
+    // rows until eight workgroups per compute unit, or 16 elements a thread
+    const int rows = (int)std::max<int64_t>(
+        1, std::min<int64_t>(std::min<int64_t>(32, 4096 / both), a.R / (8 * (int64_t)cus)));
+    const unsigned grid = (unsigned)((a.R + rows - 1) / rows);
+    if (w > 1)
+        kv_read_kernel<DT, OT, kWide><<<grid, 256, 0, s>>>(a, rows);
+    else
+        kv_read_kernel<DT, OT, 1><<<grid, 256, 0, s>>>(a, rows);
+    return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_read_as(int out, ReadArgs& a, int cus, hipStream_t s) {
+    switch (out) {
+        case XT_F32: return launch_read<DT, XT_F32>(a, cus, s);
+        case XT_F16: return launch_read<DT, XT_F16>(a, cus, s);
+        default: return launch_read<DT, XT_BF16>(a, cus, s);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_kv_store(int dtype, AppendArgs a, int cus, hipStream_t s) {
+    switch (dtype) {
+        case XT_F32: return launch_store<XT_F32>(a, cus, s);
+        case XT_F16: return launch_store<XT_F16>(a, cus, s);
+        case XT_BF16: return launch_store<XT_BF16>(a, cus, s);
+        default: return launch_store<XT_I8>(a, cus, s);
+    }
+}
+
+hipError_t launch_kv_read(int dtype, int out, ReadArgs a, int cus, hipStream_t s) {
+    switch (dtype) {
+        case XT_F32: return launch_read_as<XT_F32>(out, a, cus, s);
+        case XT_F16: return launch_read_as<XT_F16>(out, a, cus, s);
+        case XT_BF16: return launch_read_as<XT_BF16>(out, a, cus, s);
+        default: return launch_read_as<XT_I8>(out, a, cus, s);
+    }
+}
+
+}  // namespace xt

@@ -753,8 +753,8 @@ def linear_multi_q(ws, q, inv, stream=None):
     return ys
 
 
-from .cache import (XT_F32, XT_F16, XT_BF16, KvCache, kv_append, kv_evict,  # noqa: E402,F401
-                    paged_attention, token_logprobs)
+from .cache import (XT_F32, XT_F16, XT_BF16, XT_I8, KvCache, kv_append, kv_evict, kv_read,  # noqa: E402,F401
+                    paged_attention, token_logprobs, verify_drafts)
 from .layers import (TernaryLinear, DynamicLinear, TernaryRep, FastRmsNorm, Mlp,  # noqa: E402,F401
                      Int8Linear, Int4Linear, CausalSelfAttention)
 

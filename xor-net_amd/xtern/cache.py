@@ -1,5 +1,6 @@
-"""The paged key-value cache and token probabilities over the C ABI: append,
-attention, eviction (xt_kv_*, xt_paged_attention) and xt_token_logprobs.
+"""The paged key-value cache, token probabilities and the verification of
+drafted tokens over the C ABI: append, read-back, attention, eviction (xt_kv_*,
+xt_paged_attention), xt_token_logprobs and xt_verify_drafts.
 
 Tensors are on the current device; a call runs on torch's current stream or
 on `stream`.  With a `stream` of its own, results are allocated on that
@@ -10,6 +11,7 @@ import ctypes
 from . import XT_ERR_INVALID, XternError, _check, _cur_device, _i64, _lib, _stream_ptr, _torch, _torch_mod, _vp
 
 XT_F32, XT_F16, XT_BF16 = 0, 1, 2
+XT_I8 = 3  # of a cache alone
 
 
 class _KvCache(ctypes.Structure):
@@ -29,10 +31,28 @@ class _Rope(ctypes.Structure):
     _fields_ = [("cos", _vp), ("sin", _vp), ("rows", _i64), ("dim", ctypes.c_int)]
 
 
-_cache_p, _table_p, _rope_p = (ctypes.POINTER(t) for t in (_KvCache, _KvTable, _Rope))
+class _KvScales(ctypes.Structure):
+    """struct xt_kv_scales."""
+    _fields_ = [("k", _vp), ("v", _vp)]
+
+
+class _HeadNorm(ctypes.Structure):
+    """struct xt_head_norm."""
+    _fields_ = [("q", _vp), ("k", _vp), ("eps", ctypes.c_double)]
+
+
+_cache_p, _table_p, _rope_p, _scales_p, _norm_p = (ctypes.POINTER(t) for t in (_KvCache, _KvTable, _Rope, _KvScales,
+                                                                               _HeadNorm))
 _lib.xt_kv_append.argtypes = [_cache_p, _table_p, _vp, _vp, _vp, _rope_p, _vp, _i64, ctypes.c_int, _vp, _i64,
                               _vp, _i64, _vp, _i64, _i64, _vp]
 _lib.xt_kv_append_lengths.argtypes = _lib.xt_kv_append.argtypes[:-1] + [_vp, _vp]
+_lib.xt_kv_store.argtypes = [_cache_p, _scales_p, _table_p, _vp, _vp, _vp, _rope_p, _norm_p, _vp, _i64, ctypes.c_int,
+                             _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp]
+_lib.xt_kv_read.argtypes = [_cache_p, _scales_p, _table_p, _vp, _vp, _i64, ctypes.c_int, _vp, _i64, _vp, _i64, _vp]
+_lib.xt_paged_attention_window.argtypes = [_cache_p, _scales_p, _table_p, _vp, _vp, _i64, _i64, _i64, _vp, _i64,
+                                           ctypes.c_int, ctypes.c_float, _i64, _vp, _i64, _vp, ctypes.c_int, _vp]
+_lib.xt_verify_drafts.argtypes = [ctypes.c_int, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp,
+                                  ctypes.c_float, _vp, _vp, _vp, _vp, _vp]
 _lib.xt_paged_attention.argtypes = [_cache_p, _table_p, _vp, _vp, _vp, _i64, ctypes.c_int, ctypes.c_float, _i64,
                                     _vp, _i64, _vp, ctypes.c_int, _vp]
 _lib.xt_kv_evict.argtypes = [_cache_p, _table_p, _vp, _i64, _i64, _i64, _vp, _vp, _vp]
@@ -46,10 +66,11 @@ def _invalid(msg):
 
 def _torch_types():
     torch = _torch()
-    return torch.int32, torch.float32, {torch.float32: XT_F32, torch.float16: XT_F16, torch.bfloat16: XT_BF16}
+    return (torch.int32, torch.float32, torch.int8,
+            {torch.float32: XT_F32, torch.float16: XT_F16, torch.bfloat16: XT_BF16})
 
 
-_I32, _F32, _DTYPES = _torch_types() if _torch_mod is not None else (None, None, {})
+_I32, _F32, _I8, _DTYPES = _torch_types() if _torch_mod is not None else (None, None, None, {})
 _empty_strided = _torch_mod.empty_strided if _torch_mod is not None else None
 
 
@@ -145,19 +166,23 @@ def _empty(stream, dtype, device, *shape):
 
 class KvCache:
     """A pool of pages (xt_kv_cache): k and v [num_pages, page_size, kv_heads,
-    head_dim] of one type (float32, float16, bfloat16) and of equal strides
-    (any order; head_dim contiguous), score None or [num_pages, kv_heads,
-    page_size] float32, the attention weight each position has received."""
+    head_dim] of one type (float32, float16, bfloat16, int8) and of equal
+    strides (any order; head_dim contiguous), score None or [num_pages,
+    kv_heads, page_size] float32, the attention weight each position has
+    received.  int8 codes need k_scale and v_scale, shaped as score: a code
+    stands for itself times its position's and head's scale; they keep no
+    score."""
 
-    def __init__(self, k, v, score=None):
+    def __init__(self, k, v, score=None, k_scale=None, v_scale=None):
         torch = _torch()
         for t, what in ((k, "k"), (v, "v")):
             if not isinstance(t, torch.Tensor) or not t.is_cuda:
                 raise _invalid(f"{what} must be a CUDA (HIP) tensor")
             if t.dim() != 4:
                 raise _invalid(f"{what} must be [num_pages, page_size, kv_heads, head_dim], got {list(t.shape)}")
-        if k.dtype not in _DTYPES:
-            raise _invalid(f"k must be float32, float16 or bfloat16, got {k.dtype}")
+        codes = k.dtype == torch.int8
+        if not codes and k.dtype not in _DTYPES:
+            raise _invalid(f"k must be float32, float16, bfloat16 or int8, got {k.dtype}")
         if v.dtype != k.dtype or v.shape != k.shape or v.device != k.device:
             raise _invalid("k and v must have one type, shape and device")
         P, page, H, D = k.shape
@@ -165,15 +190,23 @@ class KvCache:
             raise _invalid("head_dim must be contiguous")
         if any(n > 1 and a != b for n, a, b in zip(k.shape, k.stride(), v.stride())):
             raise _invalid("k and v must have equal strides")
-        if score is not None:
-            if not isinstance(score, torch.Tensor) or score.device != k.device:
-                raise _invalid("score must be on the device of k")
-            if score.dtype != torch.float32 or tuple(score.shape) != (P, H, page) or not score.is_contiguous():
-                raise _invalid(f"score must be contiguous float32 [{P}, {H}, {page}]")
-        self.k, self.v, self.score = k, v, score
+        if codes and score is not None:
+            raise _invalid("a cache of 8-bit codes keeps no score")
+        if codes != (k_scale is not None) or codes != (v_scale is not None):
+            raise _invalid("k_scale and v_scale are needed for int8 codes, and only there")
+        for t, what in ((score, "score"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t is None:
+                continue
+            if not isinstance(t, torch.Tensor) or t.device != k.device:
+                raise _invalid(f"{what} must be on the device of k")
+            if t.dtype != torch.float32 or tuple(t.shape) != (P, H, page) or not t.is_contiguous():
+                raise _invalid(f"{what} must be contiguous float32 [{P}, {H}, {page}]")
+        self.k, self.v, self.score, self.k_scale, self.v_scale = k, v, score, k_scale, v_scale
         self.num_pages, self.page_size, self.kv_heads, self.head_dim = P, page, H, D
         self._c = _KvCache(k.data_ptr(), v.data_ptr(), score.data_ptr() if score is not None else None,
-                           _DTYPES[k.dtype], H, D, page, P, k.stride(0), k.stride(1), k.stride(2))
+                           XT_I8 if codes else _DTYPES[k.dtype], H, D, page, P, k.stride(0), k.stride(1), k.stride(2))
+        self._scales = _KvScales(k_scale.data_ptr(), v_scale.data_ptr()) if codes else None
+        self._sref = ctypes.byref(self._scales) if codes else None
         self._device, self._ref = k.get_device(), ctypes.byref(self._c)
 
     @classmethod
@@ -183,8 +216,13 @@ class KvCache:
         dtype = torch.bfloat16 if dtype is None else dtype
         k, v = (torch.zeros((num_pages, kv_heads, page_size, head_dim), dtype=dtype,
                             device=device).transpose(1, 2) for _ in range(2))
-        return cls(k, v, torch.zeros((num_pages, kv_heads, page_size), dtype=torch.float32, device=device)
-                   if score else None)
+        more = lambda want: (torch.zeros((num_pages, kv_heads, page_size), dtype=torch.float32, device=device)  # noqa: E731
+                             if want else None)
+        codes = dtype == torch.int8
+        return cls(k, v, more(score), more(codes), more(codes))
+
+    def _tensors(self):
+        return self.k, self.v, self.score, self.k_scale, self.v_scale
 
     def _on(self, here):
         if self._device != here:
@@ -202,13 +240,16 @@ def _table(table, here):
 
 
 def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=None, q_out=None, stream=None,
-              lengths=None):
+              lengths=None, norm=None):
     """xt_kv_append: R new tokens' k and v (float32 [R, kv_heads, head_dim] or
     [R, kv_heads * head_dim]) into position slots[r] (int32 [R]; -1 skips the
     row) of sequence seq[r] (default r) of table (int32 [seqs, max_pages]).
     rope = (cos, sin), float32 [rows, dim / 2] each, rotates k and q by row
     positions[r] (default slots[r]).  lengths (int32 [R], if given) receives
     what each token sees, slots[r] + 1, or 0 for a row that was skipped.
+    norm = (q weight, k weight, eps), float32 [head_dim] each, norms q's and
+    k's heads before the rotation (xt_kv_store, as for an int8 cache, which gets
+    codes and a scale for each token and head).
     Returns the rotated q (q_out if given, which may be q), or None without q."""
     here, D = _here(), cache.head_dim
     c = cache._on(here)
@@ -232,6 +273,11 @@ def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=
         if cos.dim() != 2 or not cos.is_contiguous():
             raise _invalid("cos must be contiguous [rows, dim / 2]")
         rp = ctypes.byref(_Rope(cp, _vec(sin, _F32, "sin", cos.shape, here), cos.shape[0], 2 * cos.shape[1]))
+    hp = None
+    if norm is not None:
+        wq, wk, eps = norm
+        hp = ctypes.byref(_HeadNorm(_vec(wq, _F32, "the query norm", (D,), here) if wq is not None else None,
+                                    _vec(wk, _F32, "the key norm", (D,), here), eps))
     qp = op = None
     ldq = ldo = hq = 0
     if q is not None:
@@ -242,30 +288,76 @@ def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=
     elif q_out is not None:
         raise _invalid("q_out without q")
     if stream is not None:
-        _mark(stream, cache.k, cache.v, cache.score, table, slots, k, v, q, seq, positions, q_out, lengths, *(rope or ()))
+        _mark(stream, *cache._tensors(), table, slots, k, v, q, seq, positions, q_out, lengths, *(rope or ()),
+              *(norm or ())[:2])
+    if hp is not None or cache._sref is not None:
+        _check(_lib.xt_kv_store(c, cache._sref, t, np_, sp, pp, rp, hp, qp, ldq, hq, op, ldo, kp, ldk, vp, ldv, R, lp,
+                                _stream_ptr(stream)))
+        return q_out
     _check(_lib.xt_kv_append_lengths(c, t, np_, sp, pp, rp, qp, ldq, hq, op, ldo, kp, ldk, vp, ldv, R, lp,
                                      _stream_ptr(stream)))
     return q_out
 
 
+def kv_read(cache, table, slots, seq=None, dtype=None, stream=None):
+    """xt_kv_read: keys and values of R positions as the cache holds them, row r
+    of position slots[r] (int32 [R]) of sequence seq[r] (default r) of table
+    (int32 [seqs, max_pages]), zeros where there is none.  Returns (k, v) [R,
+    kv_heads, head_dim] of dtype (float32, the default, float16 or bfloat16)."""
+    here, D = _here(), cache.head_dim
+    c = cache._on(here)
+    t, S = _table(table, here)
+    if getattr(slots, "ndim", 1) != 1:
+        raise _invalid(f"slots must be [rows], got {list(slots.shape)}")
+    sp = _vec(slots, _I32, "slots", getattr(slots, "shape", None), here)
+    R = slots.shape[0]
+    if seq is not None:
+        np_ = _vec(seq, _I32, "seq", (R,), here)
+    elif R > S:
+        raise _invalid(f"{R} rows for {S} sequences: seq is needed")
+    else:
+        np_ = None
+    dtype = _F32 if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise _invalid(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    k, v = (_empty(stream, dtype, slots.device, R, cache.kv_heads, D) for _ in range(2))
+    if stream is not None:
+        _mark(stream, *cache._tensors(), table, slots, seq)
+    ld = cache.kv_heads * D
+    _check(_lib.xt_kv_read(c, cache._sref, t, np_, sp, R, _DTYPES[dtype], k.data_ptr(), ld, v.data_ptr(), ld,
+                           _stream_ptr(stream)))
+    return k, v
+
+
 def paged_attention(cache, table, lengths, q, seq=None, scale=None, lse=False, accumulate=False, out=None,
-                    stream=None):
+                    stream=None, window=None, sink=0, tokens=1):
     """xt_paged_attention: row r of q (float32 [R, q_heads, head_dim] or [R,
     q_heads * head_dim]) attends over the first lengths[r] (int32 [R])
     positions of sequence seq[r] (default r) of table (int32 [seqs,
     max_pages]).  scale defaults to head_dim ** -0.5.  Returns out (which may
     be q), shaped as q, or (out, lse [R, q_heads]) with lse=True; accumulate=True adds the
-    weights to cache.score."""
+    weights to cache.score.
+    xt_paged_attention_window: of those positions a row sees the newest `window`
+    (1..2^30) and the first `sink`; groups of `tokens` rows belong to one
+    sequence, the one that seq names for the group's first row (default: group
+    g to sequence g), and share passes over an int8 cache."""
     here, D = _here(), cache.head_dim
     c = cache._on(here)
     t, S = _table(table, here)
     qp, ldq, hq = _head_rows(q, "q", D, here)
     R = q.shape[0]
     lp = _vec(lengths, _I32, "lengths", (R,), here)
+    if window is not None and not 1 <= window <= 1 << 30:
+        raise _invalid("window must be 1..2^30")
+    if not 0 <= sink <= 1 << 30 or (sink and window is None):
+        raise _invalid("sink must be 0..2^30, and 0 without a window")
+    if not 1 <= tokens <= 65536 or R % tokens:
+        raise _invalid("tokens must be 1..65536, a divisor of the rows")
     if seq is not None:
         sp = _vec(seq, _I32, "seq", (R,), here)
-    elif R > S:
-        raise _invalid(f"{R} rows for {S} sequences: seq is needed")
+    elif R > S * tokens:
+        raise _invalid(f"{R // tokens} groups of rows for {S} sequences: seq is needed" if tokens > 1 else
+                       f"{R} rows for {S} sequences: seq is needed")
     else:
         sp = None
     if out is None:
@@ -273,9 +365,15 @@ def paged_attention(cache, table, lengths, q, seq=None, scale=None, lse=False, a
     op, ldo, _ = _head_rows(out, "out", D, here, R, hq)
     l = _empty(stream, _F32, q.device, R, hq) if lse else None
     if stream is not None:
-        _mark(stream, cache.k, cache.v, cache.score, table, lengths, q, seq, out)
-    _check(_lib.xt_paged_attention(c, t, sp, lp, qp, ldq, hq, D ** -0.5 if scale is None else scale, R, op, ldo,
-                                   l.data_ptr() if lse else None, 1 if accumulate else 0, _stream_ptr(stream)))
+        _mark(stream, *cache._tensors(), table, lengths, q, seq, out)
+    scale = D ** -0.5 if scale is None else scale
+    if window is None and tokens == 1 and cache._sref is None:
+        _check(_lib.xt_paged_attention(c, t, sp, lp, qp, ldq, hq, scale, R, op, ldo, l.data_ptr() if lse else None,
+                                       1 if accumulate else 0, _stream_ptr(stream)))
+    else:
+        _check(_lib.xt_paged_attention_window(c, cache._sref, t, sp, lp, tokens, window or 0, sink, qp, ldq, hq, scale,
+                                              R, op, ldo, l.data_ptr() if lse else None, 1 if accumulate else 0,
+                                              _stream_ptr(stream)))
     return (out, l) if lse else out
 
 
@@ -335,3 +433,54 @@ def token_logprobs(logits, tokens=None, top=0, stream=None):
                                   entropy.data_ptr(), top, ids.data_ptr() if top else None,
                                   best.data_ptr() if top else None, _stream_ptr(stream)))
     return lp, entropy, ids, best
+
+
+def _rows_of_logits(t, what, shape, dtype, here):
+    """(address, sequence stride, row stride) of logits [S, rows, V] whose rows
+    are contiguous."""
+    p = _ptr(t, dtype, what, here)
+    if t.shape != shape:
+        raise _invalid(f"{what} must be {list(shape)}, got {list(t.shape)}")
+    if shape[2] > 1 and t.stride(2) != 1 and shape[0] and shape[1]:
+        raise _invalid(f"{what} must be contiguous within a row")
+    return p, t.stride(0), t.stride(1)
+
+
+def verify_drafts(target, drafted, uniforms, draft=None, counts=None, temperature=1.0, stream=None):
+    """xt_verify_drafts: T (0..64) drafted tokens (int32 [S, T]) of each of S
+    sequences against the target model's logits [S, T + 1, V] (float32, float16
+    or bfloat16, -inf for masked tokens) and the logits that they were drawn
+    from, draft [S, T, V] (None: each was certain).  uniforms: float32 [S, T +
+    1] in [0, 1), the first T accept, the last one draws.  counts (int32 [S]):
+    drafts of each sequence (default T; negative: no sequence).  temperature:
+    a number >= 0 or float32 [S]; 0 takes the most likely token.  Returns
+    (accepted int32 [S]: drafts that were; tokens int32 [S, T + 1]: these, the
+    one drawn after them, then -1; logprobs float32 [S, T + 1]: the target's ln
+    p of each)."""
+    here = _here()
+    dtype = getattr(target, "dtype", None)
+    if dtype not in _DTYPES:
+        raise _invalid(f"target must be a float32, float16 or bfloat16 tensor, got {dtype}")
+    if len(target.shape) != 3 or target.shape[1] < 1:
+        raise _invalid(f"target must be [seqs, drafts + 1, vocabulary], got {list(target.shape)}")
+    S, T, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    xp, ls, lr = _rows_of_logits(target, "target", (S, T + 1, V), dtype, here)
+    dp, us, cp, tp, ds, dr = (_vec(drafted, _I32, "drafted", (S, T), here), _vec(uniforms, _F32, "uniforms", (S, T + 1), here),
+                              None, None, 0, 0)
+    yp = None
+    if draft is not None:
+        yp, ds, dr = _rows_of_logits(draft, "draft", (S, T, V), dtype, here)
+    if counts is not None:
+        cp = _vec(counts, _I32, "counts", (S,), here)
+    if isinstance(temperature, (int, float)):
+        temp = float(temperature)
+    else:
+        temp, tp = 1.0, _vec(temperature, _F32, "temperature", (S,), here)
+    dev = target.device
+    accepted, tokens, logprobs = (_empty(stream, _I32, dev, S), _empty(stream, _I32, dev, S, T + 1),
+                                  _empty(stream, _F32, dev, S, T + 1))
+    if stream is not None:
+        _mark(stream, target, drafted, uniforms, draft, counts, temperature if tp is not None else None)
+    _check(_lib.xt_verify_drafts(_DTYPES[dtype], xp, ls, lr, yp, ds, dr, S, T, V, dp, cp, us, temp, tp,
+                                 accepted.data_ptr(), tokens.data_ptr(), logprobs.data_ptr(), _stream_ptr(stream)))
+    return accepted, tokens, logprobs

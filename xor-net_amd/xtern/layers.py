@@ -331,20 +331,30 @@ class Mlp:
 class CausalSelfAttention:
     """models/llama/attention.rs:42-113 over a paged cache: ternary q, k, v
     and o projections, rotary embedding, grouped-query attention and the
-    optional attn_sub_norm."""
+    optional attn_sub_norm.  Beyond the reference: norms of the query and key
+    heads (q_norm, k_norm: FastRmsNorm of head_dim, of one eps, or neither),
+    and a window of the newest positions with the first `sink` beside it."""
 
-    def __init__(self, q_proj, k_proj, v_proj, o_proj, head_dim, attn_sub_norm=None):
+    def __init__(self, q_proj, k_proj, v_proj, o_proj, head_dim, attn_sub_norm=None, q_norm=None, k_norm=None,
+                 window=None, sink=0):
         if q_proj.out_dim % head_dim or k_proj.out_dim % head_dim or v_proj.out_dim != k_proj.out_dim:
             raise XternError(XT_ERR_INVALID, "q, k and v must be whole heads, k and v of one size")
         if o_proj.in_dim != q_proj.out_dim:
             raise XternError(XT_ERR_INVALID, f"Input dimension mismatch: expected {o_proj.in_dim}, "
                                              f"got {q_proj.out_dim}")
+        if (q_norm is None) != (k_norm is None):
+            raise XternError(XT_ERR_INVALID, "q_norm and k_norm go together")
+        if q_norm is not None and (q_norm.eps != k_norm.eps
+                                   or any(tuple(n.weight.shape) != (head_dim,) for n in (q_norm, k_norm))):
+            raise XternError(XT_ERR_INVALID, "q_norm and k_norm must be of head_dim and one eps")
         self.q_proj, self.k_proj, self.v_proj, self.o_proj = q_proj, k_proj, v_proj, o_proj
         self.head_dim = int(head_dim)
         self.attn_sub_norm = attn_sub_norm
+        self.norm = (q_norm.weight, k_norm.weight, q_norm.eps) if q_norm is not None else None
+        self.window, self.sink = window, sink
 
     def forward(self, x, cache, table, slots, seq=None, positions=None, rope=None, accumulate=False,
-                mode=XT_QUANT_AVX512):
+                mode=XT_QUANT_AVX512, tokens=1):
         """x [R, hidden]: R new tokens, token r at position slots[r] (int32
         [R], -1 for a padding row) of sequence seq[r] (default r) of table
         (int32 [seqs, max_pages]).  Appends their keys and values to `cache`
@@ -354,7 +364,9 @@ class CausalSelfAttention:
         tables.  A row that cannot be appended (a slot, a page or a sequence
         that is not there, a position without a row in the tables) sees
         nothing: its attention is zero.  accumulate adds the weights to
-        cache.score.  Returns [R, hidden]."""
+        cache.score.  tokens: rows that go together, all of one sequence (the
+        drafts to verify, a chunk of a prompt; seq is needed for more than
+        one); they share passes over an int8 cache.  Returns [R, hidden]."""
         if x.dim() != 2:
             raise XternError(XT_ERR_INVALID, "x must be [rows, hidden]")
         if x.shape[-1] != self.q_proj.in_dim:
@@ -362,6 +374,8 @@ class CausalSelfAttention:
                              f"Input dimension mismatch: expected {self.q_proj.in_dim}, got {x.shape[-1]}")
         if cache.head_dim != self.head_dim or cache.kv_heads * self.head_dim != self.k_proj.out_dim:
             raise XternError(XT_ERR_INVALID, "the cache's heads are not the projections'")
+        if tokens != 1 and seq is None:
+            raise XternError(XT_ERR_INVALID, "tokens of one sequence need seq")
         x = x.contiguous()
         ws = [l.weights for l in (self.q_proj, self.k_proj, self.v_proj)]
         if all(w.fmt == ws[0].fmt and w.in_dim == ws[0].in_dim for w in ws):
@@ -369,8 +383,10 @@ class CausalSelfAttention:
         else:
             q, k, v = (linear_f32(w, x, mode=mode) for w in ws)
         lengths = _empty(None, _I32, x.device, x.shape[0])
-        kv_append(cache, table, slots, k, v, q=q, seq=seq, positions=positions, rope=rope, q_out=q, lengths=lengths)
-        y = paged_attention(cache, table, lengths, q, seq=seq, accumulate=accumulate)
+        kv_append(cache, table, slots, k, v, q=q, seq=seq, positions=positions, rope=rope, q_out=q, lengths=lengths,
+                  norm=self.norm)
+        y = paged_attention(cache, table, lengths, q, seq=seq, accumulate=accumulate, window=self.window,
+                            sink=self.sink, tokens=tokens)
         if self.attn_sub_norm is not None:
             y = self.attn_sub_norm.forward(y)
         return linear_f32(self.o_proj.weights, y, mode=mode)
