@@ -61,9 +61,28 @@ __device__ __forceinline__ const T* verify_row(const VerifyArgs& a, int b, int j
                     : static_cast<const T*>(a.draft) + b * a.ldd_seq + (j - a.T - 1) * a.ldd_row;
 }
 
-// exp((x - m) / temperature), c = 1 / temperature.
+// exp((x - m) / temperature) for x <= m, c = log2 e / temperature: with y = (x -
+// m) c = n + f, |f| <= 1/2, 2^n times a polynomial of 2^f, of degree 9 through its
+// values in Chebyshev's nodes (the constant term then made 1, so that m itself
+// gives 1): 3e-14 of the result.  0 for x = -inf; the caller sees to NaN and +inf.
 __device__ __forceinline__ double verify_exp(float x, float m, double c) {
-    return exp(((double)x - (double)m) * c);
+    const double y = fmax(((double)x - (double)m) * c, -1100.0);
+    const double magic = 0x1.8p52, z = y + magic;  // (its last bits: n)
+    const double f = y - (z - magic);
+    double p = 0x1.b6571de2f2351p-24;
+    p = fma(p, f, 0x1.63ef969a64d3cp-20);
+    p = fma(p, f, 0x1.ffcb76789860fp-17);
+    p = fma(p, f, 0x1.43088e257f341p-13);
+    p = fma(p, f, 0x1.5d87fe908f88ap-10);
+    p = fma(p, f, 0x1.3b2ab72b175eep-7);
+    p = fma(p, f, 0x1.c6b08d7044119p-5);
+    p = fma(p, f, 0x1.ebfbdff8149f2p-3);
+    p = fma(p, f, 0x1.62e42fefa39f7p-1);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)__builtin_bit_cast(int64_t, z));
+}
+__device__ __forceinline__ double verify_rate(float temp) {
+    return temp > 0.0f ? 1.4426950408889634 / (double)temp : 0.0;
 }
 
 // A lane's logits of a tile: vectors of 16 bytes (W logits), vector v at base +
@@ -127,19 +146,23 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
     const int count = verify_count(a, b);
     if (j <= a.T ? j > count : j - a.T - 1 >= count) return;
     const float temp = verify_temp(a, b);
-    const double c = temp > 0.0f ? 1.0 / (double)temp : 0.0;
+    const double c = verify_rate(temp);
     const typename R::T* x = verify_row<typename R::T>(a, b, j);
     const int per = (pl.tiles + pl.slices - 1) / pl.slices, t1 = min(pl.tiles, (slice + 1) * per);
     RowStat s{0.0, -INFINITY, 0x7fffffff};
+    bool bad = false;
     for (int t = slice * per + wave; t < t1; t += kVerifyWaves) {
         R r;
         r.load(x, t * kVerifyTile, a.V);
         float m = s.m;
 #pragma unroll
-        for (int i = 0; i < kVerifyPer; ++i) m = fmaxf(m, r.x[i]);
+        for (int i = 0; i < kVerifyPer; ++i) {
+            m = fmaxf(m, r.x[i]);
+            bad |= !(r.x[i] < INFINITY);
+        }
         if (temp > 0.0f) {
             if (m > s.m) {
-                if (s.l != 0.0) s.l *= verify_exp(s.m, m, c);  // (a NaN stays)
+                s.l *= s.m == -INFINITY ? 0.0 : verify_exp(s.m, m, c);
                 s.m = m;
             }
             const float base = s.m == -INFINITY ? 0.0f : s.m;
@@ -154,11 +177,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
                 s.m = m;
                 s.at = at;
             }
-#pragma unroll
-            for (int i = 0; i < kVerifyPer; ++i)
-                if (!(r.x[i] < INFINITY)) s.l = NAN;
         }
     }
+    if (bad) s.l = NAN;
     s = wave_join(s, c);
     if (lane == 0) waves[wave] = s;
     __syncthreads();
@@ -169,7 +190,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
     }
 }
 
-// What the second kernel draws from: max(p - q, 0), each exp((x - m) c) / l.
+// What the second kernel draws from: max(p - q, 0), each exp((x - m) / temperature) / l.
 struct VerifyDraw {
     float pm, qm;
     double pl, ql;  // 1 / l
@@ -229,7 +250,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int count = verify_count(a, b);
     const float temp = verify_temp(a, b);
-    const double c = temp > 0.0f ? 1.0 / (double)temp : 0.0;
+    const double c = verify_rate(temp);
     const bool there = count >= 0 && temp >= 0.0f && temp < INFINITY;
     // the rows' sums
     for (int j = wave; there && j < pl.rows; j += kVerifyWaves) {
@@ -277,7 +298,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
             a.tokens[at] = id;
             float lp = 0.0f;
             if (id >= 0 && temp > 0.0f)
-                lp = (float)(((double)Elem<DT>::get(verify_row<T>(a, b, i)[id]) - (double)rows[i].m) * c - log(rows[i].l));
+                lp = (float)(((double)Elem<DT>::get(verify_row<T>(a, b, i)[id]) - (double)rows[i].m) / (double)temp - log(rows[i].l));
             a.logprobs[at] = lp;
         }
     };
