@@ -44,17 +44,28 @@ __device__ __forceinline__ AttnUnit attn_unit(const AttnArgs& a, int u) {
 // is position i of the sequence below `sink`, i + gap from there on.
 struct AttnSpan {
     int n, gap;
+    int seq;  // (the unit's)
 };
 __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, int u) {
     const AttnUnit x = attn_unit(a, u);
-    AttnSpan s{0, 0};
-    if ((unsigned)x.seq >= (unsigned)a.c.nseq) return s;
+    AttnSpan s{0, 0, x.seq};
     int least = a.c.max_pages * a.c.page;  // (at most 2^30)
-    for (int t = 0; t < x.rows; ++t) {
-        const int n = kv_length(a.c, a.lengths[x.row + t]);
-        s.n = max(s.n, n);
-        if (n > 0) least = min(least, n);
+    if (x.rows == 1) {
+        s.n = kv_length(a.c, a.lengths[x.row]);
+    } else {
+        for (int t = 0; t < x.rows; t += 4) {  // (four loads in flight)
+            int n[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n[i] = a.lengths[x.row + min(t + i, x.rows - 1)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                n[i] = kv_length(a.c, n[i]);
+                s.n = max(s.n, n[i]);
+                if (n[i] > 0) least = min(least, n[i]);
+            }
+        }
     }
+    if ((unsigned)x.seq >= (unsigned)a.c.nseq) return AttnSpan{0, 0, x.seq};
     s.gap = max(0, min(s.n, least) - a.window - a.sink);
     s.n -= s.gap;
     return s;
@@ -91,6 +102,7 @@ struct AttnPlan {
     int hy;          // workgroups per share: kv heads x tiles of 16 query heads
     int tiles;       // of 16 query heads per kv head
     int shares;      // at most
+    double inv_shares;
     int units;       // of the call
     bool per_row;
 };
@@ -98,6 +110,7 @@ struct AttnPlan {
 // A unit's part of the line, and of it what one share covers.
 struct AttnSeg {
     int row, n, gap;  // the unit, its positions
+    int seq;          // its sequence
     int p0, p1;       // the share's [p0, p1) of them
     int nc;           // segments of the unit
     int64_t slot;     // of its first one
@@ -110,7 +123,7 @@ __device__ __forceinline__ int attn_steps(int len) { return max(1, (len + kAttnS
 struct AttnLine {
     const AttnArgs& a;
     const AttnPlan& pl;
-    int len, gap, upto;  // the lane's unit (at most 64)
+    int len, gap, seq, upto;  // the lane's unit (at most 64)
     int64_t* ends;       // LDS, [units] (more)
     int R;               // units
     int64_t total;       // steps
@@ -127,9 +140,10 @@ struct AttnLine {
         }
         if (R <= 64) {
             const int lane = threadIdx.x & 63;
-            const AttnSpan s = lane < R ? attn_span(a, lane) : AttnSpan{-1, 0};
+            const AttnSpan s = lane < R ? attn_span(a, lane) : AttnSpan{-1, 0, 0};
             len = s.n;
             gap = s.gap;
+            seq = s.seq;
             upto = wave_scan(len < 0 ? 0 : attn_steps(len));  // (64 rows of 2^30 positions: 2^29)
             total = __builtin_amdgcn_readlane(upto, 63);
         } else {
@@ -150,9 +164,11 @@ struct AttnLine {
             __syncthreads();
         }
         // (whole numbers below 2^53: a quotient in doubles is off by one at most)
-        per = max((int64_t)1, (int64_t)((double)total / (double)pl.shares));
+        per = max((int64_t)1, (int64_t)((double)total * pl.inv_shares));
+        if ((per - 1) * pl.shares >= total) --per;
         while (per * pl.shares < total) ++per;
-        inv = 1.0 / (double)per;
+        // (at most 2048 shares: 2^-20 of a quotient is enough)
+        inv = __builtin_amdgcn_rcp((double)per);
         x = share_of(total - 1) + 1;
     }
     // First step of share b; the share that holds a step.
@@ -182,6 +198,7 @@ struct AttnLine {
             const AttnSpan s = attn_span(a, r);
             g.n = s.n;
             g.gap = s.gap;
+            g.seq = s.seq;
             g.p0 = 0;
             g.p1 = g.n;
             g.nc = 1;
@@ -193,12 +210,14 @@ struct AttnLine {
         if (R <= 64) {
             g.n = __builtin_amdgcn_readlane(len, r);
             g.gap = __builtin_amdgcn_readlane(gap, r);
+            g.seq = __builtin_amdgcn_readlane(seq, r);
             *end = __builtin_amdgcn_readlane(upto, r);
             first = *end - attn_steps(g.n);
         } else {
             const AttnSpan s = attn_span(a, r);
             g.n = s.n;
             g.gap = s.gap;
+            g.seq = s.seq;
             *end = ends[r];
             first = r ? ends[r - 1] : 0;
         }
@@ -398,6 +417,7 @@ inline AttnPlan plan_attention(const AttnArgs& a, int cus, int rows, int residen
     pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident * cus / pl.hy));
     pl.shares = std::min(pl.shares, 64 * kJoinGroup);  // (as many as two levels join)
     if (pl.per_row) pl.shares = pl.units;
+    pl.inv_shares = 1.0 / (double)pl.shares;
     return pl;
 }
 inline bool attention_splits(const AttnArgs& a, const AttnPlan& pl) {

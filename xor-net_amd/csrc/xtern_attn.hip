@@ -212,7 +212,7 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
                            float scale2, float* lds_o, float* lds_ml, int ldo) {
     typedef Elem<DT> E;
     const KvView& c = a.c;
-    const int t = threadIdx.x, sq = attn_unit(a, it.row).seq;
+    const int t = threadIdx.x, sq = it.seq;
     __shared__ float sp[kAttnThreads];
     __shared__ int64_t so[kAttnThreads];
     __shared__ float sm[kAttnWaves];
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
         asm volatile("" : "+s"(D), "+v"(lane));
         const int n = lane & 15, g = lane >> 4;
         const bool fast = D >= S::KU;
-        const int sq = attn_unit(a, r).seq;
+        const int sq = it.seq;
         const int ntiles = it.p1 > it.p0 ? (it.p1 - it.p0 + S::TK - 1) / S::TK : 0;
 
         float m = -INFINITY, l = 0.0f, qs = scale2;
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
 // (share, kv head), every query head of the group.
 __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int hk) {
     const KvView& c = a.c;
-    const int G = a.hq / c.hkv, sq = attn_unit(a, it.row).seq;
+    const int G = a.hq / c.hkv, sq = it.seq;
     extern __shared__ float hm[];  // [G] maximum, [G] 1 / sum
     for (int h = threadIdx.x; h < G; h += kAttnThreads) {
         const float* ml = pl.ml + 2 * ((int64_t)it.row * a.hq + hk * G + h);

@@ -75,12 +75,21 @@ __device__ __forceinline__ void transpose4(const int* x, int* out) {
 // several.
 struct Attn8Cols {
     int row, h0, G, n;
+    FastDiv by_group;
     bool several;
     __device__ __forceinline__ AttnPlace operator()(int x) const {
         if (!several) return AttnPlace{row, h0 + x};
-        const int t = x / G;
+        const int t = fast_quot(x, by_group);
         return AttnPlace{row + t, h0 + x - t * G};
     }
+};
+
+struct Attn8Call {
+    AttnArgs a;
+    AttnPlan pl;
+    float scale2;
+    int G;  // query heads of a group
+    FastDiv by_group, by_tiles;
 };
 
 // Whether a row of length n sees position p.
@@ -91,7 +100,7 @@ __device__ __forceinline__ bool attn_sees(const AttnArgs& a, int n, int p) {
 // One chunk of a unit in plain f32 operations: queries and scales that are
 // infinite, NaN or beyond the digits' exponents, and head sizes below one load.
 // 256 positions at a time, one column after the other.
-__device__ void attn8_plain(const AttnArgs& a, const AttnSeg& it, int seq, int hk, const Attn8Cols& cols,
+__device__ void attn8_plain(const AttnArgs& a, const AttnSeg& it, int hk, const Attn8Cols& cols,
                             float scale2, float* lds_o, float* lds_ml, int ldo) {
     const KvView& c = a.c;
     const int t = threadIdx.x;
@@ -107,7 +116,7 @@ __device__ void attn8_plain(const AttnArgs& a, const AttnSeg& it, int seq, int h
         float m = -INFINITY, l = 0.0f, o = 0.0f;
         for (int p0 = it.p0; p0 < it.p1; p0 += kAttnThreads) {
             const int p = attn_pos(a, it.gap, p0 + t);
-            const int pg = p0 + t < it.p1 && attn_sees(a, len, p) ? kv_page(c, seq, p) : -1;
+            const int pg = p0 + t < it.p1 && attn_sees(a, len, p) ? kv_page(c, it.seq, p) : -1;
             const int64_t off = pg < 0 ? -1 : kv_offset(c, pg, p, hk);
             float s = -INFINITY, vs = 0.0f;
             if (off >= 0) {
@@ -150,12 +159,124 @@ __device__ void attn8_plain(const AttnArgs& a, const AttnSeg& it, int seq, int h
     __syncthreads();
 }
 
+// Four elements of a column's sums: into its row's result, divided by l; into
+// a segment's.
+__device__ __forceinline__ void attn8_out(const AttnArgs& a, AttnPlace w, int d, v4f sum, float l) {
+    const int D = a.c.D;
+    float* to = a.out + w.row * a.ldo + (int64_t)w.head * D + d;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    sum *= inv;
+    if (l == 0.0f) sum = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (d + 4 <= D) {
+        *reinterpret_cast<v4fu*>(to) = sum;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (d + e < D) to[e] = sum[e];
+    }
+}
+__device__ __forceinline__ void attn8_part(const AttnPlan& pl, int64_t item, int h, int d, int D, v4f sum) {
+    float* to = pl.part_o + (item * 16 + h) * pl.dp + d;
+    st2_device(to, sum[0], d + 1 < D ? sum[1] : 0.0f);
+    if (d + 2 < D) st2_device(to + 2, sum[2], d + 3 < D ? sum[3] : 0.0f);
+}
+
+// Joins `cnt` (at most 64) segments, in every `every`-th slot from slot0, of all
+// columns: into the rows' results (last), or into slot0.  As at the end of a
+// segment a thread has four elements of a column; where columns are few, 2, 4 or
+// 8 threads share them, each every 2nd, 4th or 8th segment.  Bound by the latency
+// of device-scope loads: up to 16 segments of a thread are on their way at once,
+// while the segments' statistics go through LDS (scratch, 4096 floats).
 template <int DP>
-__global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) void attention8_kernel(AttnArgs a, AttnPlan pl,
-                                                                                    float scale2) {
+__device__ void attn8_join(const AttnArgs& a, const AttnPlan& pl, const Attn8Cols& cols, int tid, int64_t slot0,
+                           int every, int cnt, bool last, float* scratch) {
+    constexpr int N = 16, Q = DP / 4;  // segments in flight, threads of a column
+    const int D = a.c.D;
+    const int64_t first = slot0 * pl.hy + blockIdx.y, step = (int64_t)every * pl.hy;
+    float2* stats = reinterpret_cast<float2*>(scratch);      // [cnt][16]
+    v4f* sums = reinterpret_cast<v4f*>(scratch + 64 * 16 * 2);  // [256]
+    // columns that are worked on at once, rounded up to a power of two
+    const int lg = cols.n > 1 ? 32 - __builtin_clz(cols.n - 1) : 0;
+    const int wide = min(Q << lg, kAttnThreads), parts = kAttnThreads / wide;
+    const int part = tid / wide, x = tid & (wide - 1), d = x % Q * 4;
+    float2 st[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int e = tid + kAttnThreads * i;
+        if (e < 16 * cnt && e % 16 < cols.n) st[i] = ld2_device(pl.part_ml + ((first + e / 16 * step) * 16 + e % 16) * 2);
+    }
+#pragma unroll 1
+    for (int h0 = 0; h0 < cols.n; h0 += wide / Q) {
+        const int h = min(h0 + x / Q, cols.n - 1);
+        const bool in = h0 + x / Q < cols.n && d < D;
+        const float* from = pl.part_o + (first * 16 + h) * pl.dp + min(d, pl.dp - 2);
+        const int more = d + 2 < pl.dp ? 2 : 0;
+        const int64_t stride = step * 16 * pl.dp;
+        float m = -INFINITY, l = 0.0f;
+        v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int c0 = 0; c0 < cnt; c0 += N * parts) {
+            float2 lo[N], hi[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = c0 + i * parts + part;
+                if (c0 + i * parts < cnt) {  // (the same for all threads)
+                    const float* y = from + min(c, cnt - 1) * stride;
+                    lo[i] = ld2_device(y);
+                    hi[i] = ld2_device(y + more);
+                }
+            }
+            if (c0 == 0) {
+                if (h0 == 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = tid + kAttnThreads * i;
+                        if (e < 16 * cnt && e % 16 < cols.n) stats[e] = st[i];
+                    }
+                    __syncthreads();
+                }
+                for (int c = 0; c < cnt; ++c) m = fmaxf(m, stats[16 * c + h].x);
+            }
+            const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = c0 + i * parts + part;
+                if (c0 + i * parts < cnt) {
+                    const float2 s = stats[16 * min(c, cnt - 1) + h];
+                    const float f = c < cnt ? pow2(s.x - base) : 0.0f;
+                    l += s.y * f;
+                    if (c < cnt) sum += f * v4f{lo[i].x, lo[i].y, hi[i].x, hi[i].y};
+                }
+            }
+        }
+        if (parts > 1) {  // (then the columns are all here)
+            float* ls = reinterpret_cast<float*>(sums + kAttnThreads);
+            sums[tid] = sum;
+            ls[tid] = l;
+            __syncthreads();
+            for (int p = 1; p < parts && part == 0; ++p) {
+                sum += sums[tid + p * wide];
+                l += ls[tid + p * wide];
+            }
+        }
+        if (!in || part) continue;
+        if (last) attn8_out(a, cols(h), d, sum, l);
+        else attn8_part(pl, first, h, d, D, sum);  // (what lay there has been read)
+        if (d) continue;
+        if (!last) {
+            st2_device(pl.part_ml + (first * 16 + h) * 2, m, l);
+        } else if (a.lse) {
+            const AttnPlace w = cols(h);
+            a.lse[(int64_t)w.row * a.hq + w.head] = row_lse(m, l);
+        }
+    }
+}
+
+template <int DP>
+__global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) void attention8_kernel(Attn8Call call) {
     typedef Attn8Shape<DP> S;
-    const KvView& c = a.c;
     constexpr int kLdsRow = DP + 4;  // floats; the pad keeps columns apart in the banks
+    constexpr int kItems = 16 * DP / 4 / kAttnThreads;
     __shared__ v4i lds_mem[kAttnWaves * 16 * kLdsRow / 4];
     v4i* lds_q = lds_mem;                              // the queries' digits, then
     float* lds_o = reinterpret_cast<float*>(lds_mem);  // the waves' sums
@@ -164,9 +285,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
     __shared__ v4f lds_scale[kAttnWaves][2][S::TK / 4];  // of a tile's keys, of its values
     __shared__ int lds_last;
     __shared__ int64_t lds_ends[kAttnPlanRows];
-    const int hk = blockIdx.y / pl.tiles;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const AttnLine line(a, pl, lds_ends);
+    const AttnLine line(call.a, call.pl, lds_ends);
     if ((int)blockIdx.x >= line.x) return;
     int64_t at = line.begin(blockIdx.x);
     const int64_t to_step = line.begin(blockIdx.x + 1);
@@ -174,19 +293,29 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
         int64_t row_end;
         const AttnSeg it = line.segment(r, at, to_step, &row_end);
         at = row_end;
-        // (opaque to the compiler: it would keep every index that follows from
-        // them in registers from segment to segment, and spill)
-        int D = c.D, lane = threadIdx.x & 63;
-        asm volatile("" : "+s"(D), "+v"(lane));
+        // The arguments and the thread, opaque to the compiler: it would compute
+        // everything that follows from them before the first segment, 1.4 us for
+        // a call that has but one, and spill it
+        typedef const __attribute__((address_space(4))) Attn8Call* Kernarg;
+        Kernarg again = (Kernarg)__builtin_amdgcn_kernarg_segment_ptr();
+        int tid = threadIdx.x;
+        asm volatile("" : "+s"(again), "+v"(tid));
+        const Attn8Call& k = *(const Attn8Call*)again;
+        const AttnArgs& a = k.a;
+        const AttnPlan& pl = k.pl;
+        const KvView& c = a.c;
+        const int D = c.D, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int n = lane & 15, g = lane >> 4;
         const bool fast = D >= 16;
         const AttnUnit unit = attn_unit(a, r);
+        const int hk = pl.tiles == 1 ? blockIdx.y : fast_quot(blockIdx.y, k.by_tiles);
         Attn8Cols cols;
         cols.row = unit.row;
-        cols.G = a.hq / c.hkv;
+        cols.G = k.G;
+        cols.by_group = k.by_group;
         cols.several = a.unit_rows > 1;
-        cols.h0 = hk * cols.G + (blockIdx.y % pl.tiles) * 16;
-        cols.n = cols.several ? unit.rows * cols.G : min(16, hk * cols.G + cols.G - cols.h0);
+        cols.h0 = hk * k.G + ((int)blockIdx.y - hk * pl.tiles) * 16;
+        cols.n = cols.several ? unit.rows * k.G : min(16, hk * k.G + k.G - cols.h0);
         const int ntiles = it.p1 > it.p0 ? (it.p1 - it.p0 + S::TK - 1) / S::TK : 0;
 
         float m = -INFINITY, l = 0.0f;
@@ -225,7 +354,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             auto pos = [&](int i, int x) { return attn_pos(a, it.gap, it.p0 + i * S::TK + x); };
             auto entry = [&](int i) {  // the lane's table entry of tile i
                 const int x = min(it.p0 + i * S::TK + lane, it.p1 - 1);
-                return c.table[(int64_t)unit.seq * c.ldt + kv_page_of(c, attn_pos(a, it.gap, x))];
+                return c.table[(int64_t)it.seq * c.ldt + kv_page_of(c, attn_pos(a, it.gap, x))];
             };
             // Row offsets of a tile's positions, one lane each, through the wave's
             // LDS (0: no position there), and the scales; whether every column
@@ -269,10 +398,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 }
             };
 
-            int next_e = entry(wave);
-            const int after_e = entry(wave + kAttnWaves);
-            // The queries' digits as the lanes' operands, to LDS, a wave every
-            // fourth piece: column n, elements from min(16 (4 s + g), D - 16);
+            // The queries' digits as the lanes' operands, to LDS, a wave each
+            // piece: column n, elements from min(16 (4 s + g), D - 16);
             // where pieces overlap (D no multiple of 16, or past D) the earlier
             // one counts, the later one holds zeros.
             const float* q = a.q + own.row * a.ldq + (int64_t)own.head * D;
@@ -285,44 +412,45 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                     for (int e = 0; e < 4; ++e) x[i + e] = n < cols.n && d + i + e >= nom ? f[e] : 0.0f;
                 }
             };
-            float mx = 0.0f;
+            // (table entries first, then the queries, then the first tile, which is
+            // on its way while the queries become digits)
+            int next_e = entry(wave);
+            const int after_e = entry(wave + kAttnWaves);
+            float x[S::KS][16], mx = 0.0f;
 #pragma unroll
-            for (int s = 0; s < S::KS; ++s) {
-                float x[16];
-                q_load(s, x);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    plain |= !(fabsf(x[i]) < INFINITY);
-                    mx = fmaxf(mx, fabsf(x[i]));
-                }
-            }
-            mx = rows_max(mx);
-            const int qk = mx < INFINITY ? digit_shift(mx) : 0;
-            const float qs = ldexpf(scale2, -qk);
-#pragma unroll 1
-            for (int s = wave; s < S::KS; s += kAttnWaves) {
-                float x[16];
-                q_load(s, x);
-                v4i dig[kDigits];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    unsigned b[4];
-                    int w[kDigits];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) b[e] = digits_of((int)rintf(ldexpf(x[4 * i + e], qk)));
-                    gather_digits(b, w);
-#pragma unroll
-                    for (int k = 0; k < kDigits; ++k) dig[k][i] = w[k];
-                }
-#pragma unroll
-                for (int k = 0; k < kDigits; ++k) lds_q[(s * kDigits + k) * 64 + lane] = dig[k];
-            }
+            for (int s = 0; s < S::KS; ++s) q_load(s, x[s]);
             bool full = false;
             if (wave < ntiles) {
                 full = offsets(wave, next_e);
                 next_e = after_e;
                 load_k(wave);
                 load_v(wave);
+            }
+#pragma unroll
+            for (int s = 0; s < S::KS; ++s)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    plain |= !(fabsf(x[s][i]) < INFINITY);
+                    mx = fmaxf(mx, fabsf(x[s][i]));
+                    if (s && s == wave) x[0][i] = x[s][i];
+                }
+            mx = rows_max(mx);
+            const int qk = mx < INFINITY ? digit_shift(mx) : 0;
+            const float qs = ldexpf(k.scale2, -qk);
+            if (wave < S::KS) {
+                v4i dig[kDigits];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unsigned b[4];
+                    int w[kDigits];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) b[e] = digits_of((int)rintf(ldexpf(x[0][4 * i + e], qk)));
+                    gather_digits(b, w);
+#pragma unroll
+                    for (int k = 0; k < kDigits; ++k) dig[k][i] = w[k];
+                }
+#pragma unroll
+                for (int k = 0; k < kDigits; ++k) lds_q[(wave * kDigits + k) * 64 + lane] = dig[k];
             }
             __syncthreads();
             for (int i = wave; i < ntiles; i += kAttnWaves) {
@@ -438,7 +566,15 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             l = rows_sum(l);
         }
 
-        // The waves' sums, relative to the largest maximum
+        // The waves' sums, relative to the largest maximum: four elements of a
+        // column a thread, kItems times
+        v4f sum[kItems];
+        auto at_item = [&](int j, int* h, int* d) {
+            const int x = tid + kAttnThreads * j;
+            *h = x / (DP / 4);
+            *d = x % (DP / 4) * 4;
+            return *h < cols.n && *d < D;
+        };
         if (fast) {
             if (g == 0) {
                 lds_ml[wave][0][n] = m;
@@ -450,14 +586,21 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             for (int w = 1; w < kAttnWaves; ++w) mm = fmaxf(mm, lds_ml[w][0][n]);
             const float f = pow2(m - (mm == -INFINITY ? 0.0f : mm));
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+            for (int y = 0; y < 4; ++y) {
+                const int nom = S::UE * (4 * g + y);
+                float* to = lds_o + (wave * 16 + n) * kLdsRow + nom;
+                if (nom + S::UE <= D) {
 #pragma unroll
-                for (int e = 0; e < S::UE; ++e) {
-                    const int nom = S::UE * (4 * g + y), d = min(nom, D - S::UE) + e;
-                    if (d >= nom) lds_o[(wave * 16 + n) * kLdsRow + d] = o[e][y] * f;
+                    for (int e = 0; e < S::UE; e += 4)
+                        *reinterpret_cast<v4f*>(to + e) = v4f{o[e][y], o[e + 1][y], o[e + 2][y], o[e + 3][y]} * f;
+                } else {  // a piece that begins at D - UE
+#pragma unroll
+                    for (int e = 0; e < S::UE; ++e)
+                        if (D - S::UE + e >= nom) lds_o[(wave * 16 + n) * kLdsRow + D - S::UE + e] = o[e][y] * f;
                 }
+            }
             __syncthreads();
-            if (threadIdx.x < 16) {
+            if (tid < 16) {
                 float lt = 0.0f;
                 for (int w = 0; w < kAttnWaves; ++w)
                     lt += lds_ml[w][1][n] * pow2(lds_ml[w][0][n] - (mm == -INFINITY ? 0.0f : mm));
@@ -465,46 +608,62 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 lds_ml[0][1][n] = lt;
                 plain |= n < cols.n && !(mm < INFINITY && lt < INFINITY);
             }
-            for (int x = threadIdx.x; x < cols.n * D; x += kAttnThreads) {
-                const int h = x / D, d = x % D;
-                float v = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kAttnWaves; ++w) v += lds_o[(w * 16 + h) * kLdsRow + d];
-                lds_o[h * kLdsRow + d] = v;
-                plain |= !(fabsf(v) < INFINITY);
+            for (int j = 0; j < kItems; ++j) {
+                int h, d;
+                if (!at_item(j, &h, &d)) continue;
+                sum[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < kAttnWaves; ++w)
+                    sum[j] += *reinterpret_cast<const v4f*>(lds_o + (w * 16 + h) * kLdsRow + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) plain |= d + e < D && !(fabsf(sum[j][e]) < INFINITY);
             }
         }
         // (A segment of nothing but holes has a maximum of -inf, sums of 0, and is
         // done.)
-        if (__syncthreads_or(plain))
-            attn8_plain(a, it, unit.seq, hk, cols, scale2, lds_o, &lds_ml[0][0][0], kLdsRow);
+        if (__syncthreads_or(plain)) {
+            attn8_plain(a, it, hk, cols, k.scale2, lds_o, &lds_ml[0][0][0], kLdsRow);
+#pragma unroll
+            for (int j = 0; j < kItems; ++j) {
+                int h, d;
+                if (at_item(j, &h, &d)) sum[j] = *reinterpret_cast<const v4f*>(lds_o + h * kLdsRow + d);
+            }
+        }
 
         if (it.nc == 1) {
-            for (int h = wave; h < cols.n; h += kAttnWaves) {
-                const AttnPlace w = cols(h);
-                float* to = a.out + w.row * a.ldo + (int64_t)w.head * D;
-                const float lt = lds_ml[0][1][h];
-                for (int d = lane; d < D; d += 64) to[d] = lt == 0.0f ? 0.0f : lds_o[h * kLdsRow + d] / lt;
+#pragma unroll
+            for (int j = 0; j < kItems; ++j) {
+                int h, d;
+                if (at_item(j, &h, &d)) attn8_out(a, cols(h), d, sum[j], lds_ml[0][1][h]);
             }
-            if (a.lse && (int)threadIdx.x < cols.n) {
+            if (a.lse && tid < cols.n) {
                 const AttnPlace w = cols(n);
                 a.lse[(int64_t)w.row * a.hq + w.head] = row_lse(lds_ml[0][0][n], lds_ml[0][1][n]);
             }
         } else {
             const int64_t slot = (int64_t)blockIdx.x + r, item = slot * pl.hy + blockIdx.y;
-            for (int h = wave; h < cols.n; h += kAttnWaves)
-                for (int d = 2 * lane; d < D; d += 128)
-                    st2_device(pl.part_o + (item * 16 + h) * pl.dp + d, lds_o[h * kLdsRow + d],
-                               d + 1 < D ? lds_o[h * kLdsRow + d + 1] : 0.0f);
-            if ((int)threadIdx.x < cols.n) st2_device(pl.part_ml + (item * 16 + n) * 2, lds_ml[0][0][n], lds_ml[0][1][n]);
-            const int64_t group = (slot - it.slot) / kJoinGroup;
+#pragma unroll
+            for (int j = 0; j < kItems; ++j) {
+                int h, d;
+                if (at_item(j, &h, &d)) attn8_part(pl, item, h, d, D, sum[j]);
+            }
+            if (tid < cols.n) st2_device(pl.part_ml + (item * 16 + n) * 2, lds_ml[0][0][n], lds_ml[0][1][n]);
+            // its group's segments, then the groups
+            const int64_t g0 = it.slot + (slot - it.slot) / kJoinGroup * kJoinGroup;
             const int groups = (it.nc + kJoinGroup - 1) / kJoinGroup;
-            const int64_t g0 = it.slot + group * kJoinGroup;
-            const int in_group = (int)min((int64_t)kJoinGroup, it.slot + it.nc - g0);
-            if (attention_count(pl.count + g0 * pl.hy + blockIdx.y, in_group, &lds_last)) {
-                attention_join<DP>(a, pl, cols, g0, 1, in_group, groups == 1, cols.n, lds_o);
-                if (groups > 1 && attention_count(pl.tops + (int64_t)r * pl.hy + blockIdx.y, groups, &lds_last))
-                    attention_join<DP>(a, pl, cols, it.slot, kJoinGroup, groups, true, cols.n, lds_o);
+            int64_t from = g0;
+            int cnt = (int)min((int64_t)kJoinGroup, it.slot + it.nc - g0), every = 1;
+            unsigned* count = pl.count + g0 * pl.hy + blockIdx.y;
+#pragma unroll 1
+            while (attention_count(count, cnt, &lds_last)) {
+                const bool last = groups == 1 || every > 1;
+                attn8_join<DP>(a, pl, cols, tid, from, every, cnt, last, lds_o);
+                if (last) break;
+                from = it.slot;
+                cnt = groups;
+                every = kJoinGroup;
+                count = pl.tops + (int64_t)r * pl.hy + blockIdx.y;
             }
         }
         __syncthreads();
@@ -535,13 +694,18 @@ hipError_t launch_paged_attention8(AttnArgs a, int cus, void* ws, void* counters
     AttnPlan pl = plan_attention(a, cus, a.unit_rows, resident(a.c.D));
     attention_memory(a, &pl, ws, counters);
     const dim3 grid((unsigned)pl.shares, (unsigned)pl.hy), block(kAttnThreads);
-    const float scale2 = (float)((double)a.scale * 1.4426950408889634);
+    const Attn8Call call = {a,
+                            pl,
+                            (float)((double)a.scale * 1.4426950408889634),
+                            a.hq / a.c.hkv,
+                            fast_div(a.hq / a.c.hkv),
+                            fast_div(pl.tiles)};
     if (a.c.D <= 64)
-        attention8_kernel<64><<<grid, block, 0, s>>>(a, pl, scale2);
+        attention8_kernel<64><<<grid, block, 0, s>>>(call);
     else if (a.c.D <= 128)
-        attention8_kernel<128><<<grid, block, 0, s>>>(a, pl, scale2);
+        attention8_kernel<128><<<grid, block, 0, s>>>(call);
     else
-        attention8_kernel<256><<<grid, block, 0, s>>>(a, pl, scale2);
+        attention8_kernel<256><<<grid, block, 0, s>>>(call);
     return hipGetLastError();
 }
 
