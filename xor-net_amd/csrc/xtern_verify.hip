@@ -46,6 +46,7 @@ struct VerifyPlan {
     unsigned* count;  // [S]: workgroups done, zero between calls
     int rows;         // of a sequence: T + 1, and T of the draft
     int slices, tiles, blocks;
+    int per;          // tiles of a slice
 };
 
 __device__ __forceinline__ float verify_temp(const VerifyArgs& a, int b) {
@@ -61,14 +62,13 @@ __device__ __forceinline__ const T* verify_row(const VerifyArgs& a, int b, int j
                     : static_cast<const T*>(a.draft) + b * a.ldd_seq + (j - a.T - 1) * a.ldd_row;
 }
 
-// exp((x - m) / temperature) for x <= m, c = log2 e / temperature: with y = (x -
-// m) c = n + f, |f| <= 1/2, 2^n times a polynomial of 2^f, of degree 9 through its
-// values in Chebyshev's nodes (the constant term then made 1, so that m itself
-// gives 1): 3e-14 of the result.  0 for x = -inf; the caller sees to NaN and +inf.
-__device__ __forceinline__ double verify_exp(float x, float m, double c) {
-    const double y = fmax(((double)x - (double)m) * c, -1100.0);
-    const double magic = 0x1.8p52, z = y + magic;  // (its last bits: n)
-    const double f = y - (z - magic);
+// 2^y for y <= 0: y = n + f, |f| <= 1/2, a polynomial of 2^f of degree 9 through
+// its values in Chebyshev's nodes (the constant term then made 1, so that 0 gives
+// 1), 3e-14 of the result, and n added to its exponent.  n: the last bits of *z.
+__device__ __forceinline__ double verify_pow2(double y, double* z) {
+    const double magic = 0x1.8p52;
+    *z = y + magic;
+    const double f = y - (*z - magic);
     double p = 0x1.b6571de2f2351p-24;
     p = fma(p, f, 0x1.63ef969a64d3cp-20);
     p = fma(p, f, 0x1.ffcb76789860fp-17);
@@ -78,8 +78,24 @@ __device__ __forceinline__ double verify_exp(float x, float m, double c) {
     p = fma(p, f, 0x1.c6b08d7044119p-5);
     p = fma(p, f, 0x1.ebfbdff8149f2p-3);
     p = fma(p, f, 0x1.62e42fefa39f7p-1);
-    p = fma(p, f, 1.0);
+    return fma(p, f, 1.0);
+}
+// exp((x - m) / temperature) for x <= m, c = log2 e / temperature; 0 for x =
+// -inf; the caller sees to NaN and +inf.
+__device__ __forceinline__ double verify_exp(float x, float m, double c) {
+    double z;
+    const double p = verify_pow2(fmax(((double)x - (double)m) * c, -1100.0), &z);
     return ldexp(p, (int)__builtin_bit_cast(int64_t, z));
+}
+// The same for a sum of at least 1: 2^-1000 instead of anything less.  (m itself
+// gives 1 to the last bit here as well: where p and q have nearly all of it on one
+// token, what is left is the difference of two numbers next to 1.)
+__device__ __forceinline__ double verify_term(float x, double m, double c) {
+    double z;
+    const double p = verify_pow2(fmax(((double)x - m) * c, -1000.0), &z);
+    const uint64_t bits = __builtin_bit_cast(uint64_t, p);
+    const unsigned hi = (unsigned)(bits >> 32) + ((unsigned)__builtin_bit_cast(uint64_t, z) << 20);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | (unsigned)bits);
 }
 __device__ __forceinline__ double verify_rate(float temp) {
     return temp > 0.0f ? 1.4426950408889634 / (double)temp : 0.0;
@@ -114,17 +130,59 @@ struct VerifyTile {
     }
 };
 
+// Over the wave, in every lane: within 16 lanes by DPP (quads, halves of a row,
+// rows), then by lane swaps; 64-bit values as two halves.
+template <int CTRL>
+__device__ __forceinline__ int dpp_to(int v) {
+    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_to(double v) {
+    return __hiloint2double(dpp_to<CTRL>(__double2hiint(v)), dpp_to<CTRL>(__double2loint(v)));
+}
 __device__ __forceinline__ double wave_add(double v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    v += dpp_to<0xb1>(v);
+    v += dpp_to<0x4e>(v);
+    v += dpp_to<0x141>(v);
+    v += dpp_to<0x140>(v);
+    auto h = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
+    auto l = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
+    v = __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
+    h = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(v), false, false);
+    l = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(v), false, false);
+    return __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
+}
+template <typename Op>
+__device__ __forceinline__ int wave_of(int v, Op op) {
+    v = op(v, dpp_to<0xb1>(v));
+    v = op(v, dpp_to<0x4e>(v));
+    v = op(v, dpp_to<0x141>(v));
+    v = op(v, dpp_to<0x140>(v));
+    auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op((int)a[0], (int)a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return op((int)b[0], (int)b[1]);
 }
 __device__ __forceinline__ float wave_most(float v) {
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return __int_as_float(wave_of(__float_as_int(v), [](int a, int b) {
+        return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
+    }));
 }
 __device__ __forceinline__ int wave_least(int v) {
-    for (int o = 32; o; o >>= 1) v = min(v, __shfl_xor(v, o));
-    return v;
+    return wave_of(v, [](int a, int b) { return min(a, b); });
+}
+// Inclusive sums over the lanes.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+    return v + __hiloint2double(dpp_id<CTRL, ROWS>(__double2hiint(v)), dpp_id<CTRL, ROWS>(__double2loint(v)));
+}
+__device__ __forceinline__ double wave_upto(double v) {
+    v = dpp_add<0x111, 0xf>(v);
+    v = dpp_add<0x112, 0xf>(v);
+    v = dpp_add<0x114, 0xf>(v);
+    v = dpp_add<0x118, 0xf>(v);
+    v = dpp_add<0x142, 0xa>(v);
+    return dpp_add<0x143, 0xc>(v);
 }
 
 // Joins stats of one a lane (neutral: l 0, m -inf).
@@ -148,35 +206,38 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
     const float temp = verify_temp(a, b);
     const double c = verify_rate(temp);
     const typename R::T* x = verify_row<typename R::T>(a, b, j);
-    const int per = (pl.tiles + pl.slices - 1) / pl.slices, t1 = min(pl.tiles, (slice + 1) * per);
+    const int per = pl.per, t1 = min(pl.tiles, (slice + 1) * per);
     RowStat s{0.0, -INFINITY, 0x7fffffff};
     bool bad = false;
     for (int t = slice * per + wave; t < t1; t += kVerifyWaves) {
         R r;
         r.load(x, t * kVerifyTile, a.V);
-        float m = s.m;
+        float m = r.x[0];
 #pragma unroll
-        for (int i = 0; i < kVerifyPer; ++i) {
-            m = fmaxf(m, r.x[i]);
-            bad |= !(r.x[i] < INFINITY);
-        }
+        for (int i = 1; i < kVerifyPer; ++i) m = __builtin_elementwise_maximum(m, r.x[i]);  // (NaN stays)
+        bad |= !(m < INFINITY);
         if (temp > 0.0f) {
             if (m > s.m) {
                 s.l *= s.m == -INFINITY ? 0.0 : verify_exp(s.m, m, c);
                 s.m = m;
             }
-            const float base = s.m == -INFINITY ? 0.0f : s.m;
+            if (s.m == -INFINITY) continue;  // (nothing yet)
+            const double base = s.m;
+            // (two sums: half the chain)
+            double l0 = 0.0, l1 = 0.0;
 #pragma unroll
-            for (int i = 0; i < kVerifyPer; ++i) s.l += verify_exp(r.x[i], base, c);
-        } else {
-            if (m > s.m) {
-                int at = 0x7fffffff;
-#pragma unroll
-                for (int i = kVerifyPer - 1; i >= 0; --i)
-                    if (r.x[i] == m) at = R::index(t * kVerifyTile, i);
-                s.m = m;
-                s.at = at;
+            for (int i = 0; i < kVerifyPer; i += 2) {
+                l0 += verify_term(r.x[i], base, c);
+                l1 += verify_term(r.x[i + 1], base, c);
             }
+            s.l += l0 + l1;
+        } else if (m > s.m) {
+            int at = 0x7fffffff;
+#pragma unroll
+            for (int i = kVerifyPer - 1; i >= 0; --i)
+                if (r.x[i] == m) at = R::index(t * kVerifyTile, i);
+            s.m = m;
+            s.at = at;
         }
     }
     if (bad) s.l = NAN;
@@ -198,16 +259,10 @@ struct VerifyDraw {
     int one;        // all of q: this token (draft NULL), -1: none of it
     bool draft;     // q of the draft's logits
 };
-template <int DT>
-__device__ __forceinline__ void verify_left(const VerifyDraw& w, const VerifyTile<DT>& p, const VerifyTile<DT>& q,
-                                            int base, double* left) {
-#pragma unroll
-    for (int i = 0; i < kVerifyPer; ++i) {
-        double v = verify_exp(p.x[i], w.pm, w.c) * w.pl;
-        if (w.draft) v = fmax(v - verify_exp(q.x[i], w.qm, w.c) * w.ql, 0.0);
-        if (VerifyTile<DT>::index(base, i) == w.one) v = 0.0;
-        left[i] = v;
-    }
+__device__ __forceinline__ double verify_left(const VerifyDraw& w, float x, float y, int at) {
+    double v = verify_exp(x, w.pm, w.c) * w.pl;
+    if (w.draft) v = fmax(v - verify_exp(y, w.qm, w.c) * w.ql, 0.0);
+    return at == w.one ? 0.0 : v;
 }
 
 __device__ __forceinline__ void st_device(double* p, double v) {
@@ -228,10 +283,9 @@ __device__ void verify_sums(const VerifyArgs& a, const VerifyPlan& pl, const Ver
         R p, q;
         p.load(prow, t * kVerifyTile, a.V);
         if (w.draft) q.load(qrow, t * kVerifyTile, a.V);
-        double left[kVerifyPer], sum = 0.0;
-        verify_left<DT>(w, p, q, t * kVerifyTile, left);
+        double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kVerifyPer; ++i) sum += left[i];
+        for (int i = 0; i < kVerifyPer; ++i) sum += verify_left(w, p.x[i], q.x[i], R::index(t * kVerifyTile, i));
         sum = wave_add(sum);
         if ((threadIdx.x & 63) == 0) st_device(pl.sums + (int64_t)b * pl.tiles + t, sum);
     }
@@ -242,53 +296,71 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
     typedef VerifyTile<DT> R;
     typedef typename R::T T;
     __shared__ RowStat rows[kVerifyRows];
-    __shared__ double chunk[kVerifyThreads];
     __shared__ double ends[kVerifyWaves];
-    __shared__ int lds_n, lds_last, lds_tile, lds_first;
-    __shared__ double lds_total, lds_before;
+    __shared__ int lds_n, lds_x, lds_last, lds_tile, lds_first;
+    __shared__ double lds_before;
     const int b = blockIdx.x / pl.blocks, block = blockIdx.x % pl.blocks;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int count = verify_count(a, b);
     const float temp = verify_temp(a, b);
     const double c = verify_rate(temp);
     const bool there = count >= 0 && temp >= 0.0f && temp < INFINITY;
-    // the rows' sums
-    for (int j = wave; there && j < pl.rows; j += kVerifyWaves) {
-        if (j <= a.T ? j > count : j - a.T - 1 >= count) continue;
-        RowStat s{0.0, -INFINITY, 0x7fffffff};
-        if (lane < pl.slices) s = pl.stats[((int64_t)b * pl.rows + j) * pl.slices + lane];
-        s = wave_join(s, c);
-        if (temp == 0.0f) s.l = s.m == -INFINITY ? NAN : s.l + 1.0;
-        if (lane == 0) rows[j] = s;
+    // (wave 0) lane t: draft t, its logits and its number, on their way while the
+    // rows' sums are joined
+    int id = -1;
+    float u = 0.0f, px = 0.0f, qx = 0.0f;
+    const bool mine = wave == 0 && there && lane < count;
+    if (mine) {
+        id = a.drafted[(int64_t)b * a.T + lane];
+        u = a.uniforms[(int64_t)b * (a.T + 1) + lane];
+        if ((unsigned)id < (unsigned)a.V) {
+            px = Elem<DT>::get(verify_row<T>(a, b, lane)[id]);
+            if (a.draft) qx = Elem<DT>::get(verify_row<T>(a, b, a.T + 1 + lane)[id]);
+        }
+    }
+    // the rows' sums, four rows of a wave at a time
+    for (int j0 = wave; there && j0 < pl.rows; j0 += 4 * kVerifyWaves) {
+        RowStat s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = j0 + i * kVerifyWaves;
+            s[i] = RowStat{0.0, -INFINITY, 0x7fffffff};
+            if (lane < pl.slices && j < pl.rows && (j <= a.T ? j <= count : j - a.T - 1 < count))
+                s[i] = pl.stats[((int64_t)b * pl.rows + j) * pl.slices + lane];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = j0 + i * kVerifyWaves;
+            if (j >= pl.rows) break;
+            s[i] = wave_join(s[i], c);
+            if (temp == 0.0f) s[i].l = s[i].m == -INFINITY ? NAN : s[i].l + 1.0;
+            if (lane == 0) rows[j] = s[i];
+        }
     }
     __syncthreads();
     // a row of probabilities: its sum is a number, and not 0
     auto fine = [&](int j) { return rows[j].l > 0.0 && rows[j].l < INFINITY; };
     auto chance = [&](int j, float x) { return verify_exp(x, rows[j].m, c) / rows[j].l; };
     if (wave == 0) {
-        // lane t: whether draft t is accepted
+        // whether the draft is accepted
         bool taken = false;
-        if (there && lane < count) {
-            const int x = a.drafted[(int64_t)b * a.T + lane];
-            const float u = a.uniforms[(int64_t)b * (a.T + 1) + lane];
-            if (x >= 0 && x < a.V && fine(lane) && (!a.draft || fine(a.T + 1 + lane))) {
-                if (temp == 0.0f) {
-                    taken = x == rows[lane].at;
-                } else {
-                    const double p = chance(lane, Elem<DT>::get(verify_row<T>(a, b, lane)[x]));
-                    const double q = a.draft ? chance(a.T + 1 + lane, Elem<DT>::get(verify_row<T>(a, b, a.T + 1 + lane)[x])) : 1.0;
-                    taken = (double)u * q < p;
-                }
-            }
+        if (mine && (unsigned)id < (unsigned)a.V && fine(lane) && (!a.draft || fine(a.T + 1 + lane))) {
+            if (temp == 0.0f)
+                taken = id == rows[lane].at;
+            else
+                taken = (double)u * (a.draft ? chance(a.T + 1 + lane, qx) : 1.0) < chance(lane, px);
         }
         const uint64_t no = ~__ballot(taken);
-        if (lane == 0) lds_n = there ? min(no ? (int)__builtin_ctzll(no) : 64, count) : 0;
+        const int accepted = there ? min(no ? (int)__builtin_ctzll(no) : 64, count) : 0;
+        if (lane == accepted) lds_x = id;
+        if (lane == 0) lds_n = accepted;
+        if (lane == 0 && accepted == 64) lds_x = -1;
     }
     __syncthreads();
     const int n = lds_n;
     // the draft that was not accepted; none, or one that is no token: all of p is left
-    const int x = there && n < count ? a.drafted[(int64_t)b * a.T + n] : -1;
-    const bool refused = x >= 0 && x < a.V;
+    const int x = lds_x;
+    const bool refused = (unsigned)x < (unsigned)a.V;
     const bool drawn = there && fine(n) && !(refused && a.draft && !fine(a.T + 1 + n));
     auto finish = [&](int token) {
         if (t == 0) a.accepted[b] = n;
@@ -321,33 +393,29 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
     if (t == 0) lds_last = atomicInc(pl.count + b, (unsigned)pl.blocks - 1) == (unsigned)pl.blocks - 1;
     __syncthreads();
     if (!lds_last) return;
-    // The tile: a run of tiles a thread, the sums before each thread
+    // Sums over the workgroup's threads before each, and of all.
+    auto scan = [&](double v, double* total) {
+        const double upto = wave_upto(v), before = __shfl_up(upto, 1);
+        if (lane == 63) ends[wave] = upto;
+        if (t == 0) lds_first = kVerifyThreads;
+        __syncthreads();
+        double first = lane ? before : 0.0;
+        *total = 0.0;
+        for (int i = 0; i < kVerifyWaves; ++i) {
+            if (i < wave) first += ends[i];
+            *total += ends[i];
+        }
+        return first;
+    };
+    // The tile: a run of tiles a thread
     const int per = (pl.tiles + kVerifyThreads - 1) / kVerifyThreads, first = t * per, end = min(pl.tiles, first + per);
     const double* sums = pl.sums + (int64_t)b * pl.tiles;
-    const double u = a.uniforms[(int64_t)b * (a.T + 1) + a.T];
-    for (int pass = 0; pass < 2; ++pass) {
-        double mine = 0.0;
-        for (int i = first; i < end; ++i) mine += ld_device(sums + i);
-        double upto = mine;
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(upto, o);
-            if (lane >= o) upto += y;
-        }
-        if (lane == 63) ends[wave] = upto;
-        __syncthreads();
-        double total = 0.0, before = 0.0;
-        for (int v = 0; v < kVerifyWaves; ++v) {
-            if (v < wave) before += ends[v];
-            total += ends[v];
-        }
-        chunk[t] = before + upto;
-        if (t == 0) {
-            lds_tile = -1;
-            lds_first = kVerifyThreads;
-            lds_total = total;
-        }
-        __syncthreads();
-        if (lds_total > 0.0) break;
+    double before, total, run;
+    for (int pass = 0;; ++pass) {
+        run = 0.0;
+        for (int i = first; i < end; ++i) run += ld_device(sums + i);
+        before = scan(run, &total);
+        if (total > 0.0 || pass) break;
         // nothing is left of p - q (a u of 1, no number): of p itself
         w.draft = false;
         w.one = -1;
@@ -355,17 +423,20 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
-    const double border = u * lds_total;
-    // the first thread whose run ends above the border; rounding may leave none:
-    // then the last one that adds anything
-    if (first < end && chunk[t] > border) atomicMin(&lds_first, t);
+    const double share = a.uniforms[(int64_t)b * (a.T + 1) + a.T];
+    const double border = share < 1.0 ? share * total : INFINITY;
+    // the first thread whose run ends above the border, in it the first tile;
+    // rounding may leave none: then the last one that adds anything
+    if (before + run > border) atomicMin(&lds_first, t);
+    if (t == 0) lds_tile = -1;
     __syncthreads();
+    const bool past = lds_first == kVerifyThreads;
     if (t == lds_first) {
-        double sum = t ? chunk[t - 1] : 0.0;
+        double sum = before;
         int at = end - 1;
-        double start = sum;
+        lds_before = sum;
         for (int i = first; i < end; ++i) {
-            start = sum;
+            lds_before = sum;
             sum += ld_device(sums + i);
             if (sum > border) {
                 at = i;
@@ -373,68 +444,45 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
             }
         }
         lds_tile = at;
-        lds_before = start;
+    } else if (past) {
+        for (int i = first; i < end; ++i)
+            if (ld_device(sums + i) > 0.0) atomicMax(&lds_tile, i);
     }
     __syncthreads();
-    if (wave == 0) {
-        int tile = lds_tile;
-        double sum = lds_before;
-        const bool past = tile < 0;
-        if (past) {  // (the last tile that holds anything)
-            int at = -1;
-            for (int i = lane; i < pl.tiles; i += 64)
-                if (ld_device(sums + i) > 0.0) at = i;
-            tile = max(0, -wave_least(-at));
-            sum = 0.0;
+    // The token: four of the tile's logits a thread
+    constexpr int kEach = kVerifyTile / kVerifyThreads;
+    const int at = max(lds_tile, 0) * kVerifyTile + t * kEach;
+    const T* prow = verify_row<T>(a, b, n);
+    const T* qrow = w.draft ? verify_row<T>(a, b, a.T + 1 + n) : prow;
+    double left[kEach], mine_left = 0.0;
+    int last = -1;  // the last that is left at all
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        left[i] = at + i < a.V ? verify_left(w, Elem<DT>::get(prow[at + i]), Elem<DT>::get(qrow[at + i]), at + i) : 0.0;
+        mine_left += left[i];
+        if (left[i] > 0.0) last = at + i;
+    }
+    double sum = past ? 0.0 : lds_before;
+    sum += scan(mine_left, &total);
+    if (!past && last >= 0 && sum + mine_left > border) atomicMin(&lds_first, t);
+    if (t == 0) lds_x = 0;
+    __syncthreads();
+    if (t == lds_first) {
+        int token = last;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            sum += left[i];
+            if (sum > border && left[i] > 0.0) {
+                token = at + i;
+                break;
+            }
         }
-        const int base = tile * kVerifyTile;
-        R p, q;
-        p.load(verify_row<T>(a, b, n), base, a.V);
-        if (w.draft) q.load(verify_row<T>(a, b, a.T + 1 + n), base, a.V);
-        double left[kVerifyPer];
-        verify_left<DT>(w, p, q, base, left);
-        int token = -1, last = -1;  // the first above the border; the last that is left at all
-#pragma unroll
-        for (int v = 0; v < R::NV; ++v) {
-            double s = 0.0;
-#pragma unroll
-            for (int i = 0; i < R::W; ++i) {
-                s += left[v * R::W + i];
-                if (left[v * R::W + i] > 0.0) last = R::index(base, v * R::W + i);
-            }
-            double upto = s;
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(upto, o);
-                if (lane >= o) upto += y;
-            }
-            double run = __shfl_up(upto, 1);
-            run = sum + (lane ? run : 0.0);
-            if (!past && token < 0) {
-                const uint64_t above = __ballot(sum + upto > border);
-                if (above) {
-                    const int l = __builtin_ctzll(above);
-                    int at = -1;
-#pragma unroll
-                    for (int i = 0; i < R::W; ++i) {
-                        run += left[v * R::W + i];
-                        const bool over = run > border || i == R::W - 1;
-                        if (at < 0 && over && left[v * R::W + i] > 0.0) at = R::index(base, v * R::W + i);
-                    }
-                    // (rounding: the lane's last that is left)
-                    if (at < 0)
-                        for (int i = 0; i < R::W; ++i)
-                            if (left[v * R::W + i] > 0.0) at = R::index(base, v * R::W + i);
-                    token = __shfl(at, l);
-                }
-            }
-            sum += __shfl(upto, 63);
-        }
-        last = -wave_least(-last);
-        if (token < 0) token = last < 0 ? 0 : last;
-        if (lane == 0) lds_tile = token;
+        lds_x = token;
+    } else if (lds_first == kVerifyThreads && last >= 0) {
+        atomicMax(&lds_x, last);
     }
     __syncthreads();
-    finish(lds_tile);
+    finish(lds_x);
 }
 
 namespace {
@@ -444,10 +492,13 @@ VerifyPlan make_plan(const VerifyArgs& a, int cus) {
     pl.rows = a.T + 1 + (a.draft ? a.T : 0);
     pl.tiles = (a.V + kVerifyTile - 1) / kVerifyTile;
     const int64_t rows = (int64_t)a.S * pl.rows, most = (pl.tiles + kVerifyWaves - 1) / kVerifyWaves;
-    const int64_t want = std::max<int64_t>(1, 8 * (int64_t)cus / rows);
+    // Slices, of a tile a wave at least, until 32 workgroups per compute unit: four
+    // times as many as run at once, for the rows behind a sequence's drafts end at
+    // once
+    const int64_t want = std::max<int64_t>(1, 32 * (int64_t)cus / rows);
     pl.slices = (int)std::min<int64_t>(std::min<int64_t>(want, kVerifySlices), most);
-    const int per = (pl.tiles + pl.slices - 1) / pl.slices;
-    pl.slices = (pl.tiles + per - 1) / per;
+    pl.per = (int)((most + pl.slices - 1) / pl.slices) * kVerifyWaves;
+    pl.slices = (pl.tiles + pl.per - 1) / pl.per;
     pl.blocks = (int)std::min<int64_t>(most, std::max<int64_t>(1, 4 * (int64_t)cus / a.S));
     pl.stats = nullptr;
     pl.sums = nullptr;
