@@ -15,7 +15,7 @@
 // each.  The first kernel reads every row that can count once (HBM bounds large
 // calls: f64 instructions go at the rate of f32 ones), rows cut into slices
 // where they are few; the second decides, reads the one row that is drawn from
-// again, in tiles of 1024 logits a wave, and the workgroup that ends the
+// again, in tiles of 512 logits a wave, and the workgroup that ends the
 // sequence's last tile finds the tile and in it the token (sums and count at
 // device scope, as the chip's eight L2s need it).
 #include <algorithm>
@@ -26,8 +26,10 @@ namespace xt {
 
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWaves = kVerifyThreads / 64;
-constexpr int kVerifyPer = 16;                     // logits of a lane and tile
-constexpr int kVerifyTile = 64 * kVerifyPer;       // of a wave
+constexpr int kStatsPer = 16;                      // logits of a lane and tile, in the first kernel
+constexpr int kDrawPer = 8;                        // and in the second
+constexpr int kStatsTile = 64 * kStatsPer;         // of a wave
+constexpr int kDrawTile = 64 * kDrawPer;
 constexpr int kVerifyRows = 2 * kVerifyDrafts + 1; // of a sequence: target, then draft
 constexpr int kVerifySlices = 64;
 
@@ -42,11 +44,11 @@ struct RowStat {
 
 struct VerifyPlan {
     RowStat* stats;   // [S][rows][slices]
-    double* sums;     // [S][tiles]
+    double* sums;     // [S][draws]
     unsigned* count;  // [S]: workgroups done, zero between calls
     int rows;         // of a sequence: T + 1, and T of the draft
-    int slices, tiles, blocks;
-    int per;          // tiles of a slice
+    int slices, tiles, per;  // of a row, in the first kernel; tiles of a slice
+    int draws, blocks;       // tiles of a row in the second kernel, workgroups of a sequence
 };
 
 __device__ __forceinline__ float verify_temp(const VerifyArgs& a, int b) {
@@ -103,13 +105,13 @@ __device__ __forceinline__ double verify_rate(float temp) {
 
 // A lane's logits of a tile: vectors of 16 bytes (W logits), vector v at base +
 // (v * 64 + lane) * W; -inf past the row.
-template <int DT>
+template <int DT, int PER>
 struct VerifyTile {
-    static constexpr int W = DT == XT_F32 ? 4 : 8, NV = kVerifyPer / W;
+    static constexpr int W = DT == XT_F32 ? 4 : 8, NV = PER / W;
     typedef typename Elem<DT>::T T;
     typedef T Vec __attribute__((ext_vector_type(W)));
     typedef Vec VecU __attribute__((aligned(sizeof(T))));
-    float x[kVerifyPer];
+    float x[PER];
     __device__ __forceinline__ static int index(int base, int i) {
         return base + ((i / W) * 64 + (int)(threadIdx.x & 63)) * W + i % W;
     }
@@ -197,7 +199,7 @@ __device__ __forceinline__ RowStat wave_join(RowStat s, double c) {
 
 template <int DT>
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs a, VerifyPlan pl) {
-    typedef VerifyTile<DT> R;
+    typedef VerifyTile<DT, kStatsPer> R;
     __shared__ RowStat waves[kVerifyWaves];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int slice = blockIdx.x % pl.slices, row = blockIdx.x / pl.slices, b = row / pl.rows, j = row % pl.rows;
@@ -211,10 +213,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
     bool bad = false;
     for (int t = slice * per + wave; t < t1; t += kVerifyWaves) {
         R r;
-        r.load(x, t * kVerifyTile, a.V);
+        r.load(x, t * kStatsTile, a.V);
         float m = r.x[0];
 #pragma unroll
-        for (int i = 1; i < kVerifyPer; ++i) m = __builtin_elementwise_maximum(m, r.x[i]);  // (NaN stays)
+        for (int i = 1; i < kStatsPer; ++i) m = __builtin_elementwise_maximum(m, r.x[i]);  // (NaN stays)
         bad |= !(m < INFINITY);
         if (temp > 0.0f) {
             if (m > s.m) {
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
             // (two sums: half the chain)
             double l0 = 0.0, l1 = 0.0;
 #pragma unroll
-            for (int i = 0; i < kVerifyPer; i += 2) {
+            for (int i = 0; i < kStatsPer; i += 2) {
                 l0 += verify_term(r.x[i], base, c);
                 l1 += verify_term(r.x[i + 1], base, c);
             }
@@ -234,8 +236,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
         } else if (m > s.m) {
             int at = 0x7fffffff;
 #pragma unroll
-            for (int i = kVerifyPer - 1; i >= 0; --i)
-                if (r.x[i] == m) at = R::index(t * kVerifyTile, i);
+            for (int i = kStatsPer - 1; i >= 0; --i)
+                if (r.x[i] == m) at = R::index(t * kStatsTile, i);
             s.m = m;
             s.at = at;
         }
@@ -276,24 +278,24 @@ __device__ __forceinline__ double ld_device(const double* p) {
 template <int DT>
 __device__ void verify_sums(const VerifyArgs& a, const VerifyPlan& pl, const VerifyDraw& w, int b, int n, int first,
                             int step) {
-    typedef VerifyTile<DT> R;
+    typedef VerifyTile<DT, kDrawPer> R;
     const typename R::T* prow = verify_row<typename R::T>(a, b, n);
     const typename R::T* qrow = w.draft ? verify_row<typename R::T>(a, b, a.T + 1 + n) : prow;
-    for (int t = first; t < pl.tiles; t += step) {
+    for (int t = first; t < pl.draws; t += step) {
         R p, q;
-        p.load(prow, t * kVerifyTile, a.V);
-        if (w.draft) q.load(qrow, t * kVerifyTile, a.V);
+        p.load(prow, t * kDrawTile, a.V);
+        if (w.draft) q.load(qrow, t * kDrawTile, a.V);
         double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kVerifyPer; ++i) sum += verify_left(w, p.x[i], q.x[i], R::index(t * kVerifyTile, i));
+        for (int i = 0; i < kDrawPer; ++i) sum += verify_left(w, p.x[i], q.x[i], R::index(t * kDrawTile, i));
         sum = wave_add(sum);
-        if ((threadIdx.x & 63) == 0) st_device(pl.sums + (int64_t)b * pl.tiles + t, sum);
+        if ((threadIdx.x & 63) == 0) st_device(pl.sums + (int64_t)b * pl.draws + t, sum);
     }
 }
 
 template <int DT>
 __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs a, VerifyPlan pl) {
-    typedef VerifyTile<DT> R;
+    typedef VerifyTile<DT, kDrawPer> R;
     typedef typename R::T T;
     __shared__ RowStat rows[kVerifyRows];
     __shared__ double ends[kVerifyWaves];
@@ -305,6 +307,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
     const float temp = verify_temp(a, b);
     const double c = verify_rate(temp);
     const bool there = count >= 0 && temp >= 0.0f && temp < INFINITY;
+    const double share = a.uniforms[(int64_t)b * (a.T + 1) + a.T];
     // (wave 0) lane t: draft t, its logits and its number, on their way while the
     // rows' sums are joined
     int id = -1;
@@ -408,8 +411,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         return first;
     };
     // The tile: a run of tiles a thread
-    const int per = (pl.tiles + kVerifyThreads - 1) / kVerifyThreads, first = t * per, end = min(pl.tiles, first + per);
-    const double* sums = pl.sums + (int64_t)b * pl.tiles;
+    const int per = (pl.draws + kVerifyThreads - 1) / kVerifyThreads, first = t * per, end = min(pl.draws, first + per);
+    const double* sums = pl.sums + (int64_t)b * pl.draws;
     double before, total, run;
     for (int pass = 0;; ++pass) {
         run = 0.0;
@@ -423,7 +426,6 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
-    const double share = a.uniforms[(int64_t)b * (a.T + 1) + a.T];
     const double border = share < 1.0 ? share * total : INFINITY;
     // the first thread whose run ends above the border, in it the first tile;
     // rounding may leave none: then the last one that adds anything
@@ -435,7 +437,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         double sum = before;
         int at = end - 1;
         lds_before = sum;
-        for (int i = first; i < end; ++i) {
+        for (int i = first; i < end && per > 1; ++i) {
             lds_before = sum;
             sum += ld_device(sums + i);
             if (sum > border) {
@@ -450,8 +452,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
     }
     __syncthreads();
     // The token: four of the tile's logits a thread
-    constexpr int kEach = kVerifyTile / kVerifyThreads;
-    const int at = max(lds_tile, 0) * kVerifyTile + t * kEach;
+    constexpr int kEach = kDrawTile / kVerifyThreads;
+    const int at = max(lds_tile, 0) * kDrawTile + t * kEach;
     const T* prow = verify_row<T>(a, b, n);
     const T* qrow = w.draft ? verify_row<T>(a, b, a.T + 1 + n) : prow;
     double left[kEach], mine_left = 0.0;
@@ -490,7 +492,8 @@ namespace {
 VerifyPlan make_plan(const VerifyArgs& a, int cus) {
     VerifyPlan pl;
     pl.rows = a.T + 1 + (a.draft ? a.T : 0);
-    pl.tiles = (a.V + kVerifyTile - 1) / kVerifyTile;
+    pl.tiles = (a.V + kStatsTile - 1) / kStatsTile;
+    pl.draws = (a.V + kDrawTile - 1) / kDrawTile;
     const int64_t rows = (int64_t)a.S * pl.rows, most = (pl.tiles + kVerifyWaves - 1) / kVerifyWaves;
     // Slices, of a tile a wave at least, until 32 workgroups per compute unit: four
     // times as many as run at once, for the rows behind a sequence's drafts end at
@@ -499,7 +502,8 @@ VerifyPlan make_plan(const VerifyArgs& a, int cus) {
     pl.slices = (int)std::min<int64_t>(std::min<int64_t>(want, kVerifySlices), most);
     pl.per = (int)((most + pl.slices - 1) / pl.slices) * kVerifyWaves;
     pl.slices = (pl.tiles + pl.per - 1) / pl.per;
-    pl.blocks = (int)std::min<int64_t>(most, std::max<int64_t>(1, 4 * (int64_t)cus / a.S));
+    pl.blocks = (int)std::min<int64_t>((pl.draws + kVerifyWaves - 1) / kVerifyWaves,
+                                       std::max<int64_t>(1, 4 * (int64_t)cus / a.S));
     pl.stats = nullptr;
     pl.sums = nullptr;
     pl.count = nullptr;
@@ -519,7 +523,7 @@ hipError_t launch(const VerifyArgs& a, const VerifyPlan& pl, hipStream_t s) {
 size_t verify_workspace(const VerifyArgs& a, int cus, size_t* counters) {
     const VerifyPlan pl = make_plan(a, cus);
     *counters = (size_t)a.S * sizeof(unsigned);
-    return (size_t)a.S * pl.rows * pl.slices * sizeof(RowStat) + (size_t)a.S * pl.tiles * sizeof(double);
+    return (size_t)a.S * pl.rows * pl.slices * sizeof(RowStat) + (size_t)a.S * pl.draws * sizeof(double);
 }
 
 hipError_t launch_verify(int dtype, const VerifyArgs& a, int cus, void* ws, void* counters, hipStream_t s) {
