@@ -22,8 +22,9 @@ namespace xt {
 //
 // A head is 16, 32 or 64 lanes of one wave, W = 4 elements each (D and h
 // multiples of four; no alignment is needed), or 64 lanes of every 64th
-// element; each lane also loads the elements that its own are rotated with.  The
-// heads of a row go to several workgroups where rows are few.
+// element; each lane also loads the elements that its own are rotated with, and
+// the next head's of both while it works on one.  The heads of a row go to
+// several workgroups where rows are few.
 template <int DT> struct Held;
 template <> struct Held<XT_I8> { typedef int8_t T; };
 template <> struct Held<XT_F32> { typedef float T; };
@@ -33,22 +34,95 @@ template <> struct Held<XT_BF16> { typedef __bf16 T; };
 constexpr int kStoreThreads = 256;
 constexpr float kLeastHead = 0x1p-119f;
 
-template <typename T>
-__device__ __forceinline__ T lanes_sum(T v, int lanes) {
-    for (int o = lanes / 2; o; o >>= 1) v += __shfl_xor(v, o);
+// Over LANES lanes side by side, in every one of them: within 16 by DPP (quads,
+// halves of a row, rows), then by lane swaps; 64 bits as two halves.
+template <int CTRL>
+__device__ __forceinline__ int dpp_to(int v) {
+    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_to(double v) {
+    return __hiloint2double(dpp_to<CTRL>(__double2hiint(v)), dpp_to<CTRL>(__double2loint(v)));
+}
+template <int LANES>
+__device__ __forceinline__ double lanes_sum(double v) {
+    v += dpp_to<0xb1>(v);
+    v += dpp_to<0x4e>(v);
+    v += dpp_to<0x141>(v);
+    v += dpp_to<0x140>(v);
+    if constexpr (LANES > 16) {
+        const auto h = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
+        const auto l = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
+        v = __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
+    }
+    if constexpr (LANES > 32) {
+        const auto h = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(v), false, false);
+        const auto l = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(v), false, false);
+        v = __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
+    }
     return v;
 }
-__device__ __forceinline__ unsigned lanes_max(unsigned v, int lanes) {
-    for (int o = lanes / 2; o; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
+template <int LANES>
+__device__ __forceinline__ unsigned lanes_max(unsigned v) {
+    v = max(v, (unsigned)dpp_to<0xb1>((int)v));
+    v = max(v, (unsigned)dpp_to<0x4e>((int)v));
+    v = max(v, (unsigned)dpp_to<0x141>((int)v));
+    v = max(v, (unsigned)dpp_to<0x140>((int)v));
+    if constexpr (LANES > 16) {
+        const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(a[0], a[1]);
+    }
+    if constexpr (LANES > 32) {
+        const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max(a[0], a[1]);
+    }
     return v;
 }
 
-template <int DT, int W>
-__global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a, int lanes) {
+template <int DT, int W, int LANES>
+__global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
     typedef typename Held<DT>::T T;
     typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+    constexpr int kGroups = kStoreThreads / LANES;
     const KvView& c = a.c;
     const int64_t r = blockIdx.x;
+    const int D = c.D, half = a.cos ? a.rot / 2 : 0, hq = a.q ? a.hq : 0, heads = hq + 2 * c.hkv;
+    const int l = threadIdx.x & (LANES - 1), group = threadIdx.x / LANES;
+    // element e of the lane; what it is rotated with, and by which pair
+    int d[4], other[4], pair[4];
+    bool turns[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        d[e] = W == 4 ? 4 * l + e : l + 64 * e;
+        turns[e] = d[W == 4 ? 0 : e] < 2 * half;  // (d and half are multiples of four: one test for the lane)
+        other[e] = !turns[e] ? d[e] : (d[e] < half ? d[e] + half : d[e] - half);
+        pair[e] = !turns[e] ? 0 : (d[e] < half ? d[e] : d[e] - half);
+    }
+    const bool any = W == 4 ? d[0] < D : true;  // (W 4: all four or none)
+    // The four elements at i[0], side by side, or those of them that are of the head
+    auto get = [&](const float* p, const int* i, float* x) {
+        if constexpr (W == 4) {
+            const F4 v = *reinterpret_cast<const F4*>(p + (any ? i[0] : 0));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = d[e] < D ? p[i[e]] : 0.0f;
+        }
+    };
+    // x of head h, and what it is rotated with
+    auto load = [&](int h, float* x, float* z) {
+        const bool isq = h < hq, isv = h >= hq + c.hkv;
+        const float* src = (isq ? a.q + r * a.ldq + (int64_t)h * D
+                                : (isv ? a.v + r * a.ldv + (int64_t)(h - hq - c.hkv) * D
+                                       : a.k + r * a.ldk + (int64_t)(h - hq) * D));
+        get(src, d, x);
+        if (half && !isv) get(src, other, z);
+    };
+    const int step = gridDim.y * kGroups;
+    int h = blockIdx.y * kGroups + group;
+    float x[4], z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (h < heads) load(h, x, z);  // (with the row's place still on its way)
     const int slot = a.slots[r];
     const int sq = a.seq ? a.seq[r] : (int)r;
     const int pos = a.cos ? a.pos[r] : 0;
@@ -59,76 +133,53 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a, i
     if (a.lengths && blockIdx.y == 0 && threadIdx.x == 0) a.lengths[r] = pg < 0 ? 0 : slot + 1;
     if (pg < 0) return;
     if (c.score && blockIdx.y == 0)
-        for (int h = threadIdx.x; h < c.hkv; h += kStoreThreads)
-            c.score[((int64_t)pg * c.hkv + h) * c.page + kv_slot(c, slot)] = 0.0f;
-    const int D = c.D, half = a.cos ? a.rot / 2 : 0, hq = a.q ? a.hq : 0;
-    const int l = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = kStoreThreads / lanes;
+        for (int i = threadIdx.x; i < c.hkv; i += kStoreThreads)
+            c.score[((int64_t)pg * c.hkv + i) * c.page + kv_slot(c, slot)] = 0.0f;
     const int64_t at = kv_offset(c, pg, slot, 0);
-    // element e of the lane; what it is rotated with, and by which pair
-    int d[4], other[4], pair[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        d[e] = W == 4 ? 4 * l + e : l + 64 * e;
-        other[e] = d[e] < half ? d[e] + half : d[e] - half;
-        pair[e] = d[e] < half ? d[e] : d[e] - half;
+    float cs[4], sn[4], wq[4], wk[4], oq[4], ok[4];  // the row's rotation, the norms' weights
+    if (half) {
+        get(a.cos + (int64_t)pos * half, pair, cs);
+        get(a.sin + (int64_t)pos * half, pair, sn);
     }
-    // The four elements at i[0], side by side, or those of them that are of the head
-    auto get = [&](const float* p, const int* i, float* x) {
-        if constexpr (W == 4) {
-            const F4 v = *reinterpret_cast<const F4*>(p + i[0]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = v[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = d[e] < D ? p[i[e]] : 0.0f;
+    if (a.k_norm) {
+        get(a.k_norm, d, wk);
+        get(a.k_norm, other, ok);
+        if (hq) {
+            get(a.q_norm, d, wq);
+            get(a.q_norm, other, oq);
         }
-    };
-    const bool any = W == 4 ? d[0] < D : true;  // (W 4: all four or none)
-    // (d and half are multiples of four then: one test for the lane)
-    auto turns = [&](int e) { return d[W == 4 ? 0 : e] < 2 * half; };
-    for (int h = blockIdx.y * groups + group; h < hq + 2 * c.hkv; h += gridDim.y * groups) {
-        const bool isq = h < hq, isv = h >= hq + c.hkv;
+    }
+#pragma unroll 1
+    for (; h < heads; h += step) {
+        float nx[4], nz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (h + step < heads) load(h + step, nx, nz);
+        const bool isq = h < hq, isv = h >= hq + c.hkv, norm = a.k_norm && !isv;
         const int head = isq ? h : (isv ? h - hq - c.hkv : h - hq);
-        const float* src = (isq ? a.q + r * a.ldq : (isv ? a.v + r * a.ldv : a.k + r * a.ldk)) + (int64_t)head * D;
-        const float* w = isq ? a.q_norm : (isv ? nullptr : a.k_norm);
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (any) get(src, d, x);
         double y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = x[e];
+        for (int e = 0; e < 4; ++e) y[e] = any ? x[e] : 0.0f;
         double inv = 1.0;
-        if (w) {
-            const double sum = lanes_sum(fma(y[0], y[0], fma(y[1], y[1], fma(y[2], y[2], y[3] * y[3]))), lanes);
+        if (norm) {
+            const double sum = lanes_sum<LANES>(fma(y[0], y[0], fma(y[1], y[1], fma(y[2], y[2], y[3] * y[3]))));
             inv = 1.0 / sqrt(sum / D + a.eps);
-            if (any) {
-                float g[4];
-                get(w, d, g);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = y[e] * inv * g[e];
-            }
+            for (int e = 0; e < 4; ++e) y[e] = y[e] * inv * (isq ? wq[e] : wk[e]);
         }
-        if (half && !isv && any) {
-            float z[4], g[4] = {1.0f, 1.0f, 1.0f, 1.0f}, cs[4], sn[4];
-            int o[4], p[4];
+        if (half && !isv) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                o[e] = turns(e) ? other[e] : d[e];
-                p[e] = turns(e) ? pair[e] : 0;
-            }
-            get(src, o, z);
-            if (w) get(w, o, g);
-            get(a.cos + (int64_t)pos * half, p, cs);
-            get(a.sin + (int64_t)pos * half, p, sn);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const double u = (double)z[e] * inv * g[e];
-                const double t = d[e] < half ? -(u * sn[e]) : u * sn[e];
-                if (turns(e)) y[e] = fma(y[e], (double)cs[e], t);
+                double u = (double)z[e] * sn[e];
+                if (norm) u = u * inv * (isq ? oq[e] : ok[e]);
+                if (turns[e]) y[e] = fma(y[e], (double)cs[e], d[e] < half ? -u : u);
             }
         }
         float f[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = (float)y[e];
+        for (int e = 0; e < 4; ++e) {
+            f[e] = (float)y[e];
+            x[e] = nx[e];
+            z[e] = nz[e];
+        }
         if (isq) {
             float* to = a.qo + r * a.ldqo + (int64_t)head * D;
             if constexpr (W == 4) {
@@ -147,7 +198,7 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a, i
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (d[e] < D) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-            const float m = __uint_as_float(lanes_max(top, lanes));
+            const float m = __uint_as_float(lanes_max<LANES>(top));
             const bool zero = !(m >= kLeastHead && m < INFINITY);  // (or NaN)
             const float scale = m < kLeastHead ? 0.0f : (m < INFINITY ? (float)((double)m / 127.0) : NAN);
             const double up = zero ? 0.0 : 1.0 / (double)scale;
@@ -238,13 +289,17 @@ hipError_t launch_store(AppendArgs& a, int cus, hipStream_t s) {
     const bool wide = D % 4 == 0 && half % 4 == 0;
     const int lanes = !wide || D > 128 ? 64 : (D > 64 ? 32 : 16), groups = kStoreThreads / lanes;
     const int64_t heads = (a.q ? a.hq : 0) + 2 * (int64_t)a.c.hkv;
-    // workgroups of a row: until two per compute unit
-    const int64_t want = std::max<int64_t>(1, 2 * (int64_t)cus / a.R);
+    // workgroups of a row: until four per compute unit
+    const int64_t want = std::max<int64_t>(1, 4 * (int64_t)cus / a.R);
     const dim3 grid((unsigned)a.R, (unsigned)std::min((heads + groups - 1) / groups, want));
-    if (wide)
-        kv_store_kernel<DT, 4><<<grid, kStoreThreads, 0, s>>>(a, lanes);
+    if (!wide)
+        kv_store_kernel<DT, 1, 64><<<grid, kStoreThreads, 0, s>>>(a);
+    else if (lanes == 64)
+        kv_store_kernel<DT, 4, 64><<<grid, kStoreThreads, 0, s>>>(a);
+    else if (lanes == 32)
+        kv_store_kernel<DT, 4, 32><<<grid, kStoreThreads, 0, s>>>(a);
     else
-        kv_store_kernel<DT, 1><<<grid, kStoreThreads, 0, s>>>(a, lanes);
+        kv_store_kernel<DT, 4, 16><<<grid, kStoreThreads, 0, s>>>(a);
     return hipGetLastError();
 }
 
