@@ -62,6 +62,7 @@ struct AppendArgs {
     const float* q_norm;      // [D] weights of a head's norm, or null (no norms)
     const float* k_norm;
     double eps;
+    double inv_dim;           // 1 / D, set by the launcher
 };
 hipError_t launch_kv_append(int dtype, AppendArgs a, hipStream_t s);
 // With norms, or into 8-bit codes; cus: compute units of the device.

@@ -136,42 +136,58 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
         for (int i = threadIdx.x; i < c.hkv; i += kStoreThreads)
             c.score[((int64_t)pg * c.hkv + i) * c.page + kv_slot(c, slot)] = 0.0f;
     const int64_t at = kv_offset(c, pg, slot, 0);
-    float cs[4], sn[4], wq[4], wk[4], oq[4], ok[4];  // the row's rotation, the norms' weights
-    if (half) {
-        get(a.cos + (int64_t)pos * half, pair, cs);
-        get(a.sin + (int64_t)pos * half, pair, sn);
-    }
-    if (a.k_norm) {
-        get(a.k_norm, d, wk);
-        get(a.k_norm, other, ok);
-        if (hq) {
-            get(a.q_norm, d, wq);
-            get(a.q_norm, other, oq);
+    // Norm and rotation of an element as inv (x A + z B), z what it is rotated
+    // with: A = w cos, B = w' (-sin or sin); of q and of k
+    double A[2][4], B[2][4];
+    {
+        float cs[4], sn[4], w[2][4], o[2][4];
+        if (half) {
+            get(a.cos + (int64_t)pos * half, pair, cs);
+            get(a.sin + (int64_t)pos * half, pair, sn);
         }
+        if (a.k_norm) {
+            get(a.k_norm, d, w[1]);
+            get(a.k_norm, other, o[1]);
+            if (hq) {
+                get(a.q_norm, d, w[0]);
+                get(a.q_norm, other, o[0]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                A[i][e] = a.k_norm ? (double)w[i][e] : 1.0;
+                B[i][e] = 0.0;
+                if (turns[e]) {
+                    B[i][e] = (a.k_norm ? (double)o[i][e] : 1.0) * (d[e] < half ? -sn[e] : sn[e]);
+                    A[i][e] *= cs[e];
+                }
+            }
     }
 #pragma unroll 1
     for (; h < heads; h += step) {
         float nx[4], nz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (h + step < heads) load(h + step, nx, nz);
-        const bool isq = h < hq, isv = h >= hq + c.hkv, norm = a.k_norm && !isv;
+        const bool isq = h < hq, isv = h >= hq + c.hkv;
         const int head = isq ? h : (isv ? h - hq - c.hkv : h - hq);
         double y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = any ? x[e] : 0.0f;
-        double inv = 1.0;
-        if (norm) {
-            const double sum = lanes_sum<LANES>(fma(y[0], y[0], fma(y[1], y[1], fma(y[2], y[2], y[3] * y[3]))));
-            inv = 1.0 / sqrt(sum / D + a.eps);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = y[e] * inv * (isq ? wq[e] : wk[e]);
-        }
-        if (half && !isv) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                double u = (double)z[e] * sn[e];
-                if (norm) u = u * inv * (isq ? oq[e] : ok[e]);
-                if (turns[e]) y[e] = fma(y[e], (double)cs[e], d[e] < half ? -u : u);
+        if (!isv) {
+            double inv = 1.0;
+            if (a.k_norm) {
+                // (the root from the hardware's estimate, 2^-23, in two steps)
+                const double v = lanes_sum<LANES>(fma(y[0], y[0], fma(y[1], y[1], fma(y[2], y[2], y[3] * y[3])))) * a.inv_dim +
+                                 a.eps;
+                inv = __builtin_amdgcn_rsq(v);
+                inv = fma(inv * 0.5, fma(-v * inv, inv, 1.0), inv);
+                inv = fma(inv * 0.5, fma(-v * inv, inv, 1.0), inv);
+                if (!(v > 0.0 && v < INFINITY)) inv = 1.0 / sqrt(v);  // (0, infinity, NaN)
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                y[e] = fma(y[e], isq ? A[0][e] : A[1][e], (turns[e] ? (double)z[e] : 0.0) * (isq ? B[0][e] : B[1][e])) * inv;
         }
         float f[4];
 #pragma unroll
@@ -200,8 +216,12 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
                 if (d[e] < D) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
             const float m = __uint_as_float(lanes_max<LANES>(top));
             const bool zero = !(m >= kLeastHead && m < INFINITY);  // (or NaN)
-            const float scale = m < kLeastHead ? 0.0f : (m < INFINITY ? (float)((double)m / 127.0) : NAN);
-            const double up = zero ? 0.0 : 1.0 / (double)scale;
+            // (m has 24 bits: m / 127 is 2^-32 or more from the middle of two floats,
+            // so that the product rounds like the quotient)
+            const float scale = m < kLeastHead ? 0.0f : (m < INFINITY ? (float)((double)m * (1.0 / 127.0)) : NAN);
+            double up = __builtin_amdgcn_rcp((double)scale);
+            up = fma(up, fma(-(double)scale, up, 1.0), up);
+            up = fma(up, fma(-(double)scale, up, 1.0), up);
 #pragma unroll
             for (int e = 0; e < 4; ++e) held[e] = zero ? 0 : (int8_t)(int)rint(y[e] * up);
             if (l == 0) (isv ? c.vs : c.ks)[((int64_t)pg * c.hkv + head) * c.page + kv_slot(c, slot)] = scale;
@@ -287,6 +307,7 @@ template <int DT>
 hipError_t launch_store(AppendArgs& a, int cus, hipStream_t s) {
     const int half = a.cos ? a.rot / 2 : 0, D = a.c.D;
     const bool wide = D % 4 == 0 && half % 4 == 0;
+    a.inv_dim = 1.0 / D;
     const int lanes = !wide || D > 128 ? 64 : (D > 64 ? 32 : 16), groups = kStoreThreads / lanes;
     const int64_t heads = (a.q ? a.hq : 0) + 2 * (int64_t)a.c.hkv;
     // workgroups of a row: until four per compute unit
