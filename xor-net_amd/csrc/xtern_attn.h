@@ -85,6 +85,13 @@ __device__ __forceinline__ int attn_pos(const AttnArgs& a, int gap, int i) { ret
 // 4000, 1000 rows, 1927 against 2040.  What the limit costs is a long row among
 // many short ones: 1000 rows, one of 60000 positions and the others of 100, 193
 // us on the line and 1018 without; 1100 rows 972 as it is, 210 on the line.
+// Parts (8-bit caches, whose cost per position is half of the others'): with half
+// as many units as workgroups at most, each unit is cut by itself, into as many
+// equal parts as the shortest length allows that gives every part a workgroup of
+// its own.  A share then is one segment; on the line most shares have the end of
+// one unit and the start of the next, and a segment costs as much as 400
+// positions.  24 sequences of 5 tokens and 1032 positions, 20 and 5 heads of 128: 34
+// us on the line, 27 in parts; 48 of one token and 1028 30 and 25.
 // The workgroup that ends the last of a row's segments joins them, from 32
 // segments on in two levels (groups of 32, then the groups): what one
 // workgroup can read at device scope, about 20 GB/s, bounds a join.  Segments
@@ -104,6 +111,7 @@ struct AttnPlan {
     int shares;      // at most
     double inv_shares;
     int units;       // of the call
+    bool parts;      // a share is a part of one unit (8-bit caches)
     bool per_row;
 };
 
@@ -130,6 +138,7 @@ struct AttnLine {
     int64_t per;         // steps of a share
     double inv;          // 1 / per
     int x;               // shares that the line is cut into
+    int cnt, each;       // parts: of the lane's unit, steps of one
 
     __device__ AttnLine(const AttnArgs& a_, const AttnPlan& pl_, int64_t* lds) : a(a_), pl(pl_), ends(lds), R(pl_.units) {
         if (pl.per_row) {
@@ -167,9 +176,31 @@ struct AttnLine {
         per = max((int64_t)1, (int64_t)((double)total * pl.inv_shares));
         if ((per - 1) * pl.shares >= total) --per;
         while (per * pl.shares < total) ++per;
+        if (pl.parts) {
+            const int steps = len < 0 ? 0 : attn_steps(len);
+            // (at most 2^23 steps of a unit, and longer parts at most twice as long)
+            for (int p = (int)per;; p += max(1, p / 8)) {
+                cnt = ceil_quot(steps, p);
+                if (__builtin_amdgcn_readlane(wave_scan(cnt), 63) <= pl.shares) break;
+            }
+            each = cnt ? ceil_quot(steps, cnt) : 1;
+            cnt = ceil_quot(steps, each);
+            upto = wave_scan(cnt);
+            total = x = __builtin_amdgcn_readlane(upto, 63);
+            per = 1;
+            inv = 1.0;
+            return;
+        }
         // (at most 2048 shares: 2^-20 of a quotient is enough)
         inv = __builtin_amdgcn_rcp((double)per);
         x = share_of(total - 1) + 1;
+    }
+    // n / d rounded up, n and d up to 2^23, the quotient up to 2^20.
+    static __device__ int ceil_quot(int n, int d) {
+        const int m = n + d - 1;
+        int q = (int)((float)m * __builtin_amdgcn_rcpf((float)d));
+        q -= (int64_t)q * d > m;
+        return q + ((int64_t)(q + 1) * d <= m);
     }
     // First step of share b; the share that holds a step.
     __device__ int64_t begin(int b) const { return min(b * per, total); }
@@ -207,6 +238,19 @@ struct AttnLine {
             return g;
         }
         int64_t first;
+        if (pl.parts) {
+            const int n = __builtin_amdgcn_readlane(each, r) * kAttnStep;
+            g.n = __builtin_amdgcn_readlane(len, r);
+            g.gap = __builtin_amdgcn_readlane(gap, r);
+            g.seq = __builtin_amdgcn_readlane(seq, r);
+            g.nc = __builtin_amdgcn_readlane(cnt, r);
+            first = __builtin_amdgcn_readlane(upto, r) - g.nc;
+            g.p0 = (int)(from - first) * n;
+            g.p1 = min(g.p0 + n, g.n);
+            g.slot = first + r;
+            *end = to;
+            return g;
+        }
         if (R <= 64) {
             g.n = __builtin_amdgcn_readlane(len, r);
             g.gap = __builtin_amdgcn_readlane(gap, r);
@@ -418,6 +462,7 @@ inline AttnPlan plan_attention(const AttnArgs& a, int cus, int rows, int residen
     pl.shares = std::min(pl.shares, 64 * kJoinGroup);  // (as many as two levels join)
     if (pl.per_row) pl.shares = pl.units;
     pl.inv_shares = 1.0 / (double)pl.shares;
+    pl.parts = false;
     return pl;
 }
 inline bool attention_splits(const AttnArgs& a, const AttnPlan& pl) {

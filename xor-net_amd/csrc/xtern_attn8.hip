@@ -188,11 +188,11 @@ __device__ __forceinline__ void attn8_part(const AttnPlan& pl, int64_t item, int
 // of device-scope loads: up to 16 segments of a thread are on their way at once,
 // while the segments' statistics go through LDS (scratch, 4096 floats).
 template <int DP>
-__device__ void attn8_join(const AttnArgs& a, const AttnPlan& pl, const Attn8Cols& cols, int tid, int64_t slot0,
-                           int every, int cnt, bool last, float* scratch) {
-    constexpr int N = 16, Q = DP / 4;  // segments in flight, threads of a column
+__device__ void attn8_join(const AttnArgs& a, const AttnPlan& pl, const Attn8Cols& cols, int tid, int heads,
+                           int64_t slot0, int every, int cnt, bool last, float* scratch) {
+    constexpr int N = DP == 64 ? 8 : 16, Q = DP / 4;  // segments in flight (as registers allow), threads of a column
     const int D = a.c.D;
-    const int64_t first = slot0 * pl.hy + blockIdx.y, step = (int64_t)every * pl.hy;
+    const int64_t first = slot0 * pl.hy + heads, step = (int64_t)every * pl.hy;
     float2* stats = reinterpret_cast<float2*>(scratch);      // [cnt][16]
     v4f* sums = reinterpret_cast<v4f*>(scratch + 64 * 16 * 2);  // [256]
     // columns that are worked on at once, rounded up to a power of two
@@ -285,10 +285,14 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
     __shared__ v4f lds_scale[kAttnWaves][2][S::TK / 4];  // of a tile's keys, of its values
     __shared__ int lds_last;
     __shared__ int64_t lds_ends[kAttnPlanRows];
+    // Neighbouring shares of one head go to one XCD: units of a sequence then find
+    // its positions in that XCD's L2
+    const int id = xcd_remap(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
+    const int heads = (unsigned)id / gridDim.x, share = id - heads * gridDim.x;
     const AttnLine line(call.a, call.pl, lds_ends);
-    if ((int)blockIdx.x >= line.x) return;
-    int64_t at = line.begin(blockIdx.x);
-    const int64_t to_step = line.begin(blockIdx.x + 1);
+    if (share >= line.x) return;
+    int64_t at = line.begin(share);
+    const int64_t to_step = line.begin(share + 1);
     for (int r = line.row_at(at); at < to_step; ++r) {
         int64_t row_end;
         const AttnSeg it = line.segment(r, at, to_step, &row_end);
@@ -308,13 +312,13 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
         const int n = lane & 15, g = lane >> 4;
         const bool fast = D >= 16;
         const AttnUnit unit = attn_unit(a, r);
-        const int hk = pl.tiles == 1 ? blockIdx.y : fast_quot(blockIdx.y, k.by_tiles);
+        const int hk = pl.tiles == 1 ? heads : fast_quot(heads, k.by_tiles);
         Attn8Cols cols;
         cols.row = unit.row;
         cols.G = k.G;
         cols.by_group = k.by_group;
         cols.several = a.unit_rows > 1;
-        cols.h0 = hk * k.G + ((int)blockIdx.y - hk * pl.tiles) * 16;
+        cols.h0 = hk * k.G + (heads - hk * pl.tiles) * 16;
         cols.n = cols.several ? unit.rows * k.G : min(16, hk * k.G + k.G - cols.h0);
         const int ntiles = it.p1 > it.p0 ? (it.p1 - it.p0 + S::TK - 1) / S::TK : 0;
 
@@ -480,10 +484,6 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                     // three times the registers)
                     asm volatile("" : "+v"(p[4 * t]), "+v"(p[4 * t + 1]), "+v"(p[4 * t + 2]), "+v"(p[4 * t + 3]));
                 }
-                const v4f* vscale = lds_scale[wave][1];
-                v4f vs[S::NT];
-#pragma unroll
-                for (int t = 0; t < S::NT; ++t) vs[t] = vscale[4 * t + g];
                 // the next tile's keys, in flight under this tile's softmax and values
                 const bool was_full = full;
                 const uint64_t was_there = there >> (4 * g);
@@ -514,12 +514,16 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 const float base = m == -INFINITY ? 0.0f : m;
                 float wm = 0.0f;
 #pragma unroll
-                for (int j = 0; j < S::NJ; ++j) {
-                    p[j] = pow2(p[j] - base);
-                    l += p[j];
-                    p[j] *= vs[j / 4][j % 4];
-                    wm = fmaxf(wm, p[j]);
-                    asm volatile("" : "+v"(l));
+                for (int t = 0; t < S::NT; ++t) {
+                    const v4f vs = lds_scale[wave][1][4 * t + g];
+#pragma unroll
+                    for (int j = 4 * t; j < 4 * t + 4; ++j) {
+                        p[j] = pow2(p[j] - base);
+                        l += p[j];
+                        p[j] *= vs[j % 4];
+                        wm = fmaxf(wm, p[j]);
+                        asm volatile("" : "+v"(l));
+                    }
                 }
                 // The weights' digits: p 2^k + 0x808080 is a whole number from
                 // 2^23 up to 2^24, so the float's last bits are its digits, the
@@ -642,7 +646,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 a.lse[(int64_t)w.row * a.hq + w.head] = row_lse(lds_ml[0][0][n], lds_ml[0][1][n]);
             }
         } else {
-            const int64_t slot = (int64_t)blockIdx.x + r, item = slot * pl.hy + blockIdx.y;
+            const int64_t slot = (int64_t)share + r, item = slot * pl.hy + heads;
 #pragma unroll
             for (int j = 0; j < kItems; ++j) {
                 int h, d;
@@ -650,20 +654,21 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             }
             if (tid < cols.n) st2_device(pl.part_ml + (item * 16 + n) * 2, lds_ml[0][0][n], lds_ml[0][1][n]);
             // its group's segments, then the groups
-            const int64_t g0 = it.slot + (slot - it.slot) / kJoinGroup * kJoinGroup;
-            const int groups = (it.nc + kJoinGroup - 1) / kJoinGroup;
+            const int size = it.nc <= 256 ? 16 : kJoinGroup, mine = (int)(slot - it.slot) & ~(size - 1);
+            const int64_t g0 = it.slot + mine;
+            const int groups = (it.nc + size - 1) / size;
             int64_t from = g0;
-            int cnt = (int)min((int64_t)kJoinGroup, it.slot + it.nc - g0), every = 1;
-            unsigned* count = pl.count + g0 * pl.hy + blockIdx.y;
+            int cnt = min(size, it.nc - mine), every = 1;
+            unsigned* count = pl.count + g0 * pl.hy + heads;
 #pragma unroll 1
             while (attention_count(count, cnt, &lds_last)) {
                 const bool last = groups == 1 || every > 1;
-                attn8_join<DP>(a, pl, cols, tid, from, every, cnt, last, lds_o);
+                attn8_join<DP>(a, pl, cols, tid, heads, from, every, cnt, last, lds_o);
                 if (last) break;
                 from = it.slot;
                 cnt = groups;
-                every = kJoinGroup;
-                count = pl.tops + (int64_t)r * pl.hy + blockIdx.y;
+                every = size;
+                count = pl.tops + (int64_t)r * pl.hy + heads;
             }
         }
         __syncthreads();
@@ -679,10 +684,16 @@ int unit_rows(const AttnArgs& a) {
 }
 int resident(int D) { return D > 128 ? 1 : (D > 64 ? 2 : 3); }
 
+AttnPlan make_plan(const AttnArgs& a, int cus) {
+    AttnPlan pl = plan_attention(a, cus, unit_rows(a), resident(a.c.D));
+    pl.parts = pl.units <= 64 && 2 * pl.units <= pl.shares;
+    return pl;
+}
+
 }  // namespace
 
 size_t attention8_workspace(const AttnArgs& a, int cus, size_t* counters) {
-    AttnPlan pl = plan_attention(a, cus, unit_rows(a), resident(a.c.D));
+    AttnPlan pl = make_plan(a, cus);
     *counters = attention_counters(a, pl);
     return place_attention(a, &pl, attention_splits(a, pl), nullptr);
 }
@@ -691,7 +702,7 @@ hipError_t launch_paged_attention8(AttnArgs a, int cus, void* ws, void* counters
     a.unit_rows = unit_rows(a);
     a.units = (a.tokens + a.unit_rows - 1) / a.unit_rows;
     a.by_units = fast_div(a.units);
-    AttnPlan pl = plan_attention(a, cus, a.unit_rows, resident(a.c.D));
+    AttnPlan pl = make_plan(a, cus);
     attention_memory(a, &pl, ws, counters);
     const dim3 grid((unsigned)pl.shares, (unsigned)pl.hy), block(kAttnThreads);
     const Attn8Call call = {a,
