@@ -423,13 +423,12 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             float x[S::KS][16], mx = 0.0f;
 #pragma unroll
             for (int s = 0; s < S::KS; ++s) q_load(s, x[s]);
-            bool full = false;
-            if (wave < ntiles) {
-                full = offsets(wave, next_e);
-                next_e = after_e;
-                load_k(wave);
-                load_v(wave);
-            }
+            // (unconditional, here and in the loop: a tile too many reads offset 0.
+            // Behind loads under a condition the compiler waits for all of them)
+            bool full = offsets(wave, next_e);
+            next_e = after_e;
+            load_k(wave);
+            load_v(wave);
 #pragma unroll
             for (int s = 0; s < S::KS; ++s)
 #pragma unroll
@@ -487,11 +486,9 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 // the next tile's keys, in flight under this tile's softmax and values
                 const bool was_full = full;
                 const uint64_t was_there = there >> (4 * g);
-                if (i + kAttnWaves < ntiles) {
-                    full = offsets(i + kAttnWaves, next_e);
-                    next_e = entry(i + 2 * kAttnWaves);
-                    load_k(i + kAttnWaves);
-                }
+                full = offsets(i + kAttnWaves, next_e);
+                next_e = entry(i + 2 * kAttnWaves);
+                load_k(i + kAttnWaves);
                 if (!was_full) {
 #pragma unroll
                     for (int j = 0; j < S::NJ; ++j) {
@@ -565,7 +562,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                         asm volatile("" : "+v"(sum));
                     }
                 }
-                if (i + kAttnWaves < ntiles) load_v(i + kAttnWaves);
+                load_v(i + kAttnWaves);
             }
             l = rows_sum(l);
         }
