@@ -611,9 +611,10 @@ int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int6
  * temperature >= 0 for every sequence, or temperatures [S]; at 0 all of p lies
  * on the largest logit (the lowest id of equals).  accepted [S]: drafts that
  * were; tokens [S][T + 1]: these, the drawn one, then -1; logprobs [S][T + 1]: ln
- * p of each, then 0.  A row that has to be looked at and has NaN, +inf or
- * nothing but -inf, or a temperature that is none, ends the sequence with -1 in
- * the drawn token's place. */
+ * p of each, then 0; these three overlap neither each other nor an input.  A row
+ * that has to be looked at and has NaN, +inf or nothing but -inf, or a
+ * temperature that is none, ends the sequence with -1 in the drawn token's
+ * place. */
 int xt_verify_drafts(int dtype, const void* target, int64_t ld_seq, int64_t ld_row,
                      const void* draft, int64_t ldd_seq, int64_t ldd_row, int64_t S, int64_t T,
                      int64_t V, const int32_t* drafted, const int32_t* counts,

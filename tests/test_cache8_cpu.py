@@ -106,6 +106,18 @@ def test_calls_without_codes_refuse_them():
     assert L.xt_kv_evict(c, t, P, 8, 0, 0, P + 64, P, None) == xtern.XT_ERR_INVALID
 
 
+def test_verify_outputs_are_arrays_of_their_own():
+    """(2 sequences of 2 drafts: arrays of 4, 2, 6 and 2 words, then 2, 6 and 6)"""
+    at = dict(drafted=P, counts=P + 16, u=P + 24, temps=P + 48, acc=P + 56, tok=P + 64, lp=P + 88)
+    for out, n in (("acc", 2), ("tok", 6), ("lp", 6)):
+        for other, size in (("drafted", 4), ("counts", 2), ("u", 6), ("temps", 2), ("acc", 2), ("tok", 6), ("lp", 6)):
+            if other == out:
+                continue
+            for where in (at[other], at[other] + 4 * size - 4, at[other] - 4 * n + 4):
+                assert verify(**{**at, out: where}) == xtern.XT_ERR_INVALID, (out, other, where)
+                assert b"overlaps" in L.xt_last_error()
+
+
 def test_no_rows_is_no_work():
     assert store(R=0, slots=None, k=None) == xtern.XT_OK
     assert read(R=0, slots=None, k=None) == xtern.XT_OK

@@ -474,7 +474,7 @@ int xt_verify_drafts(int dtype, const void* target, int64_t ld_seq, int64_t ld_r
                      int32_t* tokens, float* logprobs, void* stream) {
     if (int rc = check_dtype(dtype)) return rc;
     if (T < 0 || T > xt::kVerifyDrafts) return bad("drafts of a sequence must be 0..64");
-    if (S < 0 || S * (2 * T + 1) > kMaxRows || S > kMaxRows) return bad("sequences times 2 drafts + 1 must be 0..2^21");
+    if (S < 0 || S > kMaxRows || S * (2 * T + 1) > kMaxRows) return bad("sequences times 2 drafts + 1 must be 0..2^21");
     if (V < 1 || V > (1 << 30)) return bad("vocabulary must be 1..2^30");
     if (!temperatures && !(temperature >= 0.0f && isfinite(temperature))) return bad("temperature must be finite, >= 0");
     if (S == 0) return XT_OK;
@@ -486,11 +486,21 @@ int xt_verify_drafts(int dtype, const void* target, int64_t ld_seq, int64_t ld_r
     }
     const struct {
         const void* p;
+        int64_t n;  // words
         const char* what;
-    } words[] = {{drafted, "drafted"},   {counts, "counts"}, {uniforms, "uniforms"}, {temperatures, "temperatures"},
-                 {accepted, "accepted"}, {tokens, "tokens"}, {logprobs, "logprobs"}};
+    } words[] = {{drafted, S * T, "drafted"},   {counts, S, "counts"},           {uniforms, S * (T + 1), "uniforms"},
+                 {temperatures, S, "temperatures"}, {accepted, S, "accepted"}, {tokens, S * (T + 1), "tokens"},
+                 {logprobs, S * (T + 1), "logprobs"}};
     for (const auto& w : words)
         if (int rc = check_align(w.p, 4, w.what)) return rc;
+    // (a sequence's workgroups read the inputs at any time before its last one
+    // writes, and those of one that ends early after that, too)
+    for (int i = 4; i < 7; ++i)
+        for (int j = 0; j < i; ++j) {
+            const uintptr_t x = reinterpret_cast<uintptr_t>(words[i].p), y = reinterpret_cast<uintptr_t>(words[j].p);
+            if (y && x < y + 4 * (uintptr_t)words[j].n && y < x + 4 * (uintptr_t)words[i].n)
+                return bad(std::string(words[i].what) + " overlaps " + words[j].what);
+        }
     xt::VerifyArgs a;
     memset(&a, 0, sizeof a);
     a.target = target;
