@@ -558,7 +558,8 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
  *   (seq NULL: group g to sequence g); their lengths may be any, 0 for padding.
  *   Over an XT_I8 cache as many rows of a group as have 16 query heads between
  *   them share one pass over its positions; over the others every row makes its
- *   own.
+ *   own.  R times the key-value heads (16 query heads at most each) is below
+ *   2^31 over an XT_I8 cache.
  * Positions that no row sees are not read.  Queries and an XT_I8 cache's codes
  * meet in whole numbers of 24 and 8 bits: results keep the precision of f32. */
 int xt_paged_attention_window(const xt_kv_cache* c, const xt_kv_scales* scales,

@@ -106,6 +106,16 @@ def test_calls_without_codes_refuse_them():
     assert L.xt_kv_evict(c, t, P, 8, 0, 0, P + 64, P, None) == xtern.XT_ERR_INVALID
 
 
+def test_rows_times_heads():
+    """One int numbers the workgroups of a call over codes, a row's heads each."""
+    wide = lambda h: codes(kv_heads=h, head_dim=1, stride_slot=h, stride_page=16 * h, stride_head=1)  # noqa: E731
+    big = dict(ldq=1 << 16, ldo=1 << 16)
+    assert attend(c=wide(65535), R=32769, hq=65535, **big) == xtern.XT_ERR_INVALID
+    assert b"below 2^31" in L.xt_last_error()
+    assert attend(c=wide(16), R=1 << 21, hq=16 * 1024, **big) == xtern.XT_ERR_INVALID
+    assert b"below 2^31" in L.xt_last_error()
+
+
 def test_verify_outputs_are_arrays_of_their_own():
     """(2 sequences of 2 drafts: arrays of 4, 2, 6 and 2 words, then 2, 6 and 6)"""
     at = dict(drafted=P, counts=P + 16, u=P + 24, temps=P + 48, acc=P + 56, tok=P + 64, lp=P + 88)

@@ -574,6 +574,47 @@ def test_graph(dtype):
             assert torch.equal(a, b)
 
 
+def test_two_graphs_of_one_workspace():
+    """Graphs of a stream share its workspace and counters: replayed in turn on it,
+    with an eager call between, each gives what its calls give by themselves."""
+    c, table, ones, g = decode_state(torch.int8)
+    V = 5000
+    seq = torch.tensor([0, 0, 0, 1, 1, 1], **I32)
+    lengths = torch.tensor([1400, 900, 3, 1500, 0, 1200], **I32)
+    q = torch.randn((6, 8, 64), generator=g, device="cuda")
+    target, draft = (3 * torch.randn((4, n, V), generator=g, device="cuda") for n in (4, 3))
+    drafted = draft.argmax(2).to(torch.int32)
+    uniforms = torch.rand((4, 4), generator=g, device="cuda")
+
+    def one():
+        return (xtern.paged_attention(c, table, lengths, q, seq=seq, tokens=3),) + \
+            xtern.verify_drafts(target, drafted, uniforms, draft=draft)
+
+    def other():
+        return (xtern.paged_attention(c, table, lengths, q, seq=seq, tokens=1, window=600, sink=5),) + \
+            xtern.verify_drafts(target[:2], drafted[:2], uniforms[:2])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [[x.clone() for x in f()] for f in (one, other)]
+        graphs = []
+        for f in (one, other):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                out = f()
+            graphs.append((graph, out))
+        for i in (0, 1, 1, 0, 1, 0, 0):
+            graph, out = graphs[i]
+            for x in out:
+                x.fill_(77)
+            graph.replay()
+            eager = (one, other)[1 - i]()
+            for a, b in zip(out + eager, want[i] + want[1 - i], strict=True):
+                assert torch.equal(a, b)
+    torch.cuda.synchronize()
+
+
 def test_streams():
     """Two streams at once, each with its own workspace; a stream argument."""
     c, table, ones, g = decode_state(torch.int8)

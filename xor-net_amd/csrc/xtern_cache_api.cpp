@@ -355,6 +355,10 @@ int xt_paged_attention_window(const xt_kv_cache* c, const xt_kv_scales* scales, 
     // (in place is fine: the workgroups that read a row's head have read it
     // before the one that writes it does)
     if (q == out && ldq != ldo && R > 1) return bad("out overlaps q at another stride");
+    // (its kernel counts the workgroups of all heads in one int)
+    const int64_t tiles = (q_heads / c->kv_heads + 15) / 16;
+    if (c->dtype == XT_I8 && R * c->kv_heads * tiles > kMaxInt)
+        return bad("rows times key-value heads (a head for every 16 query heads) must be below 2^31");
     a.seq = seq;
     a.lengths = lengths;
     a.q = q;
