@@ -46,7 +46,13 @@ struct AttnSpan {
     int n, gap;
     int seq;  // (the unit's)
 };
+// SPANS false: units are rows and see all of their sequences' positions.
+template <bool SPANS>
 __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, int u) {
+    if constexpr (!SPANS) {
+        const int seq = a.seq ? a.seq[u] : u;
+        return AttnSpan{(unsigned)seq < (unsigned)a.c.nseq ? kv_length(a.c, a.lengths[u]) : 0, 0, seq};
+    }
     const AttnUnit x = attn_unit(a, u);
     AttnSpan s{0, 0, x.seq};
     int least = a.c.max_pages * a.c.page;  // (at most 2^30)
@@ -70,7 +76,10 @@ __device__ __forceinline__ AttnSpan attn_span(const AttnArgs& a, int u) {
     s.n -= s.gap;
     return s;
 }
-__device__ __forceinline__ int attn_pos(const AttnArgs& a, int gap, int i) { return i + (i >= a.sink ? gap : 0); }
+template <bool SPANS>
+__device__ __forceinline__ int attn_pos(const AttnArgs& a, int gap, int i) {
+    return SPANS ? i + (i >= a.sink ? gap : 0) : i;
+}
 
 // The split.  The steps of all rows (an empty row has one, for its zeros) form
 // one line, cut into equal shares for as many workgroups as run at once: rows
@@ -127,7 +136,9 @@ struct AttnSeg {
 __device__ __forceinline__ int attn_steps(int len) { return max(1, (len + kAttnStep - 1) / kAttnStep); }
 
 // The line as every wave of the workgroup sees it: 64 units, a lane each, in
-// registers (no barrier), or the units' ends in LDS.
+// registers (no barrier), or the units' ends in LDS.  PARTS: the plan may ask for
+// parts.
+template <bool SPANS, bool PARTS>
 struct AttnLine {
     const AttnArgs& a;
     const AttnPlan& pl;
@@ -149,7 +160,7 @@ struct AttnLine {
         }
         if (R <= 64) {
             const int lane = threadIdx.x & 63;
-            const AttnSpan s = lane < R ? attn_span(a, lane) : AttnSpan{-1, 0, 0};
+            const AttnSpan s = lane < R ? attn_span<SPANS>(a, lane) : AttnSpan{-1, 0, 0};
             len = s.n;
             gap = s.gap;
             seq = s.seq;
@@ -160,7 +171,7 @@ struct AttnLine {
             __shared__ int block[kAttnPlanRows / 64];
             const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
             for (int r = wave * 64; r < R; r += kAttnThreads) {
-                const int up = wave_scan(r + lane < R ? attn_steps(attn_span(a, r + lane).n) : 0);
+                const int up = wave_scan(r + lane < R ? attn_steps(attn_span<SPANS>(a, r + lane).n) : 0);
                 if (r + lane < R) ends[r + lane] = up;
                 if (lane == 63) block[r / 64] = up;
             }
@@ -176,7 +187,7 @@ struct AttnLine {
         per = max((int64_t)1, (int64_t)((double)total * pl.inv_shares));
         if ((per - 1) * pl.shares >= total) --per;
         while (per * pl.shares < total) ++per;
-        if (pl.parts) {
+        if (PARTS && pl.parts) {
             const int steps = len < 0 ? 0 : attn_steps(len);
             // (at most 2^23 steps of a unit, and longer parts at most twice as long)
             for (int p = (int)per;; p += max(1, p / 8)) {
@@ -226,7 +237,7 @@ struct AttnLine {
         AttnSeg g;
         g.row = r;
         if (pl.per_row) {
-            const AttnSpan s = attn_span(a, r);
+            const AttnSpan s = attn_span<SPANS>(a, r);
             g.n = s.n;
             g.gap = s.gap;
             g.seq = s.seq;
@@ -238,7 +249,7 @@ struct AttnLine {
             return g;
         }
         int64_t first;
-        if (pl.parts) {
+        if (PARTS && pl.parts) {
             const int n = __builtin_amdgcn_readlane(each, r) * kAttnStep;
             g.n = __builtin_amdgcn_readlane(len, r);
             g.gap = __builtin_amdgcn_readlane(gap, r);
@@ -258,7 +269,7 @@ struct AttnLine {
             *end = __builtin_amdgcn_readlane(upto, r);
             first = *end - attn_steps(g.n);
         } else {
-            const AttnSpan s = attn_span(a, r);
+            const AttnSpan s = attn_span<SPANS>(a, r);
             g.n = s.n;
             g.gap = s.gap;
             g.seq = s.seq;

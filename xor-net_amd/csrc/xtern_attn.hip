@@ -207,7 +207,7 @@ struct AttnShape {
 // and NaN among the inputs, sums past f32's range in a piece) and head sizes
 // below one load.  256 positions at a time, one head after the other; the sums
 // go where the matrix cores' would be.
-template <int DT>
+template <int DT, bool SPANS>
 __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int hk, int h0, int nh,
                            float scale2, float* lds_o, float* lds_ml, int ldo) {
     typedef Elem<DT> E;
@@ -222,7 +222,7 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
         const float* q = a.q + it.row * a.ldq + (int64_t)(h0 + h) * c.D;
         float m = -INFINITY, l = 0.0f, o = 0.0f;
         for (int p0 = it.p0; p0 < it.p1; p0 += kAttnThreads) {
-            const int i = p0 + t, p = attn_pos(a, it.gap, i), pg = i < it.p1 ? kv_page(c, sq, p) : -1;
+            const int i = p0 + t, p = attn_pos<SPANS>(a, it.gap, i), pg = i < it.p1 ? kv_page(c, sq, p) : -1;
             const int64_t off = pg < 0 ? -1 : kv_offset(c, pg, p, hk);
             float s = -INFINITY;
             if (off >= 0) {
@@ -262,7 +262,9 @@ __device__ void attn_plain(const AttnArgs& a, const AttnPlan& pl, const AttnSeg&
     __syncthreads();
 }
 
-template <int DT, int DP>
+// SPANS: with a window, or several rows to an entry of seq.  (Calls without either
+// would pay 10 registers and, of 180 us for 64 rows, 1.4.)
+template <int DT, int DP, bool SPANS>
 __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) void attention_kernel(AttnArgs a, AttnPlan pl,
                                                                                    float scale2) {
     typedef AttnShape<DT, DP> S;
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
     const int hk = blockIdx.y / pl.tiles, G = a.hq / c.hkv;
     const int h0 = hk * G + (blockIdx.y % pl.tiles) * 16, nh = min(16, hk * G + G - h0);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const AttnLine line(a, pl, lds_ends);
+    const AttnLine<SPANS, false> line(a, pl, lds_ends);
     if ((int)blockIdx.x >= line.x) return;
     int64_t at = line.begin(blockIdx.x);
     const int64_t to_step = line.begin(blockIdx.x + 1);
@@ -318,10 +320,10 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             // LDS; -1: no position there (masked, read from offset 0)
             auto entry = [&](int i) {  // the lane's table entry of tile i
                 const int p = it.p0 + i * S::TK + (lane & (S::TK - 1));
-                return p < it.p1 ? c.table[(int64_t)sq * c.ldt + kv_page_of(c, attn_pos(a, it.gap, p))] : -1;
+                return p < it.p1 ? c.table[(int64_t)sq * c.ldt + kv_page_of(c, attn_pos<SPANS>(a, it.gap, p))] : -1;
             };
             auto offsets = [&](int i, int e) {
-                const int p = attn_pos(a, it.gap, it.p0 + i * S::TK + (lane & (S::TK - 1)));
+                const int p = attn_pos<SPANS>(a, it.gap, it.p0 + i * S::TK + (lane & (S::TK - 1)));
                 const int64_t off = (unsigned)e < (unsigned)c.num_pages ? kv_offset(c, e, p, hk) : -1;
                 if (lane < S::TK) lds_off[wave][(i / kAttnWaves) & 1][lane] = off;
                 return __ballot(off < 0) == 0;
@@ -592,7 +594,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
         }
         // Not all finite (or a tiny head): in plain operations.  (A segment of
         // nothing but holes has a maximum of -inf, sums of 0, and is done.)
-        if (__syncthreads_or(bad)) attn_plain<DT>(a, pl, it, hk, h0, nh, scale2, lds_o, &lds_ml[0][0][0], kLdsRow);
+        if (__syncthreads_or(bad)) attn_plain<DT, SPANS>(a, pl, it, hk, h0, nh, scale2, lds_o, &lds_ml[0][0][0], kLdsRow);
 
         if (it.nc == 1) {
             float* to = a.out + it.row * a.ldo + (int64_t)h0 * D;
@@ -645,7 +647,7 @@ __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const At
     }
     __syncthreads();
     for (int i = it.p0 + threadIdx.x; i < it.p1; i += kAttnThreads) {
-        const int p = attn_pos(a, it.gap, i), pg = kv_page(c, sq, p);
+        const int p = attn_pos<true>(a, it.gap, i), pg = kv_page(c, sq, p);
         if (pg < 0) continue;
         float w = 0.0f;
         for (int h = 0; h < G; ++h)
@@ -656,7 +658,7 @@ __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const At
 
 __global__ __launch_bounds__(kAttnThreads) void attention_score_kernel(AttnArgs a, AttnPlan pl) {
     __shared__ int64_t lds_ends[kAttnPlanRows];
-    const AttnLine line(a, pl, lds_ends);
+    const AttnLine<true, false> line(a, pl, lds_ends);
     if ((int64_t)blockIdx.x >= line.x) return;
     int64_t at = line.begin(blockIdx.x);
     const int64_t to = line.begin(blockIdx.x + 1);
@@ -678,17 +680,22 @@ namespace {
 // 190; of 64, 100 with three and 102 with four).
 int resident(int D) { return D > 128 ? 1 : (D > 64 ? 2 : 3); }
 
-template <int DT>
+template <int DT, bool SPANS>
 hipError_t launch_attention(const AttnArgs& a, const AttnPlan& pl, hipStream_t s) {
     const dim3 grid((unsigned)pl.shares, (unsigned)pl.hy), block(kAttnThreads);
     const float scale2 = (float)((double)a.scale * 1.4426950408889634);
     if (a.c.D <= 64)
-        attention_kernel<DT, 64><<<grid, block, 0, s>>>(a, pl, scale2);
+        attention_kernel<DT, 64, SPANS><<<grid, block, 0, s>>>(a, pl, scale2);
     else if (a.c.D <= 128)
-        attention_kernel<DT, 128><<<grid, block, 0, s>>>(a, pl, scale2);
+        attention_kernel<DT, 128, SPANS><<<grid, block, 0, s>>>(a, pl, scale2);
     else
-        attention_kernel<DT, 256><<<grid, block, 0, s>>>(a, pl, scale2);
+        attention_kernel<DT, 256, SPANS><<<grid, block, 0, s>>>(a, pl, scale2);
     return hipGetLastError();
+}
+template <int DT>
+hipError_t launch_attention_as(const AttnArgs& a, const AttnPlan& pl, hipStream_t s) {
+    const bool spans = a.tokens > 1 || a.window < (int64_t)a.c.max_pages * a.c.page;
+    return spans ? launch_attention<DT, true>(a, pl, s) : launch_attention<DT, false>(a, pl, s);
 }
 
 }  // namespace
@@ -708,9 +715,9 @@ hipError_t launch_paged_attention(int dtype, AttnArgs a, int cus, void* ws, void
     a.by_units = fast_div(a.units);
     hipError_t e;
     switch (dtype) {
-        case XT_F32: e = launch_attention<XT_F32>(a, pl, s); break;
-        case XT_F16: e = launch_attention<XT_F16>(a, pl, s); break;
-        default: e = launch_attention<XT_BF16>(a, pl, s); break;
+        case XT_F32: e = launch_attention_as<XT_F32>(a, pl, s); break;
+        case XT_F16: e = launch_attention_as<XT_F16>(a, pl, s); break;
+        default: e = launch_attention_as<XT_BF16>(a, pl, s); break;
     }
     if (e != hipSuccess || !a.accumulate) return e;
     const size_t lds = 2 * sizeof(float) * (size_t)(a.hq / a.c.hkv);

@@ -115,7 +115,7 @@ __device__ void attn8_plain(const AttnArgs& a, const AttnSeg& it, int hk, const 
         const float* q = a.q + w.row * a.ldq + (int64_t)w.head * c.D;
         float m = -INFINITY, l = 0.0f, o = 0.0f;
         for (int p0 = it.p0; p0 < it.p1; p0 += kAttnThreads) {
-            const int p = attn_pos(a, it.gap, p0 + t);
+            const int p = attn_pos<true>(a, it.gap, p0 + t);
             const int pg = p0 + t < it.p1 && attn_sees(a, len, p) ? kv_page(c, it.seq, p) : -1;
             const int64_t off = pg < 0 ? -1 : kv_offset(c, pg, p, hk);
             float s = -INFINITY, vs = 0.0f;
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
     // its positions in that XCD's L2
     const int id = xcd_remap(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
     const int heads = (unsigned)id / gridDim.x, share = id - heads * gridDim.x;
-    const AttnLine line(call.a, call.pl, lds_ends);
+    const AttnLine<true, true> line(call.a, call.pl, lds_ends);
     if (share >= line.x) return;
     int64_t at = line.begin(share);
     const int64_t to_step = line.begin(share + 1);
@@ -355,10 +355,10 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
             const int8_t* kcol[S::KS];
 #pragma unroll
             for (int s = 0; s < S::KS; ++s) kcol[s] = kc + kd[s];
-            auto pos = [&](int i, int x) { return attn_pos(a, it.gap, it.p0 + i * S::TK + x); };
+            auto pos = [&](int i, int x) { return attn_pos<true>(a, it.gap, it.p0 + i * S::TK + x); };
             auto entry = [&](int i) {  // the lane's table entry of tile i
                 const int x = min(it.p0 + i * S::TK + lane, it.p1 - 1);
-                return c.table[(int64_t)it.seq * c.ldt + kv_page_of(c, attn_pos(a, it.gap, x))];
+                return c.table[(int64_t)it.seq * c.ldt + kv_page_of(c, attn_pos<true>(a, it.gap, x))];
             };
             // Row offsets of a tile's positions, one lane each, through the wave's
             // LDS (0: no position there), and the scales; whether every column
