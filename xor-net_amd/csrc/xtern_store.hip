@@ -270,33 +270,47 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a, int rows) {
     typedef V VU __attribute__((aligned(sizeof(T))));
     typedef O X __attribute__((ext_vector_type(W)));
     typedef X XU __attribute__((aligned(sizeof(O))));
-    for (int x = threadIdx.x >> lg; x < n; x += step) {
+    constexpr int U = 4;  // rows of a thread on their way
+    for (int x0 = threadIdx.x >> lg; x0 < n; x0 += U * step) {
+        int64_t from[U], sat[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int x = min(x0 + u * step, n - 1);
+            from[u] = off[x];
+            sat[u] = sc[x];
+        }
         for (int j = threadIdx.x & ((1 << lg) - 1); j < both; j += 1 << lg) {
             const bool isv = j >= row;
             const int k = isv ? j - row : j, h = fast_quot(k, a.by_per), e = (k - h * per) * W;
-            O* out = static_cast<O*>(isv ? a.v : a.k) + (r0 + x) * (isv ? a.ldv : a.ldk) + (int64_t)h * c.D + e;
-            X y;
-            if (off[x] < 0) {
+            O* out = static_cast<O*>(isv ? a.v : a.k) + (int64_t)h * c.D + e;
+            const T* in = static_cast<const T*>(isv ? c.v : c.k) + h * c.sh + e;
+            [[maybe_unused]] const float* scales = (isv ? c.vs : c.ks) + (int64_t)h * c.page;
+            const int64_t ld = isv ? a.ldv : a.ldk;
+            V v[U];
+            [[maybe_unused]] float s[U];
 #pragma unroll
-                for (int u = 0; u < W; ++u) y[u] = Elem<OT>::put(0.0f);
-            } else {
-                const V v = *reinterpret_cast<const VU*>(static_cast<const T*>(isv ? c.v : c.k) + off[x] + h * c.sh + e);
-                [[maybe_unused]] float s = 1.0f;
-                if constexpr (DT == XT_I8) s = (isv ? c.vs : c.ks)[sc[x] + (int64_t)h * c.page];
+            for (int u = 0; u < U; ++u) {  // (no position: the first one, and not used)
+                v[u] = *reinterpret_cast<const VU*>(in + max(from[u], (int64_t)0));
+                if constexpr (DT == XT_I8) s[u] = scales[sat[u]];
+            }
 #pragma unroll
-                for (int u = 0; u < W; ++u) {
+            for (int u = 0; u < U; ++u) {
+                if (x0 + u * step >= n) break;
+                X y;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
                     if constexpr (DT == XT_I8) {
-                        float f = s * (float)v[u];
+                        float f = s[u] * (float)v[u][i];
                         // (an f32 of its own: with one element a thread the
                         // compiler would round the product to f16 at once)
                         asm("" : "+v"(f));
-                        y[u] = Elem<OT>::put(f);
+                        y[i] = Elem<OT>::put(from[u] < 0 ? 0.0f : f);
                     } else {
-                        y[u] = Elem<OT>::put(Elem<DT>::get(v[u]));
+                        y[i] = Elem<OT>::put(from[u] < 0 ? 0.0f : Elem<DT>::get(v[u][i]));
                     }
                 }
+                *reinterpret_cast<XU*>(out + (r0 + x0 + u * step) * ld) = y;
             }
-            *reinterpret_cast<XU*>(out) = y;
         }
     }
 }
@@ -327,15 +341,17 @@ hipError_t launch_store(AppendArgs& a, int cus, hipStream_t s) {
 template <int DT, int OT>
 hipError_t launch_read(ReadArgs& a, int cus, hipStream_t s) {
     constexpr int kWide = OT == XT_F32 ? 4 : 8;
-    const int w = a.c.D % kWide == 0 ? kWide : 1;
+    const int w = a.c.D % kWide == 0 ? kWide : (a.c.D % 4 == 0 ? 4 : 1);
     a.by_per = fast_div(a.c.D / w);
     const int64_t both = 2 * (int64_t)a.c.hkv * (a.c.D / w);
     // rows until eight workgroups per compute unit, or 16 elements a thread
     const int rows = (int)std::max<int64_t>(
         1, std::min<int64_t>(std::min<int64_t>(32, 4096 / both), a.R / (8 * (int64_t)cus)));
     const unsigned grid = (unsigned)((a.R + rows - 1) / rows);
-    if (w > 1)
+    if (w == kWide)
         kv_read_kernel<DT, OT, kWide><<<grid, 256, 0, s>>>(a, rows);
+    else if (w == 4)
+        kv_read_kernel<DT, OT, 4><<<grid, 256, 0, s>>>(a, rows);
     else
         kv_read_kernel<DT, OT, 1><<<grid, 256, 0, s>>>(a, rows);
     return hipGetLastError();
