@@ -456,6 +456,15 @@ def test_store_layouts(dtype, layout, D):
     store_case(dtype, 4, 2, D, 0, 9, layout=layout, norm=False)  # (nothing to rotate: exact by either kernel)
 
 
+@pytest.mark.parametrize("dtype", [torch.int8, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("D,rot", [(100, 100), (64, 36), (64, 50), (256, 12), (192, 90), (36, 34), (252, 26), (128, 2), (4, 2)])
+def test_store_rotations(dtype, D, rot):
+    """Halves of every remainder by four, in place and not.  (16-bit caches without
+    norms: the append of 32 bits.)"""
+    store_case(dtype, 4, 2, D, rot, 16)
+    store_case(dtype, 4, 2, D, rot, 16, in_place=True, norm=dtype != torch.int8)
+
+
 def test_store_many_rows():
     for dtype in TYPES:
         for D, norm in ((64, True), (100, dtype != torch.int8), (37, True)):

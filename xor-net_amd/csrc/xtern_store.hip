@@ -20,11 +20,11 @@ namespace xt {
 // order sums are taken.  The f64 units take 4 cycles an instruction like the
 // f32 ones, and a call is bound by its bytes or by its launch.
 //
-// A head is 16, 32 or 64 lanes of one wave, W = 4 elements each (D and h
-// multiples of four; no alignment is needed), or 64 lanes of every 64th
-// element; each lane also loads the elements that its own are rotated with, and
-// the next head's of both while it works on one.  The heads of a row go to
-// several workgroups where rows are few.
+// A head is 16, 32 or 64 lanes of one wave, W = 4 elements each (D a multiple of
+// four; no alignment is needed), or 64 lanes of every 64th element.  A lane also
+// loads what its own elements are rotated with, OW = 4, 2 or 1 at a time as h is a
+// multiple of these, and the next head's of both while it works on one.  The heads
+// of a row go to several workgroups where rows are few.
 template <int DT> struct Held;
 template <> struct Held<XT_I8> { typedef int8_t T; };
 template <> struct Held<XT_F32> { typedef float T; };
@@ -79,10 +79,15 @@ __device__ __forceinline__ unsigned lanes_max(unsigned v) {
     return v;
 }
 
-template <int DT, int W, int LANES>
+template <int V> struct Width {
+    static constexpr int value = V;
+};
+
+template <int DT, int W, int OW, int LANES>
 __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
     typedef typename Held<DT>::T T;
     typedef float F4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef float F2 __attribute__((ext_vector_type(2), aligned(4)));
     constexpr int kGroups = kStoreThreads / LANES;
     const KvView& c = a.c;
     const int64_t r = blockIdx.x;
@@ -94,14 +99,23 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         d[e] = W == 4 ? 4 * l + e : l + 64 * e;
-        turns[e] = d[W == 4 ? 0 : e] < 2 * half;  // (d and half are multiples of four: one test for the lane)
+        turns[e] = d[e / OW * OW] < 2 * half;  // (OW of them turn together)
         other[e] = !turns[e] ? d[e] : (d[e] < half ? d[e] + half : d[e] - half);
         pair[e] = !turns[e] ? 0 : (d[e] < half ? d[e] : d[e] - half);
     }
     const bool any = W == 4 ? d[0] < D : true;  // (W 4: all four or none)
-    // The four elements at i[0], side by side, or those of them that are of the head
-    auto get = [&](const float* p, const int* i, float* x) {
-        if constexpr (W == 4) {
+    // The four elements at i[0], or two each at i[0] and i[2], side by side, or those
+    // of the four that are of the head
+    auto get = [&](auto width, const float* p, const int* i, float* x) {
+        constexpr int V = decltype(width)::value;
+        if constexpr (V == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const F2 v = *reinterpret_cast<const F2*>(p + (any ? i[e] : 0));
+                x[e] = v[0];
+                x[e + 1] = v[1];
+            }
+        } else if constexpr (V == 4) {
             const F4 v = *reinterpret_cast<const F4*>(p + (any ? i[0] : 0));
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = v[e];
@@ -116,8 +130,8 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
         const float* src = (isq ? a.q + r * a.ldq + (int64_t)h * D
                                 : (isv ? a.v + r * a.ldv + (int64_t)(h - hq - c.hkv) * D
                                        : a.k + r * a.ldk + (int64_t)(h - hq) * D));
-        get(src, d, x);
-        if (half && !isv) get(src, other, z);
+        get(Width<W>{}, src, d, x);
+        if (half && !isv) get(Width<OW>{}, src, other, z);
     };
     const int step = gridDim.y * kGroups;
     int h = blockIdx.y * kGroups + group;
@@ -142,15 +156,15 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
     {
         float cs[4], sn[4], w[2][4], o[2][4];
         if (half) {
-            get(a.cos + (int64_t)pos * half, pair, cs);
-            get(a.sin + (int64_t)pos * half, pair, sn);
+            get(Width<OW>{}, a.cos + (int64_t)pos * half, pair, cs);
+            get(Width<OW>{}, a.sin + (int64_t)pos * half, pair, sn);
         }
         if (a.k_norm) {
-            get(a.k_norm, d, w[1]);
-            get(a.k_norm, other, o[1]);
+            get(Width<W>{}, a.k_norm, d, w[1]);
+            get(Width<OW>{}, a.k_norm, other, o[1]);
             if (hq) {
-                get(a.q_norm, d, w[0]);
-                get(a.q_norm, other, o[0]);
+                get(Width<W>{}, a.q_norm, d, w[0]);
+                get(Width<OW>{}, a.q_norm, other, o[0]);
             }
         }
 #pragma unroll
@@ -317,10 +331,20 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a, int rows) {
 
 namespace {
 
+template <int DT, int OW>
+void launch_store_of(const AppendArgs& a, int lanes, dim3 grid, hipStream_t s) {
+    if (lanes == 64)
+        kv_store_kernel<DT, 4, OW, 64><<<grid, kStoreThreads, 0, s>>>(a);
+    else if (lanes == 32)
+        kv_store_kernel<DT, 4, OW, 32><<<grid, kStoreThreads, 0, s>>>(a);
+    else
+        kv_store_kernel<DT, 4, OW, 16><<<grid, kStoreThreads, 0, s>>>(a);
+}
+
 template <int DT>
 hipError_t launch_store(AppendArgs& a, int cus, hipStream_t s) {
     const int half = a.cos ? a.rot / 2 : 0, D = a.c.D;
-    const bool wide = D % 4 == 0 && half % 4 == 0;
+    const bool wide = D % 4 == 0;
     a.inv_dim = 1.0 / D;
     const int lanes = !wide || D > 128 ? 64 : (D > 64 ? 32 : 16), groups = kStoreThreads / lanes;
     const int64_t heads = (a.q ? a.hq : 0) + 2 * (int64_t)a.c.hkv;
@@ -328,13 +352,13 @@ hipError_t launch_store(AppendArgs& a, int cus, hipStream_t s) {
     const int64_t want = std::max<int64_t>(1, 4 * (int64_t)cus / a.R);
     const dim3 grid((unsigned)a.R, (unsigned)std::min((heads + groups - 1) / groups, want));
     if (!wide)
-        kv_store_kernel<DT, 1, 64><<<grid, kStoreThreads, 0, s>>>(a);
-    else if (lanes == 64)
-        kv_store_kernel<DT, 4, 64><<<grid, kStoreThreads, 0, s>>>(a);
-    else if (lanes == 32)
-        kv_store_kernel<DT, 4, 32><<<grid, kStoreThreads, 0, s>>>(a);
+        kv_store_kernel<DT, 1, 1, 64><<<grid, kStoreThreads, 0, s>>>(a);
+    else if (half % 4 == 0)
+        launch_store_of<DT, 4>(a, lanes, grid, s);
+    else if (half % 2 == 0)
+        launch_store_of<DT, 2>(a, lanes, grid, s);
     else
-        kv_store_kernel<DT, 4, 16><<<grid, kStoreThreads, 0, s>>>(a);
+        launch_store_of<DT, 1>(a, lanes, grid, s);
     return hipGetLastError();
 }
 
