@@ -100,7 +100,9 @@ __device__ __forceinline__ int attn_pos(const AttnArgs& a, int gap, int i) {
 // its own.  A share then is one segment; on the line most shares have the end of
 // one unit and the start of the next, and a segment costs as much as 400
 // positions.  24 sequences of 5 tokens and 1032 positions, 20 and 5 heads of 128: 34
-// us on the line, 27 in parts; 48 of one token and 1028 30 and 25.
+// us on the line, 26 in parts; 40 of one token and 1028 30 and 24; 30 of 4000, 32 and
+// 8 heads, 53 and 51; 50 of 3000, which are more than half the workgroups, 61.6 (on
+// the line, as it is) and 61.8.
 // The workgroup that ends the last of a row's segments joins them, from 32
 // segments on in two levels (groups of 32, then the groups): what one
 // workgroup can read at device scope, about 20 GB/s, bounds a join.  Segments

@@ -23,8 +23,13 @@ namespace xt {
 // transposed: S^T = K Q^T gives a lane four positions of its own column per 16,
 // which are its operand of O^T = V^T P^T; the value rows it loads as pieces and
 // transposes in registers (v_perm), and only a column's maximum crosses lanes.
-// At D = 128 a tile of 64 positions is 16.9 KB and 48 matrix instructions of 16
-// cycles.
+// At D = 128 a tile of 64 positions is 16.9 KB, 48 matrix instructions of 16 cycles
+// and about 390 others, which take the chip half of the time that HBM takes.
+// 32 and 8 heads of 128: 131072 positions 56 us (4.9 TB/s), 64 rows of up to 8192
+// 101 to 107 (5.2 to 5.5); 700 positions of 20 and 5 heads 13 us, 32 positions 10:
+// the chain of dependent loads (lengths, table, scales and codes, the join's).
+// Value rows are read with the streaming hint (without: 57 and 124 us), key rows
+// are not, whose lines several loads read (with: 61 and 117).
 
 // (rows may start at any byte)
 typedef v4i v4ib __attribute__((aligned(1)));
@@ -650,7 +655,9 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 if (at_item(j, &h, &d)) attn8_part(pl, item, h, d, D, sum[j]);
             }
             if (tid < cols.n) st2_device(pl.part_ml + (item * 16 + n) * 2, lds_ml[0][0][n], lds_ml[0][1][n]);
-            // its group's segments, then the groups
+            // its group's segments, then the groups: of 16, and of 32 where 16 of 16
+            // would not do (16384 positions 20.6 us, in groups of 32 23.8; 131072
+            // 58.5 and 60.2; 3000 16.8 and 16.1)
             const int size = it.nc <= 256 ? 16 : kJoinGroup, mine = (int)(slot - it.slot) & ~(size - 1);
             const int64_t g0 = it.slot + mine;
             const int groups = (it.nc + size - 1) / size;
@@ -679,10 +686,14 @@ int unit_rows(const AttnArgs& a) {
     const int G = a.hq / a.c.hkv;
     return G > 16 ? 1 : std::min(a.tokens, 16 / G);
 }
+// Workgroups per compute unit, as the registers allow: three of D = 128 spill (131072
+// positions 75 us, two 56), two of D = 64 are no slower for one row (38 us) and
+// slower for 64 (69.5, three 65).
 int resident(int D) { return D > 128 ? 1 : (D > 64 ? 2 : 3); }
 
 AttnPlan make_plan(const AttnArgs& a, int cus) {
     AttnPlan pl = plan_attention(a, cus, unit_rows(a), resident(a.c.D));
+    // (the line keeps 64 units in the lanes of a wave)
     pl.parts = pl.units <= 64 && 2 * pl.units <= pl.shares;
     return pl;
 }

@@ -24,7 +24,11 @@ namespace xt {
 // four; no alignment is needed), or 64 lanes of every 64th element.  A lane also
 // loads what its own elements are rotated with, OW = 4, 2 or 1 at a time as h is a
 // multiple of these, and the next head's of both while it works on one.  The heads
-// of a row go to several workgroups where rows are few.
+// of a row go to several workgroups where rows are few.  HBM bounds long calls: 4096
+// rows of 32 + 2 x 8 heads of 128 36 us (5.0 TB/s) on the same tensors again, 41 on
+// others; one row takes 3.5.  Heads of 100:
+// 34 us without a rotation, 36.5 with half of 25, 42.5 with 50 (element by element
+// all of it: 54 and 66).
 template <int DT> struct Held;
 template <> struct Held<XT_I8> { typedef int8_t T; };
 template <> struct Held<XT_F32> { typedef float T; };
@@ -258,7 +262,9 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
 // Rows r of k and v: position slots[r] of its sequence, codes times their scale
 // (or elements) rounded to the output's type; zeros for a row that names no
 // position.  Bound by HBM: a workgroup takes N rows, whose places N threads look
-// up side by side, then copies them, W elements (16 bytes of output) a thread.
+// up side by side, then copies them, W elements (16 bytes of output) a thread and
+// four rows of it at once: 65536 positions of 8 heads of 128 to bf16 85 us (4.8 TB/s
+// read and written; one row at once 93), 41493 of 5 of 192 to f32 88 (128).
 template <int DT, int OT, int W>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a, int rows) {
     typedef typename Held<DT>::T T;
@@ -348,8 +354,9 @@ hipError_t launch_store(AppendArgs& a, int cus, hipStream_t s) {
     a.inv_dim = 1.0 / D;
     const int lanes = !wide || D > 128 ? 64 : (D > 64 ? 32 : 16), groups = kStoreThreads / lanes;
     const int64_t heads = (a.q ? a.hq : 0) + 2 * (int64_t)a.c.hkv;
-    // workgroups of a row: until four per compute unit
-    const int64_t want = std::max<int64_t>(1, 4 * (int64_t)cus / a.R);
+    // workgroups of a row: until two per compute unit (77 rows of 32 + 64 heads: 5.8
+    // us, until four 6.1, eight 6.2)
+    const int64_t want = std::max<int64_t>(1, 2 * (int64_t)cus / a.R);
     const dim3 grid((unsigned)a.R, (unsigned)std::min((heads + groups - 1) / groups, want));
     if (!wide)
         kv_store_kernel<DT, 1, 1, 64><<<grid, kStoreThreads, 0, s>>>(a);
@@ -368,9 +375,10 @@ hipError_t launch_read(ReadArgs& a, int cus, hipStream_t s) {
     const int w = a.c.D % kWide == 0 ? kWide : (a.c.D % 4 == 0 ? 4 : 1);
     a.by_per = fast_div(a.c.D / w);
     const int64_t both = 2 * (int64_t)a.c.hkv * (a.c.D / w);
-    // rows until eight workgroups per compute unit, or 16 elements a thread
+    // rows until four workgroups per compute unit, or 16 pieces a thread (until
+    // eight / 16: 4096 positions of 8 heads of 128 7.1 / 8.7 us, here 6.6)
     const int rows = (int)std::max<int64_t>(
-        1, std::min<int64_t>(std::min<int64_t>(32, 4096 / both), a.R / (8 * (int64_t)cus)));
+        1, std::min<int64_t>(std::min<int64_t>(32, 4096 / both), a.R / (4 * (int64_t)cus)));
     const unsigned grid = (unsigned)((a.R + rows - 1) / rows);
     if (w == kWide)
         kv_read_kernel<DT, OT, kWide><<<grid, 256, 0, s>>>(a, rows);

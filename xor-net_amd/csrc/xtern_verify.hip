@@ -18,6 +18,10 @@
 // again, in tiles of 512 logits a wave, and the workgroup that ends the
 // sequence's last tile finds the tile and in it the token (sums and count at
 // device scope, as the chip's eight L2s need it).
+// 64 sequences of 4 drafts, 128003 bf16 logits: 52 + 30 us, where HBM would take 23:
+// 22 f64 instructions a logit are 36 us of the first kernel.  One sequence of 128256
+// f32 logits: 5.3 + 13.1 us, the second one a chain of eight dependent trips to
+// memory (sums, drafts, their logits, the row, stores, count, tile sums, the tile).
 #include <algorithm>
 
 #include "xtern_cache.h"
@@ -511,7 +515,7 @@ VerifyPlan make_plan(const VerifyArgs& a, int cus) {
     const int64_t rows = (int64_t)a.S * pl.rows, most = (pl.tiles + kVerifyWaves - 1) / kVerifyWaves;
     // Slices, of a tile a wave at least, until 32 workgroups per compute unit: four
     // times as many as run at once, for the rows behind a sequence's drafts end at
-    // once
+    // once (until 12 / 20 / 32: 64 sequences of 4 drafts 60 / 54 / 53 us)
     const int64_t want = std::max<int64_t>(1, 32 * (int64_t)cus / rows);
     pl.slices = (int)std::min<int64_t>(std::min<int64_t>(want, kVerifySlices), most);
     pl.per = (int)((most + pl.slices - 1) / pl.slices) * kVerifyWaves;
