@@ -2,6 +2,8 @@
 read back, attention over the codes; and windows and several tokens of a
 sequence over every type of cache, against plain 64-bit forms.  Memory that a
 call must not look at holds what would show."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -622,6 +624,68 @@ def test_two_graphs_of_one_workspace():
             for a, b in zip(out + eager, want[i] + want[1 - i], strict=True):
                 assert torch.equal(a, b)
     torch.cuda.synchronize()
+
+
+def test_threads():
+    """Four host threads at once, on one stream and on their own."""
+    c, table, _, g = decode_state(torch.int8)
+    seq = torch.tensor([0, 0, 0, 1, 1, 1], **I32)
+    lengths = [torch.tensor(n, **I32) for n in ([1400, 900, 3, 1500, 0, 1200], [7, 1, 1300, 64, 1100, 1490])]
+    q = torch.randn((6, 8, 64), generator=g, device="cuda")
+    target, draft = (3 * torch.randn((4, n, 5000), generator=g, device="cuda") for n in (4, 3))
+    drafted = draft.argmax(2).to(torch.int32)
+    uniforms = torch.rand((4, 4), generator=g, device="cuda")
+
+    def call(i):
+        n = lengths[i % 2]
+        return (xtern.paged_attention(c, table, n, q, seq=seq, tokens=3),
+                *xtern.kv_read(c, table, n - 1, seq=seq),
+                *xtern.verify_drafts(target[i % 2:], drafted[i % 2:], uniforms[i % 2:], draft=draft[i % 2:]))
+
+    want = [call(i) for i in range(2)]
+    torch.cuda.synchronize()
+    for own in (False, True):
+        got, streams = [[] for _ in range(4)], [torch.cuda.Stream() for _ in range(4)]
+
+        def work(i):
+            with torch.cuda.stream(streams[i if own else 0]):
+                for _ in range(20):
+                    got[i].append(call(i))
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        for i in range(4):
+            assert len(got[i]) == 20
+            for x in got[i]:
+                for a, b in zip(x, want[i % 2], strict=True):
+                    assert torch.equal(a, b)
+
+
+def test_most_rows():
+    """As many rows as a call takes: 2^21, two of which are no padding."""
+    R, D = 1 << 21, 4
+    c = xtern.KvCache.new(2, 8, 1, D, dtype=torch.int8)
+    table = torch.tensor([[1]], **I32)
+    slots = torch.full((R,), -1, **I32)
+    slots[0], slots[R - 1] = 3, 5
+    seq = torch.zeros(R, **I32)
+    k = torch.zeros((R, 1, D), device="cuda")
+    k[0, 0], k[R - 1, 0] = torch.tensor([127.0, 1, 2, 3], device="cuda"), torch.tensor([-127.0, 4, 5, 6], device="cuda")
+    lengths = torch.empty(R, **I32)
+    xtern.kv_append(c, table, slots, k, 2 * k, seq=seq, lengths=lengths)
+    assert int(lengths[0]) == 4 and int(lengths[R - 1]) == 6 and int(lengths.sum()) == 10
+    a, b = xtern.kv_read(c, table, slots, seq=seq)
+    assert torch.equal(a, k) and torch.equal(b, 2 * k)
+    # (scores beyond f32's exponents apart: one position has all of it)
+    q = torch.zeros((R, 1, D), device="cuda")
+    q[R - 1, 0, 0] = -10.0
+    out = xtern.paged_attention(c, table, lengths, q, seq=seq)
+    assert torch.equal(out[R - 1], 2 * k[R - 1]) and torch.equal(out[0], k[0] / 2)
+    assert float(out[1:R - 1].abs().max()) == 0.0
 
 
 def test_streams():

@@ -202,6 +202,20 @@ def test_no_sequences():
     assert [tuple(x.shape) for x in got] == [(0,), (0, 3), (0, 3)]
 
 
+def test_most_sequences():
+    """2^21 of them, one row each: the most likely token, and one that is certain."""
+    S = 1 << 21
+    target = torch.zeros((S, 1, 3), device="cuda")
+    target[:, 0, 1] = 200.0
+    target[S - 1, 0, 2] = 400.0
+    uniforms = torch.full((S, 1), 0.5, device="cuda")
+    drafted = torch.empty((S, 0), dtype=torch.int32, device="cuda")
+    for temperature in (0.0, 1.0):
+        accepted, tokens, logprobs = xtern.verify_drafts(target, drafted, uniforms, temperature=temperature)
+        assert int(accepted.abs().max()) == 0 and int(tokens[S - 1]) == 2
+        assert bool((tokens[:S - 1] == 1).all()) and float(logprobs.abs().max()) == 0.0
+
+
 def test_graph_and_streams():
     """Replayed several times with other inputs, eager calls between; two
     streams at once."""
