@@ -241,7 +241,15 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
             up = fma(up, fma(-(double)scale, up, 1.0), up);
             up = fma(up, fma(-(double)scale, up, 1.0), up);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) held[e] = zero ? 0 : (int8_t)(int)rint(y[e] * up);
+            for (int e = 0; e < 4; ++e) {
+                // The quotient, not the product with its divisor's reciprocal: that one
+                // misses middles between two codes (73.5 / 49, whose code is 2, gives
+                // 1.4999999999999998).  One correction: what the product leaves of y is
+                // exact in the fma, so a quotient of 53 bits comes out as it is.
+                double n = y[e] * up;
+                n = fma(fma(-n, (double)scale, y[e]), up, n);
+                held[e] = zero ? 0 : (int8_t)(int)rint(n);
+            }
             if (l == 0) (isv ? c.vs : c.ks)[((int64_t)pg * c.hkv + head) * c.page + kv_slot(c, slot)] = scale;
         } else {
 #pragma unroll
