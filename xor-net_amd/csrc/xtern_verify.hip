@@ -442,26 +442,28 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         __syncthreads();
     }
     const double border = share < 1.0 ? share * total : INFINITY;
-    // the first thread whose run ends above the border, in it the first tile;
-    // rounding may leave none: then the last one that adds anything
-    if (before + run > border) atomicMin(&lds_first, t);
+    // The first thread whose run adds anything and ends above the border, in it the
+    // first such tile; rounding may leave none: then the last one that adds
+    // anything.  (The sums before two threads are rounded in different orders, so a
+    // border on a sum may be passed between them, by a run of nothing but 0.)
+    if (run > 0.0 && before + run > border) atomicMin(&lds_first, t);
     if (t == 0) lds_tile = -1;
     __syncthreads();
     const bool past = lds_first == kVerifyThreads;
     if (t == lds_first) {
         double sum = before;
-        int at = end - 1;
+        int at = per > 1 ? -1 : first;
         lds_before = sum;
         for (int i0 = first; i0 < end && per > 1; i0 += 4) {
             if (per > 4) fetch(i0);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (i0 + i < end && sum <= border) {
+                if (i0 + i < end && four[i] > 0.0 && (at < 0 || sum <= border)) {
                     lds_before = sum;
                     sum += four[i];
                     at = i0 + i;
                 }
-            if (sum > border) break;
+            if (at >= 0 && sum > border) break;
         }
         lds_tile = at;
     } else if (past) {
