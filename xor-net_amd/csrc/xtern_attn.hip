@@ -270,6 +270,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
     typedef AttnShape<DT, DP> S;
     typedef Elem<DT> E;
     typedef typename E::T T;
+    attn_touch_args<AttnArgs, AttnPlan, float>();
     const KvView& c = a.c;
     constexpr int kLdsRow = DP + 4;  // floats; the pad keeps heads apart in the banks
     __shared__ v4i lds_mem[kAttnWaves * 16 * kLdsRow / 4];
@@ -636,6 +637,7 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
 
 // Adds the attention weights of a segment to the scores: one workgroup per
 // (share, kv head), every query head of the group.
+template <bool SPANS>
 __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const AttnSeg& it, int hk) {
     const KvView& c = a.c;
     const int G = a.hq / c.hkv, sq = it.seq;
@@ -647,7 +649,7 @@ __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const At
     }
     __syncthreads();
     for (int i = it.p0 + threadIdx.x; i < it.p1; i += kAttnThreads) {
-        const int p = attn_pos<true>(a, it.gap, i), pg = kv_page(c, sq, p);
+        const int p = attn_pos<SPANS>(a, it.gap, i), pg = kv_page(c, sq, p);
         if (pg < 0) continue;
         float w = 0.0f;
         for (int h = 0; h < G; ++h)
@@ -656,9 +658,11 @@ __device__ void attention_scores(const AttnArgs& a, const AttnPlan& pl, const At
     }
 }
 
+template <bool SPANS>
 __global__ __launch_bounds__(kAttnThreads) void attention_score_kernel(AttnArgs a, AttnPlan pl) {
+    attn_touch_args<AttnArgs, AttnPlan>();
     __shared__ int64_t lds_ends[kAttnPlanRows];
-    const AttnLine<true, false> line(a, pl, lds_ends);
+    const AttnLine<SPANS, false> line(a, pl, lds_ends);
     if ((int64_t)blockIdx.x >= line.x) return;
     int64_t at = line.begin(blockIdx.x);
     const int64_t to = line.begin(blockIdx.x + 1);
@@ -666,7 +670,7 @@ __global__ __launch_bounds__(kAttnThreads) void attention_score_kernel(AttnArgs 
         int64_t row_end;
         const AttnSeg it = line.segment(r, at, to, &row_end);
         at = row_end;
-        attention_scores(a, pl, it, blockIdx.y);
+        attention_scores<SPANS>(a, pl, it, blockIdx.y);
         __syncthreads();
     }
 }
@@ -692,10 +696,12 @@ hipError_t launch_attention(const AttnArgs& a, const AttnPlan& pl, hipStream_t s
         attention_kernel<DT, 256, SPANS><<<grid, block, 0, s>>>(a, pl, scale2);
     return hipGetLastError();
 }
+// Whether a row may see less than all of its positions, or belong to another
+// sequence than its own.
+bool has_spans(const AttnArgs& a) { return a.tokens > 1 || a.window < (int64_t)a.c.max_pages * a.c.page; }
 template <int DT>
 hipError_t launch_attention_as(const AttnArgs& a, const AttnPlan& pl, hipStream_t s) {
-    const bool spans = a.tokens > 1 || a.window < (int64_t)a.c.max_pages * a.c.page;
-    return spans ? launch_attention<DT, true>(a, pl, s) : launch_attention<DT, false>(a, pl, s);
+    return has_spans(a) ? launch_attention<DT, true>(a, pl, s) : launch_attention<DT, false>(a, pl, s);
 }
 
 }  // namespace
@@ -721,7 +727,9 @@ hipError_t launch_paged_attention(int dtype, AttnArgs a, int cus, void* ws, void
     }
     if (e != hipSuccess || !a.accumulate) return e;
     const size_t lds = 2 * sizeof(float) * (size_t)(a.hq / a.c.hkv);
-    attention_score_kernel<<<dim3((unsigned)pl.shares, (unsigned)a.c.hkv), kAttnThreads, lds, s>>>(a, pl);
+    const dim3 grid((unsigned)pl.shares, (unsigned)a.c.hkv);
+    if (has_spans(a)) attention_score_kernel<true><<<grid, kAttnThreads, lds, s>>>(a, pl);
+    else attention_score_kernel<false><<<grid, kAttnThreads, lds, s>>>(a, pl);
     return hipGetLastError();
 }
 

@@ -126,8 +126,8 @@ __device__ void attn8_plain(const AttnArgs& a, const AttnSeg& it, int hk, const 
             float s = -INFINITY, vs = 0.0f;
             if (off >= 0) {
                 const int64_t at = ((int64_t)pg * c.hkv + hk) * c.page + kv_slot(c, p);
-                const float ks = c.ks[at];
-                vs = c.vs[at];
+                const float ks = a.ks[at];
+                vs = a.vs[at];
                 float acc = 0.0f;
                 for (int d = 0; d < c.D; ++d) acc += q[d] * (ks * (float)kc[off + d]);
                 s = acc * scale2;
@@ -374,8 +374,8 @@ __global__ __launch_bounds__(kAttnThreads, DP == 256 ? 1 : (DP == 128 ? 2 : 3)) 
                 const int64_t pg = in ? e : 0, off = pg * c.sp + slot * c.ss + hk * c.sh;
                 lds_off[wave][(i / kAttnWaves) & 1][lane] = in ? off : 0;
                 const int64_t sc = (pg * c.hkv + hk) * c.page + slot;
-                ks_next = c.ks[sc];
-                vs_next = c.vs[sc];
+                ks_next = a.ks[sc];
+                vs_next = a.vs[sc];
                 there = __ballot(in);
                 return __ballot(in & (p < least) & ((p < a.sink) | (p >= most - a.window))) == ~(uint64_t)0;
             };

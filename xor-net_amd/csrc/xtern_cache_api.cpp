@@ -44,8 +44,8 @@ int check_align(const void* p, int size, const char* what) {
     return XT_OK;
 }
 
-// The cache, its scales (XT_I8) and the table as the kernels see them.  `view`
-// gets every field.
+// The cache (whose scales go with an XT_I8 one) and the table as the kernels see
+// them.  `view` gets every field.
 int check_cache(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t, xt::KvView* view) {
     if (!c || !t) return bad("cache or table is NULL");
     const bool codes = c->dtype == XT_I8;
@@ -91,8 +91,6 @@ int check_cache(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_ta
     view->k = c->k;
     view->v = c->v;
     view->score = c->score;
-    view->ks = codes ? scales->k : nullptr;
-    view->vs = codes ? scales->v : nullptr;
     view->sp = c->num_pages == 1 ? 0 : c->stride_page;
     view->ss = c->page_size == 1 ? 0 : c->stride_slot;
     view->sh = c->kv_heads == 1 ? 0 : c->stride_head;
@@ -106,6 +104,12 @@ int check_cache(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_ta
     view->nseq = (int)t->seqs;
     view->max_pages = (int)t->max_pages;
     return XT_OK;
+}
+
+template <typename Args>
+void set_scales(const xt_kv_scales* scales, Args* a) {
+    a->ks = scales ? scales->k : nullptr;
+    a->vs = scales ? scales->v : nullptr;
 }
 
 // R rows of `cols` elements (f32, or of `size` bytes) at stride ld.
@@ -233,6 +237,7 @@ int append_args(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_ta
     if (int rc = check_align(lengths, 4, "lengths")) return rc;
     if (lengths && (lengths == slots || lengths == seq || lengths == positions))
         return bad("lengths must not be slots, seq or positions");
+    set_scales(scales, &a);
     a.lengths = lengths;
     a.seq = seq;
     a.slots = slots;
@@ -312,6 +317,7 @@ int xt_kv_read(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_tab
     const int es = out == XT_F32 ? 4 : 2;
     if (int rc = check_rows(k, ldk, R, cols, "k", es)) return rc;
     if (int rc = check_rows(v, ldv, R, cols, "v", es)) return rc;
+    set_scales(scales, &a);
     a.seq = seq;
     a.slots = slots;
     a.k = k;
@@ -359,6 +365,7 @@ int xt_paged_attention_window(const xt_kv_cache* c, const xt_kv_scales* scales, 
     const int64_t tiles = (q_heads / c->kv_heads + 15) / 16;
     if (c->dtype == XT_I8 && R * c->kv_heads * tiles > kMaxInt)
         return bad("rows times key-value heads (a head for every 16 query heads) must be below 2^31");
+    set_scales(scales, &a);
     a.seq = seq;
     a.lengths = lengths;
     a.q = q;

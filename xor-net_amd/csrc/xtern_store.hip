@@ -250,7 +250,7 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
                 n = fma(fma(-n, (double)scale, y[e]), up, n);
                 held[e] = zero ? 0 : (int8_t)(int)rint(n);
             }
-            if (l == 0) (isv ? c.vs : c.ks)[((int64_t)pg * c.hkv + head) * c.page + kv_slot(c, slot)] = scale;
+            if (l == 0) (isv ? a.vs : a.ks)[((int64_t)pg * c.hkv + head) * c.page + kv_slot(c, slot)] = scale;
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) held[e] = Elem<DT>::put(f[e]);
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a, int rows) {
             const int k = isv ? j - row : j, h = fast_quot(k, a.by_per), e = (k - h * per) * W;
             O* out = static_cast<O*>(isv ? a.v : a.k) + (int64_t)h * c.D + e;
             const T* in = static_cast<const T*>(isv ? c.v : c.k) + h * c.sh + e;
-            [[maybe_unused]] const float* scales = (isv ? c.vs : c.ks) + (int64_t)h * c.page;
+            [[maybe_unused]] const float* scales = (isv ? a.vs : a.ks) + (int64_t)h * c.page;
             const int64_t ld = isv ? a.ldv : a.ldk;
             V v[U];
             [[maybe_unused]] float s[U];

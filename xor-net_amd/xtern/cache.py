@@ -329,6 +329,15 @@ def kv_read(cache, table, slots, seq=None, dtype=None, stream=None):
     return k, v
 
 
+def _check_spans(R, tokens, window, sink):
+    if window is not None and not 1 <= window <= 1 << 30:
+        raise _invalid("window must be 1..2^30")
+    if not 0 <= sink <= 1 << 30 or (sink and window is None):
+        raise _invalid("sink must be 0..2^30, and 0 without a window")
+    if not 1 <= tokens <= 65536 or R % tokens:
+        raise _invalid("tokens must be 1..65536, a divisor of the rows")
+
+
 def paged_attention(cache, table, lengths, q, seq=None, scale=None, lse=False, accumulate=False, out=None,
                     stream=None, window=None, sink=0, tokens=1):
     """xt_paged_attention: row r of q (float32 [R, q_heads, head_dim] or [R,
@@ -347,12 +356,9 @@ def paged_attention(cache, table, lengths, q, seq=None, scale=None, lse=False, a
     qp, ldq, hq = _head_rows(q, "q", D, here)
     R = q.shape[0]
     lp = _vec(lengths, _I32, "lengths", (R,), here)
-    if window is not None and not 1 <= window <= 1 << 30:
-        raise _invalid("window must be 1..2^30")
-    if not 0 <= sink <= 1 << 30 or (sink and window is None):
-        raise _invalid("sink must be 0..2^30, and 0 without a window")
-    if not 1 <= tokens <= 65536 or R % tokens:
-        raise _invalid("tokens must be 1..65536, a divisor of the rows")
+    spans = window is not None or tokens != 1 or sink
+    if spans:
+        _check_spans(R, tokens, window, sink)
     if seq is not None:
         sp = _vec(seq, _I32, "seq", (R,), here)
     elif R > S * tokens:
@@ -366,14 +372,15 @@ def paged_attention(cache, table, lengths, q, seq=None, scale=None, lse=False, a
     l = _empty(stream, _F32, q.device, R, hq) if lse else None
     if stream is not None:
         _mark(stream, *cache._tensors(), table, lengths, q, seq, out)
-    scale = D ** -0.5 if scale is None else scale
-    if window is None and tokens == 1 and cache._sref is None:
-        _check(_lib.xt_paged_attention(c, t, sp, lp, qp, ldq, hq, scale, R, op, ldo, l.data_ptr() if lse else None,
-                                       1 if accumulate else 0, _stream_ptr(stream)))
-    else:
+    if scale is None:
+        scale = D ** -0.5
+    if spans or cache._sref is not None:
         _check(_lib.xt_paged_attention_window(c, cache._sref, t, sp, lp, tokens, window or 0, sink, qp, ldq, hq, scale,
                                               R, op, ldo, l.data_ptr() if lse else None, 1 if accumulate else 0,
                                               _stream_ptr(stream)))
+    else:
+        _check(_lib.xt_paged_attention(c, t, sp, lp, qp, ldq, hq, scale, R, op, ldo, l.data_ptr() if lse else None,
+                                       1 if accumulate else 0, _stream_ptr(stream)))
     return (out, l) if lse else out
 
 
