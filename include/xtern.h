@@ -552,7 +552,8 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
  * NULL), with a window and with several tokens of a sequence:
  * window > 0: a row of length n sees position p only if p < sink or p >= n -
  *   window (the newest `window`, the last one its own); 0: every p < n, and sink
- *   has to be 0.  Both at most 2^30.
+ *   has to be 0.  Both at most 2^30.  With accumulate the workspace holds at most
+ *   window + sink scores of each row.
  * tokens (1..65536, a divisor of R): the rows go in groups of `tokens` that
  *   belong to one sequence, the one that seq names for the group's first row
  *   (seq NULL: group g to sequence g); their lengths may be any, 0 for padding.

@@ -49,8 +49,9 @@ __device__ __forceinline__ AttnUnit attn_unit(const AttnArgs& a, int u) {
         x.seq = a.seq ? a.seq[u] : u;
         return x;
     }
-    const int group = fast_quot(u, a.by_units), first = (u - group * a.units) * a.unit_rows;
-    x.row = group * a.tokens + first;
+    // (row0 > 0: units are rows, these the ones from row0 on)
+    const int v = u + a.row0, group = fast_quot(v, a.by_units), first = (v - group * a.units) * a.unit_rows;
+    x.row = group * a.tokens + first - a.row0;
     x.rows = min(a.unit_rows, a.tokens - first);
     x.seq = a.seq ? a.seq[group * a.tokens] : group;
     return x;
@@ -132,7 +133,7 @@ struct AttnPlan {
     float* ml;       // accumulate: maximum and sum of the whole row, [R][hq][2]
     int dp;          // D, made even
     float* s;        // accumulate: S in base 2, [R][hq][cap]
-    int64_t cap;     // positions of a row of s, a multiple of 32
+    int64_t cap;     // positions that a row may see, its part of s: a multiple of 32
     int hy;          // workgroups per share: kv heads x tiles of 16 query heads
     int tiles;       // of 16 query heads per kv head
     int shares;      // at most
@@ -485,8 +486,8 @@ inline AttnPlan plan_attention(const AttnArgs& a, int cus, int rows, int residen
     pl.hy = a.c.hkv * pl.tiles;
     const int64_t cap = (int64_t)a.c.max_pages * a.c.page;
     const int64_t each = (a.tokens + rows - 1) / rows;  // units of a sequence's rows
-    pl.cap = (cap + 31) / 32 * 32;
-    pl.units = (int)(a.R / a.tokens * each);
+    pl.cap = (std::min(cap, (int64_t)a.window + a.sink) + 31) / 32 * 32;
+    pl.units = (int)(rows == 1 ? a.R : a.R / a.tokens * each);
     pl.per_row = a.call_rows / a.tokens * each > kAttnPlanRows;
     const int64_t steps = pl.units * std::max<int64_t>(1, (cap + kAttnStep - 1) / kAttnStep);
     pl.shares = (int)std::min(steps, std::max<int64_t>(1, (int64_t)resident * cus / pl.hy));

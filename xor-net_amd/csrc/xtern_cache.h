@@ -98,7 +98,9 @@ struct AttnArgs {
     int64_t R;
     int64_t call_rows;       // of the call whose rows, or a part of them, these are
     int window, sink;        // a row of length n sees p < sink and p >= n - window (2^30: every p)
-    int tokens;              // rows r of one sequence: r / tokens
+    int tokens;              // rows r of one sequence: (row0 + r) / tokens, numbered as
+                             // seq and the table are (of the whole call where tokens > 1)
+    int row0;
     // set by the launcher: a sequence's rows, in units of unit_rows
     int unit_rows, units;
     FastDiv by_units;

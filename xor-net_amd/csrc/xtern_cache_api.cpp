@@ -167,15 +167,16 @@ void skip_sequences(xt::KvView* c, int64_t at) {
     c->nseq = (int)std::max<int64_t>(0, c->nseq - at);
 }
 
-// Rows [r0, r0 + n) of a call, whole groups.
+// Rows [r0, r0 + n) of a call.
 xt::AttnArgs rows_of(xt::AttnArgs a, int64_t r0, int64_t n) {
     a.R = n;
     a.q += r0 * a.ldq;
     a.out += r0 * a.ldo;
     if (a.lse) a.lse += r0 * a.hq;
     a.lengths += r0;
-    if (a.seq) a.seq += r0;
-    else skip_sequences(&a.c, r0 / a.tokens);
+    if (a.tokens > 1) a.row0 = (int)r0;  // (groups: seq and table as they are)
+    else if (a.seq) a.seq += r0;
+    else skip_sequences(&a.c, r0);
     return a;
 }
 
@@ -382,9 +383,12 @@ int xt_paged_attention_window(const xt_kv_cache* c, const xt_kv_scales* scales, 
     a.tokens = (int)tokens;
     int64_t part = R;  // rows at a time
     if (a.accumulate) {
-        const int64_t row = 4 * (int64_t)q_heads * t->max_pages * c->page_size;
-        part = part_of(R / tokens, row * tokens) * tokens;
-        if (int rc = check_fits((double)part * (double)row, "the workspace")) return rc;
+        // (a table that no device holds a row's scores of is refused, whatever the
+        // window; a row's scores are those of the positions that it may see.  Every
+        // row makes its own pass, so parts need not be whole groups.)
+        const int64_t cap = t->max_pages * c->page_size, seen = std::min(cap, (int64_t)a.window + a.sink);
+        if (int rc = check_fits(4.0 * q_heads * (double)cap, "the workspace")) return rc;
+        part = part_of(R, 4 * (int64_t)q_heads * seen);
     }
     int cus = 0;
     if (int rc = xt_internal_cus(&cus)) return rc;
