@@ -130,6 +130,23 @@ int check_logits(const void* p, int64_t ld_seq, int64_t ld_row, int64_t S, int64
     return check_align(p, size, what);
 }
 
+// Whether [out, out + bytes) shares memory with a row of those.
+bool meets_logits(uintptr_t out, uint64_t bytes, const void* p, int64_t ld_seq, int64_t ld_row, int64_t S, int64_t rows,
+                  int64_t V, int size) {
+    const uint64_t row = (uint64_t)V * size, by_row = rows > 1 ? (uint64_t)ld_row * size : 0;
+    const uint64_t by_seq = S > 1 ? (uint64_t)ld_seq * size : 0, last = (uint64_t)S - 1;
+    const uintptr_t first = reinterpret_cast<uintptr_t>(p);
+    if (out + bytes <= first || out >= first + last * by_seq + (uint64_t)(rows - 1) * by_row + row) return false;
+    for (int64_t j = 0; j < rows; ++j) {
+        const uintptr_t at = first + (uint64_t)j * by_row;
+        if (out + bytes <= at) break;  // (all of them begin behind it)
+        // the last sequence whose row begins before out's end: the others' end earlier
+        const uint64_t i = by_seq ? std::min(last, (out + bytes - 1 - at) / by_seq) : 0;
+        if (at + i * by_seq + row > out) return true;
+    }
+    return false;
+}
+
 int check_count(int64_t R) {
     if (R < 0 || R > kMaxRows) return bad("row count must be 0..2^21");
     return XT_OK;
@@ -499,11 +516,12 @@ int xt_verify_drafts(int dtype, const void* target, int64_t ld_seq, int64_t ld_r
     if (draft && T > 0) {
         if (int rc = check_logits(draft, ldd_seq, ldd_row, S, T, V, "draft", es)) return rc;
     }
-    const struct {
+    struct Words {
         const void* p;
         int64_t n;  // words
         const char* what;
-    } words[] = {{drafted, S * T, "drafted"},   {counts, S, "counts"},           {uniforms, S * (T + 1), "uniforms"},
+    };
+    const Words words[] = {{drafted, S * T, "drafted"},   {counts, S, "counts"},           {uniforms, S * (T + 1), "uniforms"},
                  {temperatures, S, "temperatures"}, {accepted, S, "accepted"}, {tokens, S * (T + 1), "tokens"},
                  {logprobs, S * (T + 1), "logprobs"}};
     for (const auto& w : words)
@@ -516,6 +534,14 @@ int xt_verify_drafts(int dtype, const void* target, int64_t ld_seq, int64_t ld_r
             if (y && x < y + 4 * (uintptr_t)words[j].n && y < x + 4 * (uintptr_t)words[i].n)
                 return bad(std::string(words[i].what) + " overlaps " + words[j].what);
         }
+    for (int i = 4; i < 7; ++i) {
+        const Words& w = words[i];
+        const uintptr_t x = reinterpret_cast<uintptr_t>(w.p);
+        if (meets_logits(x, 4 * (uint64_t)w.n, target, ld_seq, ld_row, S, T + 1, V, es))
+            return bad(std::string(w.what) + " overlaps target");
+        if (draft && T > 0 && meets_logits(x, 4 * (uint64_t)w.n, draft, ldd_seq, ldd_row, S, T, V, es))
+            return bad(std::string(w.what) + " overlaps draft");
+    }
     xt::VerifyArgs a;
     memset(&a, 0, sizeof a);
     a.target = target;
