@@ -10,6 +10,12 @@
 // is above u_T times the whole.  So the tokens are distributed as the target's.
 // At temperature 0 everything lies on the largest logit, the lowest of equals.
 //
+// p and q are e / l, e = exp((x - m) / temperature) and l the sum of a row's; both
+// sides of a comparison are multiplied by the rows' l instead: u e_q l_p < e_p l_q,
+// and what is left in units of 1 / (l_p l_q), or 1 / l_p.  Equal logits have e = 1 to
+// the bit, so that their sums are whole numbers and a border that lies on one is
+// met exactly.
+//
 // Everything that decides is in 64 bits: a token flips where a sum of V terms
 // crosses a border, and f32 exponentials would move some of V borders by 1e-8
 // each.  The first kernel reads every row that can count once (HBM bounds large
@@ -257,10 +263,11 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyArgs
     }
 }
 
-// What the second kernel draws from: max(p - q, 0), each exp((x - m) / temperature) / l.
+// What the second kernel draws from: max(p - q, 0) in units of 1 / (l_p l_q); without
+// draft logits p, or p without one token, in units of 1 / l_p.
 struct VerifyDraw {
     float pm, qm;
-    double pl, ql;  // 1 / l
+    double pl, ql;  // the factors of exp((x - m) / temperature): the other row's l; 1
     double c;
     int one;        // all of q: this token (draft NULL), -1: none of it
     bool draft;     // q of the draft's logits
@@ -347,7 +354,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
     __syncthreads();
     // a row of probabilities: its sum is a number, and not 0
     auto fine = [&](int j) { return rows[j].l > 0.0 && rows[j].l < INFINITY; };
-    auto chance = [&](int j, float x) { return verify_exp(x, rows[j].m, c) / rows[j].l; };
+    auto term = [&](int j, float x) { return verify_exp(x, rows[j].m, c); };
     if (wave == 0) {
         // whether the draft is accepted
         const bool mine = there && lane < count;
@@ -356,8 +363,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         if (mine && (unsigned)id < (unsigned)a.V && fine(lane) && (!a.draft || fine(a.T + 1 + lane))) {
             if (temp == 0.0f)
                 taken = id == rows[lane].at;
+            else if (a.draft)
+                taken = (double)u * term(a.T + 1 + lane, qx) * rows[lane].l < term(lane, px) * rows[a.T + 1 + lane].l;
             else
-                taken = (double)u * (a.draft ? chance(a.T + 1 + lane, qx) : 1.0) < chance(lane, px);
+                taken = (double)u * rows[lane].l < term(lane, px);
         }
         const uint64_t no = ~__ballot(taken);
         const int accepted = there ? min(no ? (int)__builtin_ctzll(no) : 64, count) : 0;
@@ -389,12 +398,12 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
     }
     VerifyDraw w;
     w.pm = rows[n].m;
-    w.pl = 1.0 / rows[n].l;
     w.c = c;
     w.draft = refused && a.draft;
     w.one = refused && !a.draft ? x : -1;
+    w.pl = w.draft ? rows[a.T + 1 + n].l : 1.0;
     w.qm = w.draft ? rows[a.T + 1 + n].m : 0.0f;
-    w.ql = w.draft ? 1.0 / rows[a.T + 1 + n].l : 0.0;
+    w.ql = w.draft ? rows[n].l : 0.0;
     verify_sums<DT>(a, pl, w, b, n, block * kVerifyWaves + wave, pl.blocks * kVerifyWaves);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every store has arrived
     __syncthreads();
@@ -437,6 +446,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
         // nothing is left of p - q (a u of 1, no number): of p itself
         w.draft = false;
         w.one = -1;
+        w.pl = 1.0;
         verify_sums<DT>(a, pl, w, b, n, wave, kVerifyWaves);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -471,7 +481,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_draw_kernel(VerifyArgs 
             if (ld_device(sums + i) > 0.0) atomicMax(&lds_tile, i);
     }
     __syncthreads();
-    // The token: four of the tile's logits a thread
+    // The token: kEach of the tile's logits a thread
     constexpr int kEach = kDrawTile / kVerifyThreads;
     const int at = max(lds_tile, 0) * kDrawTile + t * kEach;
     const T* prow = verify_row<T>(a, b, n);
