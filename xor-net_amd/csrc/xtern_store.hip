@@ -237,15 +237,14 @@ __global__ __launch_bounds__(kStoreThreads) void kv_store_kernel(AppendArgs a) {
             // (m has 24 bits: m / 127 is 2^-32 or more from the middle of two floats,
             // so that the product rounds like the quotient)
             const float scale = m < kLeastHead ? 0.0f : (m < INFINITY ? (float)((double)m * (1.0 / 127.0)) : NAN);
-            double up = __builtin_amdgcn_rcp((double)scale);
-            up = fma(up, fma(-(double)scale, up, 1.0), up);
+            double up = __builtin_amdgcn_rcp((double)scale);  // (2^-23, in a step 2^-46)
             up = fma(up, fma(-(double)scale, up, 1.0), up);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 // The quotient, not the product with its divisor's reciprocal: that one
                 // misses middles between two codes (73.5 / 49, whose code is 2, gives
-                // 1.4999999999999998).  One correction: what the product leaves of y is
-                // exact in the fma, so a quotient of 53 bits comes out as it is.
+                // 1.4999999999999998).  One correction, with what the product leaves of
+                // y: 2^-92, so a quotient of 53 bits comes out as it is.
                 double n = y[e] * up;
                 n = fma(fma(-n, (double)scale, y[e]), up, n);
                 held[e] = zero ? 0 : (int8_t)(int)rint(n);
