@@ -14,7 +14,7 @@ from . import (XT_ERR_INVALID, XT_PACK4, XT_PACK5, XT_QUANT_AVX512, XT_XORSPARSE
                hf_destripe, kv_append, mlp_f32, mlp_q, paged_attention, rms_norm, XT_INT8, XT_INT4, int_quantize_host,
                linear_f32, linear_multi_f32, linear_multi_q, linear_q, pack_ternary4, pack_ternary5,
                unpack_1_58bit_4pack, unpack_1_58bit_5pack)
-from .cache import _I32, _empty
+from .cache import _I32, _check_spans, _empty
 
 
 class TernaryRep(enum.Enum):
@@ -348,6 +348,7 @@ class CausalSelfAttention:
                                    or any(tuple(n.weight.shape) != (head_dim,) for n in (q_norm, k_norm))):
             raise XternError(XT_ERR_INVALID, "q_norm and k_norm must be of head_dim and one eps")
         self.q_proj, self.k_proj, self.v_proj, self.o_proj = q_proj, k_proj, v_proj, o_proj
+        _check_spans(0, 1, window, sink)
         self.head_dim = int(head_dim)
         self.attn_sub_norm = attn_sub_norm
         self.norm = (q_norm.weight, k_norm.weight, q_norm.eps) if q_norm is not None else None
@@ -376,6 +377,10 @@ class CausalSelfAttention:
             raise XternError(XT_ERR_INVALID, "the cache's heads are not the projections'")
         if tokens != 1 and seq is None:
             raise XternError(XT_ERR_INVALID, "tokens of one sequence need seq")
+        # (what the attention would refuse, before the append has written)
+        _check_spans(x.shape[0], tokens, self.window, self.sink)
+        if accumulate and cache.score is None:
+            raise XternError(XT_ERR_INVALID, "accumulate needs a cache with scores")
         x = x.contiguous()
         ws = [l.weights for l in (self.q_proj, self.k_proj, self.v_proj)]
         if all(w.fmt == ws[0].fmt and w.in_dim == ws[0].in_dim for w in ws):
