@@ -431,6 +431,7 @@ int xt_kv_evict(const xt_kv_cache* c, const xt_kv_table* t, const int32_t* lengt
                 int64_t recent, int32_t* new_lengths, int32_t* kept, void* stream) {
     xt::EvictArgs a;
     memset(&a, 0, sizeof a);
+    if (c && c->dtype == XT_I8) return bad("eviction needs a cache with scores, which one of 8-bit codes does not keep");
     if (int rc = check_cache(c, nullptr, t, &a.c)) return rc;
     if (!c->score) return bad("eviction needs a cache with scores");
     if (budget < 1 || budget > kMaxInt) return bad("budget must be 1..2^31-1");
