@@ -59,6 +59,35 @@ __device__ __forceinline__ int wave_reduce_bits(int v, Op op) {
     return __builtin_amdgcn_readlane(v, 63);
 }
 
+// Over LANES (16, 32 or 64) lanes side by side, in every one of them: within 16 by
+// DPP (quads, halves of a row, rows), then by lane swaps; 64 bits as two halves.
+template <int CTRL>
+__device__ __forceinline__ int dpp_to(int v) {
+    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_to(double v) {
+    return __hiloint2double(dpp_to<CTRL>(__double2hiint(v)), dpp_to<CTRL>(__double2loint(v)));
+}
+template <int LANES>
+__device__ __forceinline__ double lanes_sum(double v) {
+    v += dpp_to<0xb1>(v);
+    v += dpp_to<0x4e>(v);
+    v += dpp_to<0x141>(v);
+    v += dpp_to<0x140>(v);
+    if constexpr (LANES > 16) {
+        const auto h = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
+        const auto l = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
+        v = __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
+    }
+    if constexpr (LANES > 32) {
+        const auto h = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(v), false, false);
+        const auto l = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(v), false, false);
+        v = __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
+    }
+    return v;
+}
+
 struct MaxOp {
     __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };

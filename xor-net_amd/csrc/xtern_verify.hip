@@ -142,28 +142,8 @@ struct VerifyTile {
     }
 };
 
-// Over the wave, in every lane: within 16 lanes by DPP (quads, halves of a row,
-// rows), then by lane swaps; 64-bit values as two halves.
-template <int CTRL>
-__device__ __forceinline__ int dpp_to(int v) {
-    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, true);
-}
-template <int CTRL>
-__device__ __forceinline__ double dpp_to(double v) {
-    return __hiloint2double(dpp_to<CTRL>(__double2hiint(v)), dpp_to<CTRL>(__double2loint(v)));
-}
-__device__ __forceinline__ double wave_add(double v) {
-    v += dpp_to<0xb1>(v);
-    v += dpp_to<0x4e>(v);
-    v += dpp_to<0x141>(v);
-    v += dpp_to<0x140>(v);
-    auto h = __builtin_amdgcn_permlane16_swap(__double2hiint(v), __double2hiint(v), false, false);
-    auto l = __builtin_amdgcn_permlane16_swap(__double2loint(v), __double2loint(v), false, false);
-    v = __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
-    h = __builtin_amdgcn_permlane32_swap(__double2hiint(v), __double2hiint(v), false, false);
-    l = __builtin_amdgcn_permlane32_swap(__double2loint(v), __double2loint(v), false, false);
-    return __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
-}
+// Over the wave, in every lane.
+__device__ __forceinline__ double wave_add(double v) { return lanes_sum<64>(v); }
 template <typename Op>
 __device__ __forceinline__ int wave_of(int v, Op op) {
     v = op(v, dpp_to<0xb1>(v));
