@@ -508,10 +508,12 @@ typedef struct xt_head_norm {
 
 /* xt_kv_append_lengths with norms of q's and k's heads before the rotation
  * (norm NULL: none) and into a cache of any type; scales: an XT_I8 cache's, else
- * NULL.  The heads are normed, rotated and quantised in 64 bits and rounded once.
+ * NULL.  The heads are normed and rotated in 64 bits (xt_kv_append: in 32, so
+ * that results of the two may differ by its roundings) and rounded to f32 for
+ * q_out and a cache of 32 bits, and from there to one of 16 bits.
  * An XT_I8 cache gets, of a head y of k or v with a = max |y|, the scale s = a /
- * 127 (rounded to f32) and the codes round(y / s) (nearest, ties to even); s and
- * codes 0 where a < 2^-119; NaN and codes 0 where the head has an infinity or
+ * 127 (rounded to f32) and the codes round(y / s) (in 64 bits; nearest, ties to
+ * even); s and codes 0 where a < 2^-119; NaN and codes 0 where the head has an infinity or
  * NaN.  lengths may be NULL. */
 int xt_kv_store(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t,
                 const int32_t* seq, const int32_t* slots, const int32_t* positions,
@@ -521,7 +523,8 @@ int xt_kv_store(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_ta
 
 /* Keys and values of R positions as the cache holds them: row r of k and v
  * [R][kv_heads * head_dim] (row strides ldk, ldv; type out: XT_F32, XT_F16 or
- * XT_BF16, rounded to nearest even) gets position slots[r] of sequence seq[r]
+ * XT_BF16, rounded to nearest even; an XT_I8 cache's code times scale to f32
+ * first) gets position slots[r] of sequence seq[r]
  * (seq NULL: sequence r), zeros where the slot is negative or past the table or
  * the sequence or page does not exist. */
 int xt_kv_read(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t,
@@ -561,8 +564,11 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
  *   them share one pass over its positions; over the others every row makes its
  *   own.  R times the key-value heads (16 query heads at most each) is below
  *   2^31 over an XT_I8 cache.
- * Positions that no row sees are not read.  Queries and an XT_I8 cache's codes
- * meet in whole numbers of 24 and 8 bits: results keep the precision of f32. */
+ * Positions that no row sees are not read.  Over an XT_I8 cache queries and
+ * weights meet the codes as whole numbers: a query element is off by less than
+ * 2^-22 of its head's largest, a position's weight times its value scale by less
+ * than 2^-22 of the largest among the 64 positions that are read with it, and
+ * nothing is lost in the products' sums. */
 int xt_paged_attention_window(const xt_kv_cache* c, const xt_kv_scales* scales,
                               const xt_kv_table* t, const int32_t* seq, const int32_t* lengths,
                               int64_t tokens, int64_t window, int64_t sink, const float* q,
@@ -604,7 +610,7 @@ int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int6
  * drafted[b][t - 1]; draft: the logits [S][T][V] that the drafts were drawn from
  * (strides ldd_seq, ldd_row), or NULL: each was certain.  counts [S] (NULL: T
  * each): drafts of a sequence, at most T; negative: no sequence.  With p and q
- * the probabilities softmax(x / temperature) and given uniforms [S][T + 1] in
+ * the probabilities softmax(x / temperature), the temperature of both, and given uniforms [S][T + 1] in
  * [0, 1): drafts are accepted while uniforms[b][t] q(x_t) < p(x_t); the token
  * after them is drawn with uniforms[b][T] from max(p - q, 0) of the first that
  * was not (an id outside the vocabulary ends the drafts before it, as counts

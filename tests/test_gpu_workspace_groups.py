@@ -14,13 +14,13 @@ pytestmark = pytest.mark.gpu
 I32 = dict(dtype=torch.int32, device="cuda")
 
 
-@pytest.mark.parametrize("window,sink", [(None, 0), (40, 3)], ids=["all", "window"])
+@pytest.mark.parametrize("window,sink", [(None, 0), (40, 3), (1 << 19, 3)], ids=["all", "window", "wide window"])
 @pytest.mark.parametrize("named", [False, True], ids=["rows", "seq"])
 @pytest.mark.parametrize("dtype,R,tokens", [(torch.float32, 40, 8), (torch.bfloat16, 42, 42), (torch.float16, 1105, 13)],
                          ids=str)
 def test_scores_of_groups(dtype, R, tokens, named, window, sink):
     """Rows of 64 query heads over a table for 2^20 positions, 4 rows to a part
-    without a window: as over the narrow table, and as each row by itself."""
+    without a window, 7 with the wide one: as over the narrow table, and as each row by itself."""
     log(f"accumulate {dtype} {R} {tokens} {named} {window}")
     rng = np.random.default_rng(R)
     hq, H, D = 64, 2, 64

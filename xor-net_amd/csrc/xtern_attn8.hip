@@ -15,8 +15,9 @@ namespace xt {
 // weights exp(s - m) vs) is rounded to a whole number of 24 bits, x 2^k, with
 // the largest of its column near 2^23, and that to three signed 8-bit digits,
 // whose products with the codes add up in 32-bit integers without rounding.
-// What is lost is 2^-24 of the column's largest operand: of the query once, of
-// the weights in each tile of 64 positions on its own.
+// What is lost is half a unit of the column's largest operand, which is 4177856
+// or more: of the query once, of the weights in each tile of 64 positions on its
+// own.
 // The columns are the query heads of a group, and the groups of several rows
 // where rows share a sequence (16 / group rows): drafts and prompts read the
 // cache once for all of these.  As in the 16-bit kernel everything is

@@ -15,7 +15,8 @@ namespace xt {
 // 0; a head with an infinity or NaN has s = NaN, c = 0, so that what reads it
 // sees NaN.
 //
-// All of it in 64 bits, rounded once (to f32, then to the cache's type): a value
+// All of it in 64 bits, then rounded to f32 and from there to a 16-bit cache's type;
+// codes come from the 64 bits: a value
 // next to the border of two codes falls where the exact one does, in whatever
 // order sums are taken.  The f64 units take 4 cycles an instruction like the
 // f32 ones, and a call is bound by its bytes or by its launch.
@@ -25,8 +26,8 @@ namespace xt {
 // loads what its own elements are rotated with, OW = 4, 2 or 1 at a time as h is a
 // multiple of these, and the next head's of both while it works on one.  The heads
 // of a row go to several workgroups where rows are few.  HBM bounds long calls: 4096
-// rows of 32 + 2 x 8 heads of 128 36 us (5.0 TB/s) on the same tensors again, 41 on
-// others; one row takes 3.5.  Heads of 100:
+// rows of 32 + 2 x 8 heads of 128 36 us (5.0 TB/s) on the same tensors again, 40.7 on
+// others; one row takes 3.6.  Heads of 100:
 // 34 us without a rotation, 36.5 with half of 25, 42.5 with 50 (element by element
 // all of it: 54 and 66).
 template <int DT> struct Held;

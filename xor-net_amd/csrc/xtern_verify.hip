@@ -24,9 +24,9 @@
 // again, in tiles of 512 logits a wave, and the workgroup that ends the
 // sequence's last tile finds the tile and in it the token (sums and count at
 // device scope, as the chip's eight L2s need it).
-// 64 sequences of 4 drafts, 128003 bf16 logits: 52 + 30 us, where HBM would take 23:
+// 64 sequences of 4 drafts, 128003 bf16 logits: 53 + 30.5 us, where HBM would take 23:
 // 22 f64 instructions a logit are 36 us of the first kernel.  One sequence of 128256
-// f32 logits: 5.3 + 13.1 us, the second one a chain of eight dependent trips to
+// f32 logits: 5.6 + 13.1 us, the second one a chain of eight dependent trips to
 // memory (sums, drafts, their logits, the row, stores, count, tile sums, the tile).
 #include <algorithm>
 

@@ -249,7 +249,8 @@ def kv_append(cache, table, slots, k, v, q=None, seq=None, positions=None, rope=
     what each token sees, slots[r] + 1, or 0 for a row that was skipped.
     norm = (q weight, k weight, eps), float32 [head_dim] each, norms q's and
     k's heads before the rotation (xt_kv_store, as for an int8 cache, which gets
-    codes and a scale for each token and head).
+    codes and a scale for each token and head; in 64 bits, where xt_kv_append
+    rotates in 32).
     Returns the rotated q (q_out if given, which may be q), or None without q."""
     here, D = _here(), cache.head_dim
     c = cache._on(here)
@@ -457,7 +458,8 @@ def verify_drafts(target, drafted, uniforms, draft=None, counts=None, temperatur
     """xt_verify_drafts: T (0..64) drafted tokens (int32 [S, T]) of each of S
     sequences against the target model's logits [S, T + 1, V] (float32, float16
     or bfloat16, -inf for masked tokens) and the logits that they were drawn
-    from, draft [S, T, V] (None: each was certain).  uniforms: float32 [S, T +
+    from at the same temperature, draft [S, T, V] of target's type (None: each
+    was certain).  uniforms: float32 [S, T +
     1] in [0, 1), the first T accept, the last one draws.  counts (int32 [S]):
     drafts of each sequence (default T; negative: no sequence).  temperature:
     a number >= 0 or float32 [S]; 0 takes the most likely token.  Returns
