@@ -513,8 +513,8 @@ typedef struct xt_head_norm {
  * q_out and a cache of 32 bits, and from there to one of 16 bits.
  * An XT_I8 cache gets, of a head y of k or v with a = max |y|, the scale s = a /
  * 127 (rounded to f32) and the codes round(y / s) (in 64 bits; nearest, ties to
- * even); s and codes 0 where a < 2^-119; NaN and codes 0 where the head has an infinity or
- * NaN.  lengths may be NULL. */
+ * even); s and codes 0 where a < 2^-119; NaN and codes 0 where the head has an
+ * infinity or NaN.  lengths may be NULL. */
 int xt_kv_store(const xt_kv_cache* c, const xt_kv_scales* scales, const xt_kv_table* t,
                 const int32_t* seq, const int32_t* slots, const int32_t* positions,
                 const xt_rope* rope, const xt_head_norm* norm, const float* q, int64_t ldq,
@@ -567,8 +567,8 @@ int xt_paged_attention(const xt_kv_cache* c, const xt_kv_table* t, const int32_t
  * Positions that no row sees are not read.  Over an XT_I8 cache queries and
  * weights meet the codes as whole numbers: a query element is off by less than
  * 2^-22 of its head's largest, a position's weight times its value scale by less
- * than 2^-22 of the largest among the 64 positions that are read with it, and
- * nothing is lost in the products' sums. */
+ * than 2^-22 of the largest among the 64 positions that are read with it; their
+ * products' sums are whole numbers until they are rounded to f32. */
 int xt_paged_attention_window(const xt_kv_cache* c, const xt_kv_scales* scales,
                               const xt_kv_table* t, const int32_t* seq, const int32_t* lengths,
                               int64_t tokens, int64_t window, int64_t sink, const float* q,
@@ -610,12 +610,12 @@ int xt_token_logprobs(int dtype, const void* logits, int64_t ld, int64_t M, int6
  * drafted[b][t - 1]; draft: the logits [S][T][V] that the drafts were drawn from
  * (strides ldd_seq, ldd_row), or NULL: each was certain.  counts [S] (NULL: T
  * each): drafts of a sequence, at most T; negative: no sequence.  With p and q
- * the probabilities softmax(x / temperature), the temperature of both, and given uniforms [S][T + 1] in
- * [0, 1): drafts are accepted while uniforms[b][t] q(x_t) < p(x_t); the token
- * after them is drawn with uniforms[b][T] from max(p - q, 0) of the first that
- * was not (an id outside the vocabulary ends the drafts before it, as counts
- * does), or from p after the last: the lowest id up to which the sum is above
- * that share of the whole.
+ * the probabilities softmax(x / temperature), of both at one temperature, and
+ * given uniforms [S][T + 1] in [0, 1): drafts are accepted while uniforms[b][t]
+ * q(x_t) < p(x_t); the token after them is drawn with uniforms[b][T] from max(p -
+ * q, 0) of the first that was not (an id outside the vocabulary ends the drafts
+ * before it, as counts does), or from p after the last: the lowest id up to which
+ * the sum is above that share of the whole.
  * temperature >= 0 for every sequence, or temperatures [S]; at 0 all of p lies
  * on the largest logit (the lowest id of equals).  accepted [S]: drafts that
  * were; tokens [S][T + 1]: these, the drawn one, then -1; logprobs [S][T + 1]: ln
